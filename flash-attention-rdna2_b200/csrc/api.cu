@@ -80,16 +80,6 @@ static bool valid_hd(int d) {
 
 using fa::set_error;
 
-#define FA_ABI_GUARD(p, T)                                                                   \
-  do {                                                                                       \
-    if (!(p)) { set_error(#T ": null parameter block"); return FA_ERR_INVALID; }              \
-    if ((p)->struct_size != sizeof(T)) {                                                     \
-      set_error(#T ": struct_size %u != %zu (caller built against another fable_attn.h)",     \
-                (p)->struct_size, sizeof(T));                                                \
-      return FA_ERR_ABI;                                                                     \
-    }                                                                                        \
-  } while (0)
-
 static bool dtype_ok(int dt) { return dt == FA_DTYPE_F16 || dt == FA_DTYPE_BF16 || dt == FA_DTYPE_F32; }
 
 extern "C" int fa_abi_version(void) { return FA_ABI_VERSION; }

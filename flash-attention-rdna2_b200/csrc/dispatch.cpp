@@ -2,13 +2,16 @@
 // include/fable_attn.h and enqueues the launch on torch's current stream for the tensor's device.
 // Same function names and argument order as the reference's extension
 // (package/csrc/dispatch.cpp:239-267): fwd, bwd, fwd_varlen, dec; plus bwd_varlen (native varlen
-// backward), combine (flash_attn_combine on the GPU) and kernel_launch_count.
+// backward), combine (flash_attn_combine on the GPU), kv_append / kv_gather / dec8 (paged caches held in
+// 8 bits) and kernel_launch_count.
 // Outputs and workspaces (out, lse, dq/dk/dv, dsum, decode scratch) are allocated here by torch,
 // as in the reference; kernels own nothing.  No host synchronisation anywhere.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <algorithm>
 #include <cmath>
+#include <type_traits>
 #include "fable_attn.h"
 
 namespace {
@@ -384,6 +387,230 @@ std::vector<torch::Tensor> dec(torch::Tensor q, torch::Tensor k_cache, torch::Te
   return {out, lse};
 }
 
+// ------------------------------------------------------------------ paged caches held in 8 bits
+const torch::Tensor* opt_ptr(const c10::optional<torch::Tensor>& t) { return t.has_value() && t->defined() ? &*t : nullptr; }
+
+// an integer index tensor as contiguous int32 on `dev` (itself where it is that already)
+torch::Tensor index_i32(const torch::Tensor& t, const torch::Device& dev, const char* name) {
+  TORCH_CHECK_VALUE(!t.is_floating_point() && t.scalar_type() != torch::kBool, "fable_attn: ", name, " must be integers");
+  return t.to(dev, torch::kInt32).contiguous();
+}
+
+// The cache's side of a parameter block: k_cache / v_cache (num_blocks, page, nheads_k, headdim) with the scales
+// (num_blocks, nheads_k, page / block) of an 8-bit one, and the block table.
+template <typename P>
+torch::Tensor set_cache(P& p, const torch::Tensor& k_cache, const torch::Tensor& v_cache,
+                        const c10::optional<torch::Tensor>& k_scale, const c10::optional<torch::Tensor>& v_scale,
+                        const torch::Tensor& block_table) {
+  TORCH_CHECK_VALUE(k_cache.is_cuda() && v_cache.device() == k_cache.device(),
+                    "fable_attn: k_cache and v_cache must be CUDA tensors on one device");
+  TORCH_CHECK_VALUE(k_cache.dim() == 4 && k_cache.is_contiguous() && v_cache.is_contiguous() &&
+                        k_cache.sizes() == v_cache.sizes() && k_cache.scalar_type() == v_cache.scalar_type(),
+                    "fable_attn: k_cache / v_cache must be contiguous (num_blocks, page, nheads_k, headdim) of one shape and type");
+  const auto dt = k_cache.scalar_type();
+  const bool scaled = dt == torch::kInt8 || dt == torch::kFloat8_e4m3fn;
+  p.code = dt == torch::kInt8 ? FA_CODE_I8 : dt == torch::kFloat8_e4m3fn ? FA_CODE_E4M3 : dt_of(k_cache);
+  const auto *ks = opt_ptr(k_scale), *vs = opt_ptr(v_scale);
+  TORCH_CHECK_VALUE((ks != nullptr) == scaled && (vs != nullptr) == scaled,
+                    "fable_attn: k_scale and v_scale go with an int8 or float8_e4m3fn cache, and only with one");
+  p.block = 1;
+  if (scaled) {
+    for (const auto* s : {ks, vs})
+      TORCH_CHECK_VALUE(s->device() == k_cache.device() && s->scalar_type() == torch::kFloat32 && s->is_contiguous() &&
+                            s->dim() == 3 && s->size(0) == k_cache.size(0) && s->size(1) == k_cache.size(2) &&
+                            s->size(2) > 0 && k_cache.size(1) % s->size(2) == 0 && s->sizes() == ks->sizes(),
+                        "fable_attn: k_scale / v_scale must be contiguous fp32 (num_blocks, nheads_k, page / block)");
+    p.block = (int)(k_cache.size(1) / ks->size(2));
+  }
+  TORCH_CHECK_VALUE(block_table.dim() == 2, "fable_attn: block_table must be (batch, max_blocks)");
+  const torch::Tensor bt = index_i32(block_table, k_cache.device(), "block_table");
+  if constexpr (std::is_same<P, FaKvAppendParams>::value) {
+    p.Ks = scaled ? ks->data_ptr<float>() : nullptr;
+    p.Vs = scaled ? vs->data_ptr<float>() : nullptr;
+  } else {
+    p.Ks = scaled ? ks->const_data_ptr<float>() : nullptr;
+    p.Vs = scaled ? vs->const_data_ptr<float>() : nullptr;
+  }
+  p.struct_size = sizeof(P);
+  p.Kc = k_cache.data_ptr();
+  p.Vc = v_cache.data_ptr();
+  p.block_table = bt.data_ptr<int>();
+  p.batch = (int)bt.size(0);
+  p.max_blocks = (int)bt.size(1);
+  p.dim = (int)k_cache.size(3);
+  p.page = (int)k_cache.size(1);
+  p.num_blocks = k_cache.size(0);
+  return bt;
+}
+
+template <typename P>
+void set_rotary(P& p, const c10::optional<torch::Tensor>& cos, const c10::optional<torch::Tensor>& sin, bool interleaved,
+                const torch::Device& dev, torch::Tensor& c, torch::Tensor& s) {
+  const auto *hc = opt_ptr(cos), *hs = opt_ptr(sin);
+  TORCH_CHECK_VALUE((hc != nullptr) == (hs != nullptr), "fable_attn: rotary_cos and rotary_sin go together");
+  if (!hc) return;
+  TORCH_CHECK_VALUE(hc->dim() == 2 && hs->sizes() == hc->sizes() && hc->device() == dev && hs->device() == dev &&
+                        hc->size(0) > 0 && 2 * hc->size(1) <= p.dim,
+                    "fable_attn: rotary_cos / rotary_sin must be (seqlen_ro, rotary_dim / 2) on the cache's device with "
+                    "rotary_dim <= headdim");
+  c = hc->to(torch::kFloat32).contiguous();
+  s = hs->to(torch::kFloat32).contiguous();
+  p.cos = c.data_ptr<float>();
+  p.sin = s.data_ptr<float>();
+  p.rot_dim = (int)c.size(1) * 2;
+  p.rot_seqlen_ro = (int)c.size(0);
+  p.rot_interleaved = interleaved ? 1 : 0;
+}
+
+// rows of x: (batch, tokens, heads, dim) whose first two dimensions step as one, or packed
+// (total, heads, dim); a layout that strides cannot say is copied
+torch::Tensor rows_of(const torch::Tensor& x, bool packed, const char* name) {
+  TORCH_CHECK_VALUE(x.dim() == (packed ? 3 : 4), "fable_attn: ", name, " must be ",
+                    packed ? "(total, nheads, headdim) with cu_seqlens" : "(batch, seqlen, nheads, headdim)");
+  if (packed) return x.stride(2) == 1 ? x : x.contiguous();
+  const bool one = x.size(0) <= 1 || x.size(1) == 0 || x.stride(0) == x.size(1) * x.stride(1);
+  return x.stride(3) == 1 && one ? x : x.contiguous();
+}
+
+void kv_append(torch::Tensor k, torch::Tensor v, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor cache_seqlens,
+               torch::Tensor block_table, c10::optional<torch::Tensor> k_scale, c10::optional<torch::Tensor> v_scale,
+               c10::optional<torch::Tensor> cu_new, c10::optional<torch::Tensor> rotary_cos,
+               c10::optional<torch::Tensor> rotary_sin, bool rotary_interleaved, c10::optional<torch::Tensor> rotary_pos) {
+  FaKvAppendParams p{};
+  TORCH_CHECK_VALUE(k.is_cuda() && v.is_cuda(), "fable_attn: k and v must be CUDA tensors");
+  const c10::cuda::CUDAGuard guard(k.device());
+  const auto bt = set_cache(p, k_cache, v_cache, k_scale, v_scale, block_table);
+  const auto dev = k_cache.device();
+  const auto* cu = opt_ptr(cu_new);
+  TORCH_CHECK_VALUE(k.device() == dev && v.device() == dev && k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type(),
+                    "fable_attn: k and v must agree in shape and type and lie on the cache's device");
+  const torch::Tensor kr = rows_of(k, cu, "k"), vr = rows_of(v, cu, "v");
+  const int hd = cu ? 1 : 2;
+  TORCH_CHECK_VALUE(k.size(hd) == k_cache.size(2) && k.size(hd + 1) == k_cache.size(3),
+                    "fable_attn: k / v have (nheads_k, headdim) = (", k.size(hd), ", ", k.size(hd + 1),
+                    "), the cache (", k_cache.size(2), ", ", k_cache.size(3), ")");
+  TORCH_CHECK_VALUE(p.code >= FA_CODE_I8 || k.scalar_type() == k_cache.scalar_type(),
+                    "fable_attn: k / v and a cache without scales must have one type");
+  const auto lens = index_i32(cache_seqlens, dev, "cache_seqlens");
+  TORCH_CHECK_VALUE(lens.numel() == p.batch && (cu || k.size(0) == p.batch),
+                    "fable_attn: cache_seqlens, block_table and k / v must agree on the batch (", p.batch, ")");
+  torch::Tensor c32, pos32, cs, sn;
+  if (cu) {
+    c32 = index_i32(*cu, dev, "cu_seqlens_new");
+    TORCH_CHECK_VALUE(c32.numel() == p.batch + 1, "fable_attn: cu_seqlens_new must have batch + 1 = ", p.batch + 1, " entries");
+    p.cu_new = c32.data_ptr<int>();
+  } else {
+    p.tokens = (int)k.size(1);
+  }
+  if (const auto* rp = opt_ptr(rotary_pos)) {
+    pos32 = index_i32(*rp, dev, "rotary_seqlens");
+    TORCH_CHECK_VALUE(pos32.numel() == p.batch, "fable_attn: rotary_seqlens needs one entry per sequence");
+    p.rot_pos = pos32.data_ptr<int>();
+  }
+  p.heads = (int)k_cache.size(2);
+  set_rotary(p, rotary_cos, rotary_sin, rotary_interleaved, dev, cs, sn);
+  p.k = kr.data_ptr(); p.v = vr.data_ptr();
+  p.k_row = kr.stride(hd - 1); p.k_head = kr.stride(hd);
+  p.v_row = vr.stride(hd - 1); p.v_head = vr.stride(hd);
+  p.ctx_len = lens.data_ptr<int>();
+  p.total = cu ? k.size(0) : k.size(0) * k.size(1);
+  if (p.total > 0) check(fa_kv_append_launch(&p, dt_of(k), cur_stream(k)), "cache append");
+}
+
+std::vector<torch::Tensor> kv_gather(torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor block_table,
+                                     torch::Tensor cu_k, int64_t total, c10::optional<torch::Tensor> k_scale,
+                                     c10::optional<torch::Tensor> v_scale, c10::optional<torch::Tensor> starts,
+                                     c10::optional<c10::ScalarType> dtype) {
+  FaKvGatherParams p{};
+  TORCH_CHECK_VALUE(k_cache.is_cuda(), "fable_attn: k_cache must be a CUDA tensor");
+  const c10::cuda::CUDAGuard guard(k_cache.device());
+  const auto bt = set_cache(p, k_cache, v_cache, k_scale, v_scale, block_table);
+  const auto dev = k_cache.device();
+  const auto cu = index_i32(cu_k, dev, "cu_seqlens_k");
+  TORCH_CHECK_VALUE(cu.numel() == p.batch + 1, "fable_attn: cu_seqlens_k must have batch + 1 = ", p.batch + 1, " entries");
+  TORCH_CHECK_VALUE(total >= 0, "fable_attn: total_k=", total);
+  torch::Tensor st;
+  if (const auto* s = opt_ptr(starts)) {
+    st = index_i32(*s, dev, "seq_starts");
+    TORCH_CHECK_VALUE(st.numel() == p.batch, "fable_attn: seq_starts needs one entry per sequence");
+    p.starts = st.data_ptr<int>();
+  }
+  const auto odt = dtype.has_value() ? *dtype : p.code >= FA_CODE_I8 ? torch::kBFloat16 : k_cache.scalar_type();
+  auto k = torch::empty({total, k_cache.size(2), k_cache.size(3)}, k_cache.options().dtype(odt)), v = torch::empty_like(k);
+  p.heads = (int)k_cache.size(2);
+  p.cu_k = cu.data_ptr<int>();
+  p.k = k.data_ptr(); p.v = v.data_ptr();
+  p.total = total;
+  if (total > 0) check(fa_kv_gather_launch(&p, dt_of(k), cur_stream(k)), "cache gather");
+  return {k, v};
+}
+
+std::vector<torch::Tensor> dec8(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor k_scale,
+                                torch::Tensor v_scale, torch::Tensor cache_seqlens, torch::Tensor block_table, double scale,
+                                int64_t win_left, int64_t win_right, double softcap, c10::optional<torch::Tensor> alibi,
+                                c10::optional<torch::Tensor> cu_q, int64_t max_tokens, c10::optional<torch::Tensor> leftpad,
+                                c10::optional<torch::Tensor> rotary_cos, c10::optional<torch::Tensor> rotary_sin,
+                                bool rotary_interleaved, c10::optional<torch::Tensor> rotary_pos, bool return_lse) {
+  FaDec8Params p{};
+  TORCH_CHECK_VALUE(q.is_cuda(), "fable_attn: q must be a CUDA tensor");
+  const c10::cuda::CUDAGuard guard(q.device());
+  const auto bt = set_cache(p, k_cache, v_cache, k_scale, v_scale, block_table);
+  const auto dev = k_cache.device();
+  const auto* cu = opt_ptr(cu_q);
+  TORCH_CHECK_VALUE(q.device() == dev, "fable_attn: q must lie on the cache's device");
+  const torch::Tensor qr = rows_of(q, cu, "q");
+  const int hd = cu ? 1 : 2;
+  const int64_t Hq = q.size(hd), Hk = k_cache.size(2);
+  TORCH_CHECK_VALUE(q.size(hd + 1) == k_cache.size(3), "fable_attn: q has headdim ", q.size(hd + 1), ", the cache ",
+                    k_cache.size(3));
+  TORCH_CHECK_VALUE(Hk > 0 && Hq > 0 && Hq % Hk == 0, "fable_attn: nheads_q=", Hq, " is not a multiple of nheads_k=", Hk);
+  const auto lens = index_i32(cache_seqlens, dev, "cache_seqlens");
+  TORCH_CHECK_VALUE(lens.numel() == p.batch && (cu || q.size(0) == p.batch),
+                    "fable_attn: cache_seqlens, block_table and q must agree on the batch (", p.batch, ")");
+  torch::Tensor c32, lp, pos32, cs, sn, al;
+  if (cu) {
+    c32 = index_i32(*cu, dev, "cu_seqlens_q");
+    TORCH_CHECK_VALUE(c32.numel() == p.batch + 1, "fable_attn: cu_seqlens_q must have batch + 1 = ", p.batch + 1, " entries");
+    p.cu_q = c32.data_ptr<int>();
+  } else {
+    p.tokens = (int)q.size(1);
+  }
+  p.total = cu ? q.size(0) : q.size(0) * q.size(1);
+  p.max_tokens = (int)std::max<int64_t>(1, cu ? max_tokens : q.size(1));
+  if (const auto* t = opt_ptr(leftpad)) {
+    lp = index_i32(*t, dev, "cache_leftpad");
+    TORCH_CHECK_VALUE(lp.numel() == p.batch, "fable_attn: cache_leftpad needs one entry per sequence");
+    p.leftpad = lp.data_ptr<int>();
+  }
+  if (const auto* t = opt_ptr(rotary_pos)) {
+    pos32 = index_i32(*t, dev, "rotary_seqlens");
+    TORCH_CHECK_VALUE(pos32.numel() == p.batch, "fable_attn: rotary_seqlens needs one entry per sequence");
+    p.rot_pos = pos32.data_ptr<int>();
+  }
+  if (const auto* t = opt_ptr(alibi)) {
+    al = t->to(dev, torch::kFloat32).contiguous();
+    TORCH_CHECK_VALUE(al.dim() == 1 && al.numel() == Hq, "fable_attn: alibi_slopes must be (nheads,)");
+    p.alibi = al.data_ptr<float>();
+  }
+  set_rotary(p, rotary_cos, rotary_sin, rotary_interleaved, dev, cs, sn);
+  p.NH = (int)Hq; p.gqa = (int)(Hq / Hk);
+  p.q = qr.data_ptr(); p.q_row = qr.stride(hd - 1); p.q_head = qr.stride(hd);
+  p.ctx_len = lens.data_ptr<int>();
+  auto out = torch::empty(q.sizes(), q.options());
+  torch::Tensor lse;
+  if (return_lse)
+    lse = cu ? torch::empty({Hq, p.total}, q.options().dtype(torch::kFloat32))
+             : torch::empty({q.size(0), Hq, q.size(1)}, q.options().dtype(torch::kFloat32));
+  auto scratch = torch::empty({fa_decode8_scratch_floats(p.NH, p.gqa, p.dim)}, q.options().dtype(torch::kFloat32));
+  p.o = out.data_ptr();
+  p.lse = return_lse ? lse.data_ptr<float>() : nullptr;
+  p.scratch = scratch.data_ptr<float>();
+  p.scale = (float)scale; p.softcap = (float)softcap;
+  p.win_left = (int)win_left; p.win_right = (int)win_right;
+  if (p.total > 0) check(fa_decode8_launch(&p, dt_of(q), cur_stream(q)), "decode (8-bit cache)");
+  return return_lse ? std::vector<torch::Tensor>{out, lse} : std::vector<torch::Tensor>{out};
+}
+
 // ------------------------------------------------------------------ combine
 std::vector<torch::Tensor> combine(torch::Tensor out_partial, torch::Tensor lse_partial, c10::ScalarType out_dtype,
                                    bool return_lse) {
@@ -564,6 +791,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("softcap") = 0.0, py::arg("alibi") = c10::optional<torch::Tensor>(), py::arg("rotary_dim") = 0,
         py::arg("rotary_pos") = c10::optional<torch::Tensor>(), py::arg("out_fp32") = false,
         py::arg("out") = c10::optional<torch::Tensor>(), py::arg("lse_out") = c10::optional<torch::Tensor>());
+  m.def("kv_append", &kv_append, py::arg("k"), py::arg("v"), py::arg("k_cache"), py::arg("v_cache"),
+        py::arg("cache_seqlens"), py::arg("block_table"), py::arg("k_scale"), py::arg("v_scale"), py::arg("cu_new"),
+        py::arg("rotary_cos"), py::arg("rotary_sin"), py::arg("rotary_interleaved"), py::arg("rotary_pos"));
+  m.def("kv_gather", &kv_gather, py::arg("k_cache"), py::arg("v_cache"), py::arg("block_table"), py::arg("cu_k"),
+        py::arg("total"), py::arg("k_scale"), py::arg("v_scale"), py::arg("starts"), py::arg("dtype"));
+  m.def("dec8", &dec8, py::arg("q"), py::arg("k_cache"), py::arg("v_cache"), py::arg("k_scale"), py::arg("v_scale"),
+        py::arg("cache_seqlens"), py::arg("block_table"), py::arg("scale"), py::arg("win_left"), py::arg("win_right"),
+        py::arg("softcap"), py::arg("alibi"), py::arg("cu_q"), py::arg("max_tokens"), py::arg("leftpad"),
+        py::arg("rotary_cos"), py::arg("rotary_sin"), py::arg("rotary_interleaved"), py::arg("rotary_pos"),
+        py::arg("return_lse"));
   m.def("combine", &combine, py::arg("out_partial"), py::arg("lse_partial"), py::arg("out_dtype"),
         py::arg("return_lse") = false);
   m.def("combine_packed", &combine_packed, py::arg("buf"), py::arg("nsplit"), py::arg("B"), py::arg("S"),

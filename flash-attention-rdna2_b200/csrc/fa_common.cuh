@@ -230,6 +230,17 @@ void count_launch(unsigned n = 1);
 int num_sms();
 }  // namespace fa
 
+// parameter block present and of the layout this library was built with
+#define FA_ABI_GUARD(p, T)                                                                   \
+  do {                                                                                       \
+    if (!(p)) { fa::set_error(#T ": null parameter block"); return FA_ERR_INVALID; }              \
+    if ((p)->struct_size != sizeof(T)) {                                                     \
+      fa::set_error(#T ": struct_size %u != %zu (caller built against another fable_attn.h)",     \
+                (p)->struct_size, sizeof(T));                                                \
+      return FA_ERR_ABI;                                                                     \
+    }                                                                                        \
+  } while (0)
+
 #define FA_CHECK_ARG(cond, ...)             \
   do {                                      \
     if (!(cond)) {                          \

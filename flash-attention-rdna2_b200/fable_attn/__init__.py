@@ -19,6 +19,12 @@ from .flash_attn_interface import (
     flash_attn_combine,
     flash_attn_with_kvcache,
 )
+from .kvcache import (
+    flash_attn_with_kvcache_8bit,
+    kvcache_append,
+    kvcache_gather,
+    new_cache_8bit,
+)
 from . import bert_padding
 from . import torch_op
 
@@ -37,7 +43,8 @@ def device_error(clear=False):
 __all__ = [
     "device_error", "flash_attn_func", "flash_attn_qkvpacked_func", "flash_attn_kvpacked_func", "flash_attn_varlen_func",
     "flash_attn_varlen_qkvpacked_func", "flash_attn_varlen_kvpacked_func", "flash_attn_combine",
-    "flash_attn_with_kvcache", "bert_padding", "install_as_flash_attn",
+    "flash_attn_with_kvcache", "flash_attn_with_kvcache_8bit", "kvcache_append", "kvcache_gather", "new_cache_8bit",
+    "bert_padding", "install_as_flash_attn",
 ]
 
 __version__ = "0.2.0"

@@ -39,6 +39,9 @@ extern "C" {
 
 /* dtype codes — same numbering as the reference (kernels/fa_forward.hip:403) */
 enum { FA_DTYPE_F16 = 0, FA_DTYPE_BF16 = 1, FA_DTYPE_F32 = 2 };
+/* element codes of an 8-bit paged cache (fa_kv_append_launch, fa_kv_gather_launch,
+ * fa_decode8_launch only; no counterpart in the reference) */
+enum { FA_CODE_I8 = 8, FA_CODE_E4M3 = 9 };
 
 /* status codes */
 enum {
@@ -285,6 +288,113 @@ FA_API int fa_decode_num_splits(int batch, int nq, int nheads_kv, long long ctx_
 FA_API long long fa_decode_scratch_floats(int batch, int nq, int NH, int HD, int nsplit);
 
 /* ------------------------------------------------------------------------------------------
+ * Paged caches held in 8 bits (no counterpart in the reference: its caches hold the inputs'
+ * type).  A cache is Kc / Vc [num_blocks, page, heads, dim] contiguous, page a power of two,
+ * position k of sequence z in page block_table[z * max_blocks + k / page], slot k % page, with
+ *   code FA_DTYPE_*               : the elements themselves (Ks / Vs null), or
+ *   code FA_CODE_I8 / FA_CODE_E4M3: one byte an element and Ks / Vs [num_blocks, heads, page / block]
+ *       fp32, one scale >= 0 for `block` consecutive slots of a page and a head (a power of two, at
+ *       most page and 256); an element's value is code * scale.  int8 codes are in [-127, 127], e4m3
+ *       codes finite.
+ * dim is a multiple of 16 up to 256.  A block-table entry outside [0, num_blocks) or a position
+ * past the table's row is neither read (it counts as empty) nor written, and raises
+ * fa_device_error bit 8192.
+ *
+ * fa_kv_append_launch writes new tokens: token i of sequence z goes to position ctx_len[z] + i.  k is rotated
+ * on the way (cos null = not), by the table row (rot_pos ? rot_pos[z] : ctx_len[z]) + i, in fp32 with
+ * every product and the difference rounded; a position outside the table leaves its row
+ * unrotated and raises bit 16384.  One rounding to the cache's type follows.  8 bits, for each
+ * scale block that gets new tokens and each head, in fp32:
+ *     s_old = the block's scale if it holds earlier tokens of the sequence, else 0
+ *     s     = max(s_old, amax * (1 / Q), 2^-100), amax over the new tokens in it, Q = 127 or 448
+ *     new codes      = round(x * (1 / s))                      (to nearest, ties to even)
+ *     earlier codes c: round(c * (s_old / s)) where s > s_old
+ * A NaN or an infinity among the new values makes s NaN and their codes 0, and a NaN scale lasts
+ * until the block is begun anew: what is read from the block is NaN, codes are always finite.
+ *   new rows [row][heads][dim] with element strides (dim contiguous): dense rows z * tokens + i, or,
+ *   with cu_new [batch + 1], rows cu_new[z] + i.  `total` = rows.
+ * -------------------------------------------------------------------------------------------*/
+typedef struct FaKvAppendParams {
+  unsigned int struct_size;
+  const void *k, *v;                   /* new rows, dtype of the call */
+  long long k_row, k_head, v_row, v_head;
+  void *Kc, *Vc;
+  float *Ks, *Vs;
+  const int* block_table;
+  const int* ctx_len;                  /* [batch] tokens in the cache before the append */
+  const int* cu_new;                   /* [batch + 1] or null */
+  int tokens;                          /* dense: new tokens of each sequence */
+  long long total;
+  int batch, heads, dim, page, block, max_blocks, code;
+  long long num_blocks;
+  const float *cos, *sin;              /* [rot_seqlen_ro, rot_dim / 2] or null */
+  int rot_dim, rot_seqlen_ro, rot_interleaved;
+  const int* rot_pos;                  /* [batch] or null */
+} FaKvAppendParams;
+
+FA_API int fa_kv_append_launch(const FaKvAppendParams* p, int dtype, void* stream);
+
+/* fa_kv_gather_launch: positions starts[z] + i (0 + i without starts), i < cu_k[z + 1] - cu_k[z], of
+ * each sequence as packed rows k / v [total, heads, dim] (dtype of the call) from row cu_k[z] on, each
+ * value code * scale in fp32 rounded once (16/32-bit caches: converted, or copied where the types are the same).
+ * Unreadable positions give 0. */
+typedef struct FaKvGatherParams {
+  unsigned int struct_size;
+  const void *Kc, *Vc;
+  const float *Ks, *Vs;
+  const int* block_table;
+  const int* cu_k;                     /* [batch + 1] */
+  const int* starts;                   /* [batch] or null */
+  void *k, *v;
+  long long total;
+  int batch, heads, dim, page, block, max_blocks, code;
+  long long num_blocks;
+} FaKvGatherParams;
+
+FA_API int fa_kv_gather_launch(const FaKvGatherParams* p, int dtype, void* stream);
+
+/* fa_decode8_launch: attention of new tokens over an 8-bit cache that holds them already (append
+ * first).  q rows [row][NH][dim] by strides, dense rows z * tokens + t or, with cu_q, cu_q[z] + t, n_z
+ * of them in sequence z; ctx_len[z] cached tokens, the new ones included.  Row t sits at position
+ * ctx_len[z] - n_z + t and sees the keys in [max(leftpad, pos - win_left), min(ctx_len, pos + win_right + 1))
+ * (a bound < 0 is no bound; causal = win_right 0).  Scores scale * q.k, then softcap c * tanh(s / c),
+ * then alibi slope * (key - pos), as in the forward; cos / sin rotate q by its position (or rot_pos[z] + t).
+ * A row that sees nothing gives 0 and LSE -inf.
+ *   o    [total, NH, dim] contiguous, dtype of the call (fp16 / bf16 / fp32)
+ *   lse  optional fp32, natural log: dense [batch, NH, tokens], with cu_q [NH, total]
+ *   scratch  fa_decode8_scratch_floats(NH, gqa, dim) floats, whatever the batch or the lengths
+ * max_tokens is a bound on n_z (dense: ignored).  The result does not depend on it, the choice of
+ * kernel does. */
+typedef struct FaDec8Params {
+  unsigned int struct_size;
+  const void* q;
+  long long q_row, q_head;
+  const void *Kc, *Vc;
+  const float *Ks, *Vs;
+  const int* block_table;
+  const int* ctx_len;
+  const int* cu_q;                     /* [batch + 1] or null */
+  int tokens;                          /* dense: new tokens of each sequence */
+  int max_tokens;
+  long long total;
+  void* o;
+  float* lse;
+  float* scratch;
+  int batch, NH, gqa, dim, page, block, max_blocks, code;
+  long long num_blocks;
+  float scale, softcap;                /* softcap <= 0 disables */
+  int win_left, win_right;
+  const float* alibi;                  /* [NH] or null */
+  const int* leftpad;                  /* [batch] or null */
+  const float *cos, *sin;
+  int rot_dim, rot_seqlen_ro, rot_interleaved;
+  const int* rot_pos;
+} FaDec8Params;
+
+FA_API int fa_decode8_launch(const FaDec8Params* p, int dtype, void* stream);
+FA_API long long fa_decode8_scratch_floats(int NH, int gqa, int dim);
+
+/* ------------------------------------------------------------------------------------------
  * LSE-merge of split-KV partial results (flash_attn_combine).
  *   out_partial [nsplit, B, S, H, D] (dtype in_dtype), lse_partial [nsplit, B, H, S] fp32,
  *   out [B, S, H, D] (dtype out_dtype), lse_out optional [B, H, S] fp32; all contiguous.
@@ -363,7 +473,7 @@ FA_API const char* fa_last_error(void);       /* message of the last failing cal
 /* Error bits recorded on the device (0 = none).  A bounded wait in a tensor-core kernel that
  * times out records a bit here and the kernel unwinds instead of hanging (its outputs are then
  * not valid); bits 1024 / 4096 / 256 flag a paged-K/V entry outside the cache and a rotary
- * position outside the cos/sin table.  Synchronous (device -> host copy); clear != 0 resets the
+ * position outside the cos/sin table (8192 / 16384 in the 8-bit cache operators).  Synchronous (device -> host copy); clear != 0 resets the
  * bits.  No counterpart in the reference (its kernels have no waits that can give up). */
 FA_API int fa_device_error(int clear);
 /* Bit of fa_device_error set by fa_wait_selftest. */
