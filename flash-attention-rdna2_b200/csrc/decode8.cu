@@ -11,10 +11,12 @@
 // operands, fp32 sums): with 8 query rows the tensor pipe has twice the time that the bytes need, and the conversion of codes
 // has to pass through registers anyway.  A strip is 16 positions of one kv head.  Its K rows are the B operand of
 // S = Q K^T, its V rows that of O += W V.  The order of an mma's k index and of its n columns is free as long as both operands
-// agree, so each thread's operands are whole 16-byte pieces of cache rows: K, row g = lane / 4, pieces
-// lane % 4 + 4 i; V, positions 2 (lane % 4) + {0, 1, 8, 9}, piece g.  A thread copies those pieces into
-// shared memory with cp.async and reads back only its own: no barrier, no bank conflict, no ldmatrix.
-// S leaves the tensor cores in the layout in which W enters them.
+// agree, so each thread's operands are whole 16-byte pieces of cache rows (g = lane / 4, t = lane % 4):
+//   K  row at(g) (+ 8), pieces t + 4 i;      V  rows at(2 t), at(2 t + 1) (+ 8), piece g,
+// and S leaves the tensor cores in the layout in which W enters them.  Each warp has a ring of strips of its own, which
+// its lane 0 fills by TMA (one box of 16 rows x 128 bytes each for K and V) behind an mbarrier a stage: no barrier
+// between warps.  The 128-byte swizzle puts piece i of row r at i ^ (r & 7); with at(c) = c for even
+// columns and c ^ 4 for odd ones, the eight lanes of a shared-memory phase touch eight different pieces in both reads.
 //
 // Rows of a warp are (new token, query head) pairs of one kv head.  8 rows: the upper 8 rows of the
 // m16 tile carry the low parts of q and of w, so that both have 22 bits for nothing.  16 rows: a second mma.
@@ -24,18 +26,22 @@
 // adjacent in memory, are read together.  A warp's range is cut at sequence ends; a piece that is a whole sequence
 // writes its output, others leave (m, l, o) in one of the warp's two slots, and a merge kernel joins the slots of each
 // cut sequence in order (no atomics: same bits on every call).
+#include <cudaTypedefs.h>
 #include <algorithm>
 #include <type_traits>
 #include "fa_launch.h"
 #include "kv8_common.cuh"
+#include "sm100_ptx.cuh"
 
 namespace {
 
 using namespace fa_kv;
+using sm100::ex2;
 
 __device__ int g_dec8_error = 0;
 __device__ __forceinline__ void record(int bit) { atomicOr(&g_dec8_error, bit); }
 
+constexpr int ERR_WAIT = 32768;    // a copy's wait gave up
 constexpr int ST = 16;             // positions of a strip
 constexpr int NW = 4;              // warps of a CTA
 constexpr float NONE = -1e30f;     // a running maximum that nothing has moved yet
@@ -48,22 +54,19 @@ template <int W, int RT>
 struct Cfg {
   // warps of an SM and their stages: what 64 K registers and 227 KB of shared memory hold
   static constexpr int CTAS = W == 256 ? (RT == 16 ? 1 : 2) : RT == 16 ? 2 : W == 64 ? 4 : 3;   // per SM
-  static constexpr int STAGES = W == 256 && RT == 8 ? 2 : 4;
-  static constexpr bool QREG = RT == 8 && W <= 128;                        // q operands stay in registers
+  static constexpr int STAGES = RT == 16 ? 4 : W == 256 ? 2 : W == 128 ? 3 : 4;
   static constexpr int KS = W / 16;                                        // k steps of S
-  static constexpr int STAGE_B = W * 32;                                   // K and V of a strip
-  static constexpr int Q_B = QREG ? 0 : KS * 512 * (RT / 8);
-  static constexpr int WARP_B = STAGES * (STAGE_B + 128 + 16) + Q_B;
-  static constexpr int SMEM = NW * WARP_B;
+  static constexpr int ROW = W == 64 ? 64 : 128;                           // bytes of a box row
+  static constexpr int PANELS = W / ROW;                                   // boxes of a row
+  static constexpr int HALF_B = ST * W;                                    // K or V of a strip
+  static constexpr int STAGE_B = 2 * HALF_B;
+  static constexpr int Q_B = KS * 512 * (RT / 8);                          // q operands
+  static constexpr int RING_B = STAGES * STAGE_B;
+  static constexpr int SMEM = NW * (RING_B + Q_B) + 1024;                  // + what aligns the rings to 1 KB
   static_assert(SMEM * CTAS <= 227 * 1024, "shared memory of an SM");
   static constexpr int SLOT = RT * (W + 2);                                // floats of a slot: m[RT], l[RT], o[RT][W]
 };
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + e) << 23); }   // -126 <= e <= 127
 __device__ __forceinline__ int exponent(float x) { return max(((__float_as_int(x) >> 23) & 255) - 127, -120); }
 // m raised to the largest of it and a row's four values in each of its four threads; returns it
@@ -87,29 +90,17 @@ __device__ __forceinline__ float lg2(float x) {
   asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-template <int N>
-__device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool valid) {   // N bytes, zeros where not valid
-  const int n = valid ? N : 0;
-  if constexpr (N == 16)
-    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(n) : "memory");
+// 16 bytes to shared memory, zeros where not valid
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t a) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
-  return v;
-}
+// position of column c of an n tile among the tile's 8
+__device__ __forceinline__ int col_pos(int c) { return (c & 1) ? c ^ 4 : c; }
 __device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -194,23 +185,59 @@ __device__ __forceinline__ Seq seq_of(const FaDec8Params& p, const Pages& pg, in
   return s;
 }
 
-// element d.. of a q row; rotated by table row rp (rp < 0: as it is), in fp32
+// 16 elements of a row from d on
 template <typename T>
-__device__ __noinline__ void load_q4(const FaDec8Params& p, const void* row, int d, int rp, float* v) {
-  const T* x = (const T*)row;
-  const int half = p.rot_dim / 2;
+__device__ __forceinline__ void load16(const T* x, int d, bool vec, float* v) {
+  if (vec) {
+    constexpr int U = 16 / sizeof(T);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = Elem<T>::to_f(x[d + e]);
+    for (int i = 0; i < 16; i += U) {
+      union { uint4 u; T e[U]; } b;
+      b.u = *reinterpret_cast<const uint4*>(x + d + i);
+#pragma unroll
+      for (int j = 0; j < U; ++j) v[i + j] = Elem<T>::to_f(b.e[j]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = Elem<T>::to_f(x[d + i]);
+  }
+}
+// The same, rotated by table row rp (rp < 0: as they are), in fp32.
+template <typename T>
+__device__ __forceinline__ void load_q16(const FaDec8Params& p, const T* x, int d, int rp, bool vec, float* v) {
+  load16(x, d, vec, v);
   if (rp < 0 || d >= p.rot_dim) return;
+  const int half = p.rot_dim / 2;
+  const float* ct = p.cos + (long long)rp * half;
+  const float* sn = p.sin + (long long)rp * half;
+  if (p.rot_interleaved) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int i = d + e;
-    if (i >= p.rot_dim) break;
-    const bool low = p.rot_interleaved ? !(i & 1) : i < half;
-    const int j = p.rot_interleaved ? i / 2 : low ? i : i - half;
-    const float b = Elem<T>::to_f(x[p.rot_interleaved ? i ^ 1 : low ? i + half : i - half]);
-    const float c = __ldg(p.cos + (long long)rp * half + j), s = __ldg(p.sin + (long long)rp * half + j);
-    v[e] = low ? v[e] * c - b * s : v[e] * c + b * s;
+    for (int i = 0; i < 16; i += 2) {
+      if (d + i >= p.rot_dim) break;
+      const float c = __ldg(ct + (d + i) / 2), s = __ldg(sn + (d + i) / 2), a = v[i], b = v[i + 1];
+      v[i] = a * c - b * s;
+      v[i + 1] = b * c + a * s;
+    }
+  } else if (half % 16 == 0) {   // the partners are a piece too
+    const bool low = d < half;
+    float w[16];
+    load16(x, low ? d + half : d - half, vec, w);
+    ct += low ? d : d - half;
+    sn += low ? d : d - half;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float c = __ldg(ct + i), s = __ldg(sn + i);
+      v[i] = low ? v[i] * c - w[i] * s : v[i] * c + w[i] * s;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if (d + i >= p.rot_dim) break;
+      const bool low = d + i < half;
+      const int j = low ? d + i : d + i - half;
+      const float c = __ldg(ct + j), s = __ldg(sn + j), b = Elem<T>::to_f(x[low ? d + i + half : d + i - half]);
+      v[i] = low ? v[i] * c - b * s : v[i] * c + b * s;
+    }
   }
 }
 
@@ -255,15 +282,22 @@ struct Cut {   // the sequence whose strips begin in a warp's range and end in a
 // ---------------------------------------------------------------- the pass over the cache
 template <int W, typename Q, int RT>
 __global__ void __launch_bounds__(NW * 32, (Cfg<W, RT>::CTAS))
-    dec8_kernel(const FaDec8Params p, const Pages pg, const int dtype, const int ranges) {
+    dec8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const FaDec8Params p,
+                const Pages pg, const int dtype, const int ranges) {
   using C = Cfg<W, RT>;
   constexpr int STAGES = C::STAGES, KS = C::KS, NT = W / 8, KC = W / 64, VC = W == 256 ? 2 : 1;
   constexpr int RPT = RT / 8;        // rows of a thread: g, g + 8
-  extern __shared__ __align__(16) unsigned char smem[];
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ unsigned long long s_full[NW][STAGES];   // mbarrier of a stage
+  __shared__ unsigned s_have[NW][STAGES];             // its positions that lie in a page (bits)
   __shared__ long long s_pre[NW * 32 + 1], s_warp[NW];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
   const int NKV = p.NH / p.gqa;
 
+  if (lane == 0) {
+    for (int i = 0; i < STAGES; ++i) sm100::mbar_init(sm100::smem_u32(&s_full[warp][i]), 1);
+    sm100::fence_barrier_init();
+  }
   // ---- the line of strips: every thread sums a run of sequences
   const int CB = (p.batch + NW * 32 - 1) / (NW * 32);
   {
@@ -294,12 +328,18 @@ __global__ void __launch_bounds__(NW * 32, (Cfg<W, RT>::CTAS))
   const long long per = max((long long)MIN_STRIPS, (total + ranges - 1) / ranges);
   const long long begin = range * per, end = min(total, begin + per);
 
-  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * C::WARP_B;
-  const uint32_t scales = ring + STAGES * C::STAGE_B, masks = scales + STAGES * 128, qs = masks + STAGES * 16;
-  const typename Q::T* const Kc = (const typename Q::T*)p.Kc;
-  const typename Q::T* const Vc = (const typename Q::T*)p.Vc;
-  const int pmask = p.page - 1, bshift = log2_of(p.block), per_page = p.page >> bshift;
-  const bool wide = p.page >= ST;                   // a strip lies in one page
+  const uint32_t base = (sm100::smem_u32(smem_raw) + 1023u) & ~1023u, ring = base + warp * C::RING_B;
+  const unsigned char* const mine = smem_raw + (ring - sm100::smem_u32(smem_raw));
+  uint4* const qs = reinterpret_cast<uint4*>(smem_raw + (base - sm100::smem_u32(smem_raw)) + NW * C::RING_B + warp * C::Q_B);
+  const int bshift = log2_of(p.block), per_page = p.page >> bshift;
+  const int run = min(p.page, ST);                  // slots of a box
+  const bool tma = run >= 8;                        // a box keeps whole swizzle atoms
+  // the thread's pieces within K or V of a stage
+  const auto piece = [](int row, int i) { return row * C::ROW + (C::ROW == 128 ? (i ^ (row & 7)) : (i ^ ((row >> 1) & 3))) * 16; };
+  const int kat = piece(col_pos(g), t4);
+  const int vat0 = W == 64 ? piece(2 * t4, g >> 1) + (g & 1) * 8 : piece(2 * t4, g);
+  const int vat1 = W == 64 ? piece(col_pos(2 * t4 + 1), g >> 1) + (g & 1) * 8 : piece(col_pos(2 * t4 + 1), g);
+  int stage = 0, parity = 0;                        // of the next strip to consume; a piece fills the ring from there
 
   // ---- the sequence that holds the range's first strip
   int z = 0;
@@ -326,67 +366,97 @@ __global__ void __launch_bounds__(NW * 32, (Cfg<W, RT>::CTAS))
     const int tile = (int)((at - off) / sq.strips), k0 = (int)((at - off) % sq.strips);
     const int k1 = (int)min((long long)sq.strips, k0 + (end - at));
 
-    auto issue = [&](int k, int stage) {            // strip k of the sequence into a stage
+    // Lane 0: strip k of the sequence into a stage.  The page of the next strip is looked up an issue ahead.
+    int blk = lane == 0 ? pg.of(z, (sq.s0 + k0) * ST) : 0;
+    auto issue = [&](int k, int to) {
+      const uint32_t bar = sm100::smem_u32(&s_full[warp][to]), dst = ring + to * C::STAGE_B;
+      unsigned have = 0, bytes = 0;
       const int pos0 = (sq.s0 + k) * ST;
-      const uint32_t dst = ring + stage * C::STAGE_B;
-      long long blk = 0;
-      if (wide) blk = pg.of(z, pos0);
-      auto slot_of = [&](int r) -> long long {      // cache row of position pos0 + r, -1 for none
+      auto box = [&](int r, int b) {                // slots [pos0 + r, + run) lie in page b
         const int pos = pos0 + r;
-        if (pos < sq.lo || pos >= sq.L) return -1;
-        const long long b = wide ? blk : pg.of(z, pos);
-        return b < 0 ? -1 : b * p.page + (pos & pmask);
+        if (pos + run <= sq.lo || pos >= sq.L) return false;   // nothing that a row sees
+        if (b < 0) {
+          record(ERR_PAGE);
+          return false;
+        }
+        have |= ((1u << run) - 1) << r;
+        bytes += 2 * run * W;
+        return true;
       };
+      auto load = [&](int r, int b) {
+        const int slot = b * p.page + ((pos0 + r) & (p.page - 1));
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const long long s = slot_of(g + 8 * j);
-        const typename Q::T* src = Kc + (s < 0 ? 0 : (s * NKV + kvh) * p.dim);
-#pragma unroll
-        for (int c = 0; c < KC; ++c) {
-          const int d = 16 * (t4 + 4 * c);
-          const bool ok = s >= 0 && d < p.dim;
-          cp_async<16>(dst + (j * KC + c) * 512 + lane * 16, ok ? src + d : Kc, ok);
+        for (int c = 0; c < C::PANELS; ++c) {
+          sm100::tma_load_3d(dst + c * ST * C::ROW + r * C::ROW, &tmK, c * C::ROW, kvh, slot, bar);
+          sm100::tma_load_3d(dst + C::HALF_B + c * ST * C::ROW + r * C::ROW, &tmV, c * C::ROW, kvh, slot, bar);
         }
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const long long s = slot_of(2 * t4 + (j & 1) + 8 * (j >> 1));
-        const typename Q::T* src = Vc + (s < 0 ? 0 : (s * NKV + kvh) * p.dim);
-        if constexpr (W == 64) {
-          const bool ok = s >= 0 && 8 * g < p.dim;
-          cp_async<8>(dst + 2 * KC * 512 + j * 256 + lane * 8, ok ? src + 8 * g : Vc, ok);
-        } else {
-#pragma unroll
-          for (int c = 0; c < VC; ++c) {
-            const int d = 16 * (g + 8 * c);
-            const bool ok = s >= 0 && d < p.dim;
-            cp_async<16>(dst + 2 * KC * 512 + (j * VC + c) * 512 + lane * 16, ok ? src + d : Vc, ok);
-          }
-        }
-      }
-      {   // lanes 0-15: K scale of position lane; 16-31: V scale
-        const int r = lane & 15;
-        const long long s = slot_of(r);
-        const float* sc = lane < 16 ? p.Ks : p.Vs;
-        const long long b = s < 0 ? 0 : (wide ? blk : s / p.page);
-        const long long i = s < 0 ? 0 : (b * NKV + kvh) * per_page + (((pos0 + r) & pmask) >> bshift);
-        cp_async<4>(scales + stage * 128 + lane * 4, sc + i, s >= 0);
-        const bool in = pos0 + r >= sq.lo && pos0 + r < sq.L;
-        const uint32_t have = __ballot_sync(~0u, s >= 0) & 0xffffu;
-        if (in && s < 0) record(ERR_PAGE);
-        if (lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(masks + stage * 16), "r"(have) : "memory");
+      };
+      if (run == ST) {
+        const bool go = box(0, blk);
+        s_have[warp][to] = have;
+        sm100::mbar_expect_tx(bar, bytes);
+        if (go) load(0, blk);
+        if (((pos0 + ST) & (p.page - 1)) == 0) blk = k + 1 < k1 ? pg.of(z, pos0 + ST) : 0;
+      } else {
+        const int b1 = pg.of(z, pos0 + 8);          // pages of 8
+        const bool go0 = box(0, blk), go1 = box(8, b1);
+        s_have[warp][to] = have;
+        sm100::mbar_expect_tx(bar, bytes);
+        if (go0) load(0, blk);
+        if (go1) load(8, b1);
+        blk = k + 1 < k1 ? pg.of(z, pos0 + ST) : 0;
       }
     };
-
+    // Pages of less than 8 slots: the whole warp copies slot by slot, piece by piece, into the same places.
+    auto issue_small = [&](int k, int to) {
+      const int pos0 = (sq.s0 + k) * ST, r = lane & 15, pos = pos0 + r;
+      const bool in = pos >= sq.lo && pos < sq.L;
+      const int b = in ? pg.of(z, pos) : -1;
+      if (in && b < 0) record(ERR_PAGE);
+      const unsigned have = __ballot_sync(~0u, b >= 0) & 0xffffu;
+      if (lane == 0) s_have[warp][to] = have;
+      const unsigned char* src = (const unsigned char*)(lane < 16 ? p.Kc : p.Vc);   // lanes 0-15: K, 16-31: V
+      if (b >= 0) src += (((long long)b * p.page + (pos & (p.page - 1))) * NKV + kvh) * p.dim;
+      const uint32_t dst = ring + to * C::STAGE_B + (lane < 16 ? 0 : C::HALF_B);
+      for (int i = 0; i < W / 16; ++i) {
+        const bool ok = b >= 0 && 16 * i < p.dim;
+        cp_async16(dst + (16 * i / C::ROW) * ST * C::ROW + piece(r, i % (C::ROW / 16)), ok ? src + 16 * i : src, ok);
+      }
+    };
     __syncwarp();                                   // the last piece's stages and q are free
-#pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) {
-      if (k0 + i < k1) issue(k0 + i, i);
-      cp_commit();
+    for (int i = 0, to = stage; i < STAGES; ++i) {
+      if (k0 + i < k1) {
+        if (!tma) issue_small(k0 + i, to);
+        else if (lane == 0) issue(k0 + i, to);
+      }
+      if (!tma) cp_commit();
+      to = to + 1 == STAGES ? 0 : to + 1;
     }
+    // Scales of this thread's positions, pos0 + 8 j + at(2 t4 + e) at [2 j + e], loaded a strip ahead.  What lies in no
+    // page, or outside the keys, is not read.
+    float ks[4], vs[4];
+    auto scales = [&](int k) {
+      const int pos0 = (sq.s0 + k) * ST;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i && p.block >= ST && pos0 >= sq.lo && pos0 + ST <= sq.L) {   // one block: one scale
+          ks[i] = ks[0];
+          vs[i] = vs[0];
+          continue;
+        }
+        const int pos = pos0 + 8 * (i >> 1) + col_pos(2 * t4 + (i & 1));
+        const int b = pos >= sq.lo && pos < sq.L ? pg.of(z, pos) : -1;
+        const long long s = ((long long)b * NKV + kvh) * per_page + ((pos & (p.page - 1)) >> bshift);
+        ks[i] = b < 0 ? 0.f : __ldg(p.Ks + s);
+        vs[i] = b < 0 ? 0.f : __ldg(p.Vs + s);
+      }
+    };
+    scales(k0);
 
+    const bool cap = p.softcap > 0.f;
+    const int q_unit = dtype == FA_DTYPE_F32 ? 4 : 8;
+    const bool q_vec = (uintptr_t)p.q % 16 == 0 && p.q_row % q_unit == 0 && p.q_head % q_unit == 0;
     // ---- the rows: ranges of keys, factors, q operands
-    uint32_t qa[C::QREG ? KS : 1][4];
     float qf[RPT], slope[RPT], qpos[RPT];
     int rlo[RPT], rhi[RPT];
 #pragma unroll
@@ -407,40 +477,39 @@ __global__ void __launch_bounds__(NW * 32, (Cfg<W, RT>::CTAS))
         }
       }
       const long long qe = (sq.first + tok) * p.q_row + head * p.q_head;
-      float x[KS * 4], most = 0.f;
+      float x[KS * 4], most = 0.f;                  // 16 i + 4 w: piece t4 + 4 i, word w
 #pragma unroll
-      for (int c = 0; c < KS; ++c) {                // step c = 4 i + w: piece t4 + 4 i, word w
-        const int d = 16 * (t4 + 4 * (c / 4)) + 4 * (c % 4);
-        float* v = x + 4 * c;
-        v[0] = v[1] = v[2] = v[3] = 0.f;
+      for (int i = 0; i < KC; ++i) {
+        const int d = 16 * (t4 + 4 * i);
+        float* v = x + 16 * i;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] = 0.f;
         if (live && d < p.dim) {
-          if (dtype == FA_DTYPE_BF16) load_q4<__nv_bfloat16>(p, (const __nv_bfloat16*)p.q + qe, d, rp, v);
-          else if (dtype == FA_DTYPE_F16) load_q4<__half>(p, (const __half*)p.q + qe, d, rp, v);
-          else load_q4<float>(p, (const float*)p.q + qe, d, rp, v);
+          if (dtype == FA_DTYPE_BF16) load_q16(p, (const __nv_bfloat16*)p.q + qe, d, rp, q_vec, v);
+          else if (dtype == FA_DTYPE_F16) load_q16(p, (const __half*)p.q + qe, d, rp, q_vec, v);
+          else load_q16(p, (const float*)p.q + qe, d, rp, q_vec, v);
         }
-        most = fmaxf(most, fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))));
+#pragma unroll
+        for (int j = 0; j < 16; ++j) most = fmaxf(most, fabsf(v[j]));
       }
       // rows are brought to [1, 2) by a power of two, so that fp16 holds them whatever their size
       most = fmaxf(most, __shfl_xor_sync(~0u, most, 1));
       most = fmaxf(most, __shfl_xor_sync(~0u, most, 2));
       const int e = min(exponent(most), 126);
       const float down = pow2(-e);
-      qf[r] = p.scale * pow2(e);
+      qf[r] = p.scale * pow2(e) * (cap ? 1.f / p.softcap : FA_LOG2E);
 #pragma unroll
       for (int c = 0; c < KS; ++c) {
         uint32_t h0, l0, h1, l1;
         split(x[4 * c] * down, x[4 * c + 1] * down, h0, l0);
         split(x[4 * c + 2] * down, x[4 * c + 3] * down, h1, l1);
-        if constexpr (C::QREG) {
-          qa[c][0] = h0; qa[c][1] = l0; qa[c][2] = h1; qa[c][3] = l1;
-        } else if constexpr (RT == 8) {
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(qs + c * 512 + lane * 16), "r"(h0), "r"(l0), "r"(h1),
-                       "r"(l1) : "memory");
+        if constexpr (RT == 8) {
+          qs[c * 32 + lane] = make_uint4(h0, l0, h1, l1);
         } else {   // operand words: 0 row g, 1 row g + 8 (first pair); 2, 3 (second pair); low parts behind
-          asm volatile("st.shared.u32 [%0], %1;" ::"r"(qs + c * 512 + lane * 16 + 4 * r), "r"(h0) : "memory");
-          asm volatile("st.shared.u32 [%0], %1;" ::"r"(qs + c * 512 + lane * 16 + 8 + 4 * r), "r"(h1) : "memory");
-          asm volatile("st.shared.u32 [%0], %1;" ::"r"(qs + (KS + c) * 512 + lane * 16 + 4 * r), "r"(l0) : "memory");
-          asm volatile("st.shared.u32 [%0], %1;" ::"r"(qs + (KS + c) * 512 + lane * 16 + 8 + 4 * r), "r"(l1) : "memory");
+          uint32_t* const hi = reinterpret_cast<uint32_t*>(qs) + (c * 32 + lane) * 4;
+          uint32_t* const lo = hi + KS * 128;
+          hi[r] = h0; hi[2 + r] = h1;
+          lo[r] = l0; lo[2 + r] = l1;
         }
       }
     }
@@ -454,7 +523,7 @@ __global__ void __launch_bounds__(NW * 32, (Cfg<W, RT>::CTAS))
       if (!live && r == 0) { all_lo = 0; all_hi = 0x7fffffff; }
     }
     all_lo = __reduce_max_sync(~0u, all_lo);
-    all_hi = __reduce_min_sync(~0u, all_hi);
+    all_hi = cap || p.alibi ? 0 : __reduce_min_sync(~0u, all_hi);
 
     float o[NT][4];
 #pragma unroll
@@ -462,16 +531,19 @@ __global__ void __launch_bounds__(NW * 32, (Cfg<W, RT>::CTAS))
     float m[RPT], l[RPT], up[RPT];
 #pragma unroll
     for (int r = 0; r < RPT; ++r) { m[r] = NONE; l[r] = 0.f; up[r] = pow2(126); }
-    const bool cap = p.softcap > 0.f;
-    const float cap_in = cap ? 1.f / p.softcap : FA_LOG2E, cap_out = p.softcap * FA_LOG2E;
+    const float cap_out = p.softcap * FA_LOG2E;
 
+    int k_lost = -1;
     for (int k = k0; k < k1; ++k) {
-      const int stage = (k - k0) % STAGES;
-      cp_wait<STAGES - 2>();
-      __syncwarp();
-      if (k + STAGES - 1 < k1) issue(k + STAGES - 1, (k - k0 + STAGES - 1) % STAGES);
-      cp_commit();
-      const uint32_t src = ring + stage * C::STAGE_B + lane * 16;
+      if (!tma) {
+        cp_wait<STAGES - 1>();
+        __syncwarp();
+      } else if (!__all_sync(~0u, sm100::mbar_wait(sm100::smem_u32(&s_full[warp][stage]), parity))) {
+        record(ERR_WAIT);                           // copies that never land: give up (they are waited for below)
+        k_lost = k;
+        break;
+      }
+      const unsigned char* const src = mine + stage * C::STAGE_B;
 
       // ---- S = Q K^T: columns j * 8 + 2 t4 + {0, 1}
       float s[2][4];
@@ -480,22 +552,18 @@ __global__ void __launch_bounds__(NW * 32, (Cfg<W, RT>::CTAS))
 #pragma unroll
       for (int c = 0; c < KC; ++c) {
         uint4 kk[2];
-        kk[0] = lds128(src + c * 512);
-        kk[1] = lds128(src + (KC + c) * 512);
+        const int o = (c >> 1) * (ST * 128) + (kat ^ ((c & 1) * 64));
+        kk[0] = *reinterpret_cast<const uint4*>(src + o);
+        kk[1] = *reinterpret_cast<const uint4*>(src + o + 8 * C::ROW);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           uint32_t qv[4], ql[4];
-          if constexpr (C::QREG) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) qv[i] = qa[4 * c + w][i];
-          } else {
-            const uint4 u = lds128(qs + (4 * c + w) * 512 + lane * 16);
+            const uint4 u = qs[(4 * c + w) * 32 + lane];
             qv[0] = u.x; qv[1] = u.y; qv[2] = u.z; qv[3] = u.w;
             if constexpr (RT == 16) {
-              const uint4 v = lds128(qs + (KS + 4 * c + w) * 512 + lane * 16);
+              const uint4 v = qs[(KS + 4 * c + w) * 32 + lane];
               ql[0] = v.x; ql[1] = v.y; ql[2] = v.z; ql[3] = v.w;
             }
-          }
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             uint32_t b0, b1;
@@ -508,25 +576,24 @@ __global__ void __launch_bounds__(NW * 32, (Cfg<W, RT>::CTAS))
 
       // ---- weights of positions pos0 + 8 j + 2 t4 + e, row g (+ 8 r)
       const int pos0 = (sq.s0 + k) * ST;
-      uint32_t have;
-      asm volatile("ld.shared.u32 %0, [%1];" : "=r"(have) : "r"(masks + stage * 16) : "memory");
-      const bool whole = have == 0xffffu && pos0 >= all_lo && pos0 + ST <= all_hi;
-      float x[RPT][4], vs[4];
+      const uint32_t have = s_have[warp][stage];
+      // every position seen by every row, and scores that are nothing but products
+      const bool plain = have == 0xffffu && pos0 >= all_lo && pos0 + ST <= all_hi;
+      float x[RPT][4];
       bool move = false;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const uint2 ku = lds64(scales + stage * 128 + (8 * j + 2 * t4) * 4), vu = lds64(scales + stage * 128 + (16 + 8 * j + 2 * t4) * 4);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float ks = __uint_as_float(e ? ku.y : ku.x);
-          vs[2 * j + e] = __uint_as_float(e ? vu.y : vu.x);
-          const int pos = pos0 + 8 * j + 2 * t4 + e;
+          const int pos = pos0 + 8 * j + col_pos(2 * t4 + e);
 #pragma unroll
           for (int r = 0; r < RPT; ++r) {
-            float v = (RT == 8 ? s[j][e] + s[j][2 + e] : s[j][2 * r + e]) * ks * qf[r] * cap_in;
-            if (cap) v = cap_out * fa_tanh(v);
-            if (p.alibi) v = fmaf(slope[r], (float)pos - qpos[r], v);
-            if (!whole && !(pos >= rlo[r] && pos < rhi[r] && ((have >> (pos - pos0)) & 1))) v = -INFINITY;
+            float v = (RT == 8 ? s[j][e] + s[j][2 + e] : s[j][2 * r + e]) * (ks[2 * j + e] * qf[r]);
+            if (!plain) {
+              if (cap) v = cap_out * fa_tanh(v);
+              if (p.alibi) v = fmaf(slope[r], (float)pos - qpos[r], v);
+              if (!(pos >= rlo[r] && pos < rhi[r] && ((have >> (pos - pos0)) & 1))) v = -INFINITY;
+            }
             x[r][2 * j + e] = v;
             move |= v > m[r] + LAZY;
           }
@@ -548,7 +615,7 @@ __global__ void __launch_bounds__(NW * 32, (Cfg<W, RT>::CTAS))
         for (int i = 0; i < 4; ++i) {
           const float e = ex2(x[r][i] - m[r]);
           l[r] += e;
-          w[r][i] = x[r][i] == -INFINITY ? 0.f : e * vs[i];
+          w[r][i] = !plain && x[r][i] == -INFINITY ? 0.f : e * vs[i];
           move |= w[r][i] * up[r] > MOST;
         }
       }
@@ -578,12 +645,21 @@ __global__ void __launch_bounds__(NW * 32, (Cfg<W, RT>::CTAS))
           }
         }
 
+      if (k + 1 < k1) scales(k + 1);
+
       // ---- O += W V
-      const uint32_t vsrc = ring + stage * C::STAGE_B + 2 * KC * 512;
+      const unsigned char* const vsrc = src + C::HALF_B;
+      const auto hidden = [&](int j) {              // row j of the thread's four: 2 (its half) + (odd column)
+        const int r = 8 * (j >> 1) + col_pos(2 * t4 + (j & 1));
+        return !plain && !(pos0 + r >= sq.lo && pos0 + r < sq.L && ((have >> r) & 1));
+      };
       if constexpr (W == 64) {
         uint2 v[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = lds64(vsrc + j * 256 + lane * 8);
+        for (int j = 0; j < 4; ++j) {
+          v[j] = *reinterpret_cast<const uint2*>(vsrc + ((j & 1) ? vat1 : vat0) + (j >> 1) * 8 * C::ROW);
+          if (hidden(j)) v[j] = make_uint2(0, 0);   // whatever is there: 0 * NaN is not 0
+        }
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
           uint32_t b0[4], b1[4];
@@ -600,7 +676,10 @@ __global__ void __launch_bounds__(NW * 32, (Cfg<W, RT>::CTAS))
         for (int c = 0; c < VC; ++c) {
           uint4 v[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) v[j] = lds128(vsrc + (j * VC + c) * 512 + lane * 16);
+          for (int j = 0; j < 4; ++j) {
+            v[j] = *reinterpret_cast<const uint4*>(vsrc + c * (ST * 128) + ((j & 1) ? vat1 : vat0) + (j >> 1) * 8 * C::ROW);
+            if (hidden(j)) v[j] = make_uint4(0, 0, 0, 0);   // whatever is there: 0 * NaN is not 0
+          }
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
             uint32_t b0[4], b1[4];
@@ -614,8 +693,23 @@ __global__ void __launch_bounds__(NW * 32, (Cfg<W, RT>::CTAS))
           }
         }
       }
+
+      __syncwarp();                                 // every lane has read the stage
+      if (!tma) {
+        if (k + STAGES < k1) issue_small(k + STAGES, stage);
+        cp_commit();
+      } else if (lane == 0 && k + STAGES < k1) {
+        issue(k + STAGES, stage);
+      }
+      if (++stage == STAGES) { stage = 0; parity ^= 1; }
     }
-    cp_wait<0>();
+    if (k_lost >= 0) {   // let what is in flight land before the CTA's memory goes
+      for (int i = 0; i < STAGES && k_lost + i < k1; ++i) {
+        sm100::mbar_wait(sm100::smem_u32(&s_full[warp][stage]), parity, 1000000000ull);
+        if (++stage == STAGES) { stage = 0; parity ^= 1; }
+      }
+      break;
+    }
 
     // ---- the piece's result.  Column 2 t4 + h of n tile i belongs to thread g' = 2 t4 + h of the B
     // operand: dims PIECE * (g' + 8 c) + i, i < PIECE
@@ -672,52 +766,120 @@ __global__ void __launch_bounds__(NW * 32, (Cfg<W, RT>::CTAS))
 }
 
 // ---------------------------------------------------------------- the join of cut sequences
-// One CTA for the warp whose range a cut sequence begins in, one warp per row.
+// A row of a cut sequence is one item; CTAs take items in turn, the warps of a CTA every eighth part.
+// Which warps' ranges a cut begins in stands in their records: every CTA lists them for itself (a few KB from
+// L2, in the same order everywhere), so that the items of one long sequence spread over the whole GPU.
+constexpr int MW = 8;
 template <int W, int RT>
-__global__ void __launch_bounds__(RT * 32)
+__global__ void __launch_bounds__(MW * 32)
     dec8_merge_kernel(const FaDec8Params p, const Pages pg, const int dtype, const int ranges) {
   using C = Cfg<W, RT>;
+  extern __shared__ int s_cut[];                    // warps that a cut begins at
+  __shared__ int s_warp[MW];
+  __shared__ float s_l[MW], s_v[MW][W];
+  const int NKV = p.NH / p.gqa, warps = ranges * NKV, tid = threadIdx.x, w = tid / 32, lane = tid % 32;
   pdl_wait();
-  const int NKV = p.NH / p.gqa, gw = blockIdx.x, kvh = gw % NKV, r = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const Cut cut = reinterpret_cast<const Cut*>(p.scratch)[gw];
-  if (cut.parts == 0) return;
-  const Seq sq = seq_of<RT>(p, pg, cut.z);
-  const int row = cut.tile * RT + r, tok = row / p.gqa, head = kvh * p.gqa + row % p.gqa;
-  if (tok >= sq.n) return;
-  const float* slots = p.scratch + (long long)ranges * NKV * (sizeof(Cut) / 4);
-  // part 0: second slot of warp gw; part i: first slot of the warp i ranges on
-  auto part = [&](int i) { return slots + ((long long)(gw + i * NKV) * 2 + (i == 0)) * C::SLOT; };
-  float m = NONE;
-  for (int i = lane; i < cut.parts; i += 32) m = fmaxf(m, part(i)[r]);
+  const Cut* const cuts = reinterpret_cast<const Cut*>(p.scratch);
+  const int per = (warps + MW * 32 - 1) / (MW * 32), i0 = tid * per, i1 = min(warps, i0 + per);
+  int mine = 0;
+  for (int i = i0; i < i1; ++i) mine += cuts[i].parts > 0;
+  int inc = mine;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(~0u, inc, o);
+    if (lane >= o) inc += v;
+  }
+  if (lane == 31) s_warp[w] = inc;
+  __syncthreads();
+  int count = 0, at0 = inc - mine;
+#pragma unroll
+  for (int i = 0; i < MW; ++i) {
+    if (i < w) at0 += s_warp[i];
+    count += s_warp[i];
+  }
+  if (mine)
+    for (int i = i0; i < i1; ++i)
+      if (cuts[i].parts > 0) s_cut[at0++] = i;
+  __syncthreads();
+  const float* const slots = p.scratch + (long long)warps * (sizeof(Cut) / 4);
   constexpr int E = W / 32;
-  float l = 0.f, v[E];
+  for (int item = blockIdx.x; item < count * RT; item += gridDim.x) {
+    const int gw = s_cut[item / RT], r = item % RT;
+    const Cut cut = cuts[gw];
+    const Seq sq = seq_of<RT>(p, pg, cut.z);
+    const int row = cut.tile * RT + r, tok = row / p.gqa, head = gw % NKV * p.gqa + row % p.gqa;
+    if (tok >= sq.n) continue;
+    // part 0: second slot of warp gw; part i: first slot of the warp i ranges on
+    auto part = [&](int i) { return slots + ((long long)(gw + i * NKV) * 2 + (i == 0)) * C::SLOT; };
+    float m = NONE;
+    for (int i = lane; i < cut.parts; i += 32) m = fmaxf(m, part(i)[r]);
 #pragma unroll
-  for (int e = 0; e < E; ++e) v[e] = 0.f;
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+    float l = 0.f, v[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = 0.f;
 #pragma unroll 4
-  for (int i = 0; i < cut.parts; ++i) {
-    const float* s = part(i);
-    const float f = ex2(s[r] - m);
-    l = fmaf(s[RT + r], f, l);
+    for (int i = w; i < cut.parts; i += MW) {
+      const float* s = part(i);
+      const float f = ex2(s[r] - m);
+      l = fmaf(s[RT + r], f, l);
 #pragma unroll
-    for (int e = 0; e < E; e += 2) {
-      const float2 u = *reinterpret_cast<const float2*>(s + 2 * RT + r * W + lane * E + e);
-      v[e] = fmaf(u.x, f, v[e]);
-      v[e + 1] = fmaf(u.y, f, v[e + 1]);
+      for (int e = 0; e < E; e += 2) {
+        const float2 u = *reinterpret_cast<const float2*>(s + 2 * RT + r * W + lane * E + e);
+        v[e] = fmaf(u.x, f, v[e]);
+        v[e + 1] = fmaf(u.y, f, v[e + 1]);
+      }
     }
-  }
-  const float f = l == 0.f ? 0.f : 1.f / l;
-  const long long at = ((sq.first + tok) * p.NH + head) * p.dim;
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int d = lane * E + e;
-    if (d >= p.dim) break;
-    if (dtype == FA_DTYPE_BF16) ((__nv_bfloat16*)p.o)[at + d] = __float2bfloat16_rn(v[e] * f);
-    else if (dtype == FA_DTYPE_F16) ((__half*)p.o)[at + d] = __float2half_rn(v[e] * f);
-    else ((float*)p.o)[at + d] = v[e] * f;
+    for (int e = 0; e < E; ++e) s_v[w][lane * E + e] = v[e];
+    if (lane == 0) s_l[w] = l;
+    __syncthreads();
+    l = 0.f;
+#pragma unroll
+    for (int i = 0; i < MW; ++i) l += s_l[i];
+    for (int d = tid; d < p.dim; d += MW * 32) {
+      float x = 0.f;
+#pragma unroll
+      for (int i = 0; i < MW; ++i) x += s_v[i][d];
+      x = l == 0.f ? 0.f : x / l;
+      const long long at = ((sq.first + tok) * p.NH + head) * p.dim + d;
+      if (dtype == FA_DTYPE_BF16) ((__nv_bfloat16*)p.o)[at] = __float2bfloat16_rn(x);
+      else if (dtype == FA_DTYPE_F16) ((__half*)p.o)[at] = __float2half_rn(x);
+      else ((float*)p.o)[at] = x;
+    }
+    if (tid == 0) store_lse(p, cut.z, sq.first + tok, tok, head, m, l);
+    __syncthreads();
   }
-  if (lane == 0) store_lse(p, cut.z, sq.first + tok, tok, head, m, l);
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  if (!fn) {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  }
+  return fn;
+}
+
+// The cache as rows of `dim` bytes: (dim, kv heads, slots); a box is `row` bytes of one head in `run` slots, what lies past dim
+// comes as zeros.
+int map_of(CUtensorMap* m, const void* base, const FaDec8Params& p, int row) {
+  const auto enc = encode_fn();
+  const cuuint64_t heads = p.NH / p.gqa;
+  const cuuint64_t dims[3] = {(cuuint64_t)p.dim, heads, (cuuint64_t)p.num_blocks * p.page};
+  const cuuint64_t strides[2] = {(cuuint64_t)p.dim, heads * p.dim};
+  const cuuint32_t box[3] = {(cuuint32_t)row, 1, (cuuint32_t)std::min(p.page, ST)};
+  const cuuint32_t one[3] = {1, 1, 1};
+  const CUresult e = !enc ? CUDA_ERROR_NOT_FOUND
+                          : enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, one,
+                                CU_TENSOR_MAP_INTERLEAVE_NONE, row == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (e == CUDA_SUCCESS) return FA_OK;
+  fa::set_error("8-bit decode: cuTensorMapEncodeTiled failed (%d)", (int)e);
+  return FA_ERR_CUDA;
 }
 
 template <int W, typename Q, int RT>
@@ -725,13 +887,17 @@ int launch(const FaDec8Params& p, int dtype, cudaStream_t st) {
   using C = Cfg<W, RT>;
   static unsigned long long done = 0;
   if (int rc = fa::ensure_smem((const void*)dec8_kernel<W, Q, RT>, C::SMEM, &done)) return rc;
+  CUtensorMap mk, mv;
+  if (int rc = map_of(&mk, p.Kc, p, C::ROW)) return rc;
+  if (int rc = map_of(&mv, p.Vc, p, C::ROW)) return rc;
   const Pages pg{p.block_table, log2_of(p.page), p.max_blocks, p.num_blocks};
   const int NKV = p.NH / p.gqa, grid = fa::num_sms() * C::CTAS, warps = grid * NW;
   const int ranges = std::max(1, warps / NKV), need = (ranges * NKV + NW - 1) / NW;
-  dec8_kernel<W, Q, RT><<<need, NW * 32, C::SMEM, st>>>(p, pg, dtype, ranges);
+  dec8_kernel<W, Q, RT><<<need, NW * 32, C::SMEM, st>>>(mk, mv, p, pg, dtype, ranges);
   fa::count_launch();
   if (int rc = fa::cuda_status(cudaGetLastError(), "8-bit decode launch")) return rc;
-  const cudaError_t e = fa::launch_pdl(dec8_merge_kernel<W, RT>, dim3(ranges * NKV), dim3(RT * 32), 0, st, p, pg, dtype, ranges);
+  const cudaError_t e = fa::launch_pdl(dec8_merge_kernel<W, RT>, dim3(2 * fa::num_sms()), dim3(MW * 32),
+                                       (size_t)ranges * NKV * sizeof(int), st, p, pg, dtype, ranges);
   fa::count_launch();
   return fa::cuda_status(e, "8-bit decode merge launch");
 }
@@ -810,6 +976,10 @@ extern "C" FA_API int fa_decode8_launch(const FaDec8Params* pp, int dtype, void*
   FA_CHECK_ARG(p.scratch, "8-bit decode: scratch must be non-null");
   FA_CHECK_ARG(((uintptr_t)p.Kc | (uintptr_t)p.Vc | (uintptr_t)p.o | (uintptr_t)p.scratch) % 16 == 0,
                "8-bit decode: Kc, Vc, o and scratch must be 16-byte aligned");
+  if (p.num_blocks * (long long)p.page >= 1ll << 31) {
+    fa::set_error("8-bit decode: a cache of %lld pages of %d slots is more than one call takes", p.num_blocks, p.page);
+    return FA_ERR_SIZE;
+  }
   p.win_left = std::min(p.win_left, 1 << 30);   // position - win_left stays within 32 bits
   p.win_right = std::min(p.win_right, 1 << 30);
   cudaStream_t st = (cudaStream_t)stream;

@@ -33,7 +33,7 @@ struct Pages {
   int shift, max_blocks;   // page = 1 << shift
   long long num_blocks;
   // page of position pos of sequence z, or -1 where there is none
-  __device__ __forceinline__ long long of(int z, int pos) const {
+  __device__ __forceinline__ int of(int z, int pos) const {
     const int i = pos >> shift;
     if (pos < 0 || i >= max_blocks) return -1;
     const int b = __ldg(table + (long long)z * max_blocks + i);
