@@ -62,16 +62,18 @@ struct Cfg {
   static constexpr int STAGE_B = 2 * HALF_B;
   static constexpr int Q_B = KS * 512 * (RT / 8);                          // q operands
   static constexpr int RING_B = STAGES * STAGE_B;
-  static constexpr int SMEM = NW * (RING_B + Q_B) + 1024;                  // + what aligns the rings to 1 KB
+  static constexpr int WARP_B = RING_B + Q_B + STAGES * 128;               // and scales
+  static constexpr int SMEM = NW * WARP_B + 1024;                          // + what aligns the rings to 1 KB
   static_assert(SMEM * CTAS <= 227 * 1024, "shared memory of an SM");
   static constexpr int SLOT = RT * (W + 2);                                // floats of a slot: m[RT], l[RT], o[RT][W]
 };
 
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + e) << 23); }   // -126 <= e <= 127
 __device__ __forceinline__ int exponent(float x) { return max(((__float_as_int(x) >> 23) & 255) - 127, -120); }
+__device__ __forceinline__ float max4(const float* v) { return fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])); }
 // m raised to the largest of it and a row's four values in each of its four threads; returns it
 __device__ __forceinline__ float raise(float& m, const float* v) {
-  float a = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+  float a = max4(v);
   a = fmaxf(a, __shfl_xor_sync(~0u, a, 1));
   a = fmaxf(a, __shfl_xor_sync(~0u, a, 2));
   return m = fmaxf(a, m);
@@ -90,9 +92,12 @@ __device__ __forceinline__ float lg2(float x) {
   asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// 16 bytes to shared memory, zeros where not valid
+// 16 bytes to shared memory, zeros where not valid; 4 bytes
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -330,7 +335,11 @@ __global__ void __launch_bounds__(NW * 32, (Cfg<W, RT>::CTAS))
 
   const uint32_t base = (sm100::smem_u32(smem_raw) + 1023u) & ~1023u, ring = base + warp * C::RING_B;
   const unsigned char* const mine = smem_raw + (ring - sm100::smem_u32(smem_raw));
-  uint4* const qs = reinterpret_cast<uint4*>(smem_raw + (base - sm100::smem_u32(smem_raw)) + NW * C::RING_B + warp * C::Q_B);
+  unsigned char* const own = smem_raw + (base - sm100::smem_u32(smem_raw)) + NW * C::RING_B + warp * (C::Q_B + STAGES * 128);
+  uint4* const qs = reinterpret_cast<uint4*>(own);
+  const float* const scales = reinterpret_cast<const float*>(own + C::Q_B);   // a stage: 16 of K, 16 of V
+  const uint32_t scales_u = sm100::smem_u32(scales) + lane * 4;
+  const float* const my_scale = lane < 16 ? p.Ks : p.Vs;
   const int bshift = log2_of(p.block), per_page = p.page >> bshift;
   const int run = min(p.page, ST);                  // slots of a box
   const bool tma = run >= 8;                        // a box keeps whole swizzle atoms
@@ -366,44 +375,46 @@ __global__ void __launch_bounds__(NW * 32, (Cfg<W, RT>::CTAS))
     const int tile = (int)((at - off) / sq.strips), k0 = (int)((at - off) % sq.strips);
     const int k1 = (int)min((long long)sq.strips, k0 + (end - at));
 
-    // Lane 0: strip k of the sequence into a stage.  The page of the next strip is looked up an issue ahead.
-    int blk = lane == 0 ? pg.of(z, (sq.s0 + k0) * ST) : 0;
-    auto issue = [&](int k, int to) {
-      const uint32_t bar = sm100::smem_u32(&s_full[warp][to]), dst = ring + to * C::STAGE_B;
-      unsigned have = 0, bytes = 0;
-      const int pos0 = (sq.s0 + k) * ST;
-      auto box = [&](int r, int b) {                // slots [pos0 + r, + run) lie in page b
-        const int pos = pos0 + r;
-        if (pos + run <= sq.lo || pos >= sq.L) return false;   // nothing that a row sees
-        if (b < 0) {
-          record(ERR_PAGE);
-          return false;
-        }
-        have |= ((1u << run) - 1) << r;
-        bytes += 2 * run * W;
-        return true;
-      };
-      auto load = [&](int r, int b) {
-        const int slot = b * p.page + ((pos0 + r) & (p.page - 1));
+    // Strip k of the sequence into a stage: lane 0 the codes, each lane one scale (0-15: K's of position lane, 16-31: V's).
+    // What no row sees is not read: its weights are 0, and its V rows are cleared where they are used.  The page of
+    // the next strip is looked up an issue ahead.
+    int blk = pg.of(z, (sq.s0 + k0) * ST);
+    auto box = [&](int pos, int b) {                // do rows see something of the slots [pos, pos + run) in page b
+      if (pos + run <= sq.lo || pos >= sq.L) return false;
+      if (b < 0) record(ERR_PAGE);
+      return b >= 0;
+    };
+    auto load = [&](int r, int slot, int to) {
+      const uint32_t bar = sm100::smem_u32(&s_full[warp][to]), dst = ring + to * C::STAGE_B + r * C::ROW;
 #pragma unroll
-        for (int c = 0; c < C::PANELS; ++c) {
-          sm100::tma_load_3d(dst + c * ST * C::ROW + r * C::ROW, &tmK, c * C::ROW, kvh, slot, bar);
-          sm100::tma_load_3d(dst + C::HALF_B + c * ST * C::ROW + r * C::ROW, &tmV, c * C::ROW, kvh, slot, bar);
-        }
-      };
+      for (int c = 0; c < C::PANELS; ++c) {
+        sm100::tma_load_3d(dst + c * ST * C::ROW, &tmK, c * C::ROW, kvh, slot, bar);
+        sm100::tma_load_3d(dst + C::HALF_B + c * ST * C::ROW, &tmV, c * C::ROW, kvh, slot, bar);
+      }
+    };
+    auto issue = [&](int k, int to) {
+      const int pos0 = (sq.s0 + k) * ST;
       if (run == ST) {
-        const bool go = box(0, blk);
-        s_have[warp][to] = have;
-        sm100::mbar_expect_tx(bar, bytes);
-        if (go) load(0, blk);
-        if (((pos0 + ST) & (p.page - 1)) == 0) blk = k + 1 < k1 ? pg.of(z, pos0 + ST) : 0;
-      } else {
-        const int b1 = pg.of(z, pos0 + 8);          // pages of 8
-        const bool go0 = box(0, blk), go1 = box(8, b1);
-        s_have[warp][to] = have;
-        sm100::mbar_expect_tx(bar, bytes);
-        if (go0) load(0, blk);
-        if (go1) load(8, b1);
+        const int in_page = pos0 & (p.page - 1);
+        const bool go = box(pos0, blk);
+        if (lane == 0) {
+          s_have[warp][to] = go ? 0xffffu : 0u;
+          sm100::mbar_expect_tx(sm100::smem_u32(&s_full[warp][to]), go ? C::STAGE_B : 0);
+          if (go) load(0, blk * p.page + in_page, to);
+        }
+        if (go) cp_async4(scales_u + to * 128, my_scale + (long long)(blk * NKV + kvh) * per_page + ((in_page + (lane & 15)) >> bshift));
+        if (in_page + ST == p.page && k + 1 < k1) blk = pg.of(z, pos0 + ST);
+      } else {                                      // pages of 8
+        const int b1 = pg.of(z, pos0 + 8);
+        const bool go0 = box(pos0, blk), go1 = box(pos0 + 8, b1);
+        if (lane == 0) {
+          s_have[warp][to] = (go0 ? 0xffu : 0u) | (go1 ? 0xff00u : 0u);
+          sm100::mbar_expect_tx(sm100::smem_u32(&s_full[warp][to]), (go0 + go1) * (C::STAGE_B / 2));
+          if (go0) load(0, blk * 8, to);
+          if (go1) load(8, b1 * 8, to);
+        }
+        if (lane & 8 ? go1 : go0)
+          cp_async4(scales_u + to * 128, my_scale + (long long)((lane & 8 ? b1 : blk) * NKV + kvh) * per_page + ((lane & 7) >> bshift));
         blk = k + 1 < k1 ? pg.of(z, pos0 + ST) : 0;
       }
     };
@@ -422,37 +433,18 @@ __global__ void __launch_bounds__(NW * 32, (Cfg<W, RT>::CTAS))
         const bool ok = b >= 0 && 16 * i < p.dim;
         cp_async16(dst + (16 * i / C::ROW) * ST * C::ROW + piece(r, i % (C::ROW / 16)), ok ? src + 16 * i : src, ok);
       }
+      if (b >= 0)
+        cp_async4(scales_u + to * 128, my_scale + ((long long)b * NKV + kvh) * per_page + ((pos & (p.page - 1)) >> bshift));
     };
     __syncwarp();                                   // the last piece's stages and q are free
     for (int i = 0, to = stage; i < STAGES; ++i) {
       if (k0 + i < k1) {
-        if (!tma) issue_small(k0 + i, to);
-        else if (lane == 0) issue(k0 + i, to);
+        if (tma) issue(k0 + i, to);
+        else issue_small(k0 + i, to);
       }
-      if (!tma) cp_commit();
+      cp_commit();
       to = to + 1 == STAGES ? 0 : to + 1;
     }
-    // Scales of this thread's positions, pos0 + 8 j + at(2 t4 + e) at [2 j + e], loaded a strip ahead.  What lies in no
-    // page, or outside the keys, is not read.
-    float ks[4], vs[4];
-    auto scales = [&](int k) {
-      const int pos0 = (sq.s0 + k) * ST;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (i && p.block >= ST && pos0 >= sq.lo && pos0 + ST <= sq.L) {   // one block: one scale
-          ks[i] = ks[0];
-          vs[i] = vs[0];
-          continue;
-        }
-        const int pos = pos0 + 8 * (i >> 1) + col_pos(2 * t4 + (i & 1));
-        const int b = pos >= sq.lo && pos < sq.L ? pg.of(z, pos) : -1;
-        const long long s = ((long long)b * NKV + kvh) * per_page + ((pos & (p.page - 1)) >> bshift);
-        ks[i] = b < 0 ? 0.f : __ldg(p.Ks + s);
-        vs[i] = b < 0 ? 0.f : __ldg(p.Vs + s);
-      }
-    };
-    scales(k0);
-
     const bool cap = p.softcap > 0.f;
     const int q_unit = dtype == FA_DTYPE_F32 ? 4 : 8;
     const bool q_vec = (uintptr_t)p.q % 16 == 0 && p.q_row % q_unit == 0 && p.q_head % q_unit == 0;
@@ -535,8 +527,8 @@ __global__ void __launch_bounds__(NW * 32, (Cfg<W, RT>::CTAS))
 
     int k_lost = -1;
     for (int k = k0; k < k1; ++k) {
+      cp_wait<STAGES - 1>();
       if (!tma) {
-        cp_wait<STAGES - 1>();
         __syncwarp();
       } else if (!__all_sync(~0u, sm100::mbar_wait(sm100::smem_u32(&s_full[warp][stage]), parity))) {
         record(ERR_WAIT);                           // copies that never land: give up (they are waited for below)
@@ -579,7 +571,13 @@ __global__ void __launch_bounds__(NW * 32, (Cfg<W, RT>::CTAS))
       const uint32_t have = s_have[warp][stage];
       // every position seen by every row, and scores that are nothing but products
       const bool plain = have == 0xffffu && pos0 >= all_lo && pos0 + ST <= all_hi;
-      float x[RPT][4];
+      float x[RPT][4], ks[4], vs[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 8 * (i >> 1) + col_pos(2 * t4 + (i & 1));
+        ks[i] = scales[stage * 32 + r];
+        vs[i] = scales[stage * 32 + 16 + r];
+      }
       bool move = false;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -595,10 +593,11 @@ __global__ void __launch_bounds__(NW * 32, (Cfg<W, RT>::CTAS))
               if (!(pos >= rlo[r] && pos < rhi[r] && ((have >> (pos - pos0)) & 1))) v = -INFINITY;
             }
             x[r][2 * j + e] = v;
-            move |= v > m[r] + LAZY;
           }
         }
       }
+#pragma unroll
+      for (int r = 0; r < RPT; ++r) move |= max4(x[r]) > m[r] + LAZY;
       if (__any_sync(~0u, move)) {
 #pragma unroll
         for (int r = 0; r < RPT; ++r) {
@@ -616,8 +615,8 @@ __global__ void __launch_bounds__(NW * 32, (Cfg<W, RT>::CTAS))
           const float e = ex2(x[r][i] - m[r]);
           l[r] += e;
           w[r][i] = !plain && x[r][i] == -INFINITY ? 0.f : e * vs[i];
-          move |= w[r][i] * up[r] > MOST;
         }
+        move |= max4(w[r]) * up[r] > MOST;
       }
       if (__any_sync(~0u, move)) {
 #pragma unroll
@@ -644,8 +643,6 @@ __global__ void __launch_bounds__(NW * 32, (Cfg<W, RT>::CTAS))
             wl[2 * j + r] = lo;
           }
         }
-
-      if (k + 1 < k1) scales(k + 1);
 
       // ---- O += W V
       const unsigned char* const vsrc = src + C::HALF_B;
@@ -695,12 +692,11 @@ __global__ void __launch_bounds__(NW * 32, (Cfg<W, RT>::CTAS))
       }
 
       __syncwarp();                                 // every lane has read the stage
-      if (!tma) {
-        if (k + STAGES < k1) issue_small(k + STAGES, stage);
-        cp_commit();
-      } else if (lane == 0 && k + STAGES < k1) {
-        issue(k + STAGES, stage);
+      if (k + STAGES < k1) {
+        if (tma) issue(k + STAGES, stage);
+        else issue_small(k + STAGES, stage);
       }
+      cp_commit();
       if (++stage == STAGES) { stage = 0; parity ^= 1; }
     }
     if (k_lost >= 0) {   // let what is in flight land before the CTA's memory goes
