@@ -9,12 +9,12 @@
 //
 // Bound by the bytes of the cache.  What is read goes through registers to mma.sync (m16n8k16, fp16
 // operands, fp32 sums): with 8 query rows the tensor pipe has twice the time that the bytes need, and the conversion of codes
-// has to pass through registers anyway.  A strip is 16 positions of one kv head.  Its K rows are the B operand of
+// has to pass through registers anyway.  A strip is 32 (or 16) positions of one kv head.  Its K rows are the B operand of
 // S = Q K^T, its V rows that of O += W V.  The order of an mma's k index and of its n columns is free as long as both operands
 // agree, so each thread's operands are whole 16-byte pieces of cache rows (g = lane / 4, t = lane % 4):
 //   K  row at(g) (+ 8), pieces t + 4 i;      V  rows at(2 t), at(2 t + 1) (+ 8), piece g,
 // and S leaves the tensor cores in the layout in which W enters them.  Each warp has a ring of strips of its own, which
-// its lane 0 fills by TMA (one box of 16 rows x 128 bytes each for K and V) behind an mbarrier a stage: no barrier
+// its lane 0 fills by TMA (a box of its rows x 128 bytes each for K and V) behind an mbarrier a stage: no barrier
 // between warps.  The 128-byte swizzle puts piece i of row r at i ^ (r & 7); with at(c) = c for even
 // columns and c ^ 4 for odd ones, the eight lanes of a shared-memory phase touch eight different pieces in both reads.
 //
@@ -42,8 +42,6 @@ __device__ int g_dec8_error = 0;
 __device__ __forceinline__ void record(int bit) { atomicOr(&g_dec8_error, bit); }
 
 constexpr int ERR_WAIT = 32768;    // a copy's wait gave up
-constexpr int ST = 16;             // positions of a strip
-constexpr int NW = 4;              // warps of a CTA
 constexpr float NONE = -1e30f;     // a running maximum that nothing has moved yet
 constexpr float LAZY = 8.f;        // a score may exceed the running maximum by 8 (base 2) before it is moved
 constexpr int LIFT = 6;            // weights are brought to [2^6, 2^7) ...
@@ -52,9 +50,12 @@ constexpr int MIN_STRIPS = 2;      // least strips of a range
 
 template <int W, int RT>
 struct Cfg {
-  // warps of an SM and their stages: what 64 K registers and 227 KB of shared memory hold
-  static constexpr int CTAS = W == 256 ? (RT == 16 ? 1 : 2) : RT == 16 ? 2 : W == 64 ? 4 : 3;   // per SM
-  static constexpr int STAGES = RT == 16 ? 4 : W == 256 ? 2 : W == 128 ? 3 : 4;
+  // positions of a strip, warps of a CTA, CTAs of an SM, stages: what 64 K registers and 227 KB of shared memory hold
+  static constexpr int ST = RT == 8 && W <= 128 ? 32 : 16;
+  static constexpr int NW = 4;
+  static constexpr int CTAS = W == 256 ? (RT == 16 ? 1 : 2) : RT == 16 ? 2 : W == 64 ? 4 : 2;
+  static constexpr int STAGES = RT == 8 ? 2 : W == 128 ? 3 : 4;
+  static constexpr int JT = ST / 8;                                        // n tiles of S
   static constexpr int KS = W / 16;                                        // k steps of S
   static constexpr int ROW = W == 64 ? 64 : 128;                           // bytes of a box row
   static constexpr int PANELS = W / ROW;                                   // boxes of a row
@@ -62,7 +63,8 @@ struct Cfg {
   static constexpr int STAGE_B = 2 * HALF_B;
   static constexpr int Q_B = KS * 512 * (RT / 8);                          // q operands
   static constexpr int RING_B = STAGES * STAGE_B;
-  static constexpr int WARP_B = RING_B + Q_B + STAGES * 128;               // and scales
+  static constexpr int SCALE_B = ST * 8;                                   // scales of a strip: ST of K, ST of V
+  static constexpr int WARP_B = RING_B + Q_B + STAGES * SCALE_B;
   static constexpr int SMEM = NW * WARP_B + 1024;                          // + what aligns the rings to 1 KB
   static_assert(SMEM * CTAS <= 227 * 1024, "shared memory of an SM");
   static constexpr int SLOT = RT * (W + 2);                                // floats of a slot: m[RT], l[RT], o[RT][W]
@@ -70,10 +72,17 @@ struct Cfg {
 
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + e) << 23); }   // -126 <= e <= 127
 __device__ __forceinline__ int exponent(float x) { return max(((__float_as_int(x) >> 23) & 255) - 127, -120); }
-__device__ __forceinline__ float max4(const float* v) { return fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])); }
-// m raised to the largest of it and a row's four values in each of its four threads; returns it
-__device__ __forceinline__ float raise(float& m, const float* v) {
-  float a = max4(v);
+template <int N>
+__device__ __forceinline__ float max_of(const float (&v)[N]) {
+  float a = v[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) a = fmaxf(a, v[i]);
+  return a;
+}
+// m raised to the largest of it and a row's values in each of its four threads; returns it
+template <int N>
+__device__ __forceinline__ float raise(float& m, const float (&v)[N]) {
+  float a = max_of(v);
   a = fmaxf(a, __shfl_xor_sync(~0u, a, 1));
   a = fmaxf(a, __shfl_xor_sync(~0u, a, 2));
   return m = fmaxf(a, m);
@@ -147,17 +156,13 @@ struct Conv<I8> {
 };
 template <>
 struct Conv<E4M3> {
-  static __device__ __forceinline__ uint32_t two(uint32_t x, int up) {
-    const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(up ? x >> 16 : x & 0xffffu), __NV_E4M3);
-    return (uint32_t)r.x | ((uint32_t)r.y << 16);
-  }
   static __device__ __forceinline__ void along(uint32_t w, uint32_t& p0, uint32_t& p1) {
-    p0 = two(w, 0);
-    p1 = two(w, 1);
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+        : "=r"(p0), "=r"(p1) : "r"(w));
   }
   static __device__ __forceinline__ void across(uint32_t a, uint32_t b, uint32_t* p) {
-    const uint32_t x = __byte_perm(a, b, 0x5140), y = __byte_perm(a, b, 0x7362);
-    p[0] = two(x, 0); p[1] = two(x, 1); p[2] = two(y, 0); p[3] = two(y, 1);
+    along(__byte_perm(a, b, 0x5140), p[0], p[1]);
+    along(__byte_perm(a, b, 0x7362), p[2], p[3]);
   }
 };
 
@@ -168,7 +173,7 @@ struct Seq {
   long long first;        // its first row
 };
 
-template <int RT>
+template <int RT, int ST>
 __device__ __forceinline__ Seq seq_of(const FaDec8Params& p, const Pages& pg, int z) {
   Seq s;
   const RowMap rm{p.cu_q, p.tokens, p.batch};
@@ -286,11 +291,13 @@ struct Cut {   // the sequence whose strips begin in a warp's range and end in a
 
 // ---------------------------------------------------------------- the pass over the cache
 template <int W, typename Q, int RT>
-__global__ void __launch_bounds__(NW * 32, (Cfg<W, RT>::CTAS))
+__global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
     dec8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const FaDec8Params p,
                 const Pages pg, const int dtype, const int ranges) {
   using C = Cfg<W, RT>;
-  constexpr int STAGES = C::STAGES, KS = C::KS, NT = W / 8, KC = W / 64, VC = W == 256 ? 2 : 1;
+  constexpr int ST = C::ST, NW = C::NW, STAGES = C::STAGES, KS = C::KS, NT = W / 8, KC = W / 64, VC = W == 256 ? 2 : 1;
+  constexpr int JT = C::JT, NP = 2 * JT;   // n tiles of S, positions of a thread
+  constexpr unsigned ALL = ST == 32 ? ~0u : 0xffffu;
   constexpr int RPT = RT / 8;        // rows of a thread: g, g + 8
   extern __shared__ unsigned char smem_raw[];
   __shared__ unsigned long long s_full[NW][STAGES];   // mbarrier of a stage
@@ -308,7 +315,7 @@ __global__ void __launch_bounds__(NW * 32, (Cfg<W, RT>::CTAS))
   {
     long long mine = 0;
     for (int z = tid * CB; z < min(p.batch, (tid + 1) * CB); ++z) {
-      const Seq s = seq_of<RT>(p, pg, z);
+      const Seq s = seq_of<RT, C::ST>(p, pg, z);
       mine += (long long)s.strips * s.tiles;
     }
     long long inc = mine;
@@ -335,14 +342,13 @@ __global__ void __launch_bounds__(NW * 32, (Cfg<W, RT>::CTAS))
 
   const uint32_t base = (sm100::smem_u32(smem_raw) + 1023u) & ~1023u, ring = base + warp * C::RING_B;
   const unsigned char* const mine = smem_raw + (ring - sm100::smem_u32(smem_raw));
-  unsigned char* const own = smem_raw + (base - sm100::smem_u32(smem_raw)) + NW * C::RING_B + warp * (C::Q_B + STAGES * 128);
+  unsigned char* const own = smem_raw + (base - sm100::smem_u32(smem_raw)) + NW * C::RING_B + warp * (C::Q_B + STAGES * C::SCALE_B);
   uint4* const qs = reinterpret_cast<uint4*>(own);
-  const float* const scales = reinterpret_cast<const float*>(own + C::Q_B);   // a stage: 16 of K, 16 of V
+  const float* const scales = reinterpret_cast<const float*>(own + C::Q_B);   // a stage: ST of K, ST of V
   const uint32_t scales_u = sm100::smem_u32(scales) + lane * 4;
-  const float* const my_scale = lane < 16 ? p.Ks : p.Vs;
   const int bshift = log2_of(p.block), per_page = p.page >> bshift;
   const int run = min(p.page, ST);                  // slots of a box
-  const bool tma = run >= 8;                        // a box keeps whole swizzle atoms
+  const bool tma = p.page >= 16;
   // the thread's pieces within K or V of a stage
   const auto piece = [](int row, int i) { return row * C::ROW + (C::ROW == 128 ? (i ^ (row & 7)) : (i ^ ((row >> 1) & 3))) * 16; };
   const int kat = piece(col_pos(g), t4);
@@ -363,10 +369,10 @@ __global__ void __launch_bounds__(NW * 32, (Cfg<W, RT>::CTAS))
     }
     z = a * CB;
     off = s_pre[a];
-    sq = seq_of<RT>(p, pg, z);
+    sq = seq_of<RT, C::ST>(p, pg, z);
     while (off + (long long)sq.strips * sq.tiles <= begin) {
       off += (long long)sq.strips * sq.tiles;
-      sq = seq_of<RT>(p, pg, ++z);
+      sq = seq_of<RT, C::ST>(p, pg, ++z);
     }
   }
 
@@ -375,10 +381,10 @@ __global__ void __launch_bounds__(NW * 32, (Cfg<W, RT>::CTAS))
     const int tile = (int)((at - off) / sq.strips), k0 = (int)((at - off) % sq.strips);
     const int k1 = (int)min((long long)sq.strips, k0 + (end - at));
 
-    // Strip k of the sequence into a stage: lane 0 the codes, each lane one scale (0-15: K's of position lane, 16-31: V's).
-    // What no row sees is not read: its weights are 0, and its V rows are cleared where they are used.  The page of
-    // the next strip is looked up an issue ahead.
-    int blk = pg.of(z, (sq.s0 + k0) * ST);
+    // Strip k of the sequence into a stage: lane 0 the codes, the lanes one scale each (two where a strip has 32).
+    // What no row sees is not read: its weights are 0, and its V rows are cleared where they are used.  The pages of
+    // the next strip (two where a page is half a strip) are looked up an issue ahead.
+    int b0 = pg.of(z, (sq.s0 + k0) * ST), b1 = run < ST ? pg.of(z, (sq.s0 + k0) * ST + run) : b0;
     auto box = [&](int pos, int b) {                // do rows see something of the slots [pos, pos + run) in page b
       if (pos + run <= sq.lo || pos >= sq.L) return false;
       if (b < 0) record(ERR_PAGE);
@@ -392,49 +398,58 @@ __global__ void __launch_bounds__(NW * 32, (Cfg<W, RT>::CTAS))
         sm100::tma_load_3d(dst + C::HALF_B + c * ST * C::ROW, &tmV, c * C::ROW, kvh, slot, bar);
       }
     };
+    auto scale_to = [&](int e, int b, int in_page, int to) {   // entry e of a stage's scales
+      cp_async4(scales_u + to * C::SCALE_B + (e - lane) * 4,
+                (e < ST ? p.Ks : p.Vs) + (long long)(b * NKV + kvh) * per_page + (in_page >> bshift));
+    };
     auto issue = [&](int k, int to) {
-      const int pos0 = (sq.s0 + k) * ST;
-      if (run == ST) {
-        const int in_page = pos0 & (p.page - 1);
-        const bool go = box(pos0, blk);
-        if (lane == 0) {
-          s_have[warp][to] = go ? 0xffffu : 0u;
-          sm100::mbar_expect_tx(sm100::smem_u32(&s_full[warp][to]), go ? C::STAGE_B : 0);
-          if (go) load(0, blk * p.page + in_page, to);
+      const int pos0 = (sq.s0 + k) * ST, in_page = pos0 & (p.page - 1);
+      const bool go0 = box(pos0, b0), go1 = run < ST && box(pos0 + run, b1);
+      if (lane == 0) {
+        unsigned have = 0, bytes = 0;
+        if (run == ST) {
+          have = go0 ? ALL : 0u;
+          bytes = go0 ? C::STAGE_B : 0;
+        } else {
+          have = (go0 ? 0xffffu : 0u) | (go1 ? 0xffff0000u : 0u);
+          bytes = (go0 + go1) * (C::STAGE_B / 2);
         }
-        if (go) cp_async4(scales_u + to * 128, my_scale + (long long)(blk * NKV + kvh) * per_page + ((in_page + (lane & 15)) >> bshift));
-        if (in_page + ST == p.page && k + 1 < k1) blk = pg.of(z, pos0 + ST);
-      } else {                                      // pages of 8
-        const int b1 = pg.of(z, pos0 + 8);
-        const bool go0 = box(pos0, blk), go1 = box(pos0 + 8, b1);
-        if (lane == 0) {
-          s_have[warp][to] = (go0 ? 0xffu : 0u) | (go1 ? 0xff00u : 0u);
-          sm100::mbar_expect_tx(sm100::smem_u32(&s_full[warp][to]), (go0 + go1) * (C::STAGE_B / 2));
-          if (go0) load(0, blk * 8, to);
-          if (go1) load(8, b1 * 8, to);
-        }
-        if (lane & 8 ? go1 : go0)
-          cp_async4(scales_u + to * 128, my_scale + (long long)((lane & 8 ? b1 : blk) * NKV + kvh) * per_page + ((lane & 7) >> bshift));
-        blk = k + 1 < k1 ? pg.of(z, pos0 + ST) : 0;
+        s_have[warp][to] = have;
+        sm100::mbar_expect_tx(sm100::smem_u32(&s_full[warp][to]), bytes);
+        if (go0) load(0, b0 * p.page + in_page, to);
+        if (go1) load(run, b1 * p.page, to);
+      }
+#pragma unroll
+      for (int i = 0; i < ST / 16; ++i) {
+        const int e = lane + 32 * i, r = e % ST;
+        if (r < run ? go0 : go1) scale_to(e, r < run ? b0 : b1, (in_page + r) & (p.page - 1), to);
+      }
+      if (in_page + ST >= p.page && k + 1 < k1) {
+        b0 = pg.of(z, pos0 + ST);
+        if (run < ST) b1 = pg.of(z, pos0 + ST + run);
       }
     };
-    // Pages of less than 8 slots: the whole warp copies slot by slot, piece by piece, into the same places.
+    // Pages of less than 16 slots: the whole warp copies slot by slot, piece by piece, into the same places.
     auto issue_small = [&](int k, int to) {
-      const int pos0 = (sq.s0 + k) * ST, r = lane & 15, pos = pos0 + r;
-      const bool in = pos >= sq.lo && pos < sq.L;
-      const int b = in ? pg.of(z, pos) : -1;
-      if (in && b < 0) record(ERR_PAGE);
-      const unsigned have = __ballot_sync(~0u, b >= 0) & 0xffffu;
-      if (lane == 0) s_have[warp][to] = have;
-      const unsigned char* src = (const unsigned char*)(lane < 16 ? p.Kc : p.Vc);   // lanes 0-15: K, 16-31: V
-      if (b >= 0) src += (((long long)b * p.page + (pos & (p.page - 1))) * NKV + kvh) * p.dim;
-      const uint32_t dst = ring + to * C::STAGE_B + (lane < 16 ? 0 : C::HALF_B);
-      for (int i = 0; i < W / 16; ++i) {
-        const bool ok = b >= 0 && 16 * i < p.dim;
-        cp_async16(dst + (16 * i / C::ROW) * ST * C::ROW + piece(r, i % (C::ROW / 16)), ok ? src + 16 * i : src, ok);
+      const int pos0 = (sq.s0 + k) * ST;
+      unsigned have = 0;
+#pragma unroll 1
+      for (int i = 0; i < ST / 16; ++i) {           // lane's entry: K or V of position pos0 + r
+        const int e = lane + 32 * i, r = e % ST, pos = pos0 + r;
+        const bool in = pos >= sq.lo && pos < sq.L;
+        const int b = in ? pg.of(z, pos) : -1;
+        if (in && b < 0) record(ERR_PAGE);
+        have = __ballot_sync(~0u, b >= 0) & ALL;
+        const unsigned char* src = (const unsigned char*)(e < ST ? p.Kc : p.Vc);
+        if (b >= 0) src += (((long long)b * p.page + (pos & (p.page - 1))) * NKV + kvh) * p.dim;
+        const uint32_t dst = ring + to * C::STAGE_B + (e < ST ? 0 : C::HALF_B);
+        for (int j = 0; j < W / 16; ++j) {
+          const bool ok = b >= 0 && 16 * j < p.dim;
+          cp_async16(dst + (16 * j / C::ROW) * ST * C::ROW + piece(r, j % (C::ROW / 16)), ok ? src + 16 * j : src, ok);
+        }
+        if (b >= 0) scale_to(e, b, pos & (p.page - 1), to);
       }
-      if (b >= 0)
-        cp_async4(scales_u + to * 128, my_scale + ((long long)b * NKV + kvh) * per_page + ((pos & (p.page - 1)) >> bshift));
+      if (lane == 0) s_have[warp][to] = have;
     };
     __syncwarp();                                   // the last piece's stages and q are free
     for (int i = 0, to = stage; i < STAGES; ++i) {
@@ -537,67 +552,67 @@ __global__ void __launch_bounds__(NW * 32, (Cfg<W, RT>::CTAS))
       }
       const unsigned char* const src = mine + stage * C::STAGE_B;
 
-      // ---- S = Q K^T: columns j * 8 + 2 t4 + {0, 1}
-      float s[2][4];
+      // ---- S = Q K^T: column c of n tile j is position pos0 + 8 j + col_pos(c)
+      float s[JT][4];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+      for (int j = 0; j < JT; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
 #pragma unroll
       for (int c = 0; c < KC; ++c) {
-        uint4 kk[2];
-        const int o = (c >> 1) * (ST * 128) + (kat ^ ((c & 1) * 64));
-        kk[0] = *reinterpret_cast<const uint4*>(src + o);
-        kk[1] = *reinterpret_cast<const uint4*>(src + o + 8 * C::ROW);
+        uint4 kk[JT];
+#pragma unroll
+        for (int j = 0; j < JT; ++j)
+          kk[j] = *reinterpret_cast<const uint4*>(src + (c >> 1) * (ST * 128) + (kat ^ ((c & 1) * 64)) + j * 8 * C::ROW);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          uint32_t qv[4], ql[4];
-            const uint4 u = qs[(4 * c + w) * 32 + lane];
-            qv[0] = u.x; qv[1] = u.y; qv[2] = u.z; qv[3] = u.w;
-            if constexpr (RT == 16) {
-              const uint4 v = qs[(KS + 4 * c + w) * 32 + lane];
-              ql[0] = v.x; ql[1] = v.y; ql[2] = v.z; ql[3] = v.w;
-            }
+          const uint4 qu = qs[(4 * c + w) * 32 + lane];
+          const uint32_t qv[4] = {qu.x, qu.y, qu.z, qu.w};
+          uint32_t ql[4];
+          if constexpr (RT == 16) {
+            const uint4 lu = qs[(KS + 4 * c + w) * 32 + lane];
+            ql[0] = lu.x; ql[1] = lu.y; ql[2] = lu.z; ql[3] = lu.w;
+          }
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            uint32_t b0, b1;
-            Conv<Q>::along((&kk[j].x)[w], b0, b1);
-            mma(s[j], qv, b0, b1);
-            if constexpr (RT == 16) mma(s[j], ql, b0, b1);
+          for (int j = 0; j < JT; ++j) {
+            uint32_t k0, k1;
+            Conv<Q>::along((&kk[j].x)[w], k0, k1);
+            mma(s[j], qv, k0, k1);
+            if constexpr (RT == 16) mma(s[j], ql, k0, k1);
           }
         }
       }
 
-      // ---- weights of positions pos0 + 8 j + 2 t4 + e, row g (+ 8 r)
+      // ---- weights of positions pos0 + 8 j + col_pos(2 t4 + e), row g (+ 8 r), at [2 j + e]
       const int pos0 = (sq.s0 + k) * ST;
-      const uint32_t have = s_have[warp][stage];
+      const unsigned have = s_have[warp][stage];
       // every position seen by every row, and scores that are nothing but products
-      const bool plain = have == 0xffffu && pos0 >= all_lo && pos0 + ST <= all_hi;
-      float x[RPT][4], ks[4], vs[4];
+      const bool plain = have == ALL && pos0 >= all_lo && pos0 + ST <= all_hi;
+      float x[RPT][NP], vs[NP];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < NP; ++i) {
         const int r = 8 * (i >> 1) + col_pos(2 * t4 + (i & 1));
-        ks[i] = scales[stage * 32 + r];
-        vs[i] = scales[stage * 32 + 16 + r];
+        const float ks = scales[stage * (2 * ST) + r];
+        vs[i] = scales[stage * (2 * ST) + ST + r];
+#pragma unroll
+        for (int h = 0; h < RPT; ++h)
+          x[h][i] = (RT == 8 ? s[i >> 1][i & 1] + s[i >> 1][2 + (i & 1)] : s[i >> 1][2 * h + (i & 1)]) * (ks * qf[h]);
       }
-      bool move = false;
+      if (!plain) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+        for (int i = 0; i < NP; ++i) {
+          const int r = 8 * (i >> 1) + col_pos(2 * t4 + (i & 1)), pos = pos0 + r;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int pos = pos0 + 8 * j + col_pos(2 * t4 + e);
-#pragma unroll
-          for (int r = 0; r < RPT; ++r) {
-            float v = (RT == 8 ? s[j][e] + s[j][2 + e] : s[j][2 * r + e]) * (ks[2 * j + e] * qf[r]);
-            if (!plain) {
-              if (cap) v = cap_out * fa_tanh(v);
-              if (p.alibi) v = fmaf(slope[r], (float)pos - qpos[r], v);
-              if (!(pos >= rlo[r] && pos < rhi[r] && ((have >> (pos - pos0)) & 1))) v = -INFINITY;
-            }
-            x[r][2 * j + e] = v;
+          for (int h = 0; h < RPT; ++h) {
+            float v = x[h][i];
+            if (cap) v = cap_out * fa_tanh(v);
+            if (p.alibi) v = fmaf(slope[h], (float)pos - qpos[h], v);
+            if (!(pos >= rlo[h] && pos < rhi[h] && ((have >> r) & 1))) v = -INFINITY;
+            x[h][i] = v;
           }
         }
       }
+      bool move = false;
 #pragma unroll
-      for (int r = 0; r < RPT; ++r) move |= max4(x[r]) > m[r] + LAZY;
+      for (int r = 0; r < RPT; ++r) move |= max_of(x[r]) > m[r] + LAZY;
       if (__any_sync(~0u, move)) {
 #pragma unroll
         for (int r = 0; r < RPT; ++r) {
@@ -606,17 +621,21 @@ __global__ void __launch_bounds__(NW * 32, (Cfg<W, RT>::CTAS))
           scale_rows<NT, RT>(o, r, f);
         }
       }
-      float w[RPT][4];
+      float w[RPT][NP];
       move = false;
 #pragma unroll
       for (int r = 0; r < RPT; ++r) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < NP; ++i) {
           const float e = ex2(x[r][i] - m[r]);
           l[r] += e;
-          w[r][i] = !plain && x[r][i] == -INFINITY ? 0.f : e * vs[i];
+          w[r][i] = e * vs[i];
         }
-        move |= max4(w[r]) * up[r] > MOST;
+        if (!plain)
+#pragma unroll
+          for (int i = 0; i < NP; ++i)
+            if (x[r][i] == -INFINITY) w[r][i] = 0.f;   // whatever the scale is
+        move |= max_of(w[r]) * up[r] > MOST;
       }
       if (__any_sync(~0u, move)) {
 #pragma unroll
@@ -628,64 +647,57 @@ __global__ void __launch_bounds__(NW * 32, (Cfg<W, RT>::CTAS))
           up[r] = to;
         }
       }
-      uint32_t wa[4], wl[4];
-#pragma unroll
-      for (int r = 0; r < RPT; ++r)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          uint32_t hi, lo;
-          split(w[r][2 * j] * up[r], w[r][2 * j + 1] * up[r], hi, lo);
-          if constexpr (RT == 8) {
-            wa[2 * j] = hi;
-            wa[2 * j + 1] = lo;
-          } else {
-            wa[2 * j + r] = hi;
-            wl[2 * j + r] = lo;
-          }
-        }
 
-      // ---- O += W V
-      const unsigned char* const vsrc = src + C::HALF_B;
-      const auto hidden = [&](int j) {              // row j of the thread's four: 2 (its half) + (odd column)
-        const int r = 8 * (j >> 1) + col_pos(2 * t4 + (j & 1));
-        return !plain && !(pos0 + r >= sq.lo && pos0 + r < sq.L && ((have >> r) & 1));
-      };
-      if constexpr (W == 64) {
-        uint2 v[4];
+      // ---- O += W V, 16 positions (two n tiles of S) a time
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          v[j] = *reinterpret_cast<const uint2*>(vsrc + ((j & 1) ? vat1 : vat0) + (j >> 1) * 8 * C::ROW);
-          if (hidden(j)) v[j] = make_uint2(0, 0);   // whatever is there: 0 * NaN is not 0
-        }
+      for (int b = 0; b < ST / 16; ++b) {
+        uint32_t wa[4], wl[4];
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          uint32_t b0[4], b1[4];
-          Conv<Q>::across((&v[0].x)[w], (&v[1].x)[w], b0);
-          Conv<Q>::across((&v[2].x)[w], (&v[3].x)[w], b1);
+        for (int r = 0; r < RPT; ++r)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            mma(o[4 * w + i], wa, b0[i], b1[i]);
-            if constexpr (RT == 16) mma(o[4 * w + i], wl, b0[i], b1[i]);
+          for (int j = 0; j < 2; ++j) {
+            uint32_t hi, lo;
+            split(w[r][4 * b + 2 * j] * up[r], w[r][4 * b + 2 * j + 1] * up[r], hi, lo);
+            if constexpr (RT == 8) {
+              wa[2 * j] = hi;
+              wa[2 * j + 1] = lo;
+            } else {
+              wa[2 * j + r] = hi;
+              wl[2 * j + r] = lo;
+            }
           }
-        }
-      } else {
-#pragma unroll
-        for (int c = 0; c < VC; ++c) {
-          uint4 v[4];
+        // the thread's rows: positions 16 b + 8 (j >> 1) + col_pos(2 t4 + (j & 1)); what no row sees may be
+        // anything, and 0 * NaN is not 0
+        const unsigned char* const vsrc = src + C::HALF_B + b * 16 * C::ROW;
+        unsigned hidden = 0;
+        if (!plain) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            v[j] = *reinterpret_cast<const uint4*>(vsrc + c * (ST * 128) + ((j & 1) ? vat1 : vat0) + (j >> 1) * 8 * C::ROW);
-            if (hidden(j)) v[j] = make_uint4(0, 0, 0, 0);   // whatever is there: 0 * NaN is not 0
+            const int r = 16 * b + 8 * (j >> 1) + col_pos(2 * t4 + (j & 1));
+            if (!(pos0 + r >= sq.lo && pos0 + r < sq.L && ((have >> r) & 1))) hidden |= 1u << j;
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < VC; ++c) {
+          using Piece = std::conditional_t<W == 64, uint2, uint4>;
+          Piece v[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            v[j] = *reinterpret_cast<const Piece*>(vsrc + c * (ST * 128) + ((j & 1) ? vat1 : vat0) + (j >> 1) * 8 * C::ROW);
+          if (hidden) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if ((hidden >> j) & 1) v[j] = Piece{};
           }
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            uint32_t b0[4], b1[4];
-            Conv<Q>::across((&v[0].x)[w], (&v[1].x)[w], b0);
-            Conv<Q>::across((&v[2].x)[w], (&v[3].x)[w], b1);
+          for (int i = 0; i < (int)sizeof(Piece) / 4; ++i) {
+            uint32_t v0[4], v1[4];
+            Conv<Q>::across((&v[0].x)[i], (&v[1].x)[i], v0);
+            Conv<Q>::across((&v[2].x)[i], (&v[3].x)[i], v1);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              mma(o[16 * c + 4 * w + i], wa, b0[i], b1[i]);
-              if constexpr (RT == 16) mma(o[16 * c + 4 * w + i], wl, b0[i], b1[i]);
+            for (int n = 0; n < 4; ++n) {
+              mma(o[16 * c + 4 * i + n], wa, v0[n], v1[n]);
+              if constexpr (RT == 16) mma(o[16 * c + 4 * i + n], wl, v0[n], v1[n]);
             }
           }
         }
@@ -753,7 +765,7 @@ __global__ void __launch_bounds__(NW * 32, (Cfg<W, RT>::CTAS))
     if (at < end && at - off >= (long long)sq.strips * sq.tiles) {
       do {
         off += (long long)sq.strips * sq.tiles;
-        sq = seq_of<RT>(p, pg, ++z);
+        sq = seq_of<RT, C::ST>(p, pg, ++z);
       } while (sq.tiles == 0);
     }
   }
@@ -802,7 +814,7 @@ __global__ void __launch_bounds__(MW * 32)
   for (int item = blockIdx.x; item < count * RT; item += gridDim.x) {
     const int gw = s_cut[item / RT], r = item % RT;
     const Cut cut = cuts[gw];
-    const Seq sq = seq_of<RT>(p, pg, cut.z);
+    const Seq sq = seq_of<RT, C::ST>(p, pg, cut.z);
     const int row = cut.tile * RT + r, tok = row / p.gqa, head = gw % NKV * p.gqa + row % p.gqa;
     if (tok >= sq.n) continue;
     // part 0: second slot of warp gw; part i: first slot of the warp i ranges on
@@ -862,12 +874,12 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 
 // The cache as rows of `dim` bytes: (dim, kv heads, slots); a box is `row` bytes of one head in `run` slots, what lies past dim
 // comes as zeros.
-int map_of(CUtensorMap* m, const void* base, const FaDec8Params& p, int row) {
+int map_of(CUtensorMap* m, const void* base, const FaDec8Params& p, int row, int strip) {
   const auto enc = encode_fn();
   const cuuint64_t heads = p.NH / p.gqa;
   const cuuint64_t dims[3] = {(cuuint64_t)p.dim, heads, (cuuint64_t)p.num_blocks * p.page};
   const cuuint64_t strides[2] = {(cuuint64_t)p.dim, heads * p.dim};
-  const cuuint32_t box[3] = {(cuuint32_t)row, 1, (cuuint32_t)std::min(p.page, ST)};
+  const cuuint32_t box[3] = {(cuuint32_t)row, 1, (cuuint32_t)std::min(p.page, strip)};
   const cuuint32_t one[3] = {1, 1, 1};
   const CUresult e = !enc ? CUDA_ERROR_NOT_FOUND
                           : enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, one,
@@ -884,12 +896,12 @@ int launch(const FaDec8Params& p, int dtype, cudaStream_t st) {
   static unsigned long long done = 0;
   if (int rc = fa::ensure_smem((const void*)dec8_kernel<W, Q, RT>, C::SMEM, &done)) return rc;
   CUtensorMap mk, mv;
-  if (int rc = map_of(&mk, p.Kc, p, C::ROW)) return rc;
-  if (int rc = map_of(&mv, p.Vc, p, C::ROW)) return rc;
+  if (int rc = map_of(&mk, p.Kc, p, C::ROW, C::ST)) return rc;
+  if (int rc = map_of(&mv, p.Vc, p, C::ROW, C::ST)) return rc;
   const Pages pg{p.block_table, log2_of(p.page), p.max_blocks, p.num_blocks};
-  const int NKV = p.NH / p.gqa, grid = fa::num_sms() * C::CTAS, warps = grid * NW;
-  const int ranges = std::max(1, warps / NKV), need = (ranges * NKV + NW - 1) / NW;
-  dec8_kernel<W, Q, RT><<<need, NW * 32, C::SMEM, st>>>(mk, mv, p, pg, dtype, ranges);
+  const int NKV = p.NH / p.gqa, grid = fa::num_sms() * C::CTAS, warps = grid * C::NW;
+  const int ranges = std::max(1, warps / NKV), need = (ranges * NKV + C::NW - 1) / C::NW;
+  dec8_kernel<W, Q, RT><<<need, C::NW * 32, C::SMEM, st>>>(mk, mv, p, pg, dtype, ranges);
   fa::count_launch();
   if (int rc = fa::cuda_status(cudaGetLastError(), "8-bit decode launch")) return rc;
   const cudaError_t e = fa::launch_pdl(dec8_merge_kernel<W, RT>, dim3(2 * fa::num_sms()), dim3(MW * 32),
@@ -914,7 +926,7 @@ int by_dim(const FaDec8Params& p, int dtype, cudaStream_t st) {
 template <int W, int RT>
 long long scratch_of(int NKV) {
   using C = Cfg<W, RT>;
-  const long long warps = (long long)fa::num_sms() * C::CTAS * NW, used = std::max<long long>(1, warps / NKV) * NKV;
+  const long long warps = (long long)fa::num_sms() * C::CTAS * C::NW, used = std::max<long long>(1, warps / NKV) * NKV;
   return used * (sizeof(Cut) / 4 + 2ll * C::SLOT);
 }
 
