@@ -309,7 +309,11 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
   if (lane == 0) {
     for (int i = 0; i < STAGES; ++i) sm100::mbar_init(sm100::smem_u32(&s_full[warp][i]), 1);
     sm100::fence_barrier_init();
+    sm100::prefetch_tmap(&tmK);
+    sm100::prefetch_tmap(&tmV);
   }
+  pdl_wait();      // what comes before on the stream (an append) is done
+  pdl_trigger();   // the merge may be set up; it waits for this grid itself
   // ---- the line of strips: every thread sums a run of sequences
   const int CB = (p.batch + NW * 32 - 1) / (NW * 32);
   {
@@ -770,7 +774,6 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
     }
   }
   if (lane == 0) cuts[gw] = cut;
-  pdl_trigger();
 }
 
 // ---------------------------------------------------------------- the join of cut sequences
@@ -787,6 +790,7 @@ __global__ void __launch_bounds__(MW * 32)
   __shared__ float s_l[MW], s_v[MW][W];
   const int NKV = p.NH / p.gqa, warps = ranges * NKV, tid = threadIdx.x, w = tid / 32, lane = tid % 32;
   pdl_wait();
+  pdl_trigger();
   const Cut* const cuts = reinterpret_cast<const Cut*>(p.scratch);
   const int per = (warps + MW * 32 - 1) / (MW * 32), i0 = tid * per, i1 = min(warps, i0 + per);
   int mine = 0;
@@ -901,10 +905,10 @@ int launch(const FaDec8Params& p, int dtype, cudaStream_t st) {
   const Pages pg{p.block_table, log2_of(p.page), p.max_blocks, p.num_blocks};
   const int NKV = p.NH / p.gqa, grid = fa::num_sms() * C::CTAS, warps = grid * C::NW;
   const int ranges = std::max(1, warps / NKV), need = (ranges * NKV + C::NW - 1) / C::NW;
-  dec8_kernel<W, Q, RT><<<need, C::NW * 32, C::SMEM, st>>>(mk, mv, p, pg, dtype, ranges);
+  cudaError_t e = fa::launch_pdl(dec8_kernel<W, Q, RT>, dim3(need), dim3(C::NW * 32), C::SMEM, st, mk, mv, p, pg, dtype, ranges);
   fa::count_launch();
-  if (int rc = fa::cuda_status(cudaGetLastError(), "8-bit decode launch")) return rc;
-  const cudaError_t e = fa::launch_pdl(dec8_merge_kernel<W, RT>, dim3(2 * fa::num_sms()), dim3(MW * 32),
+  if (int rc = fa::cuda_status(e, "8-bit decode launch")) return rc;
+  e = fa::launch_pdl(dec8_merge_kernel<W, RT>, dim3(2 * fa::num_sms()), dim3(MW * 32),
                                        (size_t)ranges * NKV * sizeof(int), st, p, pg, dtype, ranges);
   fa::count_launch();
   return fa::cuda_status(e, "8-bit decode merge launch");
