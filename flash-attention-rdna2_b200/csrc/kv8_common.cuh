@@ -75,10 +75,20 @@ struct RowMap {
   }
 };
 
-__host__ __device__ constexpr int log2_of(int x) {
-  int s = 0;
-  while ((1 << s) < x) ++s;
-  return s;
+__host__ __device__ __forceinline__ int log2_of(int x) {   // of a power of two
+#ifdef __CUDA_ARCH__
+  return 31 - __clz(x);
+#else
+  return 31 - __builtin_clz((unsigned)x);
+#endif
 }
+
+// n / d for 0 <= n < 2^31 / d, d known to the host: one multiplication
+struct Div {
+  unsigned d, m;
+  Div() = default;
+  explicit Div(int d_) : d((unsigned)d_), m((unsigned)((0x100000000ull + d_ - 1) / d_)) {}
+  __device__ __forceinline__ int of(int n) const { return d == 1 ? n : (int)__umulhi((unsigned)n, m); }
+};
 
 }  // namespace fa_kv

@@ -157,18 +157,21 @@ __device__ __forceinline__ void to_float8(const Raw8<T>& r, float* v) {
   for (int i = 0; i < 8; ++i) v[i] = Elem<T>::to_f(e[i]);
 }
 template <typename T>
+__device__ __forceinline__ void store_raw(T* x, const Raw8<T>& r) {
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(x)[i] = r.u[i];
+}
+template <typename T>
 __device__ __forceinline__ void store8(T* x, const float* v) {
   Raw8<T> r;
   T* e = reinterpret_cast<T*>(&r);
 #pragma unroll
   for (int i = 0; i < 8; ++i) e[i] = Elem<T>::from_f(v[i]);
-#pragma unroll
-  for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(x)[i] = r.u[i];
+  store_raw(x, r);
 }
-
 // Groups of unit u of a row: rotated NeoX pieces pair group 8 u with the one rot_dim / 2 further, all others their neighbour.
-__device__ __forceinline__ void groups_of(int u, const Turn& r, bool turn, int& d1, int& d2) {
-  if (turn && !r.interleaved && 16 * u < r.dim) {
+__device__ __forceinline__ void groups_of(int u, const Turn& r, bool is_k, int& d1, int& d2) {
+  if (is_k && r.cos && !r.interleaved && 16 * u < r.dim) {
     d1 = 8 * u;
     d2 = d1 + r.dim / 2;
   } else {
@@ -176,25 +179,24 @@ __device__ __forceinline__ void groups_of(int u, const Turn& r, bool turn, int& 
     d2 = d1 + 8;
   }
 }
-// rotates a unit's groups a, b by table row tp: every product and the sum rounded in fp32
-__device__ __forceinline__ void turn8(float* a, float* b, int u, const Turn& r, int tp) {
-  const int half = r.dim / 2;
-  const float4* ct = reinterpret_cast<const float4*>(r.cos + (long long)tp * half + 8 * u);
-  const float4* st = reinterpret_cast<const float4*>(r.sin + (long long)tp * half + 8 * u);
-  float c[8], s[8];
+__device__ __forceinline__ void turn2(float& x, float& y, float c, float s) {   // every product and the sum rounded in fp32
+  const float lo = __fsub_rn(__fmul_rn(x, c), __fmul_rn(y, s)), hi = __fadd_rn(__fmul_rn(y, c), __fmul_rn(x, s));
+  x = lo;
+  y = hi;
+}
+// rotates a unit's groups v[0, 8) and v[8, 16) by table row tp
+__device__ __forceinline__ void turn16(float* v, int u, const Turn& r, int tp) {
+  const long long at = (long long)tp * (r.dim / 2) + 8 * u;
+  const float4* ct = reinterpret_cast<const float4*>(r.cos + at);
+  const float4* st = reinterpret_cast<const float4*>(r.sin + at);
+  const float4 c0 = __ldg(ct), c1 = __ldg(ct + 1), s0 = __ldg(st), s1 = __ldg(st + 1);
+  const float c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+  if (r.interleaved) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const float4 x = __ldg(ct + i), y = __ldg(st + i);
-    c[4 * i] = x.x; c[4 * i + 1] = x.y; c[4 * i + 2] = x.z; c[4 * i + 3] = x.w;
-    s[4 * i] = y.x; s[4 * i + 1] = y.y; s[4 * i + 2] = y.z; s[4 * i + 3] = y.w;
-  }
+    for (int i = 0; i < 8; ++i) turn2(v[2 * i], v[2 * i + 1], c[i], s[i]);
+  } else {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    float& x = r.interleaved ? (i < 4 ? a[2 * i] : b[2 * i - 8]) : a[i];
-    float& y = r.interleaved ? (i < 4 ? a[2 * i + 1] : b[2 * i - 7]) : b[i];
-    const float lo = __fsub_rn(__fmul_rn(x, c[i]), __fmul_rn(y, s[i])), hi = __fadd_rn(__fmul_rn(y, c[i]), __fmul_rn(x, s[i]));
-    x = lo;
-    y = hi;
+    for (int i = 0; i < 8; ++i) turn2(v[i], v[8 + i], c[i], s[i]);
   }
 }
 
@@ -202,7 +204,8 @@ __device__ __forceinline__ void turn8(float* a, float* b, int u, const Turn& r, 
 // A CTA takes `rows` new rows; where each goes stands in shared memory before its threads walk the units of their K and V.
 constexpr int AT = 256, MAX_ROWS = 16;
 template <typename T>
-__global__ void __launch_bounds__(AT) append_vec_kernel(const FaKvAppendParams p, const Pages pg, const int rows) {
+__global__ void __launch_bounds__(AT) append_vec_kernel(const FaKvAppendParams p, const Pages pg, const int rows, const Div per_row,
+                                                        const Div per_head) {
   __shared__ long long s_slot[MAX_ROWS];   // cache row, -1: none
   __shared__ int s_turn[MAX_ROWS];
   pdl_wait();
@@ -229,24 +232,31 @@ __global__ void __launch_bounds__(AT) append_vec_kernel(const FaKvAppendParams p
   }
   __syncthreads();
   const Turn r{p.cos, p.sin, p.rot_dim, p.rot_seqlen_ro, p.rot_interleaved};
-  const int per_head = p.dim / 16, per_row = 2 * p.heads * per_head;   // K's units, then V's
+  const bool is_k = blockIdx.y == 0;
+  const T* const src = (const T*)(is_k ? p.k : p.v);
+  T* const cache = (T*)(is_k ? p.Kc : p.Vc);
+  const long long row_step = is_k ? p.k_row : p.v_row, head_step = is_k ? p.k_head : p.v_head;
 #pragma unroll 4
-  for (int e = threadIdx.x; e < rows * per_row; e += AT) {
-    const int i = e / per_row, w = e % per_row, hu = w % (p.heads * per_head), h = hu / per_head, u = hu % per_head;
-    const bool is_k = w < p.heads * per_head;
-    const long long slot = s_slot[i], row = row0 + i;
+  for (int e = threadIdx.x; e < rows * (int)per_row.d; e += AT) {
+    const int i = per_row.of(e), w = e - i * per_row.d, h = per_head.of(w), u = w - h * per_head.d;
+    const long long slot = s_slot[i];
     if (slot < 0) continue;
-    const T* x = is_k ? (const T*)p.k + row * p.k_row + h * p.k_head : (const T*)p.v + row * p.v_row + h * p.v_head;
-    T* out = (T*)(is_k ? p.Kc : p.Vc) + (slot * p.heads + h) * p.dim;
-    const int tp = is_k ? s_turn[i] : -1;
+    const T* x = src + (row0 + i) * row_step + h * head_step;
+    T* out = cache + (slot * p.heads + h) * p.dim;
     int d1, d2;
-    groups_of(u, r, tp >= 0, d1, d2);
-    float a[8], b[8];
-    to_float8(load8(x + d1), a);
-    to_float8(load8(x + d2), b);
-    if (tp >= 0 && 16 * u < r.dim) turn8(a, b, u, r, tp);
-    store8(out + d1, a);
-    store8(out + d2, b);
+    groups_of(u, r, is_k, d1, d2);
+    const Raw8<T> a = load8(x + d1), b = load8(x + d2);
+    if (is_k && s_turn[i] >= 0 && 16 * u < r.dim) {
+      float v[16];
+      to_float8(a, v);
+      to_float8(b, v + 8);
+      turn16(v, u, r, s_turn[i]);
+      store8(out + d1, v);
+      store8(out + d2, v + 8);
+    } else {
+      store_raw(out + d1, a);
+      store_raw(out + d2, b);
+    }
   }
 }
 
@@ -286,135 +296,153 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return y;
 }
 
-// A warp holds 16 positions (an aligned group) of one head of K or V in registers: LP lanes a row, each one unit, 32 / LP
-// rows a pass.  The largest magnitude of a scale block comes from the row's lanes, then from the rows of the block: lanes, passes and,
-// where a block has more than 16 slots, the block's warps.  One read of the new rows, one write of the codes; earlier codes of the
-// first block are touched only where its scale grew.  The warps of a CTA take the heads of the same rows, which share
-// their cos / sin rows in L1.
-template <typename T, typename Q, int LP>
+// A warp holds 16 positions (an aligned group, within one page) of one head of K or V in registers: LP lanes a row, each one
+// unit, 32 / LP rows a pass.  The largest magnitude of a scale block comes from the row's lanes, then from the rows of the
+// block: lanes, passes and, where a block has more than 16 slots, the block's warps.  One read of the new rows, one write of the
+// codes; earlier codes of the first block are touched only where its scale grew.  The warps of a CTA take the heads of the
+// same rows, which share their cos / sin rows in L1.  BIG: a block has 16 slots or more, so a warp has one scale.
+template <typename T, typename Q, int LP, bool BIG>
 __global__ void __launch_bounds__(512, 1) append8_vec_kernel(const FaKvAppendParams p, const Pages pg, const long long slots) {
   constexpr int RPP = 32 / LP, PASS = 16 / RPP;
   constexpr bool KEEP = LP <= 8;                      // values stay in registers; rows of more than 128 are read again (from L1)
+  constexpr int NB = BIG ? 1 : PASS;                  // scales of a thread
   __shared__ float s_most[16];
   pdl_wait();
   pdl_trigger();
-  const int SB = p.block, wpb = SB > 16 ? SB / 16 : 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int units = (blockDim.x >> 5) / wpb;          // (slot, K or V, head) items of a CTA
-  const long long item = (long long)blockIdx.x * units + warp / wpb;
-  const int h = (int)(item % p.heads), gs = log2_of(max(SB, 16));
-  const bool is_k = (item / p.heads) % 2 == 0;
-  const long long slot = item / p.heads / 2;
+  const int SB = p.block, bs = log2_of(SB), gs = BIG ? bs : 4, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int ws = BIG ? bs - 4 : 0, in_block = warp & ((1 << ws) - 1);   // warps of a block; this one's place
+  const int units = (int)(blockDim.x >> 5) >> ws;     // (slot, K or V, head) items of a CTA
+  const unsigned item = blockIdx.x * units + (warp >> ws);
+  const int h = (int)(item % (unsigned)p.heads);
+  const bool is_k = ((item / (unsigned)p.heads) & 1) == 0;
+  const long long slot = item / (unsigned)p.heads / 2;
   const RowMap rm{p.cu_new, p.tokens, p.batch};
   // ---- positions [c0, c0 + 16) of this warp; new tokens are [n0, n1)
-  int z = 0, ctx = 0, n0 = 0, n1 = 0, c0 = 0;
+  int z = 0, n0 = 0, n1 = 0, c0 = 0;
+  long long row0 = 0;                                 // row of position 0, so to say
   if (slot < slots) {
     z = rm.seq_of_slot(slot, gs);
-    ctx = p.ctx_len[z];
-    if (ctx < 0) record(ERR_PAGE);
-    else {
-      const long long i = slot - ((rm.first(z) >> gs) + 2 * z);
-      c0 = (int)((((ctx >> gs) + i) << gs) + 16 * (warp % wpb));
-      n0 = ctx;
-      n1 = ctx + rm.count(z);
+    n0 = p.ctx_len[z];
+    if (n0 < 0) {
+      record(ERR_PAGE);
+      n0 = 0;
+    } else {
+      const long long first = rm.first(z);
+      c0 = (int)(((n0 >> gs) + slot - ((first >> gs) + 2 * z)) << gs) + 16 * in_block;
+      n1 = n0 + rm.count(z);
+      row0 = first - n0;
     }
   }
-  const bool any = n1 > n0 && c0 < n1 && c0 + 16 > n0;   // new tokens among them
+  const int block0 = c0 & ~(SB - 1);                  // first position of the block (of the warp's first block)
+  bool any = block0 < n1 && max(c0 + 16, block0 + SB) > n0;   // new tokens in the warp's blocks
+  const int blk = any ? pg.of(z, c0) : -1;
+  if (any && blk < 0) record(ERR_PAGE);
+  any = blk >= 0;
+
   const Turn r{p.cos, p.sin, p.rot_dim, p.rot_seqlen_ro, p.rot_interleaved};
-  const int u = lane % LP, per_head = p.dim / 16;
-  const bool mine = u < per_head;
-  const int blk0 = p.page >= 16 && n1 > n0 ? pg.of(z, c0) : -1;
-  auto page_of = [&](int pos) { return p.page >= 16 ? blk0 : pg.of(z, pos); };
-  // this lane's unit of the new token at pos, rotated; d1, d2: where its groups lie
-  auto load = [&](int pos, int& d1, int& d2, float* x) {
-    const long long row = rm.first(z) + pos - ctx;
-    const T* src = is_k ? (const T*)p.k + row * p.k_row + h * p.k_head : (const T*)p.v + row * p.v_row + h * p.v_head;
-    const int tp = turn_pos(p, z, pos - ctx, is_k);
-    groups_of(u, r, tp >= 0, d1, d2);
-    to_float8(load8(src + d1), x);
-    to_float8(load8(src + d2), x + 8);
-    if (tp >= 0 && 16 * u < r.dim) turn8(x, x + 8, u, r, tp);
+  const int u = lane % LP, rp = lane / LP;            // unit; row of a pass
+  const bool mine = any && u < p.dim / 16;
+  int d1, d2;
+  groups_of(u, r, is_k, d1, d2);
+  const long long row_step = is_k ? p.k_row : p.v_row;
+  const T* const src = (const T*)(is_k ? p.k : p.v) + (row0 + c0 + rp) * row_step + h * (is_k ? p.k_head : p.v_head);
+  const bool turn = is_k && p.cos && 16 * u < r.dim;
+  const int tp0 = turn && mine ? (p.rot_pos ? p.rot_pos[z] - n0 : 0) + c0 + rp : 0;   // table row of the first pass
+  auto fresh = [&](int i) { const int pos = c0 + i * RPP + rp; return mine && pos >= n0 && pos < n1; };
+  auto finish = [&](const Raw8<T>& a, const Raw8<T>& b, int i, float* v) {
+    to_float8(a, v);
+    to_float8(b, v + 8);
+    if (turn) {
+      const int tp = tp0 + i * RPP;
+      if (tp >= 0 && tp < r.rows) turn16(v, u, r, tp);
+      else record(ERR_ROTARY);
+    }
   };
-  int d1[PASS], d2[PASS];
-  float x[KEEP ? PASS : 1][16];
-  float most[PASS];
-  bool fresh[PASS];
+  float x[KEEP ? PASS : 1][16], most[NB];
 #pragma unroll
-  for (int i = 0; i < PASS; ++i) {
-    const int pos = c0 + i * RPP + lane / LP;
-    fresh[i] = any && pos >= n0 && pos < n1;
-    most[i] = 0.f;
-    d1[i] = d2[i] = 0;
-    if (fresh[i] && page_of(pos) < 0) {
-      record(ERR_PAGE);
-      fresh[i] = false;
-    }
-    if (fresh[i] && mine) {
-      float* const v = x[KEEP ? i : 0];
-      load(pos, d1[i], d2[i], v);
+  for (int i = 0; i < NB; ++i) most[i] = 0.f;
+  if constexpr (KEEP) {
+    Raw8<T> a[PASS], b[PASS];                         // all loads first
 #pragma unroll
-      for (int j = 0; j < 16; ++j) most[i] = max_nan(most[i], fabsf(v[j]));
-    }
+    for (int i = 0; i < PASS; ++i)
+      if (fresh(i)) {
+        a[i] = load8(src + i * RPP * row_step + d1);
+        b[i] = load8(src + i * RPP * row_step + d2);
+      }
+#pragma unroll
+    for (int i = 0; i < PASS; ++i)
+      if (fresh(i)) {
+        finish(a[i], b[i], i, x[i]);
+        float& m = most[BIG ? 0 : i];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) m = max_nan(m, fabsf(x[i][j]));
+      }
+  } else {
+#pragma unroll
+    for (int i = 0; i < PASS; ++i)
+      if (fresh(i)) {
+        finish(load8(src + i * RPP * row_step + d1), load8(src + i * RPP * row_step + d2), i, x[0]);
+        float& m = most[BIG ? 0 : i];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) m = max_nan(m, fabsf(x[0][j]));
+      }
   }
   // ---- the blocks' largest: lanes of a row, rows of a pass, passes, warps
 #pragma unroll
-  for (int i = 0; i < PASS; ++i) {
+  for (int i = 0; i < NB; ++i)
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1)
-      if (o < LP * SB) most[i] = max_nan(most[i], __shfl_xor_sync(~0u, most[i], o));
-  }
+      if (BIG || o < LP * SB) most[i] = max_nan(most[i], __shfl_xor_sync(~0u, most[i], o));
+  if constexpr (!BIG) {
 #pragma unroll
-  for (int o = 1; o < PASS; o <<= 1)
-    if (o * RPP < SB) {
+    for (int o = 1; o < PASS; o <<= 1)
+      if (o * RPP < SB) {
 #pragma unroll
-      for (int i = 0; i < PASS; ++i)
-        if (!(i & o)) most[i] = most[i | o] = max_nan(most[i], most[i | o]);
-    }
-  if (wpb > 1) {
+        for (int i = 0; i < PASS; ++i)
+          if (!(i & o)) most[i] = most[i | o] = max_nan(most[i], most[i | o]);
+      }
+  } else if (ws) {
     if (lane == 0) s_most[warp] = most[0];
     __syncthreads();
-    float a = 0.f;
-    for (int w = 0; w < wpb; ++w) a = max_nan(a, s_most[warp / wpb * wpb + w]);
-#pragma unroll
-    for (int i = 0; i < PASS; ++i) most[i] = a;
+    for (int w = 0; w < 1 << ws; ++w) most[0] = max_nan(most[0], s_most[(warp & ~((1 << ws) - 1)) + w]);
   }
-  // ---- scales, codes
+  // ---- scales
+  const int in_page = c0 & (p.page - 1);
+  float* const sc = (is_k ? p.Ks : p.Vs) + ((long long)max(blk, 0) * p.heads + h) * (p.page >> bs);
+  float s[NB], old[NB];
+#pragma unroll
+  for (int i = 0; i < NB; ++i) {
+    const int pos = c0 + i * RPP + rp, first = BIG ? block0 : pos & ~(SB - 1);
+    const bool touched = any && first < n1 && first + SB > n0;
+    old[i] = touched && first < n0 ? sc[(first & (p.page - 1)) >> bs] : 0.f;   // the block holds earlier tokens
+    s[i] = fmaxf(fmaxf(__fmul_rn(most[i], 1.f / Q::QMAX), MIN_SCALE), old[i]);
+    if (!(most[i] <= 3.402823466e38f) || isnan(old[i])) s[i] = __int_as_float(0x7fc00000);
+    if (!touched) s[i] = -1.f;
+  }
+  // ---- codes
   const long long step = (long long)p.heads * p.dim;
-  float* const scales = is_k ? p.Ks : p.Vs;
-  typename Q::T* const cache = (typename Q::T*)(is_k ? p.Kc : p.Vc);
-  const int bs = log2_of(SB);
-  float news[PASS];
-  int where[PASS];                                    // index of the block's scale within its page and head
+  typename Q::T* const out = (typename Q::T*)(is_k ? p.Kc : p.Vc) + ((long long)max(blk, 0) * p.page + in_page + rp) * step + (long long)h * p.dim;
 #pragma unroll
   for (int i = 0; i < PASS; ++i) {
-    const int pos = c0 + i * RPP + lane / LP, first = pos & ~(SB - 1);   // of its block
-    const bool touched = n1 > n0 && first < n1 && first + SB > n0;
-    const int blk = touched ? page_of(pos) : -1;
-    where[i] = (pos & (p.page - 1)) >> bs;
-    news[i] = 0.f;
-    if (blk < 0) continue;
-    float* const sc = scales + ((long long)blk * p.heads + h) * (p.page >> bs) + where[i];
-    const bool kept = first < n0;                     // the block holds earlier tokens
-    const float old = kept ? *sc : 0.f;
-    float s = fmaxf(__fmul_rn(most[i], 1.f / Q::QMAX), MIN_SCALE);
-    if (old > s) s = old;
-    if (!(most[i] <= 3.402823466e38f) || isnan(old)) s = __int_as_float(0x7fc00000);
-    news[i] = s;
-    typename Q::T* const out = cache + ((long long)blk * p.page + (pos & (p.page - 1))) * step + (long long)h * p.dim;
-    if (mine && fresh[i]) {
-      if (isnan(s)) {
-        *reinterpret_cast<uint2*>(out + d1[i]) = *reinterpret_cast<uint2*>(out + d2[i]) = make_uint2(0, 0);
-      } else {
-        const float inv = __frcp_rn(s);
+    const int pos = c0 + i * RPP + rp;
+    const float si = s[BIG ? 0 : i], was = old[BIG ? 0 : i];
+    typename Q::T* const o = out + i * RPP * step;
+    if (fresh(i)) {
+      uint2 c1 = make_uint2(0, 0), c2 = c1;
+      if (!isnan(si)) {
+        const float inv = __frcp_rn(si);
         float* const v = x[KEEP ? i : 0];
-        if constexpr (!KEEP) load(pos, d1[i], d2[i], v);
-        *reinterpret_cast<uint2*>(out + d1[i]) = codes8<Q>(v, inv);
-        *reinterpret_cast<uint2*>(out + d2[i]) = codes8<Q>(v + 8, inv);
+        if constexpr (!KEEP) finish(load8(src + i * RPP * row_step + d1), load8(src + i * RPP * row_step + d2), i, v);
+        c1 = codes8<Q>(v, inv);
+        c2 = codes8<Q>(v + 8, inv);
       }
-    } else if (mine && kept && pos < n0 && s > old) { // earlier token: onto the scale that grew (never where s is NaN)
-      const float ratio = __fdiv_rn(old, s);
+      *reinterpret_cast<uint2*>(o + d1) = c1;
+      *reinterpret_cast<uint2*>(o + d2) = c2;
+    } else if (mine && pos < n0 && was > 0.f && si > was) {   // earlier token: onto the scale that grew (never where it is NaN)
+      const float ratio = __fdiv_rn(was, si);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        uint2* const at = reinterpret_cast<uint2*>(out + 16 * u + 8 * j);
+        uint2* const at = reinterpret_cast<uint2*>(o + 16 * u + 8 * j);
         float v[8];
         values8<Q>(*at, v);
         *at = codes8<Q>(v, ratio);
@@ -422,27 +450,49 @@ __global__ void __launch_bounds__(512, 1) append8_vec_kernel(const FaKvAppendPar
     }
   }
   // every reader of the old scale is done before the new one is written
-  if (wpb > 1) __syncthreads();
+  if (BIG && ws) __syncthreads();
   else __syncwarp();
 #pragma unroll
-  for (int i = 0; i < PASS; ++i) {
-    const int pos = c0 + i * RPP + lane / LP;
-    if (news[i] != 0.f && u == 0 && (pos & (SB - 1)) == 0)
-      scales[((long long)page_of(pos) * p.heads + h) * (p.page >> bs) + where[i]] = news[i];
+  for (int i = 0; i < NB; ++i) {
+    const int pos = c0 + i * RPP + rp;
+    if (s[i] == -1.f || (BIG ? lane != 0 || c0 != block0 : u != 0 || (pos & (SB - 1)) != 0)) continue;
+    sc[(pos & (p.page - 1)) >> bs] = s[i];
   }
 }
 
 // ---------------------------------------------------------------- gather
-// A CTA takes `rows` rows; a thread makes 16 bytes of the output at a time (8 or 4 elements), K's and then V's.
+// A CTA takes `rows` rows of K or of V; a thread makes 32 bytes of the output at a time (16 or 8 elements).
 constexpr int GT = 256;
+struct __align__(32) Out32 { uint32_t u[8]; };
+__device__ __forceinline__ void store32(void* o, const Out32& v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(o), "r"(v.u[0]), "r"(v.u[1]), "r"(v.u[2]),
+               "r"(v.u[3]), "r"(v.u[4]), "r"(v.u[5]), "r"(v.u[6]), "r"(v.u[7]) : "memory");
+}
+// values of 4 codes in a word, times s
+template <typename Q>
+__device__ __forceinline__ void values4(uint32_t w, float s, float* v) {
+  if constexpr (std::is_same<Q, I8>::value) {
+    const uint32_t x = w ^ 0x80808080u;   // c + 128 as the low byte of 2^23 + (c + 128)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v[i] = __fmul_rn(__fsub_rn(__uint_as_float(__byte_perm(x, 0x4B000000u, 0x7440 + i)), 8388736.f), s);
+  } else {
+    uint32_t a, b;
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+        : "=r"(a), "=r"(b) : "r"(w));
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a)), g = __half22float2(*reinterpret_cast<const __half2*>(&b));
+    v[0] = __fmul_rn(f.x, s); v[1] = __fmul_rn(f.y, s); v[2] = __fmul_rn(g.x, s); v[3] = __fmul_rn(g.y, s);
+  }
+}
 template <typename T, typename C, bool SCALED>
-__global__ void __launch_bounds__(GT) gather_kernel(const FaKvGatherParams p, const Pages pg, const int rows) {
+__global__ void __launch_bounds__(GT) gather_kernel(const FaKvGatherParams p, const Pages pg, const int rows, const Div per_row,
+                                                    const Div per_head) {
   __shared__ long long s_slot[MAX_ROWS], s_scale[MAX_ROWS];   // cache row; scale of its head 0
-  constexpr int N = 16 / sizeof(T);
+  constexpr int N = 32 / sizeof(T);
   pdl_wait();
   pdl_trigger();
   const long long row0 = (long long)blockIdx.x * rows;
-  const int per_page = SCALED ? p.page / p.block : 1;
+  const int bs = SCALED ? log2_of(p.block) : 0, per_page = p.page >> bs;
   if (threadIdx.x < rows) {
     const long long row = row0 + threadIdx.x;
     const RowMap rm{p.cu_k, 0, p.batch};
@@ -455,7 +505,7 @@ __global__ void __launch_bounds__(GT) gather_kernel(const FaKvGatherParams p, co
         else {
           const int in_page = pos & (p.page - 1);
           slot = (long long)blk * p.page + in_page;
-          sc = (long long)blk * p.heads * per_page + (SCALED ? in_page / p.block : 0);
+          sc = (long long)blk * p.heads * per_page + (in_page >> bs);
         }
       }
     }
@@ -463,34 +513,40 @@ __global__ void __launch_bounds__(GT) gather_kernel(const FaKvGatherParams p, co
     s_scale[threadIdx.x] = sc;
   }
   __syncthreads();
-  const int per_row = p.heads * p.dim / N, live = (int)min((long long)rows, p.total - row0);
+  const int n = (int)min((long long)rows, p.total - row0) * per_row.d;
   const bool is_v = blockIdx.y;
   const void* const cache = is_v ? p.Vc : p.Kc;
   const float* const scales = is_v ? p.Vs : p.Ks;
   T* const out = (T*)(is_v ? p.v : p.k) + row0 * p.heads * p.dim;
 #pragma unroll 4
-  for (int e = threadIdx.x; e < live * per_row; e += GT) {
-    const int i = e / per_row, w = e - i * per_row;
-    const long long slot = s_slot[i];
-    uint4 u = make_uint4(0, 0, 0, 0);
-    T* const o = reinterpret_cast<T*>(&u);
+  for (int e = threadIdx.x; e < n; e += GT) {
+    const int i = per_row.of(e), w = e - i * per_row.d;
+    const long long slot = s_slot[i], at = slot * p.heads * p.dim + w * N;
+    Out32 o = {};
+    T* const t = reinterpret_cast<T*>(&o);
     if (slot >= 0) {
-      const long long at = slot * p.heads * p.dim + (long long)w * N;
-      if constexpr (SCALED) {
-        const float s = __ldg(scales + s_scale[i] + w * N / p.dim * per_page);
-        typename C::T c[N];
-        if constexpr (N == 8) *reinterpret_cast<uint2*>(c) = __ldg(reinterpret_cast<const uint2*>((const unsigned char*)cache + at));
-        else *reinterpret_cast<uint32_t*>(c) = __ldg(reinterpret_cast<const uint32_t*>((const unsigned char*)cache + at));
-#pragma unroll
-        for (int j = 0; j < N; ++j) o[j] = Elem<T>::from_f(C::to_f(c[j]) * s);
-      } else if constexpr (std::is_same<T, C>::value) {
-        u = __ldg(reinterpret_cast<const uint4*>((const C*)cache + at));
+      if constexpr (std::is_same<T, C>::value) {
+        const uint4* x = reinterpret_cast<const uint4*>((const C*)cache + at);
+        reinterpret_cast<uint4*>(&o)[0] = __ldg(x);
+        reinterpret_cast<uint4*>(&o)[1] = __ldg(x + 1);
       } else {
+        float v[N];
+        if constexpr (SCALED) {
+          const float s = __ldg(scales + s_scale[i] + per_head.of(w) * per_page);
+          uint32_t c[N / 4];
+          if constexpr (N == 16) *reinterpret_cast<uint4*>(c) = __ldg(reinterpret_cast<const uint4*>((const unsigned char*)cache + at));
+          else *reinterpret_cast<uint2*>(c) = __ldg(reinterpret_cast<const uint2*>((const unsigned char*)cache + at));
 #pragma unroll
-        for (int j = 0; j < N; ++j) o[j] = Elem<T>::from_f(Elem<C>::to_f(((const C*)cache)[at + j]));
+          for (int j = 0; j < N / 4; ++j) values4<C>(c[j], s, v + 4 * j);
+        } else {
+#pragma unroll
+          for (int j = 0; j < N; j += 8) to_float8(load8((const C*)cache + at + j), v + j);
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j) t[j] = Elem<T>::from_f(v[j]);
       }
     }
-    *reinterpret_cast<uint4*>(out + (long long)e * N) = u;
+    store32(out + (long long)e * N, o);
   }
 }
 
@@ -508,8 +564,8 @@ bool cache_ok(const P& p, const char* who) {
                   p.max_blocks, p.num_blocks);
     return false;
   }
-  if (!(p.batch >= 0 && p.heads > 0)) {
-    fa::set_error("%s: batch=%d heads=%d", who, p.batch, p.heads);
+  if (!(p.batch >= 0 && p.heads > 0 && p.heads <= 256)) {
+    fa::set_error("%s: batch=%d heads=%d (up to 256)", who, p.batch, p.heads);
     return false;
   }
   const bool scaled = p.code == FA_CODE_I8 || p.code == FA_CODE_E4M3;
@@ -540,17 +596,19 @@ Pages pages_of(const P& p) {
 
 template <typename T, typename Q>
 cudaError_t append8(const FaKvAppendParams& p, const Pages& pg, bool vec, cudaStream_t st) {
-  if (!vec) {
+  if (!vec || p.page < 16) {
     const long long slots = p.total / p.block + 2ll * p.batch, warps = slots * p.heads * 2;
     return fa::launch_pdl(append8_kernel<T, Q>, dim3((unsigned)((warps + 3) / 4)), dim3(128), 0, st, p, pg, slots);
   }
   const int group = std::max(p.block, 16), wpb = group / 16, warps = std::max(4, wpb), units = warps / wpb;
   const long long slots = p.total / group + 2ll * p.batch, items = slots * p.heads * 2;
   const dim3 grid((unsigned)((items + units - 1) / units)), block(32 * warps);
-  if (p.dim <= 32) return fa::launch_pdl(append8_vec_kernel<T, Q, 2>, grid, block, 0, st, p, pg, slots);
-  if (p.dim <= 64) return fa::launch_pdl(append8_vec_kernel<T, Q, 4>, grid, block, 0, st, p, pg, slots);
-  if (p.dim <= 128) return fa::launch_pdl(append8_vec_kernel<T, Q, 8>, grid, block, 0, st, p, pg, slots);
-  return fa::launch_pdl(append8_vec_kernel<T, Q, 16>, grid, block, 0, st, p, pg, slots);
+  const auto go = [&](auto kernel) { return fa::launch_pdl(kernel, grid, block, 0, st, p, pg, slots); };
+  const bool big = p.block >= 16;
+  if (p.dim <= 32) return big ? go(append8_vec_kernel<T, Q, 2, true>) : go(append8_vec_kernel<T, Q, 2, false>);
+  if (p.dim <= 64) return big ? go(append8_vec_kernel<T, Q, 4, true>) : go(append8_vec_kernel<T, Q, 4, false>);
+  if (p.dim <= 128) return big ? go(append8_vec_kernel<T, Q, 8, true>) : go(append8_vec_kernel<T, Q, 8, false>);
+  return big ? go(append8_vec_kernel<T, Q, 16, true>) : go(append8_vec_kernel<T, Q, 16, false>);
 }
 
 template <typename T>
@@ -567,8 +625,9 @@ int append(const FaKvAppendParams& p, cudaStream_t st) {
   } else if (p.code == FA_CODE_E4M3) {
     e = append8<T, E4M3>(p, pg, vec, st);
   } else if (vec) {
-    const int rows = rows_of_cta(p.total, MAX_ROWS);
-    e = fa::launch_pdl(append_vec_kernel<T>, dim3((unsigned)((p.total + rows - 1) / rows)), dim3(AT), 0, st, p, pg, rows);
+    const int rows = rows_of_cta(p.total * 2, MAX_ROWS);
+    e = fa::launch_pdl(append_vec_kernel<T>, dim3((unsigned)((p.total + rows - 1) / rows), 2), dim3(AT), 0, st, p, pg, rows,
+                       Div(p.heads * p.dim / 16), Div(p.dim / 16));
   } else {
     e = fa::launch_pdl(append_kernel<T, T>, dim3((unsigned)((p.total * p.heads * 2 + 3) / 4)), dim3(128), 0, st, p, pg);
   }
@@ -581,12 +640,14 @@ int gather(const FaKvGatherParams& p, cudaStream_t st) {
   const Pages pg = pages_of(p);
   const int rows = rows_of_cta(p.total * 2, MAX_ROWS);
   const dim3 grid((unsigned)((p.total + rows - 1) / rows), 2), block(GT);
-  cudaError_t e;
-  if (p.code == FA_CODE_I8) e = fa::launch_pdl(gather_kernel<T, I8, true>, grid, block, 0, st, p, pg, rows);
-  else if (p.code == FA_CODE_E4M3) e = fa::launch_pdl(gather_kernel<T, E4M3, true>, grid, block, 0, st, p, pg, rows);
-  else if (p.code == FA_DTYPE_F16) e = fa::launch_pdl(gather_kernel<T, __half, false>, grid, block, 0, st, p, pg, rows);
-  else if (p.code == FA_DTYPE_BF16) e = fa::launch_pdl(gather_kernel<T, __nv_bfloat16, false>, grid, block, 0, st, p, pg, rows);
-  else e = fa::launch_pdl(gather_kernel<T, float, false>, grid, block, 0, st, p, pg, rows);
+  constexpr int N = 32 / sizeof(T);
+  const Div per_row(p.heads * p.dim / N), per_head(p.dim / N);
+  const auto go = [&](auto kernel) { return fa::launch_pdl(kernel, grid, block, 0, st, p, pg, rows, per_row, per_head); };
+  const cudaError_t e = p.code == FA_CODE_I8      ? go(gather_kernel<T, I8, true>)
+                        : p.code == FA_CODE_E4M3  ? go(gather_kernel<T, E4M3, true>)
+                        : p.code == FA_DTYPE_F16  ? go(gather_kernel<T, __half, false>)
+                        : p.code == FA_DTYPE_BF16 ? go(gather_kernel<T, __nv_bfloat16, false>)
+                                                  : go(gather_kernel<T, float, false>);
   fa::count_launch();
   return fa::cuda_status(e, "kv gather launch");
 }
@@ -640,8 +701,8 @@ extern "C" FA_API int fa_kv_gather_launch(const FaKvGatherParams* pp, int dtype,
   if (!cache_ok(p, "kv gather")) return FA_ERR_INVALID;
   if (!dim_ok(p.dim, "kv gather")) return FA_ERR_UNSUPPORTED;
   FA_CHECK_ARG(p.total >= 0, "kv gather: total=%lld", p.total);
-  FA_CHECK_ARG(((uintptr_t)p.Kc | (uintptr_t)p.Vc | (uintptr_t)p.k | (uintptr_t)p.v) % 16 == 0,
-               "kv gather: Kc, Vc, k and v must be 16-byte aligned");
+  FA_CHECK_ARG(((uintptr_t)p.Kc | (uintptr_t)p.Vc) % 16 == 0 && ((uintptr_t)p.k | (uintptr_t)p.v) % 32 == 0,
+               "kv gather: Kc and Vc must be 16-byte, k and v 32-byte aligned");
   if (p.total == 0 || p.batch == 0) return FA_OK;
   if (p.total * p.heads >= 1ll << 31) {
     fa::set_error("kv gather: %lld rows of %d heads are more than one call takes", p.total, p.heads);
