@@ -41,6 +41,7 @@ using sm100::ex2;
 __device__ int g_dec8_error = 0;
 __device__ __forceinline__ void record(int bit) { atomicOr(&g_dec8_error, bit); }
 
+#define UNLIKELY(x) __builtin_expect(!!(x), 0)
 constexpr int ERR_WAIT = 32768;    // a copy's wait gave up
 constexpr float NONE = -1e30f;     // a running maximum that nothing has moved yet
 constexpr float LAZY = 8.f;        // a score may exceed the running maximum by 8 (base 2) before it is moved
@@ -279,10 +280,8 @@ __device__ __forceinline__ void store_n(void* o, int dtype, long long at, const 
   }
 }
 
-__device__ __forceinline__ void store_lse(const FaDec8Params& p, int z, long long row, int t, int head, float m, float l) {
-  if (!p.lse) return;
-  p.lse[p.cu_q ? head * p.total + row : ((long long)z * p.NH + head) * p.tokens + t] =
-      l == 0.f ? -INFINITY : (m + lg2(l)) * FA_LN2;
+__device__ __forceinline__ void store_lse(const FaDec8Params& p, long long row, int head, float m, float l) {
+  if (p.lse) p.lse[head * p.total + row] = l == 0.f ? -INFINITY : (m + lg2(l)) * FA_LN2;
 }
 
 struct Cut {   // the sequence whose strips begin in a warp's range and end in a later one
@@ -290,7 +289,7 @@ struct Cut {   // the sequence whose strips begin in a warp's range and end in a
 };
 
 // ---------------------------------------------------------------- the pass over the cache
-template <int W, typename Q, int RT>
+template <int W, typename Q, int RT, bool TMA>
 __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
     dec8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const FaDec8Params p,
                 const Pages pg, const int dtype, const int ranges) {
@@ -352,7 +351,7 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
   const uint32_t scales_u = sm100::smem_u32(scales) + lane * 4;
   const int bshift = log2_of(p.block), per_page = p.page >> bshift;
   const int run = min(p.page, ST);                  // slots of a box
-  const bool tma = p.page >= 16;
+  const bool two = run < ST;                        // a page is half a strip
   // the thread's pieces within K or V of a stage
   const auto piece = [](int row, int i) { return row * C::ROW + (C::ROW == 128 ? (i ^ (row & 7)) : (i ^ ((row >> 1) & 3))) * 16; };
   const int kat = piece(col_pos(g), t4);
@@ -389,11 +388,6 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
     // What no row sees is not read: its weights are 0, and its V rows are cleared where they are used.  The pages of
     // the next strip (two where a page is half a strip) are looked up an issue ahead.
     int b0 = pg.of(z, (sq.s0 + k0) * ST), b1 = run < ST ? pg.of(z, (sq.s0 + k0) * ST + run) : b0;
-    auto box = [&](int pos, int b) {                // do rows see something of the slots [pos, pos + run) in page b
-      if (pos + run <= sq.lo || pos >= sq.L) return false;
-      if (b < 0) record(ERR_PAGE);
-      return b >= 0;
-    };
     auto load = [&](int r, int slot, int to) {
       const uint32_t bar = sm100::smem_u32(&s_full[warp][to]), dst = ring + to * C::STAGE_B + r * C::ROW;
 #pragma unroll
@@ -408,29 +402,26 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
     };
     auto issue = [&](int k, int to) {
       const int pos0 = (sq.s0 + k) * ST, in_page = pos0 & (p.page - 1);
-      const bool go0 = box(pos0, b0), go1 = run < ST && box(pos0 + run, b1);
+      // do rows see something of the slots of either page; are they there
+      const bool see0 = pos0 + run > sq.lo && pos0 < sq.L, see1 = two && pos0 + ST > sq.lo && pos0 + run < sq.L;
+      const bool go0 = see0 && b0 >= 0, go1 = see1 && b1 >= 0;
+      if (UNLIKELY(see0 != go0 || see1 != go1)) record(ERR_PAGE);
       if (lane == 0) {
-        unsigned have = 0, bytes = 0;
-        if (run == ST) {
-          have = go0 ? ALL : 0u;
-          bytes = go0 ? C::STAGE_B : 0;
-        } else {
-          have = (go0 ? 0xffffu : 0u) | (go1 ? 0xffff0000u : 0u);
-          bytes = (go0 + go1) * (C::STAGE_B / 2);
-        }
-        s_have[warp][to] = have;
-        sm100::mbar_expect_tx(sm100::smem_u32(&s_full[warp][to]), bytes);
+        const uint32_t half = (uint32_t)run * (2 * W);
+        s_have[warp][to] = (go0 ? (two ? 0xffffu : ALL) : 0u) | (go1 ? 0xffff0000u : 0u);
+        sm100::mbar_expect_tx(sm100::smem_u32(&s_full[warp][to]), (go0 ? half : 0) + (go1 ? half : 0));
         if (go0) load(0, b0 * p.page + in_page, to);
-        if (go1) load(run, b1 * p.page, to);
+        if (UNLIKELY(go1)) load(run, b1 * p.page, to);
       }
 #pragma unroll
       for (int i = 0; i < ST / 16; ++i) {
         const int e = lane + 32 * i, r = e % ST;
-        if (r < run ? go0 : go1) scale_to(e, r < run ? b0 : b1, (in_page + r) & (p.page - 1), to);
+        const bool first = ST == 16 || r < run;
+        if (first ? go0 : go1) scale_to(e, first ? b0 : b1, (in_page + r) & (p.page - 1), to);
       }
       if (in_page + ST >= p.page && k + 1 < k1) {
         b0 = pg.of(z, pos0 + ST);
-        if (run < ST) b1 = pg.of(z, pos0 + ST + run);
+        if (UNLIKELY(two)) b1 = pg.of(z, pos0 + ST + run);
       }
     };
     // Pages of less than 16 slots: the whole warp copies slot by slot, piece by piece, into the same places.
@@ -458,7 +449,7 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
     __syncwarp();                                   // the last piece's stages and q are free
     for (int i = 0, to = stage; i < STAGES; ++i) {
       if (k0 + i < k1) {
-        if (tma) issue(k0 + i, to);
+        if constexpr (TMA) issue(k0 + i, to);
         else issue_small(k0 + i, to);
       }
       cp_commit();
@@ -547,9 +538,8 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
     int k_lost = -1;
     for (int k = k0; k < k1; ++k) {
       cp_wait<STAGES - 1>();
-      if (!tma) {
-        __syncwarp();
-      } else if (!__all_sync(~0u, sm100::mbar_wait(sm100::smem_u32(&s_full[warp][stage]), parity))) {
+      __syncwarp();
+      if (TMA && UNLIKELY(!__all_sync(~0u, sm100::mbar_wait(sm100::smem_u32(&s_full[warp][stage]), parity)))) {
         record(ERR_WAIT);                           // copies that never land: give up (they are waited for below)
         k_lost = k;
         break;
@@ -600,7 +590,7 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
         for (int h = 0; h < RPT; ++h)
           x[h][i] = (RT == 8 ? s[i >> 1][i & 1] + s[i >> 1][2 + (i & 1)] : s[i >> 1][2 * h + (i & 1)]) * (ks * qf[h]);
       }
-      if (!plain) {
+      if (UNLIKELY(!plain)) {
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
           const int r = 8 * (i >> 1) + col_pos(2 * t4 + (i & 1)), pos = pos0 + r;
@@ -617,7 +607,7 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
       bool move = false;
 #pragma unroll
       for (int r = 0; r < RPT; ++r) move |= max_of(x[r]) > m[r] + LAZY;
-      if (__any_sync(~0u, move)) {
+      if (UNLIKELY(__any_sync(~0u, move))) {
 #pragma unroll
         for (int r = 0; r < RPT; ++r) {
           const float was = m[r], f = ex2(was - raise(m[r], x[r]));
@@ -635,13 +625,13 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
           l[r] += e;
           w[r][i] = e * vs[i];
         }
-        if (!plain)
+        if (UNLIKELY(!plain))
 #pragma unroll
           for (int i = 0; i < NP; ++i)
             if (x[r][i] == -INFINITY) w[r][i] = 0.f;   // whatever the scale is
         move |= max_of(w[r]) * up[r] > MOST;
       }
-      if (__any_sync(~0u, move)) {
+      if (UNLIKELY(__any_sync(~0u, move))) {
 #pragma unroll
         for (int r = 0; r < RPT; ++r) {
           float most = 0.f;
@@ -674,7 +664,7 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
         // anything, and 0 * NaN is not 0
         const unsigned char* const vsrc = src + C::HALF_B + b * 16 * C::ROW;
         unsigned hidden = 0;
-        if (!plain) {
+        if (UNLIKELY(!plain)) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int r = 16 * b + 8 * (j >> 1) + col_pos(2 * t4 + (j & 1));
@@ -688,7 +678,7 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             v[j] = *reinterpret_cast<const Piece*>(vsrc + c * (ST * 128) + ((j & 1) ? vat1 : vat0) + (j >> 1) * 8 * C::ROW);
-          if (hidden) {
+          if (UNLIKELY(hidden)) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
               if ((hidden >> j) & 1) v[j] = Piece{};
@@ -709,7 +699,7 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
 
       __syncwarp();                                 // every lane has read the stage
       if (k + STAGES < k1) {
-        if (tma) issue(k + STAGES, stage);
+        if constexpr (TMA) issue(k + STAGES, stage);
         else issue_small(k + STAGES, stage);
       }
       cp_commit();
@@ -738,7 +728,7 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
       if (tok >= sq.n) continue;
       if (t4 == 0) {
         if (whole_seq) {
-          store_lse(p, z, sq.first + tok, tok, head, m[r], l[r]);
+          store_lse(p, sq.first + tok, head, m[r], l[r]);
         } else {
           slot[g + 8 * r] = m[r];
           slot[RT + g + 8 * r] = l[r];
@@ -859,7 +849,7 @@ __global__ void __launch_bounds__(MW * 32)
       else if (dtype == FA_DTYPE_F16) ((__half*)p.o)[at] = __float2half_rn(x);
       else ((float*)p.o)[at] = x;
     }
-    if (tid == 0) store_lse(p, cut.z, sq.first + tok, tok, head, m, l);
+    if (tid == 0) store_lse(p, sq.first + tok, head, m, l);
     __syncthreads();
   }
 }
@@ -894,21 +884,25 @@ int map_of(CUtensorMap* m, const void* base, const FaDec8Params& p, int row, int
   return FA_ERR_CUDA;
 }
 
-template <int W, typename Q, int RT>
+template <int W, typename Q, int RT, bool TMA>
 int launch(const FaDec8Params& p, int dtype, cudaStream_t st) {
   using C = Cfg<W, RT>;
   static unsigned long long done = 0;
-  if (int rc = fa::ensure_smem((const void*)dec8_kernel<W, Q, RT>, C::SMEM, &done)) return rc;
+  if (int rc = fa::ensure_smem((const void*)dec8_kernel<W, Q, RT, TMA>, C::SMEM, &done)) return rc;
   CUtensorMap mk, mv;
   if (int rc = map_of(&mk, p.Kc, p, C::ROW, C::ST)) return rc;
   if (int rc = map_of(&mv, p.Vc, p, C::ROW, C::ST)) return rc;
   const Pages pg{p.block_table, log2_of(p.page), p.max_blocks, p.num_blocks};
-  const int NKV = p.NH / p.gqa, grid = fa::num_sms() * C::CTAS, warps = grid * C::NW;
-  const int ranges = std::max(1, warps / NKV), need = (ranges * NKV + C::NW - 1) / C::NW;
-  cudaError_t e = fa::launch_pdl(dec8_kernel<W, Q, RT>, dim3(need), dim3(C::NW * 32), C::SMEM, st, mk, mv, p, pg, dtype, ranges);
+  const int NKV = p.NH / p.gqa, warps = fa::num_sms() * C::CTAS * C::NW;
+  // no more ranges than the block table's width allows strips for: a small call then starts and joins few warps
+  const long long tiles = ((long long)(p.cu_q ? p.max_tokens : p.tokens) * p.gqa + RT - 1) / RT;
+  const long long strips = p.batch * tiles * (((long long)p.max_blocks * p.page + C::ST - 1) / C::ST);
+  const int ranges = (int)std::max(1ll, std::min<long long>(warps / NKV, (strips + MIN_STRIPS - 1) / MIN_STRIPS));
+  const int need = (ranges * NKV + C::NW - 1) / C::NW;
+  cudaError_t e = fa::launch_pdl(dec8_kernel<W, Q, RT, TMA>, dim3(need), dim3(C::NW * 32), C::SMEM, st, mk, mv, p, pg, dtype, ranges);
   fa::count_launch();
   if (int rc = fa::cuda_status(e, "8-bit decode launch")) return rc;
-  e = fa::launch_pdl(dec8_merge_kernel<W, RT>, dim3(2 * fa::num_sms()), dim3(MW * 32),
+  e = fa::launch_pdl(dec8_merge_kernel<W, RT>, dim3(std::min(2 * fa::num_sms(), ranges * NKV * RT)), dim3(MW * 32),
                                        (size_t)ranges * NKV * sizeof(int), st, p, pg, dtype, ranges);
   fa::count_launch();
   return fa::cuda_status(e, "8-bit decode merge launch");
@@ -918,7 +912,8 @@ template <int W, typename Q>
 int by_rows(const FaDec8Params& p, int dtype, cudaStream_t st) {
   // more than 8 rows share one pass over the cache; fp32 keeps to 8, whose q and weights have 22 bits
   const long long rows = (long long)p.gqa * (p.cu_q ? p.max_tokens : p.tokens);
-  return rows > 8 ? launch<W, Q, 16>(p, dtype, st) : launch<W, Q, 8>(p, dtype, st);
+  if (p.page < 16) return rows > 8 ? launch<W, Q, 16, false>(p, dtype, st) : launch<W, Q, 8, false>(p, dtype, st);
+  return rows > 8 ? launch<W, Q, 16, true>(p, dtype, st) : launch<W, Q, 8, true>(p, dtype, st);
 }
 template <typename Q>
 int by_dim(const FaDec8Params& p, int dtype, cudaStream_t st) {

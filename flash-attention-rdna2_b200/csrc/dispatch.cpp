@@ -393,7 +393,11 @@ const torch::Tensor* opt_ptr(const c10::optional<torch::Tensor>& t) { return t.h
 // an integer index tensor as contiguous int32 on `dev` (itself where it is that already)
 torch::Tensor index_i32(const torch::Tensor& t, const torch::Device& dev, const char* name) {
   TORCH_CHECK_VALUE(!t.is_floating_point() && t.scalar_type() != torch::kBool, "fable_attn: ", name, " must be integers");
+  if (t.scalar_type() == torch::kInt32 && t.device() == dev && t.is_contiguous()) return t;
   return t.to(dev, torch::kInt32).contiguous();
+}
+torch::Tensor table_f32(const torch::Tensor& t) {
+  return t.scalar_type() == torch::kFloat32 && t.is_contiguous() ? t : t.to(torch::kFloat32).contiguous();
 }
 
 // The cache's side of a parameter block: k_cache / v_cache (num_blocks, page, nheads_k, headdim) with the scales
@@ -453,8 +457,8 @@ void set_rotary(P& p, const c10::optional<torch::Tensor>& cos, const c10::option
                         hc->size(0) > 0 && 2 * hc->size(1) <= p.dim,
                     "fable_attn: rotary_cos / rotary_sin must be (seqlen_ro, rotary_dim / 2) on the cache's device with "
                     "rotary_dim <= headdim");
-  c = hc->to(torch::kFloat32).contiguous();
-  s = hs->to(torch::kFloat32).contiguous();
+  c = table_f32(*hc);
+  s = table_f32(*hs);
   p.cos = c.data_ptr<float>();
   p.sin = s.data_ptr<float>();
   p.rot_dim = (int)c.size(1) * 2;
@@ -598,9 +602,7 @@ std::vector<torch::Tensor> dec8(torch::Tensor q, torch::Tensor k_cache, torch::T
   p.ctx_len = lens.data_ptr<int>();
   auto out = torch::empty(q.sizes(), q.options());
   torch::Tensor lse;
-  if (return_lse)
-    lse = cu ? torch::empty({Hq, p.total}, q.options().dtype(torch::kFloat32))
-             : torch::empty({q.size(0), Hq, q.size(1)}, q.options().dtype(torch::kFloat32));
+  if (return_lse) lse = torch::empty({Hq, p.total}, q.options().dtype(torch::kFloat32));
   auto scratch = torch::empty({fa_decode8_scratch_floats(p.NH, p.gqa, p.dim)}, q.options().dtype(torch::kFloat32));
   p.o = out.data_ptr();
   p.lse = return_lse ? lse.data_ptr<float>() : nullptr;
@@ -608,7 +610,9 @@ std::vector<torch::Tensor> dec8(torch::Tensor q, torch::Tensor k_cache, torch::T
   p.scale = (float)scale; p.softcap = (float)softcap;
   p.win_left = (int)win_left; p.win_right = (int)win_right;
   if (p.total > 0) check(fa_decode8_launch(&p, dt_of(q), cur_stream(q)), "decode (8-bit cache)");
-  return return_lse ? std::vector<torch::Tensor>{out, lse} : std::vector<torch::Tensor>{out};
+  if (!return_lse) return {out};
+  if (!cu) lse = lse.view({Hq, q.size(0), q.size(1)}).transpose(0, 1);   // (batch, nheads, seqlen_q)
+  return {out, lse};
 }
 
 // ------------------------------------------------------------------ combine

@@ -13,7 +13,7 @@ element's value is code * scale.  `new_cache_8bit` makes one.
 
 The reference has no counterpart: its caches hold the inputs' type and its FP8 arguments raise.
 headdim is a multiple of 16 up to 256.  All calls run on the current stream and read lengths and
-tables on the device, with no host synchronisation.
+tables on the device, with no host synchronisation.  None of them carries gradients.
 """
 import torch
 
@@ -35,7 +35,6 @@ def new_cache_8bit(num_blocks, page_block_size, nheads_k, headdim, dtype=torch.i
     return k, v, ks, vs
 
 
-@torch.no_grad()
 def kvcache_append(k, v, k_cache, v_cache, cache_seqlens, block_table, *, k_scale=None, v_scale=None,
                    cu_seqlens_new=None, rotary_cos=None, rotary_sin=None, rotary_interleaved=True,
                    rotary_seqlens=None):
@@ -56,7 +55,6 @@ def kvcache_append(k, v, k_cache, v_cache, cache_seqlens, block_table, *, k_scal
                  rotary_sin, bool(rotary_interleaved), rotary_seqlens)
 
 
-@torch.no_grad()
 def kvcache_gather(k_cache, v_cache, block_table, cu_seqlens_k, total_k, *, k_scale=None, v_scale=None,
                    seq_starts=None, dtype=None):
     """(k, v), each (total_k, nheads_k, headdim): of sequence b the positions seq_starts[b] + i (0 + i without
@@ -67,7 +65,6 @@ def kvcache_gather(k_cache, v_cache, block_table, cu_seqlens_k, total_k, *, k_sc
                               dtype))
 
 
-@torch.no_grad()
 def flash_attn_with_kvcache_8bit(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block_table, softmax_scale=None,
                                  causal=True, window_size=(-1, -1), softcap=0.0, alibi_slopes=None, *,
                                  cu_seqlens_q=None, max_seqlen_q=None, cache_leftpad=None, rotary_cos=None,

@@ -361,7 +361,7 @@ FA_API int fa_kv_gather_launch(const FaKvGatherParams* p, int dtype, void* strea
  * then alibi slope * (key - pos), as in the forward; cos / sin rotate q by its position (or rot_pos[z] + t).
  * A row that sees nothing gives 0 and LSE -inf.
  *   o    [total, NH, dim] contiguous, dtype of the call (fp16 / bf16 / fp32)
- *   lse  optional fp32, natural log: dense [batch, NH, tokens], with cu_q [NH, total]
+ *   lse  optional fp32 [NH, total], natural log
  *   scratch  fa_decode8_scratch_floats(NH, gqa, dim) floats, whatever the batch or the lengths
  * max_tokens is a bound on n_z (dense: ignored).  The result does not depend on it, the choice of
  * kernel does. */
@@ -473,7 +473,7 @@ FA_API const char* fa_last_error(void);       /* message of the last failing cal
 /* Error bits recorded on the device (0 = none).  A bounded wait in a tensor-core kernel that
  * times out records a bit here and the kernel unwinds instead of hanging (its outputs are then
  * not valid); bits 1024 / 4096 / 256 flag a paged-K/V entry outside the cache and a rotary
- * position outside the cos/sin table (8192 / 16384 in the 8-bit cache operators).  Synchronous (device -> host copy); clear != 0 resets the
+ * position outside the cos/sin table (8192 / 16384 in the 8-bit cache operators, where 32768 is a copy whose wait gave up).  Synchronous (device -> host copy); clear != 0 resets the
  * bits.  No counterpart in the reference (its kernels have no waits that can give up). */
 FA_API int fa_device_error(int clear);
 /* Bit of fa_device_error set by fa_wait_selftest. */
