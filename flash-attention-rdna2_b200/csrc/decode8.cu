@@ -47,14 +47,14 @@ constexpr float NONE = -1e30f;     // a running maximum that nothing has moved y
 constexpr float LAZY = 8.f;        // a score may exceed the running maximum by 8 (base 2) before it is moved
 constexpr int LIFT = 6;            // weights are brought to [2^6, 2^7) ...
 constexpr float MOST = 16384.f;    // ... when one exceeds 2^14: fp16 then reaches 2^-30 of the largest
-constexpr int MIN_STRIPS = 2;      // least strips of a range
+constexpr int MIN_STRIPS = 1;      // least strips of a range
 
 template <int W, int RT>
 struct Cfg {
   // positions of a strip, warps of a CTA, CTAs of an SM, stages: what 64 K registers and 227 KB of shared memory hold
   static constexpr int ST = RT == 8 && W <= 128 ? 32 : 16;
   static constexpr int NW = 4;
-  static constexpr int CTAS = W == 256 ? (RT == 16 ? 1 : 2) : RT == 16 ? 2 : W == 64 ? 4 : 2;
+  static constexpr int CTAS = W == 64 && RT == 8 ? 4 : 2;
   static constexpr int STAGES = RT == 8 ? 2 : W == 128 ? 3 : 4;
   static constexpr int JT = ST / 8;                                        // n tiles of S
   static constexpr int KS = W / 16;                                        // k steps of S
@@ -284,9 +284,12 @@ __device__ __forceinline__ void store_lse(const FaDec8Params& p, long long row, 
   if (p.lse) p.lse[head * p.total + row] = l == 0.f ? -INFINITY : (m + lg2(l)) * FA_LN2;
 }
 
-struct Cut {   // the sequence whose strips begin in a warp's range and end in a later one
-  int z, tile, parts, pad;
+struct Cut {   // the row tile of a sequence whose strips begin in a warp's range and end in a later one
+  long long first;   // the sequence's first row
+  int tile, rows;    // row tile; rows of a kv head in the sequence (tokens x query heads)
+  int parts, pad[3]; // ranges that it lies in; 0: none
 };
+static_assert(sizeof(Cut) == 32, "the slots behind the records are stored to 16 bytes at a time");
 
 // ---------------------------------------------------------------- the pass over the cache
 template <int W, typename Q, int RT, bool TMA>
@@ -339,7 +342,7 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
   if (range >= ranges) return;
   Cut* const cuts = reinterpret_cast<Cut*>(p.scratch);
   float* const slots = p.scratch + (long long)ranges * NKV * (sizeof(Cut) / 4) + (long long)gw * 2 * C::SLOT;
-  Cut cut{0, 0, 0, 0};
+  Cut cut{};
   const long long per = max((long long)MIN_STRIPS, (total + ranges - 1) / ranges);
   const long long begin = range * per, end = min(total, begin + per);
 
@@ -751,8 +754,9 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
         }
     }
     if (k0 == 0 && k1 < sq.strips) {   // goes on in the ranges that follow
-      cut.z = z;
+      cut.first = sq.first;
       cut.tile = tile;
+      cut.rows = sq.n * p.gqa;
       cut.parts = (int)((at + sq.strips - 1) / per - range) + 1;
     }
     at += k1 - k0;
@@ -767,89 +771,160 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
 }
 
 // ---------------------------------------------------------------- the join of cut sequences
-// A row of a cut sequence is one item; CTAs take items in turn, the warps of a CTA every eighth part.
-// Which warps' ranges a cut begins in stands in their records: every CTA lists them for itself (a few KB from
-// L2, in the same order everywhere), so that the items of one long sequence spread over the whole GPU.
-constexpr int MW = 8;
+// A row of a cut sequence and kv head is one item.  Which ranges a cut begins in stands in their records, the same for every kv
+// head: each CTA lists them for itself (a few KB from L2, in the same order everywhere).  Items of few parts, the rule in a batch,
+// are taken by a warp each; those of many, a long sequence's, by a CTA each, so that one sequence's items spread over the
+// whole GPU.  Either way an item takes two rounds of loads, all of each under way at once: the parts' maxima and
+// sums, a thread each, then their outputs.  (Every item by a CTA: 27 us of 128 for 48 sequences of 1-9k tokens.)
+constexpr int MW = 8, FEW = 16;
+template <int E>
+__device__ __forceinline__ void store_row(const FaDec8Params& p, int dtype, long long at, int d, const float* v) {
+  if (d >= p.dim) return;
+  at = at * p.dim + d;
+#pragma unroll
+  for (int e = 0; e < E; e += 2) {
+    if (dtype == FA_DTYPE_BF16) *reinterpret_cast<__nv_bfloat162*>((__nv_bfloat16*)p.o + at + e) = __floats2bfloat162_rn(v[e], v[e + 1]);
+    else if (dtype == FA_DTYPE_F16) *reinterpret_cast<__half2*>((__half*)p.o + at + e) = __floats2half2_rn(v[e], v[e + 1]);
+    else *reinterpret_cast<float2*>((float*)p.o + at + e) = make_float2(v[e], v[e + 1]);
+  }
+}
 template <int W, int RT>
-__global__ void __launch_bounds__(MW * 32)
-    dec8_merge_kernel(const FaDec8Params p, const Pages pg, const int dtype, const int ranges) {
+__global__ void __launch_bounds__(MW * 32) dec8_merge_kernel(const FaDec8Params p, const int dtype, const int ranges) {
   using C = Cfg<W, RT>;
-  extern __shared__ int s_cut[];                    // warps that a cut begins at
-  __shared__ int s_warp[MW];
-  __shared__ float s_l[MW], s_v[MW][W];
-  const int NKV = p.NH / p.gqa, warps = ranges * NKV, tid = threadIdx.x, w = tid / 32, lane = tid % 32;
+  extern __shared__ int s_cut[];                    // ranges that a cut begins in, few parts from the front, many from
+  float* const s_f = reinterpret_cast<float*>(s_cut + ranges);   // the back; the factors of an item's parts
+  __shared__ int s_few[MW], s_many[MW];
+  __shared__ float s_m[MW], s_l[MW];
+  __shared__ __align__(16) float s_v[MW][W];
+  const int NKV = p.NH / p.gqa, tid = threadIdx.x, w = tid / 32, lane = tid % 32;
   pdl_wait();
   pdl_trigger();
   const Cut* const cuts = reinterpret_cast<const Cut*>(p.scratch);
-  const int per = (warps + MW * 32 - 1) / (MW * 32), i0 = tid * per, i1 = min(warps, i0 + per);
-  int mine = 0;
-  for (int i = i0; i < i1; ++i) mine += cuts[i].parts > 0;
-  int inc = mine;
+  int few = 0, many = 0;
+  for (int base = 0; base < ranges; base += MW * 32) {
+    const int parts = base + tid < ranges ? cuts[(long long)(base + tid) * NKV].parts : 0;
+    const unsigned vf = __ballot_sync(~0u, parts > 0 && parts <= FEW), vm = __ballot_sync(~0u, parts > FEW);
+    if (lane == 0) {
+      s_few[w] = __popc(vf);
+      s_many[w] = __popc(vm);
+    }
+    __syncthreads();
+    const unsigned below = (1u << lane) - 1;
+    int af = few + __popc(vf & below), am = many + __popc(vm & below);
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(~0u, inc, o);
-    if (lane >= o) inc += v;
+    for (int i = 0; i < MW; ++i) {
+      if (i < w) {
+        af += s_few[i];
+        am += s_many[i];
+      }
+      few += s_few[i];
+      many += s_many[i];
+    }
+    if (parts > FEW) s_cut[ranges - 1 - am] = base + tid;
+    else if (parts > 0) s_cut[af] = base + tid;
+    __syncthreads();
   }
-  if (lane == 31) s_warp[w] = inc;
-  __syncthreads();
-  int count = 0, at0 = inc - mine;
-#pragma unroll
-  for (int i = 0; i < MW; ++i) {
-    if (i < w) at0 += s_warp[i];
-    count += s_warp[i];
-  }
-  if (mine)
-    for (int i = i0; i < i1; ++i)
-      if (cuts[i].parts > 0) s_cut[at0++] = i;
-  __syncthreads();
-  const float* const slots = p.scratch + (long long)warps * (sizeof(Cut) / 4);
+  const float* const slots = p.scratch + (long long)ranges * NKV * (sizeof(Cut) / 4);
   constexpr int E = W / 32;
-  for (int item = blockIdx.x; item < count * RT; item += gridDim.x) {
-    const int gw = s_cut[item / RT], r = item % RT;
+  // part 0 of a cut that begins in the range of warp gw: its second slot; part i: first slot of the warp i ranges on
+  auto part = [&](int gw, int i) { return slots + ((long long)(gw + i * NKV) * 2 + (i == 0)) * C::SLOT; };
+
+  for (int item = blockIdx.x * MW + w; item < few * NKV * RT; item += gridDim.x * MW) {
+    const int r = item % RT, kvh = item / RT % NKV, gw = s_cut[item / RT / NKV] * NKV + kvh;
     const Cut cut = cuts[gw];
-    const Seq sq = seq_of<RT, C::ST>(p, pg, cut.z);
-    const int row = cut.tile * RT + r, tok = row / p.gqa, head = gw % NKV * p.gqa + row % p.gqa;
-    if (tok >= sq.n) continue;
-    // part 0: second slot of warp gw; part i: first slot of the warp i ranges on
-    auto part = [&](int i) { return slots + ((long long)(gw + i * NKV) * 2 + (i == 0)) * C::SLOT; };
-    float m = NONE;
-    for (int i = lane; i < cut.parts; i += 32) m = fmaxf(m, part(i)[r]);
+    const int row = cut.tile * RT + r;
+    if (row >= cut.rows) continue;
+    float m = NONE, f = 0.f, l = 0.f, v[E];
+    if (lane < cut.parts) {
+      m = part(gw, lane)[r];
+      l = part(gw, lane)[RT + r];
+    }
+    float all = m;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-    float l = 0.f, v[E];
+    for (int o = 16; o; o >>= 1) all = fmaxf(all, __shfl_xor_sync(~0u, all, o));
+    if (lane < cut.parts) f = ex2(m - all);
+    l *= f;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] = 0.f;
 #pragma unroll 4
-    for (int i = w; i < cut.parts; i += MW) {
-      const float* s = part(i);
-      const float f = ex2(s[r] - m);
-      l = fmaf(s[RT + r], f, l);
+    for (int i = 0; i < cut.parts; ++i) {
+      const float* const o = part(gw, i) + 2 * RT + r * W + lane * E;
+      const float fi = __shfl_sync(~0u, f, i);
 #pragma unroll
       for (int e = 0; e < E; e += 2) {
-        const float2 u = *reinterpret_cast<const float2*>(s + 2 * RT + r * W + lane * E + e);
+        const float2 u = *reinterpret_cast<const float2*>(o + e);
+        v[e] = fmaf(u.x, fi, v[e]);
+        v[e + 1] = fmaf(u.y, fi, v[e + 1]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = l == 0.f ? 0.f : v[e] / l;
+    const int head = kvh * p.gqa + row % p.gqa;
+    store_row<E>(p, dtype, (cut.first + row / p.gqa) * p.NH + head, lane * E, v);
+    if (lane == 0) store_lse(p, cut.first + row / p.gqa, head, all, l);
+  }
+
+  for (int item = blockIdx.x; item < many * NKV * RT; item += gridDim.x) {
+    const int r = item % RT, kvh = item / RT % NKV, gw = s_cut[ranges - 1 - item / RT / NKV] * NKV + kvh;
+    const Cut cut = cuts[gw];
+    const int row = cut.tile * RT + r;
+    if (row >= cut.rows) continue;
+    float m = NONE;
+    for (int i = tid; i < cut.parts; i += MW * 32) {
+      s_f[i] = part(gw, i)[r];
+      m = fmaxf(m, s_f[i]);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+    if (lane == 0) s_m[w] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < MW; ++i) m = fmaxf(m, s_m[i]);
+    float l = 0.f;
+    for (int i = tid; i < cut.parts; i += MW * 32) {
+      const float f = ex2(s_f[i] - m);
+      s_f[i] = f;
+      l = fmaf(part(gw, i)[RT + r], f, l);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
+    if (lane == 0) s_l[w] = l;
+    __syncthreads();
+    float v[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = 0.f;
+#pragma unroll 8
+    for (int i = w; i < cut.parts; i += MW) {
+      const float* const o = part(gw, i) + 2 * RT + r * W + lane * E;
+      const float f = s_f[i];
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        const float2 u = *reinterpret_cast<const float2*>(o + e);
         v[e] = fmaf(u.x, f, v[e]);
         v[e + 1] = fmaf(u.y, f, v[e + 1]);
       }
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) s_v[w][lane * E + e] = v[e];
-    if (lane == 0) s_l[w] = l;
     __syncthreads();
     l = 0.f;
 #pragma unroll
     for (int i = 0; i < MW; ++i) l += s_l[i];
-    for (int d = tid; d < p.dim; d += MW * 32) {
-      float x = 0.f;
+    const int head = kvh * p.gqa + row % p.gqa;
+    for (int d = 2 * tid; d < p.dim; d += MW * 64) {
+      float x[2] = {0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < MW; ++i) x += s_v[i][d];
-      x = l == 0.f ? 0.f : x / l;
-      const long long at = ((sq.first + tok) * p.NH + head) * p.dim + d;
-      if (dtype == FA_DTYPE_BF16) ((__nv_bfloat16*)p.o)[at] = __float2bfloat16_rn(x);
-      else if (dtype == FA_DTYPE_F16) ((__half*)p.o)[at] = __float2half_rn(x);
-      else ((float*)p.o)[at] = x;
+      for (int i = 0; i < MW; ++i) {
+        x[0] += s_v[i][d];
+        x[1] += s_v[i][d + 1];
+      }
+      x[0] = l == 0.f ? 0.f : x[0] / l;
+      x[1] = l == 0.f ? 0.f : x[1] / l;
+      store_row<2>(p, dtype, (cut.first + row / p.gqa) * p.NH + head, d, x);
     }
-    if (tid == 0) store_lse(p, sq.first + tok, head, m, l);
+    if (tid == 0) store_lse(p, cut.first + row / p.gqa, head, m, l);
     __syncthreads();
   }
 }
@@ -902,18 +977,26 @@ int launch(const FaDec8Params& p, int dtype, cudaStream_t st) {
   cudaError_t e = fa::launch_pdl(dec8_kernel<W, Q, RT, TMA>, dim3(need), dim3(C::NW * 32), C::SMEM, st, mk, mv, p, pg, dtype, ranges);
   fa::count_launch();
   if (int rc = fa::cuda_status(e, "8-bit decode launch")) return rc;
-  e = fa::launch_pdl(dec8_merge_kernel<W, RT>, dim3(std::min(2 * fa::num_sms(), ranges * NKV * RT)), dim3(MW * 32),
-                                       (size_t)ranges * NKV * sizeof(int), st, p, pg, dtype, ranges);
+  e = fa::launch_pdl(dec8_merge_kernel<W, RT>, dim3(std::min(4 * fa::num_sms(), ranges * NKV * RT)), dim3(MW * 32),
+                                       (size_t)ranges * 8, st, p, dtype, ranges);
   fa::count_launch();
   return fa::cuda_status(e, "8-bit decode merge launch");
 }
 
+template <int W, typename Q, int RT>
+int by_page(const FaDec8Params& p, int dtype, cudaStream_t st) {
+  return p.page < 16 ? launch<W, Q, RT, false>(p, dtype, st) : launch<W, Q, RT, true>(p, dtype, st);
+}
 template <int W, typename Q>
 int by_rows(const FaDec8Params& p, int dtype, cudaStream_t st) {
-  // more than 8 rows share one pass over the cache; fp32 keeps to 8, whose q and weights have 22 bits
-  const long long rows = (long long)p.gqa * (p.cu_q ? p.max_tokens : p.tokens);
-  if (p.page < 16) return rows > 8 ? launch<W, Q, 16, false>(p, dtype, st) : launch<W, Q, 8, false>(p, dtype, st);
-  return rows > 8 ? launch<W, Q, 16, true>(p, dtype, st) : launch<W, Q, 8, true>(p, dtype, st);
+  // More than 8 rows a sequence: one pass over the cache with 16 rows, or tiles of 8 that each make a pass.  16 rows win
+  // where every sequence has them (16 x 16-32k tokens, 16 heads a kv head, headdim 128: 291 against 330 us); tiles win where
+  // counts are ragged, since most tiles of 16 are then half empty (1 to 4 tokens of 4 heads, 24 x 1-20k tokens: 124 against 104
+  // us), and for rows of 256, whose 16-row form has one warp a scheduler (16 x 1-9k tokens, 16 heads: 127 against 108 us).
+  const bool full = p.gqa > 8 || (!p.cu_q && (long long)p.gqa * p.tokens > 8);
+  if constexpr (W <= 128)
+    if (full) return by_page<W, Q, 16>(p, dtype, st);
+  return by_page<W, Q, 8>(p, dtype, st);
 }
 template <typename Q>
 int by_dim(const FaDec8Params& p, int dtype, cudaStream_t st) {
@@ -948,7 +1031,7 @@ extern "C" FA_API long long fa_decode8_scratch_floats(int NH, int gqa, int dim) 
   const int n = NH / gqa;
   if (dim <= 64) return std::max(scratch_of<64, 8>(n), scratch_of<64, 16>(n));
   if (dim <= 128) return std::max(scratch_of<128, 8>(n), scratch_of<128, 16>(n));
-  return std::max(scratch_of<256, 8>(n), scratch_of<256, 16>(n));
+  return scratch_of<256, 8>(n);
 }
 
 extern "C" FA_API int fa_decode8_launch(const FaDec8Params* pp, int dtype, void* stream) {
