@@ -43,7 +43,7 @@ __device__ __forceinline__ void record(int bit) { atomicOr(&g_dec8_error, bit); 
 
 #define UNLIKELY(x) __builtin_expect(!!(x), 0)
 constexpr int ERR_WAIT = 32768;    // a copy's wait gave up
-constexpr float NONE = -1e30f;     // a running maximum that nothing has moved yet
+constexpr float NONE = -1e30f;     // maximum of a part that saw nothing
 constexpr float LAZY = 8.f;        // a score may exceed the running maximum by 8 (base 2) before it is moved
 constexpr int LIFT = 6;            // weights are brought to [2^6, 2^7) ...
 constexpr float MOST = 16384.f;    // ... when one exceeds 2^14: fp16 then reaches 2^-30 of the largest
@@ -533,9 +533,9 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
     float o[NT][4];
 #pragma unroll
     for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m[RPT], l[RPT], up[RPT];
+    float m[RPT], above[RPT], l[RPT], up[RPT];      // above: how far over m a score moves it
 #pragma unroll
-    for (int r = 0; r < RPT; ++r) { m[r] = NONE; l[r] = 0.f; up[r] = pow2(126); }
+    for (int r = 0; r < RPT; ++r) { m[r] = l[r] = 0.f; above[r] = -INFINITY; up[r] = pow2(126); }
     const float cap_out = p.softcap * FA_LOG2E;
 
     int k_lost = -1;
@@ -578,7 +578,8 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
         }
       }
 
-      // ---- weights of positions pos0 + 8 j + col_pos(2 t4 + e), row g (+ 8 r), at [2 j + e]
+      // ---- weights of positions pos0 + 8 j + col_pos(2 t4 + e), row g (+ 8 r), at [2 j + e]; x: scores less m, rounded
+      // once (a score of 50 by itself is good to 2^-19 only, and so would its weight be)
       const int pos0 = (sq.s0 + k) * ST;
       const unsigned have = s_have[warp][stage];
       // every position seen by every row, and scores that are nothing but products
@@ -591,7 +592,7 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
         vs[i] = scales[stage * (2 * ST) + ST + r];
 #pragma unroll
         for (int h = 0; h < RPT; ++h)
-          x[h][i] = (RT == 8 ? s[i >> 1][i & 1] + s[i >> 1][2 + (i & 1)] : s[i >> 1][2 * h + (i & 1)]) * (ks * qf[h]);
+          x[h][i] = fmaf(RT == 8 ? s[i >> 1][i & 1] + s[i >> 1][2 + (i & 1)] : s[i >> 1][2 * h + (i & 1)], ks * qf[h], -m[h]);
       }
       if (UNLIKELY(!plain)) {
 #pragma unroll
@@ -599,23 +600,31 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
           const int r = 8 * (i >> 1) + col_pos(2 * t4 + (i & 1)), pos = pos0 + r;
 #pragma unroll
           for (int h = 0; h < RPT; ++h) {
-            float v = x[h][i];
+            float v = x[h][i] + m[h];
             if (cap) v = cap_out * fa_tanh(v);
             if (p.alibi) v = fmaf(slope[h], (float)pos - qpos[h], v);
             if (!(pos >= rlo[h] && pos < rhi[h] && ((have >> r) & 1))) v = -INFINITY;
-            x[h][i] = v;
+            x[h][i] = v - m[h];
           }
         }
       }
       bool move = false;
 #pragma unroll
-      for (int r = 0; r < RPT; ++r) move |= max_of(x[r]) > m[r] + LAZY;
+      for (int r = 0; r < RPT; ++r) move |= max_of(x[r]) > above[r];
       if (UNLIKELY(__any_sync(~0u, move))) {
 #pragma unroll
         for (int r = 0; r < RPT; ++r) {
-          const float was = m[r], f = ex2(was - raise(m[r], x[r]));
+          // the reference moves by what fp32 has room for, and everything else by the same
+          float top = above[r] == LAZY ? 0.f : -INFINITY;   // a row's first keys may lower it
+          raise(top, x[r]);
+          if (top == -INFINITY) continue;          // nothing seen yet
+          const float by = (m[r] + top) - m[r], f = ex2(-by);
+          m[r] += by;
+          above[r] = LAZY;
           l[r] *= f;
           scale_rows<NT, RT>(o, r, f);
+#pragma unroll
+          for (int i = 0; i < NP; ++i) x[r][i] -= by;
         }
       }
       float w[RPT][NP];
@@ -624,7 +633,7 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
       for (int r = 0; r < RPT; ++r) {
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
-          const float e = ex2(x[r][i] - m[r]);
+          const float e = ex2(x[r][i]);
           l[r] += e;
           w[r][i] = e * vs[i];
         }
@@ -733,7 +742,7 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
         if (whole_seq) {
           store_lse(p, sq.first + tok, head, m[r], l[r]);
         } else {
-          slot[g + 8 * r] = m[r];
+          slot[g + 8 * r] = above[r] == LAZY ? m[r] : NONE;
           slot[RT + g + 8 * r] = l[r];
         }
       }
