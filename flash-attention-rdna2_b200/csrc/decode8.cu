@@ -401,7 +401,7 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
     };
     auto scale_to = [&](int e, int b, int in_page, int to) {   // entry e of a stage's scales
       cp_async4(scales_u + to * C::SCALE_B + (e - lane) * 4,
-                (e < ST ? p.Ks : p.Vs) + (long long)(b * NKV + kvh) * per_page + (in_page >> bshift));
+                (e < ST ? p.Ks : p.Vs) + ((long long)b * NKV + kvh) * per_page + (in_page >> bshift));
     };
     auto issue = [&](int k, int to) {
       const int pos0 = (sq.s0 + k) * ST, in_page = pos0 & (p.page - 1);
@@ -582,8 +582,10 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
       // once (a score of 50 by itself is good to 2^-19 only, and so would its weight be)
       const int pos0 = (sq.s0 + k) * ST;
       const unsigned have = s_have[warp][stage];
-      // every position seen by every row, and scores that are nothing but products
-      const bool plain = have == ALL && pos0 >= all_lo && pos0 + ST <= all_hi;
+      // strips that every row sees whole, with scores that are nothing but products, run code without masks (16 x 16-32k
+      // int8 tokens: one form with branches 182 us, two forms 173; e4m3 165 and 160)
+      const auto weigh = [&](auto plain) {
+      constexpr bool PLAIN = decltype(plain)::value;
       float x[RPT][NP], vs[NP];
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
@@ -594,7 +596,7 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
         for (int h = 0; h < RPT; ++h)
           x[h][i] = fmaf(RT == 8 ? s[i >> 1][i & 1] + s[i >> 1][2 + (i & 1)] : s[i >> 1][2 * h + (i & 1)], ks * qf[h], -m[h]);
       }
-      if (UNLIKELY(!plain)) {
+      if constexpr (!PLAIN) {
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
           const int r = 8 * (i >> 1) + col_pos(2 * t4 + (i & 1)), pos = pos0 + r;
@@ -637,7 +639,7 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
           l[r] += e;
           w[r][i] = e * vs[i];
         }
-        if (UNLIKELY(!plain))
+        if constexpr (!PLAIN)
 #pragma unroll
           for (int i = 0; i < NP; ++i)
             if (x[r][i] == -INFINITY) w[r][i] = 0.f;   // whatever the scale is
@@ -676,7 +678,7 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
         // anything, and 0 * NaN is not 0
         const unsigned char* const vsrc = src + C::HALF_B + b * 16 * C::ROW;
         unsigned hidden = 0;
-        if (UNLIKELY(!plain)) {
+        if constexpr (!PLAIN) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int r = 16 * b + 8 * (j >> 1) + col_pos(2 * t4 + (j & 1));
@@ -708,6 +710,10 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
           }
         }
       }
+
+      };
+      if (have == ALL && pos0 >= all_lo && pos0 + ST <= all_hi) weigh(std::true_type{});
+      else weigh(std::false_type{});
 
       __syncwarp();                                 // every lane has read the stage
       if (k + STAGES < k1) {
