@@ -7,9 +7,10 @@
 // largest weight so far in fp16's range whatever the scales: the tensor cores take codes (exact in
 // fp16) and weights (fp16 high and low part, 22 bits) as they are, and dividing by u at the end is exact.
 //
-// Bound by the bytes of the cache.  What is read goes through registers to mma.sync (m16n8k16, fp16
+// The floor is the bytes of the cache.  What is read goes through registers to mma.sync (m16n8k16, fp16
 // operands, fp32 sums): with 8 query rows the tensor pipe has twice the time that the bytes need, and the conversion of codes
-// has to pass through registers anyway.  A strip is 32 (or 16) positions of one kv head.  Its K rows are the B operand of
+// has to pass through registers anyway (a tcgen05 form with the converted operands in tensor and shared memory: 343 against
+// 189 us at the time).  A strip is 32 (or 16) positions of one kv head.  Its K rows are the B operand of
 // S = Q K^T, its V rows that of O += W V.  The order of an mma's k index and of its n columns is free as long as both operands
 // agree, so each thread's operands are whole 16-byte pieces of cache rows (g = lane / 4, t = lane % 4):
 //   K  row at(g) (+ 8), pieces t + 4 i;      V  rows at(2 t), at(2 t + 1) (+ 8), piece g,
@@ -26,6 +27,12 @@
 // adjacent in memory, are read together.  A warp's range is cut at sequence ends; a piece that is a whole sequence
 // writes its output, others leave (m, l, o) in one of the warp's two slots, and a merge kernel joins the slots of each
 // cut sequence in order (no atomics: same bits on every call).
+//
+// Measured, both kernels: 16 x 16-32k tokens, 8 kv heads, headdim 128, one token of 32 heads (806 MB): int8 173 us
+// (4.7 TB/s), e4m3 160 us (5.0 TB/s); 48 x 1-9k e4m3 108 us (4.6 TB/s); one document of 131k 76 us (3.5 TB/s); 24 tables of 4k
+// with 1-4 tokens each 93 us; 1 x 900 12.5 us.  What bounds it: an SM holds 8 warps of 240 registers, whose conversions,
+// mma and softmax (135 us by themselves in the first case, before strips without masks had code of their own) and copies (141 us by themselves)
+// overlap only in part; DRAM is at 55 % of its peak, issue slots at 41 %.
 #include <cudaTypedefs.h>
 #include <algorithm>
 #include <type_traits>
@@ -47,11 +54,12 @@ constexpr float NONE = -1e30f;     // maximum of a part that saw nothing
 constexpr float LAZY = 8.f;        // a score may exceed the running maximum by 8 (base 2) before it is moved
 constexpr int LIFT = 6;            // weights are brought to [2^6, 2^7) ...
 constexpr float MOST = 16384.f;    // ... when one exceeds 2^14: fp16 then reaches 2^-30 of the largest
-constexpr int MIN_STRIPS = 1;      // least strips of a range
 
 template <int W, int RT>
 struct Cfg {
-  // positions of a strip, warps of a CTA, CTAs of an SM, stages: what 64 K registers and 227 KB of shared memory hold
+  // Positions of a strip, warps of a CTA, CTAs of an SM, stages: what 64 K registers and 227 KB of shared memory hold.
+  // Strips of 32 with 8 warps an SM against strips of 16 with 12: 173 and 188 us (16 x 16-32k int8), 108 and 134 us (48 x 1-9k
+  // e4m3), 12.5 and 12.3 us (1 x 900).
   static constexpr int ST = RT == 8 && W <= 128 ? 32 : 16;
   static constexpr int NW = 4;
   static constexpr int CTAS = W == 64 && RT == 8 ? 4 : 2;
@@ -343,7 +351,7 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
   Cut* const cuts = reinterpret_cast<Cut*>(p.scratch);
   float* const slots = p.scratch + (long long)ranges * NKV * (sizeof(Cut) / 4) + (long long)gw * 2 * C::SLOT;
   Cut cut{};
-  const long long per = max((long long)MIN_STRIPS, (total + ranges - 1) / ranges);
+  const long long per = max(1ll, (total + ranges - 1) / ranges);
   const long long begin = range * per, end = min(total, begin + per);
 
   const uint32_t base = (sm100::smem_u32(smem_raw) + 1023u) & ~1023u, ring = base + warp * C::RING_B;
@@ -987,7 +995,7 @@ int launch(const FaDec8Params& p, int dtype, cudaStream_t st) {
   // no more ranges than the block table's width allows strips for: a small call then starts and joins few warps
   const long long tiles = ((long long)(p.cu_q ? p.max_tokens : p.tokens) * p.gqa + RT - 1) / RT;
   const long long strips = p.batch * tiles * (((long long)p.max_blocks * p.page + C::ST - 1) / C::ST);
-  const int ranges = (int)std::max(1ll, std::min<long long>(warps / NKV, (strips + MIN_STRIPS - 1) / MIN_STRIPS));
+  const int ranges = (int)std::max(1ll, std::min<long long>(warps / NKV, strips));
   const int need = (ranges * NKV + C::NW - 1) / C::NW;
   cudaError_t e = fa::launch_pdl(dec8_kernel<W, Q, RT, TMA>, dim3(need), dim3(C::NW * 32), C::SMEM, st, mk, mv, p, pg, dtype, ranges);
   fa::count_launch();
@@ -998,6 +1006,8 @@ int launch(const FaDec8Params& p, int dtype, cudaStream_t st) {
   return fa::cuda_status(e, "8-bit decode merge launch");
 }
 
+// A box takes slots of one page: pages of 8 and less would make four or more copies of a strip of 32, and go by the warp's own
+// 16-byte copies.
 template <int W, typename Q, int RT>
 int by_page(const FaDec8Params& p, int dtype, cudaStream_t st) {
   return p.page < 16 ? launch<W, Q, RT, false>(p, dtype, st) : launch<W, Q, RT, true>(p, dtype, st);

@@ -201,7 +201,9 @@ __device__ __forceinline__ void turn16(float* v, int u, const Turn& r, int tp) {
 }
 
 // ---------------------------------------------------------------- append, caches of the inputs' type
-// A CTA takes `rows` new rows; where each goes stands in shared memory before its threads walk the units of their K and V.
+// A CTA takes `rows` new rows of K or of V; where each goes stands in shared memory before its threads walk the rows' units.
+// 67k fp16 rows of 8 x 128, rotated: 105 us, 5.4 TB/s (the floor is 89 us; a warp a row and head, element by element: 400 us).
+// Left over is the latency of a CTA's own chain: sequence, page, rows.
 constexpr int AT = 256, MAX_ROWS = 16;
 template <typename T>
 __global__ void __launch_bounds__(AT) append_vec_kernel(const FaKvAppendParams p, const Pages pg, const int rows, const Div per_row,
@@ -301,6 +303,10 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // block: lanes, passes and, where a block has more than 16 slots, the block's warps.  One read of the new rows, one write of the
 // codes; earlier codes of the first block are touched only where its scale grew.  The warps of a CTA take the heads of the
 // same rows, which share their cos / sin rows in L1.  BIG: a block has 16 slots or more, so a warp has one scale.
+// 67k bf16 rows of 8 x 128 to e4m3, rotated: 131 us, 3.1 TB/s (106 us unrotated; the floor is 64 us; element by element: 1.5 ms).
+// Bound by the latency of warps that live for one group: a warp has 16 rows of loads under way, an SM 16 warps of 127
+// registers, DRAM is at 36 %.  Keeping rows as loaded and rotating them twice for fewer registers: 158 us; several heads a
+// warp: 193 us.
 template <typename T, typename Q, int LP, bool BIG>
 __global__ void __launch_bounds__(512, 1) append8_vec_kernel(const FaKvAppendParams p, const Pages pg, const long long slots) {
   constexpr int RPP = 32 / LP, PASS = 16 / RPP;
@@ -462,6 +468,7 @@ __global__ void __launch_bounds__(512, 1) append8_vec_kernel(const FaKvAppendPar
 
 // ---------------------------------------------------------------- gather
 // A CTA takes `rows` rows of K or of V; a thread makes 32 bytes of the output at a time (16 or 8 elements).
+// 393k e4m3 rows of 8 x 128 to bf16: 365 us, 6.6 TB/s; what a copy of as many bytes takes (element by element: 4.2 ms).
 constexpr int GT = 256;
 struct __align__(32) Out32 { uint32_t u[8]; };
 __device__ __forceinline__ void store32(void* o, const Out32& v) {
@@ -550,7 +557,8 @@ __global__ void __launch_bounds__(GT) gather_kernel(const FaKvGatherParams p, co
   }
 }
 
-// rows of a CTA: as many as leave every SM two CTAs
+// rows of a CTA: as many as leave every SM two CTAs.  A call of few rows spreads over the SMs, one of many finds its rows'
+// pages once for 16.
 int rows_of_cta(long long total, int most) {
   int r = most;
   while (r > 1 && (total + r - 1) / r < 2 * fa::num_sms()) r /= 2;
