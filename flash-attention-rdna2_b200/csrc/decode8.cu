@@ -4,7 +4,7 @@
 // One pass over the cache with a running maximum and sum.  For a key j with codes c_j, d_j and block
 // scales ks_j, vs_j, and in base 2:  x_j = scale log2(e) ks_j (q . c_j),  o = sum 2^(x_j - m) vs_j d_j / sum 2^(x_j - m).
 // The value scale joins the weight, w_j = 2^(x_j - m) vs_j u, where u is a power of two of the row's own that keeps the
-// largest weight so far in fp16's range whatever the scales: the tensor cores take codes (exact in
+// largest weight so far in fp16's range whatever the scales: the tensor cores take V codes (exact in
 // fp16) and weights (fp16 high and low part, 22 bits) as they are, and dividing by u at the end is exact.
 //
 // The floor is the bytes of the cache.  What is read goes through registers to mma.sync (m16n8k16, fp16
@@ -21,6 +21,8 @@
 //
 // Rows of a warp are (new token, query head) pairs of one kv head.  8 rows: the upper 8 rows of the
 // m16 tile carry the low parts of q and of w, so that both have 22 bits for nothing.  16 rows: a second mma.
+// int8 K rows need no conversion: q becomes integers of 24 bits, relative to the row's largest, whose three bytes are the
+// rows of integer mma (m16n8k32) with the codes as they are, and whose sums are exact.
 //
 // Work split: the strips of all sequences (times the row tiles of each) form one line, cut into equal
 // ranges, one for each warp of a kv head; the warps of a CTA take the heads of one range, so that the heads' rows,
@@ -128,6 +130,23 @@ __device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, ui
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// int8 K: q (signed or unsigned bytes) times codes, 32 dims, exact sums
+template <bool SIGNED>
+__device__ __forceinline__ void mma8(int* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (SIGNED)
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// byte i of four words
+__device__ __forceinline__ uint32_t bytes_of(const int* n, int i) {
+  const int sel = i | (4 + i) << 4;
+  return __byte_perm(__byte_perm(n[0], n[1], sel), __byte_perm(n[2], n[3], sel), 0x5410);
+}
 __device__ __forceinline__ uint32_t pack(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -150,12 +169,6 @@ struct Conv<I8> {
     const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&u), __half2half2(__ushort_as_half(0x6480)));
     return *reinterpret_cast<const uint32_t*>(&h);
   }
-  // 4 bytes of one word -> (0, 1), (2, 3)
-  static __device__ __forceinline__ void along(uint32_t w, uint32_t& p0, uint32_t& p1) {
-    const uint32_t x = w ^ 0x80808080u;
-    p0 = half_pair(x, 0x4140);
-    p1 = half_pair(x, 0x4342);
-  }
   // bytes i of two words -> (a_i, b_i)
   static __device__ __forceinline__ void across(uint32_t a, uint32_t b, uint32_t* p) {
     const uint32_t x = __byte_perm(a, b, 0x5140) ^ 0x80808080u, y = __byte_perm(a, b, 0x7362) ^ 0x80808080u;
@@ -165,6 +178,7 @@ struct Conv<I8> {
 };
 template <>
 struct Conv<E4M3> {
+  // 4 bytes of one word -> (0, 1), (2, 3)
   static __device__ __forceinline__ void along(uint32_t w, uint32_t& p0, uint32_t& p1) {
     asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
         : "=r"(p0), "=r"(p1) : "r"(w));
@@ -309,6 +323,7 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
   constexpr int JT = C::JT, NP = 2 * JT;   // n tiles of S, positions of a thread
   constexpr unsigned ALL = ST == 32 ? ~0u : 0xffffu;
   constexpr int RPT = RT / 8;        // rows of a thread: g, g + 8
+  constexpr bool INT = std::is_same<Q, I8>::value;
   extern __shared__ unsigned char smem_raw[];
   __shared__ unsigned long long s_full[NW][STAGES];   // mbarrier of a stage
   __shared__ unsigned s_have[NW][STAGES];             // its positions that lie in a page (bits)
@@ -490,7 +505,7 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
         }
       }
       const long long qe = (sq.first + tok) * p.q_row + head * p.q_head;
-      float x[KS * 4], most = 0.f;                  // 16 i + 4 w: piece t4 + 4 i, word w
+      float x[KS * 4], most = 0.f, bad = 0.f;       // 16 i + 4 w: piece t4 + 4 i, word w; bad: NaN where one is not finite
 #pragma unroll
       for (int i = 0; i < KC; ++i) {
         const int d = 16 * (t4 + 4 * i);
@@ -503,7 +518,10 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
           else load_q16(p, (const float*)p.q + qe, d, rp, q_vec, v);
         }
 #pragma unroll
-        for (int j = 0; j < 16; ++j) most = fmaxf(most, fabsf(v[j]));
+        for (int j = 0; j < 16; ++j) {
+          most = fmaxf(most, fabsf(v[j]));
+          if constexpr (INT) bad = fmaf(v[j], 0.f, bad);
+        }
       }
       // rows are brought to [1, 2) by a power of two, so that fp16 holds them whatever their size
       most = fmaxf(most, __shfl_xor_sync(~0u, most, 1));
@@ -511,18 +529,41 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
       const int e = min(exponent(most), 126);
       const float down = pow2(-e);
       qf[r] = p.scale * pow2(e) * (cap ? 1.f / p.softcap : FA_LOG2E);
+      if constexpr (INT) {   // q as integers of 24 bits, 2^22 to 1: three bytes, the upper one signed
+        bad += __shfl_xor_sync(~0u, bad, 1);
+        bad += __shfl_xor_sync(~0u, bad, 2);
+        qf[r] = fmaf(qf[r], 0x1p-22f, bad);
 #pragma unroll
-      for (int c = 0; c < KS; ++c) {
-        uint32_t h0, l0, h1, l1;
-        split(x[4 * c] * down, x[4 * c + 1] * down, h0, l0);
-        split(x[4 * c + 2] * down, x[4 * c + 3] * down, h1, l1);
-        if constexpr (RT == 8) {
-          qs[c * 32 + lane] = make_uint4(h0, l0, h1, l1);
-        } else {   // operand words: 0 row g, 1 row g + 8 (first pair); 2, 3 (second pair); low parts behind
-          uint32_t* const hi = reinterpret_cast<uint32_t*>(qs) + (c * 32 + lane) * 4;
-          uint32_t* const lo = hi + KS * 128;
-          hi[r] = h0; hi[2 + r] = h1;
-          lo[r] = l0; lo[2 + r] = l1;
+        for (int c = 0; c < KS; ++c) {
+          int n[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) n[i] = min(__float2int_rn(x[4 * c + i] * down * 0x1p22f), (1 << 23) - 1);
+          uint32_t* const at = reinterpret_cast<uint32_t*>(qs);
+          const int step = (c >> 1) * 32 + lane;
+          if constexpr (RT == 8) {   // the upper bytes of a step's two words; of each, the middle ones and the lower ones
+            at[2 * step + (c & 1)] = bytes_of(n, 2);
+            uint32_t* const low = at + KS * 32 + 4 * step + 2 * (c & 1);
+            low[0] = bytes_of(n, 1);
+            low[1] = bytes_of(n, 0);
+          } else {                   // as the operand has them: word 0 of rows g, g + 8, word 1 of both
+#pragma unroll
+            for (int i = 0; i < 3; ++i) at[i * (KS * 64) + 4 * step + 2 * (c & 1) + r] = bytes_of(n, 2 - i);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < KS; ++c) {
+          uint32_t h0, l0, h1, l1;
+          split(x[4 * c] * down, x[4 * c + 1] * down, h0, l0);
+          split(x[4 * c + 2] * down, x[4 * c + 3] * down, h1, l1);
+          if constexpr (RT == 8) {
+            qs[c * 32 + lane] = make_uint4(h0, l0, h1, l1);
+          } else {   // operand words: 0 row g, 1 row g + 8 (first pair); 2, 3 (second pair); low parts behind
+            uint32_t* const hi = reinterpret_cast<uint32_t*>(qs) + (c * 32 + lane) * 4;
+            uint32_t* const lo = hi + KS * 128;
+            hi[r] = h0; hi[2 + r] = h1;
+            lo[r] = l0; lo[2 + r] = l1;
+          }
         }
       }
     }
@@ -558,32 +599,89 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
       const unsigned char* const src = mine + stage * C::STAGE_B;
 
       // ---- S = Q K^T: column c of n tile j is position pos0 + 8 j + col_pos(c)
-      float s[JT][4];
+      float s[RPT][NP];                             // as the weights are, below
+      if constexpr (INT) {
+        // Integer mma on the codes as they are.  With q = 65536 h + 256 m + l the three sums stay below 2^31 for 256
+        // dims, and so does 256 m + l.  8 rows: h in one, m and l in the two halves of another.  (K as fp16: 175 against
+        // 166 us for 16 x 16-32k tokens of 4 heads a kv head, 279 against 256 us with 16 heads.)
+        constexpr int ACCS = RT == 8 ? 2 : 3;
+        int a[ACCS][JT][4];
 #pragma unroll
-      for (int j = 0; j < JT; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+        for (int i = 0; i < ACCS; ++i)
 #pragma unroll
-      for (int c = 0; c < KC; ++c) {
-        uint4 kk[JT];
+          for (int j = 0; j < JT; ++j) a[i][j][0] = a[i][j][1] = a[i][j][2] = a[i][j][3] = 0;
 #pragma unroll
-        for (int j = 0; j < JT; ++j)
-          kk[j] = *reinterpret_cast<const uint4*>(src + (c >> 1) * (ST * 128) + (kat ^ ((c & 1) * 64)) + j * 8 * C::ROW);
+        for (int c = 0; c < KC; ++c) {
+          uint4 kk[JT];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const uint4 qu = qs[(4 * c + w) * 32 + lane];
-          const uint32_t qv[4] = {qu.x, qu.y, qu.z, qu.w};
-          uint32_t ql[4];
-          if constexpr (RT == 16) {
-            const uint4 lu = qs[(KS + 4 * c + w) * 32 + lane];
-            ql[0] = lu.x; ql[1] = lu.y; ql[2] = lu.z; ql[3] = lu.w;
-          }
+          for (int j = 0; j < JT; ++j)
+            kk[j] = *reinterpret_cast<const uint4*>(src + (c >> 1) * (ST * 128) + (kat ^ ((c & 1) * 64)) + j * 8 * C::ROW);
 #pragma unroll
-          for (int j = 0; j < JT; ++j) {
-            uint32_t k0, k1;
-            Conv<Q>::along((&kk[j].x)[w], k0, k1);
-            mma(s[j], qv, k0, k1);
-            if constexpr (RT == 16) mma(s[j], ql, k0, k1);
+          for (int w = 0; w < 2; ++w) {
+            const int step = (2 * c + w) * 32 + lane;
+            if constexpr (RT == 8) {
+              const uint2 h = reinterpret_cast<const uint2*>(qs)[step];
+              const uint4 ml = qs[KS * 8 + step];
+#pragma unroll
+              for (int j = 0; j < JT; ++j) {
+                const uint32_t k0 = (&kk[j].x)[2 * w], k1 = (&kk[j].x)[2 * w + 1];
+                mma8<true>(a[0][j], h.x, 0, h.y, 0, k0, k1);
+                mma8<false>(a[1][j], ml.x, ml.y, ml.z, ml.w, k0, k1);
+              }
+            } else {
+              const uint4 h = qs[step], m = qs[KS * 16 + step], l = qs[KS * 32 + step];
+#pragma unroll
+              for (int j = 0; j < JT; ++j) {
+                const uint32_t k0 = (&kk[j].x)[2 * w], k1 = (&kk[j].x)[2 * w + 1];
+                mma8<true>(a[0][j], h.x, h.y, h.z, h.w, k0, k1);
+                mma8<false>(a[1][j], m.x, m.y, m.z, m.w, k0, k1);
+                mma8<false>(a[2][j], l.x, l.y, l.z, l.w, k0, k1);
+              }
+            }
           }
         }
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          const int j = i >> 1, e = i & 1;
+#pragma unroll
+          for (int h = 0; h < RPT; ++h) {
+            const int ml = RT == 8 ? a[1][j][e] * 256 + a[1][j][2 + e] : a[1][j][2 * h + e] * 256 + a[ACCS - 1][j][2 * h + e];
+            s[h][i] = fmaf((float)a[0][j][2 * h + e], 65536.f, (float)ml);
+          }
+        }
+      } else {
+        float a[JT][4];
+#pragma unroll
+        for (int j = 0; j < JT; ++j) a[j][0] = a[j][1] = a[j][2] = a[j][3] = 0.f;
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+          uint4 kk[JT];
+#pragma unroll
+          for (int j = 0; j < JT; ++j)
+            kk[j] = *reinterpret_cast<const uint4*>(src + (c >> 1) * (ST * 128) + (kat ^ ((c & 1) * 64)) + j * 8 * C::ROW);
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint4 qu = qs[(4 * c + w) * 32 + lane];
+            const uint32_t qv[4] = {qu.x, qu.y, qu.z, qu.w};
+            uint32_t ql[4];
+            if constexpr (RT == 16) {
+              const uint4 lu = qs[(KS + 4 * c + w) * 32 + lane];
+              ql[0] = lu.x; ql[1] = lu.y; ql[2] = lu.z; ql[3] = lu.w;
+            }
+#pragma unroll
+            for (int j = 0; j < JT; ++j) {
+              uint32_t k0, k1;
+              Conv<Q>::along((&kk[j].x)[w], k0, k1);
+              mma(a[j], qv, k0, k1);
+              if constexpr (RT == 16) mma(a[j], ql, k0, k1);
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+#pragma unroll
+          for (int h = 0; h < RPT; ++h)
+            s[h][i] = RT == 8 ? a[i >> 1][i & 1] + a[i >> 1][2 + (i & 1)] : a[i >> 1][2 * h + (i & 1)];
       }
 
       // ---- weights of positions pos0 + 8 j + col_pos(2 t4 + e), row g (+ 8 r), at [2 j + e]; x: scores less m, rounded
@@ -602,7 +700,7 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
         vs[i] = scales[stage * (2 * ST) + ST + r];
 #pragma unroll
         for (int h = 0; h < RPT; ++h)
-          x[h][i] = fmaf(RT == 8 ? s[i >> 1][i & 1] + s[i >> 1][2 + (i & 1)] : s[i >> 1][2 * h + (i & 1)], ks * qf[h], -m[h]);
+          x[h][i] = fmaf(s[h][i], ks * qf[h], -m[h]);
       }
       if constexpr (!PLAIN) {
 #pragma unroll
