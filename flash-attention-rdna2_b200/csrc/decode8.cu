@@ -30,11 +30,10 @@
 // writes its output, others leave (m, l, o) in one of the warp's two slots, and a merge kernel joins the slots of each
 // cut sequence in order (no atomics: same bits on every call).
 //
-// Measured, both kernels: 16 x 16-32k tokens, 8 kv heads, headdim 128, one token of 32 heads (806 MB): int8 173 us
-// (4.7 TB/s), e4m3 160 us (5.0 TB/s); 48 x 1-9k e4m3 108 us (4.6 TB/s); one document of 131k 76 us (3.5 TB/s); 24 tables of 4k
-// with 1-4 tokens each 93 us; 1 x 900 12.5 us.  What bounds it: an SM holds 8 warps of 240 registers, whose conversions,
-// mma and softmax (135 us by themselves in the first case, before strips without masks had code of their own) and copies (141 us by themselves)
-// overlap only in part; DRAM is at 55 % of its peak, issue slots at 41 %.
+// Measured, both kernels: 16 x 16-32k tokens, 8 kv heads, headdim 128, one token of 32 heads (806 MB): int8 166 us
+// (4.9 TB/s), e4m3 160 us (5.0 TB/s); 48 x 1-9k e4m3 108 us (4.6 TB/s); one int8 document of 131k 73 us (3.7 TB/s); 24 windows
+// of 4k with 1-4 tokens each, int8, 90 us; 1 x 611 12.5 us.  What bounds it: an SM holds 8 warps of 240 registers, whose conversions,
+// mma and softmax (135 us by themselves when the first case took 181) and copies (141 us) overlap only in part.
 #include <cudaTypedefs.h>
 #include <algorithm>
 #include <type_traits>
@@ -60,8 +59,8 @@ constexpr float MOST = 16384.f;    // ... when one exceeds 2^14: fp16 then reach
 template <int W, int RT>
 struct Cfg {
   // Positions of a strip, warps of a CTA, CTAs of an SM, stages: what 64 K registers and 227 KB of shared memory hold.
-  // Strips of 32 with 8 warps an SM against strips of 16 with 12: 173 and 188 us (16 x 16-32k int8), 108 and 134 us (48 x 1-9k
-  // e4m3), 12.5 and 12.3 us (1 x 900).
+  // Strips of 32 with 8 warps an SM against strips of 16 with 12: 160 and 181 us (16 x 16-32k e4m3), 108 and 134 us (48 x 1-9k
+  // e4m3), 12.5 and 12.3 us (1 x 611).
   static constexpr int ST = RT == 8 && W <= 128 ? 32 : 16;
   static constexpr int NW = 4;
   static constexpr int CTAS = W == 64 && RT == 8 ? 4 : 2;
@@ -1113,9 +1112,10 @@ int by_page(const FaDec8Params& p, int dtype, cudaStream_t st) {
 template <int W, typename Q>
 int by_rows(const FaDec8Params& p, int dtype, cudaStream_t st) {
   // More than 8 rows a sequence: one pass over the cache with 16 rows, or tiles of 8 that each make a pass.  16 rows win
-  // where every sequence has them (16 x 16-32k tokens, 16 heads a kv head, headdim 128: 291 against 330 us); tiles win where
-  // counts are ragged, since most tiles of 16 are then half empty (1 to 4 tokens of 4 heads, 24 x 1-20k tokens: 124 against 104
-  // us), and for rows of 256, whose 16-row form has one warp a scheduler (16 x 1-9k tokens, 16 heads: 127 against 108 us).
+  // where every sequence has them (16 x 16-32k tokens, 16 heads a kv head, headdim 128: int8 256 against 299 us, e4m3 260
+  // against 286); tiles win where counts are ragged, since most tiles of 16 are then half empty (1 to 4 tokens of 4 heads, 24
+  // x 1-20k int8 tokens: 105 against 90 us), and for rows of 256, whose 16-row form has one warp a scheduler (16 x 1-9k tokens, 16 heads,
+  // before int8 took integer mma: 127 against 108 us).
   const bool full = p.gqa > 8 || (!p.cu_q && (long long)p.gqa * p.tokens > 8);
   if constexpr (W <= 128)
     if (full) return by_page<W, Q, 16>(p, dtype, st);

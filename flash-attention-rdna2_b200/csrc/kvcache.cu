@@ -709,13 +709,13 @@ extern "C" FA_API int fa_kv_gather_launch(const FaKvGatherParams* pp, int dtype,
   if (!cache_ok(p, "kv gather")) return FA_ERR_INVALID;
   if (!dim_ok(p.dim, "kv gather")) return FA_ERR_UNSUPPORTED;
   FA_CHECK_ARG(p.total >= 0, "kv gather: total=%lld", p.total);
-  FA_CHECK_ARG(((uintptr_t)p.Kc | (uintptr_t)p.Vc) % 16 == 0 && ((uintptr_t)p.k | (uintptr_t)p.v) % 32 == 0,
-               "kv gather: Kc and Vc must be 16-byte, k and v 32-byte aligned");
   if (p.total == 0 || p.batch == 0) return FA_OK;
   if (p.total * p.heads >= 1ll << 31) {
     fa::set_error("kv gather: %lld rows of %d heads are more than one call takes", p.total, p.heads);
     return FA_ERR_SIZE;
   }
+  FA_CHECK_ARG(((uintptr_t)p.Kc | (uintptr_t)p.Vc) % 16 == 0 && ((uintptr_t)p.k | (uintptr_t)p.v) % 32 == 0,
+               "kv gather: Kc and Vc must be 16-byte, k and v 32-byte aligned");
   cudaStream_t st = (cudaStream_t)stream;
   if (dtype == FA_DTYPE_F16) return gather<__half>(p, st);
   if (dtype == FA_DTYPE_BF16) return gather<__nv_bfloat16>(p, st);
