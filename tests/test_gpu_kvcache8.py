@@ -383,6 +383,38 @@ def test_decode_large_and_small_scores(code):
     check_decode(got, want, lse, wl, "fp32")
 
 
+@pytest.mark.parametrize("hq,dim", [(4, 256), (8, 128), (16, 128), (16, 64)])
+def test_decode_sums_of_the_largest_codes(hq, dim):
+    """Every code at an end of int8 and every |q| just below a power of two: the largest sums that a score can need.
+    Scores stay within 4, each good to a few units of 2^-23 of that: far below the fp32 bar of 1e-5."""
+    rng = np.random.default_rng(31)
+    c = R.Cache(rng, 1, 1, dim, 16, 16, "int8", 200)
+    ends = torch.from_numpy(rng.choice(np.array([-128, 127]), (c.n, 16, 1, 1))).to(torch.int8)
+    c.k.copy_(ends.expand(-1, -1, 1, dim))
+    c.ks.copy_(torch.from_numpy(rng.uniform(1, 4, tuple(c.ks.shape))).float())
+    q = np.full((1, hq, dim), np.nextafter(np.float32(2), np.float32(0)))
+    q[0, 1] *= -1
+    q[0, 2:] *= rng.choice([-1, 1], (hq - 2, dim))
+    got, want, lse, wl = run_decode(c, torch.from_numpy(q).to("cuda", torch.float32), [200], [1], "fp32", False, scale=1 / (256 * dim))
+    check_decode(got, want, lse, wl, "fp32")
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("hq", [4, 16])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_decode_nonfinite_q_stays_in_its_row(code, hq, bad):
+    rng = np.random.default_rng(32)
+    c = R.Cache(rng, 2, 1, 128, 16, 16, code, 100)
+    q = torch.from_numpy(rng.standard_normal((2, 1, hq, 128))).to("cuda", torch.float32)
+    args = (c.k, c.v, c.ks, c.vs, i32([100, 37]), c.bt)
+    clean = fa.flash_attn_with_kvcache_8bit(q, *args)
+    q[1, 0, 2, 77] = bad
+    got = fa.flash_attn_with_kvcache_8bit(q, *args)
+    assert torch.isnan(got[1, 0, 2]).all()
+    got[1, 0, 2] = clean[1, 0, 2]
+    assert torch.equal(got, clean)
+
+
 @pytest.mark.parametrize("code", ["int8", "e4m3"])
 @pytest.mark.parametrize("hq", [2, 12])
 def test_decode_hidden_places_may_hold_anything(code, hq):
