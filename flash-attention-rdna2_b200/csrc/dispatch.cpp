@@ -472,9 +472,12 @@ torch::Tensor rows_of(const torch::Tensor& x, bool packed, const char* name) {
   TORCH_CHECK_VALUE(x.dim() == (packed ? 3 : 4), "fable_attn: ", name, " must be ",
                     packed ? "(total, nheads, headdim) with cu_seqlens" : "(batch, seqlen, nheads, headdim)");
   if (packed) return x.stride(2) == 1 ? x : x.contiguous();
-  const bool one = x.size(0) <= 1 || x.size(1) == 0 || x.stride(0) == x.size(1) * x.stride(1);
+  const bool one = x.size(0) <= 1 || x.size(1) <= 1 || x.stride(0) == x.size(1) * x.stride(1);
   return x.stride(3) == 1 && one ? x : x.contiguous();
 }
+// step between rows that lie along dimension `dim` (or, where that has one entry, along dimension 0): the stride of one entry
+// says nothing, not even of a tensor that counts as contiguous
+int64_t row_step(const torch::Tensor& x, int dim) { return x.size(dim) == 1 ? x.stride(0) : x.stride(dim); }
 
 void kv_append(torch::Tensor k, torch::Tensor v, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor cache_seqlens,
                torch::Tensor block_table, c10::optional<torch::Tensor> k_scale, c10::optional<torch::Tensor> v_scale,
@@ -514,8 +517,8 @@ void kv_append(torch::Tensor k, torch::Tensor v, torch::Tensor k_cache, torch::T
   p.heads = (int)k_cache.size(2);
   set_rotary(p, rotary_cos, rotary_sin, rotary_interleaved, dev, cs, sn);
   p.k = kr.data_ptr(); p.v = vr.data_ptr();
-  p.k_row = kr.stride(hd - 1); p.k_head = kr.stride(hd);
-  p.v_row = vr.stride(hd - 1); p.v_head = vr.stride(hd);
+  p.k_row = row_step(kr, hd - 1); p.k_head = kr.stride(hd);
+  p.v_row = row_step(vr, hd - 1); p.v_head = vr.stride(hd);
   p.ctx_len = lens.data_ptr<int>();
   p.total = cu ? k.size(0) : k.size(0) * k.size(1);
   if (p.total > 0) check(fa_kv_append_launch(&p, dt_of(k), cur_stream(k)), "cache append");
@@ -598,7 +601,7 @@ std::vector<torch::Tensor> dec8(torch::Tensor q, torch::Tensor k_cache, torch::T
   }
   set_rotary(p, rotary_cos, rotary_sin, rotary_interleaved, dev, cs, sn);
   p.NH = (int)Hq; p.gqa = (int)(Hq / Hk);
-  p.q = qr.data_ptr(); p.q_row = qr.stride(hd - 1); p.q_head = qr.stride(hd);
+  p.q = qr.data_ptr(); p.q_row = row_step(qr, hd - 1); p.q_head = qr.stride(hd);
   p.ctx_len = lens.data_ptr<int>();
   auto out = torch::empty(q.sizes(), q.options());
   torch::Tensor lse;

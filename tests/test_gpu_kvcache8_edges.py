@@ -1,0 +1,174 @@
+"""Paged 8-bit caches at the edges of their calls, on the GPU: layouts whose strides say nothing, counts of zero or beyond
+the rows, scores far below zero, scales that fall while scores rise, softcap in fp32, and warps that read many strips.
+
+The reference is attention in 64 bits over what the codes stand for, on the device, one sequence at a time (`exact`).
+Tolerances are the framework's bars, rel_rms 3e-4 (fp16), 2.5e-3 (bf16), 1e-5 (fp32), and 1e-5 of an LSE's rms, unless a test
+says otherwise."""
+import math
+
+import pytest
+import torch
+
+import fable_attn as fa
+
+pytestmark = pytest.mark.gpu
+TDT = {"fp16": torch.float16, "bf16": torch.bfloat16, "fp32": torch.float32}
+CDT = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
+QMAX = {"int8": 127.0, "e4m3": 448.0}
+BAR = {"fp16": 3e-4, "bf16": 2.5e-3, "fp32": 1e-5}
+
+
+def i32(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def cum(v):
+    out = [0]
+    for x in v:
+        out.append(out[-1] + x)
+    return i32(out)
+
+
+def rel(a, b):
+    return float((a - b).norm() / b.norm().clamp_min(1e-30))
+
+
+class Pool:
+    """A random paged cache: pages in no order, every slot full of codes, scales about 3 / Q."""
+
+    def __init__(self, seed, lens, heads, dim, page, block, code):
+        self.gen = g = torch.Generator("cuda").manual_seed(seed)
+        self.page, self.block, self.code, self.heads, self.dim = page, block, code, heads, dim
+        per = [(n + page - 1) // page for n in lens]
+        n = sum(per) + 2
+        order = torch.randperm(n, generator=g, device="cuda").to(torch.int32).cpu()
+        self.table = torch.zeros(len(lens), max(max(per), 1), dtype=torch.int32)
+        at = 0
+        for z, p in enumerate(per):
+            self.table[z, :p] = order[at:at + p]
+            at += p
+        self.bt = self.table.cuda()
+        x = lambda: (torch.randn(n, page, heads, dim, generator=g, device="cuda") * (QMAX[code] / 3)).clamp(-QMAX[code], QMAX[code])
+        self.k, self.v = ((x().round() if code == "int8" else x()).to(CDT[code]) for _ in range(2))
+        self.ks, self.vs = (torch.randn(n, heads, page // block, generator=g, device="cuda").mul(0.5).exp() * (3 / QMAX[code])
+                            for _ in range(2))
+
+    def randn(self, *shape):
+        return torch.randn(*shape, generator=self.gen, device="cuda")
+
+    def values(self, which, z, n):
+        """fp64 (n, heads, dim): what the first n positions of sequence z stand for."""
+        c, s = (self.k, self.ks) if which == "k" else (self.v, self.vs)
+        pages = self.bt[z, :(n + self.page - 1) // self.page].long()
+        x = c.view(torch.int8)[pages].view(c.dtype).float().double()
+        return (x * s[pages].double().repeat_interleave(self.block, 2).transpose(1, 2)[..., None]).flatten(0, 1)[:n]
+
+    def blocks_of(self, z):
+        """[(page, block in it)] of sequence z in the order of its positions."""
+        return [(int(p), j) for p in self.table[z] for j in range(self.page // self.block)]
+
+
+def exact(c, q, lens, news, scale=None, softcap=0.0, window=-1, alibi=None, leftpad=None, causal=True):
+    """Packed out (total, Hq, D) and LSE (total, Hq), fp64."""
+    hq, d = q.shape[-2:]
+    g, outs, lses, at = hq // c.heads, [], [], 0
+    for z, (L, n) in enumerate(zip(lens, news)):
+        k, v = c.values("k", z, L), c.values("v", z, L)
+        x = q[at:at + n].double().view(n, c.heads, g, d)
+        at += n
+        s = torch.einsum("nhgd,lhd->nhgl", x, k) * (scale or d ** -0.5)
+        if softcap:
+            s = softcap * torch.tanh(s / softcap)
+        j, pos = torch.arange(L, device="cuda"), torch.arange(L - n, L, device="cuda")[:, None]
+        if alibi is not None:
+            s = s + alibi.double().view(1, c.heads, g, 1) * (j - pos)[:, None, None].double()
+        seen = torch.ones(n, L, dtype=torch.bool, device="cuda")
+        if causal:
+            seen &= j <= pos
+        if window >= 0:
+            seen &= j >= pos - window
+        if leftpad is not None:
+            seen &= j >= leftpad[z]
+        s = s.masked_fill(~seen[:, None, None], -math.inf)
+        lse = torch.logsumexp(s, -1)
+        p = (s - lse.masked_fill(lse == -math.inf, 0.0)[..., None]).exp()
+        outs.append(torch.einsum("nhgl,lhd->nhgd", p, v).reshape(n, hq, d))
+        lses.append(lse.reshape(n, hq))
+    return torch.cat(outs), torch.cat(lses)
+
+
+def decode(c, q, lens, news, packed=False, scale=None, softcap=0.0, window=-1, alibi=None, leftpad=None, causal=True):
+    """The framework's, laid out the same."""
+    hq, d = q.shape[-2:]
+    qq = q if packed else q.view(len(lens), news[0], hq, d)
+    out, lse = fa.flash_attn_with_kvcache_8bit(
+        qq, c.k, c.v, c.ks, c.vs, i32(lens), c.bt, softmax_scale=scale, causal=causal, window_size=(window, -1), softcap=softcap,
+        alibi_slopes=alibi, cu_seqlens_q=cum(news) if packed else None, max_seqlen_q=max(news) if packed else None,
+        cache_leftpad=None if leftpad is None else i32(leftpad), return_softmax_lse=True)
+    lse = lse.t() if packed else lse.transpose(1, 2).reshape(-1, hq)
+    return out.reshape(-1, hq, d), lse
+
+
+def check(got, want, dt, bar=None):
+    (o, l), (wo, wl) = got, want
+    assert torch.isfinite(o).all() and (torch.isneginf(l) == torch.isneginf(wl)).all()
+    live = ~torch.isneginf(wl)
+    assert rel(o.double(), wo) <= (bar or BAR[dt]), rel(o.double(), wo)
+    err = (l.double() - wl)[live].abs().max()
+    assert float(err) <= 1e-5 * max(1.0, float(wl[live].square().mean().sqrt())), float(err)
+
+
+def strips_a_warp(c, lens, news, gqa, packed=False):
+    """(strips that a warp takes, stages of its ring) by the kernel's rule for equal ranges."""
+    w = 64 if c.dim <= 64 else 128 if c.dim <= 128 else 256
+    rt = 16 if w <= 128 and (gqa > 8 or (not packed and gqa * news[0] > 8)) else 8
+    st = 32 if rt == 8 and w <= 128 else 16
+    ctas = 4 if w == 64 and rt == 8 else 2
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    tiles = (max(news) * gqa + rt - 1) // rt
+    bound = len(lens) * tiles * ((c.bt.shape[1] * c.page + st - 1) // st)
+    ranges = max(1, min(sms * ctas * 4 // c.heads, bound))
+    line = sum(max(1, (n + st - 1) // st) * ((k * gqa + rt - 1) // rt) for n, k in zip(lens, news))
+    return -(-line // ranges), 2 if rt == 8 else 3 if w == 128 else 4
+
+
+# ---------------------------------------------------------------------------------------- layouts
+def seq_first(x):
+    """(batch, 1, heads, dim) as a view of (1, batch, heads, dim): dimension 1 has one entry and batch's stride.  The storage goes on
+    to where that stride would lead."""
+    b, _, h, d = x.shape
+    wide = torch.zeros(b * b, h, d, dtype=x.dtype, device=x.device)
+    wide[:b] = x[:, 0]
+    y = wide[:b][None].transpose(0, 1)
+    assert y.stride(1) == b * h * d and y.is_contiguous() and torch.equal(y, x)
+    return y
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3", "none"])
+def test_one_token_with_the_sequence_dimension_first(code):
+    """A dimension of one entry has a stride that says nothing, and such a tensor counts as contiguous whatever it is."""
+    lens = [3, 40, 17]
+    a, b = (Pool(1, [n + 1 for n in lens], 2, 64, 16, 8, "int8" if code == "none" else code) for _ in range(2))
+    for c in (a, b):
+        if code == "none":
+            c.k, c.v, c.ks, c.vs = c.k.bfloat16(), c.v.bfloat16(), None, None
+    k, v, q = a.randn(3, 1, 2, 64).bfloat16(), a.randn(3, 1, 2, 64).bfloat16(), a.randn(3, 1, 8, 64).bfloat16()
+    for c, lay in ((a, lambda t: t), (b, seq_first)):
+        fa.kvcache_append(lay(k), lay(v), c.k, c.v, i32(lens), c.bt, k_scale=c.ks, v_scale=c.vs)
+    same = lambda x, y: torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+    assert same(a.k, b.k) and same(a.v, b.v)
+    if code == "none":
+        return
+    assert torch.equal(a.ks, b.ks) and torch.equal(a.vs, b.vs)
+    out = [fa.flash_attn_with_kvcache_8bit(x, a.k, a.v, a.ks, a.vs, i32([n + 1 for n in lens]), a.bt) for x in (q, seq_first(q))]
+    assert torch.equal(*out)
+
+
+@pytest.mark.parametrize("rows", [1, 3])
+def test_rows_of_a_slice_need_no_copy_to_be_right(rows):
+    """(batch, 1) rows cut out of longer sequences, and batches of one."""
+    c = Pool(2, [30, 30], 2, 64, 16, 8, "int8")
+    wide = c.randn(2, 9, 8, 64).half()
+    for q in (wide[:, 4:4 + rows], wide[1:, 4:4 + rows]):
+        args = (c.k, c.v, c.ks, c.vs, i32([30] * len(q)), c.bt[:len(q)])
+        assert torch.equal(fa.flash_attn_with_kvcache_8bit(q, *args), fa.flash_attn_with_kvcache_8bit(q.clone(), *args))
