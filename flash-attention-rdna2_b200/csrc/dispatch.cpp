@@ -40,6 +40,10 @@ FaStrides S4(const torch::Tensor& x) { return FaStrides{x.stride(0), x.stride(1)
 // (total, H, D) varlen tensors: token stride = stride(0), head stride = stride(1)
 FaStrides S3(const torch::Tensor& x) { return FaStrides{0, x.stride(1), x.stride(0)}; }
 
+// step between rows that lie along dimension `dim` (or, where that has one entry, along dimension 0): the stride of one entry
+// says nothing, not even of a tensor that counts as contiguous
+int64_t row_step(const torch::Tensor& x, int dim) { return x.size(dim) == 1 ? x.stride(0) : x.stride(dim); }
+
 void need_cuda_lastdim(const torch::Tensor& t, const char* name) {
   TORCH_CHECK_VALUE(t.is_cuda(), "fable_attn: ", name, " must be a CUDA tensor");
   TORCH_CHECK_VALUE(t.stride(-1) == 1, "fable_attn: ", name, " must have a contiguous last dimension");
@@ -125,7 +129,7 @@ RotaryArgs rotary_args(const c10::optional<torch::Tensor>& cos, const c10::optio
 torch::Tensor rotate_k_rows(const torch::Tensor& k, const RotaryArgs& r, const int* cu_k, int batch, bool varlen) {
   torch::Tensor src = k;
   // dense rows (b, s) must form one strided dimension: batch stride = SK * row stride
-  if (!varlen && k.size(0) > 1 && k.stride(0) != k.size(2) * k.stride(2)) src = k.contiguous();
+  if (!varlen && k.size(0) > 1 && k.size(2) > 1 && k.stride(0) != k.size(2) * k.stride(2)) src = k.contiguous();
   auto out = torch::empty_like(src);
   FaRotaryParams rp{};
   rp.struct_size = sizeof(FaRotaryParams);
@@ -137,8 +141,8 @@ torch::Tensor rotate_k_rows(const torch::Tensor& k, const RotaryArgs& r, const i
     rp.cu_seqlens = cu_k; rp.batch = batch;
   } else {   // (B, Hk, SK, D) view
     rp.rows = src.size(0) * src.size(2); rp.heads = (int)src.size(1); rp.dim = (int)src.size(3);
-    rp.x_row_stride = src.stride(2); rp.x_head_stride = src.stride(1);
-    rp.out_row_stride = out.stride(2); rp.out_head_stride = out.stride(1);
+    rp.x_row_stride = row_step(src, 2); rp.x_head_stride = src.stride(1);
+    rp.out_row_stride = row_step(out, 2); rp.out_head_stride = out.stride(1);
     rp.seqlen = (int)src.size(2); rp.batch = (int)src.size(0);
   }
   rp.rotary_dim = (int)r.cos.size(1) * 2;
@@ -475,10 +479,6 @@ torch::Tensor rows_of(const torch::Tensor& x, bool packed, const char* name) {
   const bool one = x.size(0) <= 1 || x.size(1) <= 1 || x.stride(0) == x.size(1) * x.stride(1);
   return x.stride(3) == 1 && one ? x : x.contiguous();
 }
-// step between rows that lie along dimension `dim` (or, where that has one entry, along dimension 0): the stride of one entry
-// says nothing, not even of a tensor that counts as contiguous
-int64_t row_step(const torch::Tensor& x, int dim) { return x.size(dim) == 1 ? x.stride(0) : x.stride(dim); }
-
 void kv_append(torch::Tensor k, torch::Tensor v, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor cache_seqlens,
                torch::Tensor block_table, c10::optional<torch::Tensor> k_scale, c10::optional<torch::Tensor> v_scale,
                c10::optional<torch::Tensor> cu_new, c10::optional<torch::Tensor> rotary_cos,
@@ -727,7 +727,7 @@ torch::Tensor rotary(torch::Tensor x, torch::Tensor cos, torch::Tensor sin, bool
                     "(batch, seqlen, heads, dim)");
   // rows must be one strided dimension: (batch, seqlen) merge when batch stride = seqlen * row stride
   torch::Tensor src = x;
-  if (!varlen && x.size(0) > 1 && x.stride(0) != x.size(1) * x.stride(1)) src = x.contiguous();
+  if (!varlen && x.size(0) > 1 && x.size(1) > 1 && x.stride(0) != x.size(1) * x.stride(1)) src = x.contiguous();
   auto c = cos.to(torch::kFloat32).contiguous(), s = sin.to(torch::kFloat32).contiguous();
   TORCH_CHECK_VALUE(c.dim() == 2 && s.sizes() == c.sizes(), "fable_attn: cos/sin must be (seqlen_ro, rotary_dim/2)");
   torch::Tensor out = (inplace && src.is_same(x)) ? x : torch::empty_like(src);
@@ -737,8 +737,8 @@ torch::Tensor rotary(torch::Tensor x, torch::Tensor cos, torch::Tensor sin, bool
   const int hd = varlen ? 1 : 2;
   p.rows = varlen ? src.size(0) : src.size(0) * src.size(1);
   p.heads = (int)src.size(hd); p.dim = (int)src.size(hd + 1); p.rotary_dim = (int)c.size(1) * 2;
-  p.x_row_stride = src.stride(hd - 1); p.x_head_stride = src.stride(hd);
-  p.out_row_stride = out.stride(hd - 1); p.out_head_stride = out.stride(hd);
+  p.x_row_stride = row_step(src, hd - 1); p.x_head_stride = src.stride(hd);
+  p.out_row_stride = row_step(out, hd - 1); p.out_head_stride = out.stride(hd);
   torch::Tensor cu, offs;
   if (varlen) {
     cu = cu_seqlens->to(torch::kInt32).contiguous();
