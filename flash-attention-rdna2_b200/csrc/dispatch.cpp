@@ -128,9 +128,11 @@ RotaryArgs rotary_args(const c10::optional<torch::Tensor>& cos, const c10::optio
 }
 torch::Tensor rotate_k_rows(const torch::Tensor& k, const RotaryArgs& r, const int* cu_k, int batch, bool varlen) {
   torch::Tensor src = k;
-  // dense rows (b, s) must form one strided dimension: batch stride = SK * row stride
-  if (!varlen && k.size(0) > 1 && k.size(2) > 1 && k.stride(0) != k.size(2) * k.stride(2)) src = k.contiguous();
-  auto out = torch::empty_like(src);
+  // dense rows (b, s) must form one strided dimension, of the input and of the output: batch stride = SK * row stride
+  if (!varlen && k.size(0) > 1 && k.size(2) > 1 && k.stride(0) != k.size(2) * k.stride(2))
+    src = k.transpose(1, 2).contiguous().transpose(1, 2);
+  auto out = varlen ? torch::empty_like(src)
+                    : torch::empty({k.size(0), k.size(2), k.size(1), k.size(3)}, k.options()).transpose(1, 2);
   FaRotaryParams rp{};
   rp.struct_size = sizeof(FaRotaryParams);
   rp.x = src.data_ptr(); rp.out = out.data_ptr();

@@ -45,3 +45,26 @@ def test_attention_that_rotates(sq):
         want = fa.flash_attn_func(q, k, v, rotary_cos=cos, rotary_sin=sin)
         got = fa.flash_attn_func(q, seq_first(k), v, rotary_cos=cos, rotary_sin=sin)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_attention_that_rotates_a_slice_of_longer_sequences(interleaved):
+    """k cut out of a longer buffer: its batches do not follow one another."""
+    q = torch.randn(3, 5, 4, 64, device="cuda", dtype=torch.float16)
+    wide = torch.randn(2, 3, 9, 2, 64, device="cuda", dtype=torch.float16)
+    k, v = wide[0, :, 2:7], wide[1, :, 2:7]
+    cos, sin = tables(8, 32)
+    with torch.no_grad():
+        want = fa.flash_attn_func(q, k.clone(), v.clone(), causal=True, rotary_cos=cos, rotary_sin=sin, rotary_interleaved=interleaved)
+        got = fa.flash_attn_func(q, k, v, causal=True, rotary_cos=cos, rotary_sin=sin, rotary_interleaved=interleaved)
+    assert torch.equal(got, want)
+
+
+def test_attention_that_rotates_one_head_given_as_several():
+    q = torch.randn(3, 5, 4, 64, device="cuda", dtype=torch.float16)
+    k, v = (torch.randn(3, 5, 1, 64, device="cuda", dtype=torch.float16).expand(-1, -1, 2, -1) for _ in range(2))
+    cos, sin = tables(8, 32)
+    with torch.no_grad():
+        want = fa.flash_attn_func(q, k.contiguous(), v.contiguous(), causal=True, rotary_cos=cos, rotary_sin=sin)
+        got = fa.flash_attn_func(q, k, v, causal=True, rotary_cos=cos, rotary_sin=sin)
+    assert torch.equal(got, want)
