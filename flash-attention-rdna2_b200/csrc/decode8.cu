@@ -200,8 +200,7 @@ __device__ __forceinline__ Seq seq_of(const FaDec8Params& p, const Pages& pg, in
   Seq s;
   const RowMap rm{p.cu_q, p.tokens, p.batch};
   s.first = rm.first(z);
-  s.n = (int)max(0ll, min((long long)rm.count(z), p.total - s.first));
-  if (s.first < 0) s.n = 0;
+  s.n = rm.count(z, p.total);
   s.L = max(p.ctx_len[z], 0);
   const long long cap = (long long)p.max_blocks << pg.shift;
   if (s.L > cap) {

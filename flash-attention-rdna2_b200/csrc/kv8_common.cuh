@@ -50,10 +50,10 @@ struct RowMap {
   const int* cu;
   int tokens, batch;
   __device__ __forceinline__ long long first(int z) const { return cu ? (long long)__ldg(cu + z) : (long long)z * tokens; }
-  __device__ __forceinline__ int count(int z) const {
-    if (!cu) return tokens;
-    const int n = __ldg(cu + z + 1) - __ldg(cu + z);
-    return n > 0 ? n : 0;
+  // rows of sequence z, of those that lie in [0, total): the offsets come from the device, unchecked by the host
+  __device__ __forceinline__ int count(int z, long long total) const {
+    const long long a = first(z), n = cu ? __ldg(cu + z + 1) - a : tokens;
+    return a < 0 ? 0 : (int)max(0ll, min(n, total - a));
   }
   __device__ __forceinline__ int seq_of_slot(long long slot, int gs) const {
     int lo = 0, hi = batch - 1;

@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(128) append_kernel(const FaKvAppendParams p, c
   const long long row = w / 2 / p.heads;
   const RowMap rm{p.cu_new, p.tokens, p.batch};
   const int z = rm.seq_of_row(row), i = (int)(row - rm.first(z)), pos = p.ctx_len[z] + i;
-  if (i < 0 || i >= rm.count(z)) return;   // a row of no sequence
+  if (i < 0 || i >= rm.count(z, p.total)) return;   // a row of no sequence
   const long long blk = pg.of(z, pos);
   if (blk < 0) {
     record(ERR_PAGE);
@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(128) append8_kernel(const FaKvAppendParams p, 
   const int h = (int)(w / 2 % p.heads), SB = p.block, gs = log2_of(SB);
   const long long slot = w / 2 / p.heads;
   const RowMap rm{p.cu_new, p.tokens, p.batch};
-  const int z = rm.seq_of_slot(slot, gs), n = rm.count(z), ctx = p.ctx_len[z];
+  const int z = rm.seq_of_slot(slot, gs), n = rm.count(z, p.total), ctx = p.ctx_len[z];
   if (ctx < 0) {
     record(ERR_PAGE);
     return;
@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(AT) append_vec_kernel(const FaKvAppendParams p
     int tp = -1;
     if (row < p.total) {
       const int z = rm.seq_of_row(row), i = (int)(row - rm.first(z)), pos = p.ctx_len[z] + i;
-      if (i >= 0 && i < rm.count(z)) {   // else a row of no sequence
+      if (i >= 0 && i < rm.count(z, p.total)) {   // else a row of no sequence
         const int blk = pg.of(z, pos);
         if (blk < 0) record(ERR_PAGE);
         else {
@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(512, 1) append8_vec_kernel(const FaKvAppendPar
     } else {
       const long long first = rm.first(z);
       c0 = (int)(((n0 >> gs) + slot - ((first >> gs) + 2 * z)) << gs) + 16 * in_block;
-      n1 = n0 + rm.count(z);
+      n1 = n0 + rm.count(z, p.total);
       row0 = first - n0;
     }
   }
@@ -506,7 +506,7 @@ __global__ void __launch_bounds__(GT) gather_kernel(const FaKvGatherParams p, co
     long long slot = -1, sc = 0;
     if (row < p.total) {
       const int z = rm.seq_of_row(row), i = (int)(row - rm.first(z));
-      if (i >= 0 && i < rm.count(z)) {   // else a row of no sequence
+      if (i >= 0 && i < rm.count(z, p.total)) {   // else a row of no sequence
         const int pos = i + (p.starts ? p.starts[z] : 0), blk = pg.of(z, pos);
         if (blk < 0) record(ERR_PAGE);
         else {

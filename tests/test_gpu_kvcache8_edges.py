@@ -172,3 +172,25 @@ def test_rows_of_a_slice_need_no_copy_to_be_right(rows):
     for q in (wide[:, 4:4 + rows], wide[1:, 4:4 + rows]):
         args = (c.k, c.v, c.ks, c.vs, i32([30] * len(q)), c.bt[:len(q)])
         assert torch.equal(fa.flash_attn_with_kvcache_8bit(q, *args), fa.flash_attn_with_kvcache_8bit(q.clone(), *args))
+
+
+# ---------------------------------------------------------------------------------------- counts
+@pytest.mark.parametrize("code,page,block", [("int8", 16, 16), ("e4m3", 64, 64), ("int8", 32, 4), ("e4m3", 256, 256), ("int8", 8, 8)])
+def test_append_counts_beyond_the_rows(code, page, block):
+    """cu_seqlens_new that ends past the rows given: the rows given are appended, nothing else is written.  (The rows lie in a
+    longer buffer, so that what a call must not read is there.)"""
+    lens, total = [5, 0], 20
+    a, b = (Pool(3, [300, 300], 2, 64, page, block, code) for _ in range(2))
+    wide = a.randn(400, 2, 64)
+    k, v = wide[:total], wide[200:200 + total]
+    kw = lambda c: dict(k_scale=c.ks, v_scale=c.vs)
+    fa.kvcache_append(k, v, a.k, a.v, i32(lens), a.bt, cu_seqlens_new=i32([0, 7, 20]), **kw(a))
+    fa.kvcache_append(k, v, b.k, b.v, i32(lens), b.bt, cu_seqlens_new=i32([0, 7, 130]), **kw(b))
+    for x, y in ((a.k, b.k), (a.v, b.v), (a.ks, b.ks), (a.vs, b.vs)):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+    # a sequence that begins past them, or before them, has none
+    before = [t.clone() for t in (b.k, b.v, b.ks, b.vs)]
+    fa.kvcache_append(k, v, b.k, b.v, i32(lens), b.bt, cu_seqlens_new=i32([25, 60, 99]), **kw(b))
+    fa.kvcache_append(k, v, b.k, b.v, i32(lens), b.bt, cu_seqlens_new=i32([-9, -9, -4]), **kw(b))
+    for x, y in zip(before, (b.k, b.v, b.ks, b.vs)):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
