@@ -340,7 +340,8 @@ __global__ void __launch_bounds__(512, 1) append8_vec_kernel(const FaKvAppendPar
     }
   }
   const int block0 = c0 & ~(SB - 1);                  // first position of the block (of the warp's first block)
-  bool any = block0 < n1 && max(c0 + 16, block0 + SB) > n0;   // new tokens in the warp's blocks
+  // new tokens in the warp's blocks (a sequence that has none may name pages that another one is appending to)
+  bool any = n0 < n1 && block0 < n1 && max(c0 + 16, block0 + SB) > n0;
   const int blk = any ? pg.of(z, c0) : -1;
   if (any && blk < 0) record(ERR_PAGE);
   any = blk >= 0;

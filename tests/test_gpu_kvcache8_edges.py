@@ -194,3 +194,41 @@ def test_append_counts_beyond_the_rows(code, page, block):
     fa.kvcache_append(k, v, b.k, b.v, i32(lens), b.bt, cu_seqlens_new=i32([-9, -9, -4]), **kw(b))
     for x, y in zip(before, (b.k, b.v, b.ks, b.vs)):
         assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
+@pytest.mark.parametrize("code,page,block", [("int8", 16, 16), ("e4m3", 64, 64), ("int8", 16, 4), ("e4m3", 16, 1), ("int8", 8, 8)])
+def test_append_leaves_sequences_without_new_tokens_alone(code, page, block):
+    """Counts of 0 beside others: their blocks keep codes and scales bit by bit (a scale of 0 among them), their table rows are not
+    looked at, and a page that such a sequence shares with one that appends gets what the latter writes."""
+    lens, news = [3, 5, 6, 2], [2, 0, 0, 0]
+    c = Pool(4, [40] * 4, 2, 64, page, block, code)
+    c.ks.zero_()
+    c.vs[::2] = 1e-35
+    c.table[2, 0] = c.table[0, 0]     # shares the first sequence's page
+    c.table[3] = -1                   # has no pages at all
+    c.bt = c.table.cuda()
+    before = [t.clone() for t in (c.k, c.v, c.ks, c.vs)]
+    x = c.randn(2, 2, 64) * 5
+    fa.device_error(clear=True)
+    fa.kvcache_append(x, x, c.k, c.v, i32(lens), c.bt, k_scale=c.ks, v_scale=c.vs, cu_seqlens_new=cum(news))
+    assert fa.device_error(clear=True) == 0
+    pg, touched = int(c.table[0, 0]), sorted({3 // block, 4 // block})
+    for old, new in zip(before[2:], (c.ks, c.vs)):
+        want = old.clone()
+        for b in touched:
+            rows = x[[i for i in range(2) if (3 + i) // block == b]]
+            want[pg, :, b] = torch.maximum(rows.abs().amax((0, 2)) / QMAX[code], old[pg, :, b] if b * block < 3 else torch.zeros(2, device="cuda"))
+        torch.testing.assert_close(new, want, rtol=1e-6, atol=0)
+        keep = torch.ones_like(old, dtype=torch.bool)
+        keep[pg, :, touched] = False
+        assert torch.equal(new[keep], old[keep])
+    slots = torch.ones(c.k.shape[:2], dtype=torch.bool, device="cuda")
+    slots[pg, touched[0] * block:5] = False   # earlier codes of a block may go onto its larger scale
+    for old, new in zip(before, (c.k, c.v)):
+        assert torch.equal(old.view(torch.int8)[slots], new.view(torch.int8)[slots])
+    # as whole batches do: all of them idle
+    before = [t.clone() for t in (c.k, c.v, c.ks, c.vs)]
+    fa.kvcache_append(x, x, c.k, c.v, i32(lens), c.bt, k_scale=c.ks, v_scale=c.vs, cu_seqlens_new=i32([0] * 5))
+    assert fa.device_error(clear=True) == 0
+    for old, new in zip(before, (c.k, c.v, c.ks, c.vs)):
+        assert torch.equal(old.view(torch.uint8), new.view(torch.uint8))
