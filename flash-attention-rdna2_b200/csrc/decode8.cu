@@ -724,7 +724,8 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
           float top = above[r] == LAZY ? 0.f : -INFINITY;   // a row's first keys may lower it
           raise(top, x[r]);
           if (top == -INFINITY) continue;          // nothing seen yet
-          const float by = (m[r] + top) - m[r], f = ex2(-by);
+          // before a row's first keys l and o hold 0 (or NaN): scaled by 2^-by, infinite where by <= -128, they would be NaN
+          const float by = (m[r] + top) - m[r], f = above[r] == LAZY ? ex2(-by) : 1.f;
           m[r] += by;
           above[r] = LAZY;
           l[r] *= f;

@@ -232,3 +232,34 @@ def test_append_leaves_sequences_without_new_tokens_alone(code, page, block):
     assert fa.device_error(clear=True) == 0
     for old, new in zip(before, (c.k, c.v, c.ks, c.vs)):
         assert torch.equal(old.view(torch.uint8), new.view(torch.uint8))
+
+
+# ---------------------------------------------------------------------------------------- scores
+@pytest.mark.parametrize("code,dt,gqa", [("int8", "bf16", 2), ("e4m3", "fp32", 1), ("int8", "fp32", 12), ("e4m3", "fp16", 16)])
+@pytest.mark.parametrize("lens", [[300, 41], [3000, 130]])
+def test_decode_alibi_over_long_contexts(code, dt, gqa, lens):
+    """The usual slopes 2^-1 .. 2^-8: the first keys' scores lie hundreds below the last ones'."""
+    c = Pool(5, lens, 8, 64, 16, 16, code)
+    q = c.randn(2, 8 * gqa, 64).to(TDT[dt])
+    slopes = (2.0 ** -(1.0 + torch.arange(8, device="cuda"))).repeat_interleave(gqa)
+    check(decode(c, q, lens, [1, 1], alibi=slopes), exact(c, q, lens, [1, 1], alibi=slopes), dt)
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("gqa", [1, 12])
+@pytest.mark.parametrize("opt", [dict(), dict(window=0), dict(leftpad=[32, 40]), dict(window=3)])
+def test_decode_scores_far_below_zero(code, gqa, opt):
+    """Every visible score at about -120 .. -2000, in strips of many and of one visible key."""
+    lens = [33, 41]
+    c = Pool(6, lens, 2, 64, 16, 1, code)
+    q = c.randn(2, 2 * gqa, 64)
+    for z, n in enumerate(lens):      # each key the opposite of the first query of its head, at a size of its own
+        for pos in range(n):
+            x = -q[z, ::gqa].sign() * (100 if code == "int8" else 256)
+            at = int(c.table[z, pos // 16]), pos % 16
+            c.k[at] = x.to(CDT[code])
+            c.ks[at[0], :, at[1]] = (5 + 2 * ((7 * pos + 11 * z) % 40)) / (100 if code == "int8" else 256)
+    q[:, :] = q[:, ::gqa].repeat_interleave(gqa, 1)
+    want = exact(c, q, lens, [1, 1], scale=1.0, **opt)
+    assert float(want[1].max()) < -89
+    check(decode(c, q, lens, [1, 1], scale=1.0, **opt), want, "fp32")
