@@ -724,12 +724,18 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
           float top = above[r] == LAZY ? 0.f : -INFINITY;   // a row's first keys may lower it
           raise(top, x[r]);
           if (top == -INFINITY) continue;          // nothing seen yet
+          const float by = (m[r] + top) - m[r];
           // before a row's first keys l and o hold 0 (or NaN): scaled by 2^-by, infinite where by <= -128, they would be NaN
-          const float by = (m[r] + top) - m[r], f = above[r] == LAZY ? ex2(-by) : 1.f;
+          if (above[r] == LAZY) {
+            // u rises by what whole powers of two the weights so far fall by: o keeps its size, and the weights that count
+            // from now on keep their bits however large the V scales of keys that no longer do
+            const int lift = min(__float2int_rz(by), 253 - (__float_as_int(up[r]) >> 23));   // to 2^126 at most
+            up[r] = __int_as_float(__float_as_int(up[r]) + (lift << 23));
+            l[r] *= ex2(-by);
+            scale_rows<NT, RT>(o, r, ex2((float)lift - by));
+          }
           m[r] += by;
           above[r] = LAZY;
-          l[r] *= f;
-          scale_rows<NT, RT>(o, r, f);
 #pragma unroll
           for (int i = 0; i < NP; ++i) x[r][i] -= by;
         }

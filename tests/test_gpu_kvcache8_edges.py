@@ -63,9 +63,9 @@ class Pool:
         x = c.view(torch.int8)[pages].view(c.dtype).float().double()
         return (x * s[pages].double().repeat_interleave(self.block, 2).transpose(1, 2)[..., None]).flatten(0, 1)[:n]
 
-    def blocks_of(self, z):
-        """[(page, block in it)] of sequence z in the order of its positions."""
-        return [(int(p), j) for p in self.table[z] for j in range(self.page // self.block)]
+    def blocks_of(self, z, n):
+        """[(page, block in it)] of the first n positions of sequence z, in order."""
+        return [(int(p), j) for p in self.table[z, :(n + self.page - 1) // self.page] for j in range(self.page // self.block)]
 
 
 def exact(c, q, lens, news, scale=None, softcap=0.0, window=-1, alibi=None, leftpad=None, causal=True):
@@ -263,3 +263,29 @@ def test_decode_scores_far_below_zero(code, gqa, opt):
     want = exact(c, q, lens, [1, 1], scale=1.0, **opt)
     assert float(want[1].max()) < -89
     check(decode(c, q, lens, [1, 1], scale=1.0, **opt), want, "fp32")
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("gqa,dim", [(1, 128), (12, 128), (2, 64), (1, 256)])
+@pytest.mark.parametrize("fall,rise", [(0, 0), (14, 20), (20, 30), (30, 60), (40, 60), (90, 300)])
+def test_decode_value_scales_fall_while_scores_rise(code, gqa, dim, fall, rise):
+    """A block whose V scale is 2^fall times the others' and whose scores lie `rise` (base 2) below: what it leaves behind must not
+    cost the later weights a bit.  Each row to 1e-5."""
+    lens = [1400, 1100]
+    c = Pool(7, lens, 64, dim, 32, 16, code)
+    per, stages = strips_a_warp(c, lens, [1, 1], gqa)
+    assert per > stages
+    q = c.randn(2, 64 * gqa, dim)
+    slope = torch.zeros(64 * gqa, device="cuda")
+    for z in range(2):
+        every = c.blocks_of(z, lens[z])
+        # the large block begins a stretch of a third of the sequence: whichever strips a warp takes, some hold it and smaller ones
+        for i in range(0, len(every), 6):
+            p, j = every[i]
+            c.vs[p, :, j] *= 2.0 ** fall
+    # scores rise with the position: rise over the 96 positions from one large block to the next
+    slope += rise * math.log(2.0) / 96
+    got, want = decode(c, q, lens, [1, 1], alibi=slope), exact(c, q, lens, [1, 1], alibi=slope)
+    check(got, want, "fp32")
+    err = (got[0].double() - want[0]).norm(dim=-1) / want[0].norm(dim=-1)
+    assert float(err.max()) <= 1e-5, float(err.max())
