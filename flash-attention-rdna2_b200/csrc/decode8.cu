@@ -683,7 +683,8 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
       }
 
       // ---- weights of positions pos0 + 8 j + col_pos(2 t4 + e), row g (+ 8 r), at [2 j + e]; x: scores less m, rounded
-      // once (a score of 50 by itself is good to 2^-19 only, and so would its weight be)
+      // once (a score of 50 by itself is good to 2^-19 only, and so would its weight be).  What a softcap takes is the score
+      // itself, not its difference from m, which would be rounded at m's size.
       const int pos0 = (sq.s0 + k) * ST;
       const unsigned have = s_have[warp][stage];
       // strips that every row sees whole, with scores that are nothing but products, run code without masks (16 x 16-32k
@@ -697,20 +698,22 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
         const float ks = scales[stage * (2 * ST) + r];
         vs[i] = scales[stage * (2 * ST) + ST + r];
 #pragma unroll
-        for (int h = 0; h < RPT; ++h)
-          x[h][i] = fmaf(s[h][i], ks * qf[h], -m[h]);
+        for (int h = 0; h < RPT; ++h) x[h][i] = fmaf(s[h][i], ks * qf[h], !PLAIN && cap ? 0.f : -m[h]);
       }
       if constexpr (!PLAIN) {
+        if (cap) {
+#pragma unroll
+          for (int i = 0; i < NP; ++i)
+#pragma unroll
+            for (int h = 0; h < RPT; ++h) x[h][i] = fmaf(cap_out, fa_tanh(x[h][i]), -m[h]);
+        }
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
           const int r = 8 * (i >> 1) + col_pos(2 * t4 + (i & 1)), pos = pos0 + r;
 #pragma unroll
           for (int h = 0; h < RPT; ++h) {
-            float v = x[h][i] + m[h];
-            if (cap) v = cap_out * fa_tanh(v);
-            if (p.alibi) v = fmaf(slope[h], (float)pos - qpos[h], v);
-            if (!(pos >= rlo[h] && pos < rhi[h] && ((have >> r) & 1))) v = -INFINITY;
-            x[h][i] = v - m[h];
+            if (p.alibi) x[h][i] = fmaf(slope[h], (float)pos - qpos[h], x[h][i]);
+            if (!(pos >= rlo[h] && pos < rhi[h] && ((have >> r) & 1))) x[h][i] = -INFINITY;
           }
         }
       }

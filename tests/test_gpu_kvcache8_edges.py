@@ -289,3 +289,19 @@ def test_decode_value_scales_fall_while_scores_rise(code, gqa, dim, fall, rise):
     check(got, want, "fp32")
     err = (got[0].double() - want[0]).norm(dim=-1) / want[0].norm(dim=-1)
     assert float(err.max()) <= 1e-5, float(err.max())
+
+
+@pytest.mark.parametrize("code,gqa,dim", [("int8", 1, 128), ("e4m3", 2, 64), ("int8", 12, 64), ("e4m3", 12, 128)])
+@pytest.mark.parametrize("cap", [20.0, 30.0, 50.0])
+@pytest.mark.parametrize("size", [3.0, 10.0])
+def test_decode_softcap_in_fp32(code, gqa, dim, cap, size):
+    """fp32 outputs under a softcap, several strips a warp.  The tanh is good to about 2^-24 of 1 (rms), which cap makes a relative
+    error of a weight: 3e-6 at cap 50, with signs that differ from key to key; 1e-6 for the rest.  The bar is 5e-6."""
+    lens = [1500, 1130]
+    c = Pool(8, lens, 64, dim, 64, 16, code)
+    per, stages = strips_a_warp(c, lens, [1, 1], gqa)
+    assert per > stages
+    q = c.randn(2, 64 * gqa, dim)
+    k = c.values("k", 0, 1500)
+    scale = size / float(torch.einsum("hgd,lhd->hgl", q[0].double().view(64, gqa, dim), k).square().mean().sqrt())
+    check(decode(c, q, lens, [1, 1], softcap=cap, scale=scale), exact(c, q, lens, [1, 1], softcap=cap, scale=scale), "fp32", 5e-6)
