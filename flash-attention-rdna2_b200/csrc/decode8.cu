@@ -705,7 +705,7 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
 #pragma unroll
           for (int i = 0; i < NP; ++i)
 #pragma unroll
-            for (int h = 0; h < RPT; ++h) x[h][i] = fmaf(cap_out, fa_tanh(x[h][i]), -m[h]);
+            for (int h = 0; h < RPT; ++h) x[h][i] = fmaf(cap_out, fa_tanh<true>(x[h][i]), -m[h]);
         }
 #pragma unroll
         for (int i = 0; i < NP; ++i) {

@@ -305,3 +305,29 @@ def test_decode_softcap_in_fp32(code, gqa, dim, cap, size):
     k = c.values("k", 0, 1500)
     scale = size / float(torch.einsum("hgd,lhd->hgl", q[0].double().view(64, gqa, dim), k).square().mean().sqrt())
     check(decode(c, q, lens, [1, 1], softcap=cap, scale=scale), exact(c, q, lens, [1, 1], softcap=cap, scale=scale), "fp32", 5e-6)
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("gqa", [2, 12])
+@pytest.mark.parametrize("softcap", [0.0, 30.0])
+def test_decode_nan_shows_with_and_without_softcap(code, gqa, softcap):
+    """A NaN scale of K or of V, or a NaN in q, makes every row that sees it NaN, and no other."""
+    lens = [70, 90]
+    c = Pool(9, lens, 2, 128, 16, 16, code)
+    q = c.randn(2, 1, 2 * gqa, 128)
+    run = lambda: fa.flash_attn_with_kvcache_8bit(q, c.k, c.v, c.ks, c.vs, i32(lens), c.bt, softcap=softcap)
+    clean = run()
+    p = int(c.table[1, 2])
+    for t in (c.ks, c.vs):
+        was = t[p, 1, 0].clone()
+        t[p, 1, 0] = float("nan")
+        got = run()
+        assert torch.isnan(got[1, :, gqa:]).all()
+        got[1, :, gqa:] = clean[1, :, gqa:]
+        assert torch.equal(got, clean)
+        t[p, 1, 0] = was
+    q[0, 0, 1, 5] = float("nan")
+    got = run()
+    assert torch.isnan(got[0, 0, 1]).all()
+    got[0, 0, 1] = clean[0, 0, 1]
+    assert torch.equal(got, clean)
