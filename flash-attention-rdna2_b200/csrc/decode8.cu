@@ -1056,6 +1056,16 @@ __global__ void __launch_bounds__(MW * 32) dec8_merge_kernel(const FaDec8Params 
     if (tid == 0) store_lse(p, cut.first + row / p.gqa, head, m, l);
     __syncthreads();
   }
+
+  if (!p.cu_q) return;   // rows of no sequence (a padded batch's): 0 and -infinity, a warp a row and head
+  const long long from = min(max((long long)__ldg(p.cu_q), 0ll), p.total), to = min(max((long long)__ldg(p.cu_q + p.batch), from), p.total);
+  for (long long item = blockIdx.x * MW + w; item < (from + p.total - to) * p.NH; item += gridDim.x * MW) {
+    const long long i = item / p.NH, row = i < from ? i : to + i - from;
+    const int head = (int)(item % p.NH);
+    const float zero[2] = {0.f, 0.f};
+    for (int d = 2 * lane; d < p.dim; d += 64) store_row<2>(p, dtype, row * p.NH + head, d, zero);
+    if (lane == 0) store_lse(p, row, head, 0.f, 0.f);
+  }
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {

@@ -79,7 +79,8 @@ def flash_attn_with_kvcache_8bit(q, k_cache, v_cache, k_scale, v_scale, cache_se
     its position, or by rotary_seqlens + t.  max_seqlen_q is a bound on the ragged counts that helps to choose the kernel.
 
     Returns out, shaped as q, or (out, softmax_lse) with return_softmax_lse: (batch, nheads, seqlen_q), or (nheads,
-    total_q) with cu_seqlens_q.  Meant for up to some tens of query rows (tokens times query heads of a kv
+    total_q) with cu_seqlens_q.  Rows that see nothing, and packed rows outside [cu_seqlens_q[0], cu_seqlens_q[-1]) as
+    padded batches have them, are 0 with an LSE of -infinity.  Meant for up to some tens of query rows (tokens times query heads of a kv
     head) per sequence; longer chunks: kvcache_gather and flash_attn_varlen_func."""
     if k_cache.dtype not in _CODE_TYPES:
         raise ValueError(f"fable_attn: an 8-bit cache is torch.int8 or torch.float8_e4m3fn, not {k_cache.dtype}")

@@ -359,7 +359,7 @@ FA_API int fa_kv_gather_launch(const FaKvGatherParams* p, int dtype, void* strea
  * ctx_len[z] - n_z + t and sees the keys in [max(leftpad, pos - win_left), min(ctx_len, pos + win_right + 1))
  * (a bound < 0 is no bound; causal = win_right 0).  Scores scale * q.k, then softcap c * tanh(s / c),
  * then alibi slope * (key - pos), as in the forward; cos / sin rotate q by its position (or rot_pos[z] + t).
- * A row that sees nothing gives 0 and LSE -inf.
+ * A row that sees nothing, or that belongs to no sequence (before cu_q[0], from cu_q[batch] on), gives 0 and LSE -inf.
  *   o    [total, NH, dim] contiguous, dtype of the call (fp16 / bf16 / fp32)
  *   lse  optional fp32 [NH, total], natural log
  *   scratch  fa_decode8_scratch_floats(NH, gqa, dim) floats, whatever the batch or the lengths

@@ -331,3 +331,24 @@ def test_decode_nan_shows_with_and_without_softcap(code, gqa, softcap):
     assert torch.isnan(got[0, 0, 1]).all()
     got[0, 0, 1] = clean[0, 0, 1]
     assert torch.equal(got, clean)
+
+
+@pytest.mark.parametrize("dt", ["fp16", "fp32"])
+@pytest.mark.parametrize("news,cu", [([1, 1], [0, 1, 2]), ([3, 2], [2, 5, 7]), ([0, 0], [0, 0, 0]), ([0, 4], [1, 1, 5])])
+def test_decode_rows_of_no_sequence_are_empty(dt, news, cu):
+    """A padded batch: rows before cu_seqlens_q[0] and from cu_seqlens_q[-1] on give 0 and an LSE of -infinity."""
+    lens, total = [40, 33], 12
+    c = Pool(10, lens, 2, 80, 16, 8, "int8")
+    q = c.randn(total, 6, 80).to(TDT[dt])
+    for _ in range(2):   # what the allocator hands out holds something
+        junk = [torch.full((total, 6, 80), 7.0, dtype=TDT[dt], device="cuda"), torch.full((6, total), 7.0, device="cuda")]
+        del junk
+        out, lse = fa.flash_attn_with_kvcache_8bit(q, c.k, c.v, c.ks, c.vs, i32(lens), c.bt, cu_seqlens_q=i32(cu), max_seqlen_q=4,
+                                                   return_softmax_lse=True)
+    own = slice(cu[0], cu[-1])
+    free = torch.ones(total, dtype=torch.bool, device="cuda")
+    free[own] = False
+    assert (out[free] == 0).all() and torch.isneginf(lse[:, free]).all()
+    if cu[-1] > cu[0]:
+        want = exact(c, q[own], lens, news)
+        check((out[own], lse.t()[own]), want, dt)
