@@ -10,6 +10,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <algorithm>
+#include <climits>
 #include <cmath>
 #include <type_traits>
 #include "fable_attn.h"
@@ -554,6 +555,9 @@ std::vector<torch::Tensor> kv_gather(torch::Tensor k_cache, torch::Tensor v_cach
   return {k, v};
 }
 
+// a bound of any size as an int
+int as_int(int64_t x) { return (int)std::min<int64_t>(x, INT_MAX); }
+
 std::vector<torch::Tensor> dec8(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor k_scale,
                                 torch::Tensor v_scale, torch::Tensor cache_seqlens, torch::Tensor block_table, double scale,
                                 int64_t win_left, int64_t win_right, double softcap, c10::optional<torch::Tensor> alibi,
@@ -585,7 +589,7 @@ std::vector<torch::Tensor> dec8(torch::Tensor q, torch::Tensor k_cache, torch::T
     p.tokens = (int)q.size(1);
   }
   p.total = cu ? q.size(0) : q.size(0) * q.size(1);
-  p.max_tokens = (int)std::max<int64_t>(1, cu ? max_tokens : q.size(1));
+  p.max_tokens = as_int(std::max<int64_t>(1, cu ? max_tokens : q.size(1)));
   if (const auto* t = opt_ptr(leftpad)) {
     lp = index_i32(*t, dev, "cache_leftpad");
     TORCH_CHECK_VALUE(lp.numel() == p.batch, "fable_attn: cache_leftpad needs one entry per sequence");
@@ -613,7 +617,7 @@ std::vector<torch::Tensor> dec8(torch::Tensor q, torch::Tensor k_cache, torch::T
   p.lse = return_lse ? lse.data_ptr<float>() : nullptr;
   p.scratch = scratch.data_ptr<float>();
   p.scale = (float)scale; p.softcap = (float)softcap;
-  p.win_left = (int)win_left; p.win_right = (int)win_right;
+  p.win_left = as_int(win_left); p.win_right = as_int(win_right);
   if (p.total > 0) check(fa_decode8_launch(&p, dt_of(q), cur_stream(q)), "decode (8-bit cache)");
   if (!return_lse) return {out};
   if (!cu) lse = lse.view({Hq, q.size(0), q.size(1)}).transpose(0, 1);   // (batch, nheads, seqlen_q)

@@ -352,3 +352,13 @@ def test_decode_rows_of_no_sequence_are_empty(dt, news, cu):
     if cu[-1] > cu[0]:
         want = exact(c, q[own], lens, news)
         check((out[own], lse.t()[own]), want, dt)
+
+
+def test_window_sizes_beyond_32_bits():
+    c = Pool(11, [60], 2, 64, 16, 8, "int8")
+    q = c.randn(1, 2, 4, 64)
+    args = (q, c.k, c.v, c.ks, c.vs, i32([60]), c.bt)
+    for big in (2 ** 31, 2 ** 32, 2 ** 32 + 3, 2 ** 40):
+        assert torch.equal(fa.flash_attn_with_kvcache_8bit(*args, window_size=(big, 0)), fa.flash_attn_with_kvcache_8bit(*args))
+        assert torch.equal(fa.flash_attn_with_kvcache_8bit(*args, causal=False, window_size=(-1, big)),
+                           fa.flash_attn_with_kvcache_8bit(*args, causal=False))
