@@ -1200,7 +1200,8 @@ extern "C" FA_API int fa_decode8_launch(const FaDec8Params* pp, int dtype, void*
     fa::set_error("8-bit decode: dim=%d must be a multiple of 16 up to 256", p.dim);
     return FA_ERR_UNSUPPORTED;
   }
-  if (p.total == 0 || p.batch == 0) return FA_OK;
+  if (p.total == 0) return FA_OK;
+  FA_CHECK_ARG(p.batch > 0, "8-bit decode: %lld rows of no sequence", p.total);
   if (p.total * p.NH >= 1ll << 31) {
     fa::set_error("8-bit decode: %lld rows of %d heads are more than one call takes", p.total, p.NH);
     return FA_ERR_SIZE;

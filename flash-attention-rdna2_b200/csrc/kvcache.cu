@@ -690,7 +690,8 @@ extern "C" FA_API int fa_kv_append_launch(const FaKvAppendParams* pp, int dtype,
     FA_CHECK_ARG(p.sin && p.rot_dim > 0 && p.rot_dim % 2 == 0 && p.rot_dim <= p.dim && p.rot_seqlen_ro > 0,
                  "kv append: rotary needs sin, an even rot_dim=%d in (0, dim], rot_seqlen_ro=%d > 0", p.rot_dim,
                  p.rot_seqlen_ro);
-  if (p.total == 0 || p.batch == 0) return FA_OK;
+  if (p.total == 0) return FA_OK;
+  FA_CHECK_ARG(p.batch > 0, "kv append: %lld rows of no sequence", p.total);
   if ((p.total + 2ll * p.batch) * p.heads >= 1ll << 30) {
     fa::set_error("kv append: %lld rows of %d heads are more than one call takes", p.total, p.heads);
     return FA_ERR_SIZE;
@@ -710,7 +711,8 @@ extern "C" FA_API int fa_kv_gather_launch(const FaKvGatherParams* pp, int dtype,
   if (!cache_ok(p, "kv gather")) return FA_ERR_INVALID;
   if (!dim_ok(p.dim, "kv gather")) return FA_ERR_UNSUPPORTED;
   FA_CHECK_ARG(p.total >= 0, "kv gather: total=%lld", p.total);
-  if (p.total == 0 || p.batch == 0) return FA_OK;
+  if (p.total == 0) return FA_OK;
+  FA_CHECK_ARG(p.batch > 0, "kv gather: %lld rows of no sequence", p.total);
   if (p.total * p.heads >= 1ll << 31) {
     fa::set_error("kv gather: %lld rows of %d heads are more than one call takes", p.total, p.heads);
     return FA_ERR_SIZE;
