@@ -362,3 +362,64 @@ def test_window_sizes_beyond_32_bits():
         assert torch.equal(fa.flash_attn_with_kvcache_8bit(*args, window_size=(big, 0)), fa.flash_attn_with_kvcache_8bit(*args))
         assert torch.equal(fa.flash_attn_with_kvcache_8bit(*args, causal=False, window_size=(-1, big)),
                            fa.flash_attn_with_kvcache_8bit(*args, causal=False))
+
+
+# ---------------------------------------------------------------------------------------- warps with many strips
+STRIPS = [
+    # code, dtype, page, block, heads, gqa, dim, lens, news, options
+    ("int8", "bf16", 256, 64, 64, 4, 128, [2500, 1], [1, 1], {}),
+    ("e4m3", "bf16", 256, 64, 64, 4, 128, [2500, 1700], [1, 1], {}),
+    ("int8", "fp32", 16, 16, 64, 1, 128, [1999, 2100], [1, 1], {}),
+    ("e4m3", "fp32", 16, 1, 64, 2, 128, [1999, 2100], [1, 1], dict(window=900)),
+    ("int8", "fp16", 4, 4, 64, 2, 128, [1301, 900], [1, 1], {}),
+    ("e4m3", "fp16", 4, 1, 64, 2, 64, [2300, 1900], [1, 1], dict(leftpad=[70, 3])),
+    ("int8", "fp32", 64, 16, 64, 12, 128, [1003, 700], [1, 1], {}),
+    ("e4m3", "fp32", 64, 64, 64, 16, 128, [1003, 700], [1, 1], dict(softcap=30.0)),
+    ("int8", "fp16", 16, 8, 64, 9, 64, [1003, 900], [1, 1], dict(window=333)),
+    ("e4m3", "bf16", 256, 256, 64, 16, 64, [1600, 31], [1, 1], {}),
+    ("int8", "fp32", 64, 8, 64, 1, 64, [3000, 2600], [1, 1], dict(alibi=True)),
+    ("e4m3", "fp32", 256, 32, 64, 8, 64, [3000, 2600], [1, 1], {}),
+    ("int8", "fp16", 16, 16, 64, 4, 256, [700, 650], [1, 1], {}),
+    ("e4m3", "fp32", 64, 2, 64, 2, 192, [700, 650], [1, 1], dict(softcap=20.0)),
+    ("int8", "fp32", 4, 2, 64, 2, 256, [500, 444], [1, 1], dict(alibi=True)),
+    ("int8", "bf16", 64, 16, 64, 4, 128, [900, 1000], [3, 3], {}),
+    ("e4m3", "fp16", 32, 16, 64, 4, 128, [1300, 0, 1], [4, 0, 1], dict(packed=True)),
+    ("int8", "fp32", 32, 16, 64, 2, 96, [1300, 40, 700], [7, 1, 5], dict(packed=True, window=500, softcap=30.0)),
+    ("e4m3", "fp32", 16, 8, 64, 2, 128, [900, 800], [2, 2], dict(causal=False)),
+    ("int8", "fp16", 16, 16, 64, 1, 128, [33 + 11 * i for i in range(40)], [1] * 40, {}),
+    ("e4m3", "fp16", 64, 16, 64, 12, 64, [33 + 11 * i for i in range(30)], [1] * 30, {}),
+    ("int8", "fp32", 128, 32, 128, 1, 128, [3 * i for i in range(60)], [1] * 60, dict(alibi=True)),
+]
+
+
+@pytest.mark.parametrize("case", STRIPS, ids=lambda c: "-".join(map(str, (*c[:7], max(c[7]), max(c[8])))))
+def test_decode_many_strips_a_warp(case):
+    """So many heads and positions that every warp fills its ring again and again: the steady loop, the ring's later rounds,
+    pages ahead, sequences written whole, warps that go on from one sequence to the next."""
+    code, dt, page, block, heads, gqa, dim, lens, news, opt = case
+    opt = dict(opt)
+    c = Pool(12, lens, heads, dim, page, block, code)
+    packed = opt.pop("packed", False)
+    per, stages = strips_a_warp(c, lens, news, gqa, packed)
+    assert per > stages, (per, stages)
+    q = c.randn(sum(news), heads * gqa, dim).to(TDT[dt])
+    if opt.pop("alibi", False):
+        opt["alibi"] = torch.rand(heads * gqa, generator=c.gen, device="cuda") * 0.2
+    check(decode(c, q, lens, news, packed, **opt), exact(c, q, lens, news, **opt), dt)
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("gqa", [1, 12])
+@pytest.mark.parametrize("way", [1, -1])
+def test_decode_maxima_that_grow_or_shrink_along_a_warp(code, gqa, way):
+    """K scales from 2^-6 to 2^6 along the positions, either way: the running maximum moves again and again within a warp."""
+    lens = [1500, 1234]
+    c = Pool(13, lens, 64, 128, 32, 32, code)
+    per, stages = strips_a_warp(c, lens, [1, 1], gqa)
+    assert per > stages
+    for z in range(2):
+        every = c.blocks_of(z, lens[z])
+        for i, (p, j) in enumerate(every):
+            c.ks[p, :, j] = 2.0 ** (way * (12.0 * i / len(every) - 6)) / QMAX[code]
+    q = c.randn(2, 64 * gqa, 128)
+    check(decode(c, q, lens, [1, 1]), exact(c, q, lens, [1, 1]), "fp32")
