@@ -111,6 +111,17 @@ __device__ __forceinline__ float lg2(float x) {
   asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// tanh to a few units of its own last place (a score far below the softcap keeps its bits, which 1 - 2 / (e^2x + 1) would take from
+// it), NaN where x is.  Below 1 the fifth convergent of Lambert's continued fraction x / (1 + x^2 / (3 + x^2 / (5 + ...))), which
+// is 6e-8 off at 1 and less below; above, (e^2x - 1) / (e^2x + 1), with an exponent that keeps the power finite.
+__device__ __forceinline__ float tanh_rel(float x) {
+  const float y = x * x;
+  float e = 2.f * FA_LOG2E * x;
+  asm("min.NaN.f32 %0, %0, %1;" : "+f"(e) : "f"(64.f));
+  e = ex2(e);
+  const bool small = fabsf(x) < 1.f;
+  return __fdividef(small ? x * fmaf(y, y + 105.f, 945.f) : e - 1.f, small ? fmaf(y, fmaf(y, 15.f, 420.f), 945.f) : e + 1.f);
+}
 // 16 bytes to shared memory, zeros where not valid; 4 bytes
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
@@ -705,7 +716,7 @@ __global__ void __launch_bounds__((Cfg<W, RT>::NW * 32), (Cfg<W, RT>::CTAS))
 #pragma unroll
           for (int i = 0; i < NP; ++i)
 #pragma unroll
-            for (int h = 0; h < RPT; ++h) x[h][i] = fmaf(cap_out, fa_tanh<true>(x[h][i]), -m[h]);
+            for (int h = 0; h < RPT; ++h) x[h][i] = fmaf(cap_out, tanh_rel(x[h][i]), -m[h]);
         }
 #pragma unroll
         for (int i = 0; i < NP; ++i) {

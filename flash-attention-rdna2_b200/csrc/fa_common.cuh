@@ -198,13 +198,10 @@ __host__ __device__ __forceinline__ void fa_query_range(int k, int SQ, int SK, i
 // tanh from the identity tanh x = 1 - 2 / (e^(2x) + 1), with e^(2x) = 2^(2x log2 e) on the SFU.
 // The exponent is clamped so the power stays finite (tanh is 1 in fp32 long before); below, the
 // power flushes to 0 and the result is -1.  Absolute error is a few ulp of 1, which is what the
-// softcapped logit cap * tanh(.) needs: its error is then a few ulp of cap.  A NaN gives 1, or, with KEEP_NAN, NaN.
-template <bool KEEP_NAN = false>
+// softcapped logit cap * tanh(.) needs: its error is then a few ulp of cap.
 __device__ __forceinline__ float fa_tanh(float x) {
-  float a = 2.f * FA_LOG2E * x, e;
-  if constexpr (KEEP_NAN) asm("min.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(64.f));
-  else a = fminf(a, 64.f);
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(a));
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fminf(2.f * FA_LOG2E * x, 64.f)));
   return 1.f - __fdividef(2.f, e + 1.f);
 }
 

@@ -423,3 +423,17 @@ def test_decode_maxima_that_grow_or_shrink_along_a_warp(code, gqa, way):
             c.ks[p, :, j] = 2.0 ** (way * (12.0 * i / len(every) - 6)) / QMAX[code]
     q = c.randn(2, 64 * gqa, 128)
     check(decode(c, q, lens, [1, 1]), exact(c, q, lens, [1, 1]), "fp32")
+
+
+@pytest.mark.parametrize("code,gqa,dim", [("int8", 1, 128), ("e4m3", 2, 64), ("int8", 12, 64), ("e4m3", 4, 256)])
+@pytest.mark.parametrize("cap", [30.0, 50.0, 1000.0])
+@pytest.mark.parametrize("size", [1.0, 3.0])
+def test_decode_softcap_far_above_the_scores(code, gqa, dim, cap, size):
+    """Scores far below the cap are the tanh's near 0: a relative error of some 1.5e-7 (rms) of the tanh is as much of a score, 4.5e-7
+    at scores of rms 3, beside 3e-7 of what a decode without softcap is off.  The bar is 1e-6, whatever the cap."""
+    lens = [700, 530]
+    c = Pool(14, lens, 64, dim, 64, 16, code)
+    q = c.randn(2, 64 * gqa, dim)
+    k = c.values("k", 0, 700)
+    scale = size / float(torch.einsum("hgd,lhd->hgl", q[0].double().view(64, gqa, dim), k).square().mean().sqrt())
+    check(decode(c, q, lens, [1, 1], softcap=cap, scale=scale), exact(c, q, lens, [1, 1], softcap=cap, scale=scale), "fp32", 1e-6)
