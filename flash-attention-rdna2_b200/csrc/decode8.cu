@@ -4,7 +4,8 @@
 // One pass over the cache with a running maximum and sum.  For a key j with codes c_j, d_j and block
 // scales ks_j, vs_j, and in base 2:  x_j = scale log2(e) ks_j (q . c_j),  o = sum 2^(x_j - m) vs_j d_j / sum 2^(x_j - m).
 // The value scale joins the weight, w_j = 2^(x_j - m) vs_j u, where u is a power of two of the row's own that keeps the
-// largest weight so far in fp16's range whatever the scales: the tensor cores take V codes (exact in
+// largest weight that still counts in fp16's range, whatever the scales (for V values up to 2^100, that sums stay finite): it
+// falls where a weight would leave that range, and rises as m does.  The tensor cores take V codes (exact in
 // fp16) and weights (fp16 high and low part, 22 bits) as they are, and dividing by u at the end is exact.
 //
 // The floor is the bytes of the cache.  What is read goes through registers to mma.sync (m16n8k16, fp16
@@ -30,10 +31,11 @@
 // writes its output, others leave (m, l, o) in one of the warp's two slots, and a merge kernel joins the slots of each
 // cut sequence in order (no atomics: same bits on every call).
 //
-// Measured, both kernels: 16 x 16-32k tokens, 8 kv heads, headdim 128, one token of 32 heads (806 MB): int8 166 us
-// (4.9 TB/s), e4m3 160 us (5.0 TB/s); 48 x 1-9k e4m3 108 us (4.6 TB/s); one int8 document of 131k 73 us (3.7 TB/s); 24 windows
-// of 4k with 1-4 tokens each, int8, 90 us; 1 x 611 12.5 us.  What bounds it: an SM holds 8 warps of 240 registers, whose conversions,
-// mma and softmax (135 us by themselves when the first case took 181) and copies (141 us) overlap only in part.
+// Measured, both kernels, replayed as a graph: 16 x 16-32k tokens, 8 kv heads, headdim 128, one token of 32 heads (806 MB): int8
+// 166 us (4.8 TB/s), e4m3 163 us (4.9 TB/s), and 170 to 179 us either in a long loop, which the card's power limit slows; with 16
+// heads a kv head 252 and 253 us; 48 x 1-9k e4m3 108 us (4.6 TB/s); one int8 document of 131k 73 us (3.7 TB/s); 24 windows
+// of 4k with 1-4 tokens each, int8, softcap, 88 us; 1 x 611 12.5 us.  What bounds it: an SM holds 8 warps of 240 registers, whose
+// conversions, mma and softmax (135 us by themselves when the first case took 181) and copies (141 us) overlap only in part.
 #include <cudaTypedefs.h>
 #include <algorithm>
 #include <type_traits>
@@ -1142,10 +1144,11 @@ int by_page(const FaDec8Params& p, int dtype, cudaStream_t st) {
 template <int W, typename Q>
 int by_rows(const FaDec8Params& p, int dtype, cudaStream_t st) {
   // More than 8 rows a sequence: one pass over the cache with 16 rows, or tiles of 8 that each make a pass.  16 rows win
-  // where every sequence has them (16 x 16-32k tokens, 16 heads a kv head, headdim 128: int8 256 against 299 us, e4m3 260
-  // against 286); tiles win where counts are ragged, since most tiles of 16 are then half empty (1 to 4 tokens of 4 heads, 24
-  // x 1-20k int8 tokens: 105 against 90 us), and for rows of 256, whose 16-row form has one warp a scheduler (16 x 1-9k tokens, 16 heads,
-  // before int8 took integer mma: 127 against 108 us).
+  // where every sequence has them (16 x 16-32k tokens, 16 heads a kv head, headdim 128: int8 252 against 301 us, e4m3 254
+  // against 299; headdim 64, int8: 205 against 193); tiles win where counts are ragged, since most tiles of 16 are then half
+  // empty (1 to 4 tokens of 4 heads, 24 x 1-20k int8 tokens, window 4096 and softcap: 104 against 88 us, without either 185
+  // against 157), and for rows of 256, whose 16-row form has one warp a scheduler (16 x 1-9k tokens, 16 heads, before int8 took
+  // integer mma: 127 against 108 us).
   const bool full = p.gqa > 8 || (!p.cu_q && (long long)p.gqa * p.tokens > 8);
   if constexpr (W <= 128)
     if (full) return by_page<W, Q, 16>(p, dtype, st);

@@ -44,7 +44,11 @@ def kvcache_append(k, v, k_cache, v_cache, cache_seqlens, block_table, *, k_scal
     as (total_new, nheads_k, headdim); fp16, bf16 or fp32.  cache_seqlens (batch): tokens in the cache BEFORE
     the call; token i goes to position cache_seqlens + i (the caller advances cache_seqlens).
     rotary_cos / rotary_sin (seqlen_ro, rotary_dim / 2) rotate k at its position, or at rotary_seqlens + i, in fp32
-    with one rounding at the end.
+    with one rounding at the end.  A sequence with no new tokens is left alone, and so is what cu_seqlens_new names beyond
+    the rows given.
+
+    Fast are rows on 16-byte boundaries, a rotary_dim that is a multiple of 16 and, in 8 bits, pages of 16 slots or more; other
+    calls go element by element and take 5 to 7 times as long.
 
     The cache has k's type, or is 8-bit with k_scale / v_scale.  Then each touched block of slots gets
     s = max(its scale so far, amax / Q, 2**-100), Q = 127 or 448, its scale so far counting only where the block holds
@@ -81,7 +85,8 @@ def flash_attn_with_kvcache_8bit(q, k_cache, v_cache, k_scale, v_scale, cache_se
     Returns out, shaped as q, or (out, softmax_lse) with return_softmax_lse: (batch, nheads, seqlen_q), or (nheads,
     total_q) with cu_seqlens_q.  Rows that see nothing, and packed rows outside [cu_seqlens_q[0], cu_seqlens_q[-1]) as
     padded batches have them, are 0 with an LSE of -infinity.  Meant for up to some tens of query rows (tokens times query heads of a kv
-    head) per sequence; longer chunks: kvcache_gather and flash_attn_varlen_func."""
+    head) per sequence; longer chunks: kvcache_gather and flash_attn_varlen_func.  V's values may be up to 2**100.  Pages of
+    less than 16 slots take about 1.7 times as long."""
     if k_cache.dtype not in _CODE_TYPES:
         raise ValueError(f"fable_attn: an 8-bit cache is torch.int8 or torch.float8_e4m3fn, not {k_cache.dtype}")
     if softmax_scale is None:

@@ -312,7 +312,8 @@ FA_API long long fa_decode_scratch_floats(int batch, int nq, int NH, int HD, int
  * A NaN or an infinity among the new values makes s NaN and their codes 0, and a NaN scale lasts
  * until the block is begun anew: what is read from the block is NaN, codes are always finite.
  *   new rows [row][heads][dim] with element strides (dim contiguous): dense rows z * tokens + i, or,
- *   with cu_new [batch + 1], rows cu_new[z] + i.  `total` = rows.
+ *   with cu_new [batch + 1], rows cu_new[z] + i.  `total` = rows; what cu_new names outside [0, total) is not read, and a
+ *   sequence without rows is left alone, its pages not looked at.
  * -------------------------------------------------------------------------------------------*/
 typedef struct FaKvAppendParams {
   unsigned int struct_size;
@@ -357,7 +358,7 @@ FA_API int fa_kv_gather_launch(const FaKvGatherParams* p, int dtype, void* strea
  * first).  q rows [row][NH][dim] by strides, dense rows z * tokens + t or, with cu_q, cu_q[z] + t, n_z
  * of them in sequence z; ctx_len[z] cached tokens, the new ones included.  Row t sits at position
  * ctx_len[z] - n_z + t and sees the keys in [max(leftpad, pos - win_left), min(ctx_len, pos + win_right + 1))
- * (a bound < 0 is no bound; causal = win_right 0).  Scores scale * q.k, then softcap c * tanh(s / c),
+ * (a bound < 0 is no bound; causal = win_right 0; V values up to 2^100).  Scores scale * q.k, then softcap c * tanh(s / c),
  * then alibi slope * (key - pos), as in the forward; cos / sin rotate q by its position (or rot_pos[z] + t).
  * A row that sees nothing, or that belongs to no sequence (before cu_q[0], from cu_q[batch] on), gives 0 and LSE -inf.
  *   o    [total, NH, dim] contiguous, dtype of the call (fp16 / bf16 / fp32)
