@@ -437,3 +437,23 @@ def test_decode_softcap_far_above_the_scores(code, gqa, dim, cap, size):
     k = c.values("k", 0, 700)
     scale = size / float(torch.einsum("hgd,lhd->hgl", q[0].double().view(64, gqa, dim), k).square().mean().sqrt())
     check(decode(c, q, lens, [1, 1], softcap=cap, scale=scale), exact(c, q, lens, [1, 1], softcap=cap, scale=scale), "fp32", 1e-6)
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("gqa", [1, 12])
+@pytest.mark.parametrize("power", [-100, 100])
+def test_decode_values_at_the_ends_of_their_range(code, gqa, power):
+    """V up to 2^100 in size, and as small, in long sums whose maximum grows: finite, and each row to 1e-5."""
+    lens = [1500, 1234]
+    c = Pool(15, lens, 64, 128, 32, 32, code)
+    c.vs.copy_(torch.full_like(c.vs, 2.0 ** power / QMAX[code]))
+    for z in range(2):
+        every = c.blocks_of(z, lens[z])
+        for i, (p, j) in enumerate(every):
+            c.ks[p, :, j] = 2.0 ** (6.0 * i / len(every) - 4) / QMAX[code]
+    q = c.randn(2, 64 * gqa, 128)
+    got, want = decode(c, q, lens, [1, 1]), exact(c, q, lens, [1, 1])
+    assert torch.isfinite(got[0]).all()
+    f = 2.0 ** -power                 # norms of such values are beyond fp32, and 2^-100 squared is
+    err = (got[0].double() * f - want[0] * f).norm(dim=-1) / (want[0] * f).norm(dim=-1)
+    assert float(err.max()) <= 1e-5, float(err.max())
