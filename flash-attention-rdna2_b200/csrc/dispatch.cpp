@@ -3,10 +3,11 @@
 // Same function names and argument order as the reference's extension
 // (package/csrc/dispatch.cpp:239-267): fwd, bwd, fwd_varlen, dec; plus bwd_varlen (native varlen
 // backward), combine (flash_attn_combine on the GPU), kv_append / kv_gather / dec8 (paged caches held in
-// 8 bits) and kernel_launch_count.
+// 8 bits), linear_fwd / linear_bwd (linear attention), rotary_qk and kernel_launch_count.
 // Outputs and workspaces (out, lse, dq/dk/dv, dsum, decode scratch) are allocated here by torch,
 // as in the reference; kernels own nothing.  No host synchronisation anywhere.
 #include <torch/extension.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <algorithm>
@@ -718,6 +719,218 @@ void peer_step_end(torch::Tensor peer_bufs, torch::Tensor peer_signals, int64_t 
   check(fa_peer_step_end_launch(&p, cur_stream(step)), "peer step end");
 }
 
+// ------------------------------------------------------------------ linear attention with a decay per head
+// (batch, seqlen, heads, dim) or, packed, (total, heads, dim), dim contiguous, as strides of [batch, heads, seq, dim]
+FaStrides rows_of_heads(const torch::Tensor& x) {
+  if (x.dim() == 3) return FaStrides{0, x.stride(1), x.stride(0)};
+  return FaStrides{x.stride(0), x.stride(2), x.stride(1)};
+}
+
+// what the forward and the backward check alike: shapes, types, the device, the packed rows' bounds
+template <typename P>
+struct LinearCall {
+  torch::Tensor q, k, v, decay, cu;
+  bool packed = false;
+  LinearCall(P& p, const torch::Tensor& q_, const torch::Tensor& k_, const torch::Tensor& v_, const torch::Tensor& log_decay,
+             double scale, const c10::optional<torch::Tensor>& cu_, int64_t max_seqlen) {
+    const auto* c = opt_ptr(cu_);
+    packed = c != nullptr;
+    const int hd = packed ? 1 : 2;
+    const char* shape = packed ? "(total, nheads, headdim) with cu_seqlens" : "(batch, seqlen, nheads, headdim)";
+    for (const auto* x : {&q_, &k_, &v_}) {
+      TORCH_CHECK_VALUE(x->is_cuda(), "fable_attn: linear attention needs CUDA tensors");
+      TORCH_CHECK_VALUE(x->dim() == hd + 2, "fable_attn: linear attention expects ", shape, ", got ", x->sizes());
+      TORCH_CHECK_VALUE(x->device() == q_.device() && x->scalar_type() == q_.scalar_type(),
+                        "fable_attn: q, k and v must have one type and lie on one device");
+      for (int d = 0; d < hd; ++d)
+        TORCH_CHECK_VALUE(x->size(d) == q_.size(d) && x->size(d) <= INT_MAX, "fable_attn: q, k and v must agree on batch and length, got ",
+                          q_.sizes(), ", ", x->sizes());
+    }
+    dt_of(q_);
+    const int64_t hq = q_.size(hd), hk = k_.size(hd);
+    TORCH_CHECK_VALUE(hk > 0 && hq > 0 && hq % hk == 0 && v_.size(hd) == hk, "fable_attn: nheads_q=", hq,
+                      " must be a multiple of nheads_k=", hk, ", and v has ", v_.size(hd), " heads");
+    TORCH_CHECK_VALUE(q_.size(hd + 1) == k_.size(hd + 1), "fable_attn: q and k must have one headdim, got ", q_.size(hd + 1), " and ",
+                      k_.size(hd + 1));
+    for (const int64_t d : {q_.size(hd + 1), v_.size(hd + 1)})
+      TORCH_CHECK_VALUE(d > 0 && d <= 256 && d % 8 == 0, "fable_attn: headdim=", d, " must be a multiple of 8 up to 256");
+    TORCH_CHECK_VALUE(log_decay.is_cuda() && log_decay.device() == q_.device() && log_decay.dim() == 1 && log_decay.size(0) == hk &&
+                          log_decay.is_floating_point(),
+                      "fable_attn: log_decay must be (nheads_k,) = (", hk, ",) floating point values on q's device");
+    const auto last = [](const torch::Tensor& x) { return x.stride(-1) == 1 ? x : x.contiguous(); };
+    q = last(q_); k = last(k_); v = last(v_);
+    decay = table_f32(log_decay);
+    p.struct_size = sizeof(P);
+    p.log_decay = decay.template data_ptr<float>();
+    if (packed) {
+      cu = index_i32(*c, q.device(), "cu_seqlens");
+      TORCH_CHECK_VALUE(cu.dim() == 1 && cu.numel() >= 1, "fable_attn: cu_seqlens must be (batch + 1,)");
+      p.cu = cu.template data_ptr<int>();
+      p.batch = (int)cu.numel() - 1;
+      p.total = q.size(0);
+      p.S = max_seqlen > 0 ? (int)std::min<int64_t>(max_seqlen, p.total) : (int)p.total;
+      TORCH_CHECK_VALUE(p.batch > 0 || p.total == 0, "fable_attn: ", p.total, " rows and no sequence in cu_seqlens");
+    } else {
+      p.batch = (int)q.size(0);
+      p.S = (int)q.size(1);
+    }
+    p.q = q.data_ptr(); p.k = k.data_ptr(); p.v = v.data_ptr();
+    p.sQ = rows_of_heads(q); p.sK = rows_of_heads(k); p.sV = rows_of_heads(v);
+    p.NH = (int)hq; p.gqa = (int)(hq / hk);
+    p.dk = (int)q.size(hd + 1); p.dv = (int)v.size(hd + 1);
+    p.scale = (float)scale;
+  }
+  // states (slots, nheads_k, dk, dv) fp32
+  void check_states(const P& p, const torch::Tensor& s, const char* name, int64_t slots) const {
+    TORCH_CHECK_VALUE(s.is_cuda() && s.device() == q.device() && s.scalar_type() == torch::kFloat32 && s.is_contiguous() && s.dim() == 4 &&
+                          (slots < 0 || s.size(0) == slots) && s.size(1) == p.NH / p.gqa && s.size(2) == p.dk && s.size(3) == p.dv,
+                      "fable_attn: ", name, " must be contiguous fp32 (", slots < 0 ? std::string("slots") : std::to_string(slots), ", ",
+                      p.NH / p.gqa, ", ", p.dk, ", ", p.dv, ") on q's device, got ", s.sizes());
+  }
+};
+
+// (out, states kept for the backward, seg_len, nseg).  state_in / state_out are pools found by index, or (index None) one slot for
+// each sequence.
+std::tuple<torch::Tensor, torch::Tensor, int64_t, int64_t> linear_fwd(
+    torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor log_decay, double scale, c10::optional<torch::Tensor> state_in,
+    c10::optional<torch::Tensor> state_out, c10::optional<torch::Tensor> index, c10::optional<torch::Tensor> seen,
+    c10::optional<torch::Tensor> cu, int64_t max_seqlen, bool keep_states) {
+  TORCH_CHECK_VALUE(q.is_cuda(), "fable_attn: linear attention needs CUDA tensors");
+  const c10::cuda::CUDAGuard guard(q.device());
+  FaLinearParams p{};
+  const LinearCall<FaLinearParams> call(p, q, k, v, log_decay, scale, cu, max_seqlen);
+  torch::Tensor idx, sn;
+  const auto *si = opt_ptr(state_in), *so = opt_ptr(state_out);
+  if (const auto* i = opt_ptr(index)) {
+    TORCH_CHECK_VALUE(si || so, "fable_attn: state_indices without a state");
+    idx = index_i32(*i, q.device(), "state_indices");
+    TORCH_CHECK_VALUE(idx.numel() == p.batch, "fable_attn: state_indices needs one entry per sequence");
+    p.state_index = idx.data_ptr<int>();
+  }
+  if (const auto* s = opt_ptr(seen)) {
+    sn = index_i32(*s, q.device(), "cache_seqlens");
+    TORCH_CHECK_VALUE(sn.numel() == p.batch, "fable_attn: cache_seqlens needs one entry per sequence");
+    p.seen = sn.data_ptr<int>();
+  }
+  const int64_t slots = p.state_index ? -1 : p.batch;
+  if (si) call.check_states(p, *si, "the state", slots);
+  if (so) call.check_states(p, *so, "the new state", si ? si->size(0) : slots);
+  p.slots = si ? si->size(0) : so ? so->size(0) : 0;
+  p.state_in = si ? si->const_data_ptr<float>() : nullptr;
+  p.state_out = so ? so->data_ptr<float>() : nullptr;
+  auto shape = call.q.sizes().vec();
+  shape.back() = p.dv;
+  auto out = torch::empty(shape, call.q.options());
+  p.o = out.data_ptr();
+  p.sO = rows_of_heads(out);
+  p.keep_states = keep_states ? 1 : 0;
+  const long long floats = fa_linear_plan(p.batch, p.S, p.total, p.NH, p.gqa, p.dk, p.dv, dt_of(q), &p.seg_len, &p.nseg);
+  auto work = torch::empty({floats}, call.decay.options());
+  p.states = floats ? work.data_ptr<float>() : nullptr;
+  if (p.batch > 0) check(fa_linear_launch(&p, dt_of(q), cur_stream(q)), "linear attention");
+  return {out, work, p.seg_len, p.nseg};
+}
+
+// (dq, dk, dv, dinitial or an empty tensor)
+std::vector<torch::Tensor> linear_bwd(torch::Tensor dout, torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor log_decay,
+                                      double scale, c10::optional<torch::Tensor> initial, c10::optional<torch::Tensor> dfinal,
+                                      bool want_dinitial, c10::optional<torch::Tensor> cu, int64_t max_seqlen, torch::Tensor states,
+                                      int64_t seg_len, int64_t nseg) {
+  const c10::cuda::CUDAGuard guard(q.device());
+  FaLinearBwdParams p{};
+  const LinearCall<FaLinearBwdParams> call(p, q, k, v, log_decay, scale, cu, max_seqlen);
+  auto shape = call.q.sizes().vec();
+  shape.back() = p.dv;
+  TORCH_CHECK_VALUE(dout.is_cuda() && dout.sizes() == c10::IntArrayRef(shape) && dout.scalar_type() == q.scalar_type() && dout.device() == q.device(),
+                    "fable_attn: the output's gradient must have the output's shape and type");
+  const torch::Tensor d = dout.stride(-1) == 1 ? dout : dout.contiguous();
+  torch::Tensor df;
+  if (const auto* x = opt_ptr(dfinal)) {
+    df = x->contiguous();
+    call.check_states(p, df, "the final state's gradient", p.batch);
+    p.dfinal = df.const_data_ptr<float>();
+  }
+  if (const auto* x = opt_ptr(initial)) {
+    call.check_states(p, *x, "the initial state", p.batch);
+    p.initial = x->const_data_ptr<float>();
+  }
+  auto dq = torch::empty(call.q.sizes(), call.q.options()), dk = torch::empty(call.k.sizes(), call.k.options()),
+       dv = torch::empty(call.v.sizes(), call.v.options());
+  auto dinit = torch::empty({0}, call.decay.options());
+  if (want_dinitial) {
+    dinit = torch::empty({p.batch, p.NH / p.gqa, p.dk, p.dv}, call.decay.options());
+    p.dinitial = dinit.data_ptr<float>();
+  }
+  auto work = torch::empty_like(states);
+  p.dO = d.data_ptr(); p.dQ = dq.data_ptr(); p.dK = dk.data_ptr(); p.dV = dv.data_ptr();
+  p.sdO = rows_of_heads(d); p.sdQ = rows_of_heads(dq); p.sdK = rows_of_heads(dk); p.sdV = rows_of_heads(dv);
+  p.seg_len = (int)seg_len; p.nseg = (int)nseg;
+  TORCH_CHECK_VALUE(nseg <= 1 || states.numel() == nseg * p.batch * (p.NH / p.gqa) * p.dk * p.dv,
+                    "fable_attn: `states` is not this forward's");
+  p.states = states.numel() ? states.const_data_ptr<float>() : nullptr;
+  p.work = states.numel() ? work.data_ptr<float>() : nullptr;
+  if (p.batch > 0) check(fa_linear_backward_launch(&p, dt_of(q), cur_stream(q)), "linear attention backward");
+  return {dq, dk, dv, dinit};
+}
+
+// ------------------------------------------------------------------ rotary of q and k at given positions
+std::tuple<torch::Tensor, torch::Tensor> rotary_qk(torch::Tensor q, torch::Tensor k, torch::Tensor inv_freq,
+                                                   c10::optional<torch::Tensor> positions, py::object offsets, bool interleaved,
+                                                   bool inplace, double factor, bool inverse) {
+  TORCH_CHECK_VALUE(q.is_cuda() && k.is_cuda() && k.device() == q.device() && k.scalar_type() == q.scalar_type(),
+                    "fable_attn: rotary needs q and k of one type on one CUDA device");
+  const int hd = (int)q.dim() - 2;
+  TORCH_CHECK_VALUE((hd == 1 || hd == 2) && k.dim() == q.dim(), "fable_attn: rotary expects (batch, seqlen, nheads, headdim) or (total, "
+                    "nheads, headdim), got ", q.sizes(), " and ", k.sizes());
+  for (int d = 0; d < hd; ++d)
+    TORCH_CHECK_VALUE(k.size(d) == q.size(d), "fable_attn: q and k must agree on batch and length, got ", q.sizes(), " and ", k.sizes());
+  TORCH_CHECK_VALUE(k.size(hd + 1) == q.size(hd + 1), "fable_attn: q and k must have one headdim");
+  const c10::cuda::CUDAGuard guard(q.device());
+  FaRotaryQkParams p{};
+  p.struct_size = sizeof(p);
+  p.batch = hd == 2 ? (int)q.size(0) : 1;
+  p.seqlen = (int)q.size(hd - 1);
+  TORCH_CHECK_VALUE(q.size(0) <= INT_MAX && q.size(hd - 1) <= INT_MAX, "fable_attn: rotary of ", q.sizes());
+  p.heads_q = (int)q.size(hd); p.heads_k = (int)k.size(hd); p.dim = (int)q.size(hd + 1);
+  TORCH_CHECK_VALUE(p.heads_q > 0 && p.heads_k > 0, "fable_attn: rotary needs heads, got ", q.sizes(), " and ", k.sizes());
+  TORCH_CHECK_VALUE(inv_freq.is_cuda() && inv_freq.device() == q.device() && inv_freq.dim() == 1 && inv_freq.is_floating_point() &&
+                        inv_freq.numel() > 0 && 2 * inv_freq.numel() <= p.dim,
+                    "fable_attn: inv_freq must be (rotary_dim / 2,) floating point values on q's device with rotary_dim <= headdim");
+  const torch::Tensor f = inv_freq.to(torch::kFloat64).contiguous();
+  p.inv_freq = f.const_data_ptr<double>();
+  p.rot_dim = 2 * (int)f.numel();
+  torch::Tensor pos, offs;
+  if (const auto* t = opt_ptr(positions)) {
+    TORCH_CHECK_VALUE(t->scalar_type() == torch::kInt32 || t->scalar_type() == torch::kInt64, "fable_attn: positions must be int32 or int64");
+    TORCH_CHECK_VALUE(t->device() == q.device() && t->sizes() == q.sizes().slice(0, hd), "fable_attn: positions must be ",
+                      q.sizes().slice(0, hd), " on q's device, got ", t->sizes());
+    TORCH_CHECK_VALUE(py::isinstance<py::int_>(offsets) && offsets.cast<int64_t>() == 0, "fable_attn: positions and seqlen_offsets exclude each other");
+    pos = t->contiguous();
+    p.positions = pos.const_data_ptr();
+    p.pos_bytes = (int)pos.element_size();
+  } else if (py::isinstance<py::int_>(offsets)) {
+    p.offset = offsets.cast<int64_t>();
+  } else {
+    offs = index_i32(offsets.cast<torch::Tensor>(), q.device(), "seqlen_offsets");
+    TORCH_CHECK_VALUE(offs.numel() == p.batch, "fable_attn: seqlen_offsets needs one entry per sequence");
+    p.offsets = offs.data_ptr<int>();
+  }
+  const auto last = [](const torch::Tensor& x) { return x.stride(-1) == 1 || x.size(-1) == 1 ? x : x.contiguous(); };
+  const torch::Tensor qs = last(q), ks = last(k);
+  if (inplace) {
+    TORCH_CHECK_VALUE(qs.is_same(q) && ks.is_same(k), "fable_attn: inplace rotary needs a contiguous last dimension");
+    at::assert_no_internal_overlap(q);
+    at::assert_no_internal_overlap(k);
+  }
+  const torch::Tensor qo = inplace ? q : torch::empty(q.sizes(), q.options()), ko = inplace ? k : torch::empty(k.sizes(), k.options());
+  p.q = qs.const_data_ptr(); p.k = ks.const_data_ptr(); p.q_out = qo.data_ptr(); p.k_out = ko.data_ptr();
+  p.sQ = rows_of_heads(qs); p.sK = rows_of_heads(ks); p.sQo = rows_of_heads(qo); p.sKo = rows_of_heads(ko);
+  p.interleaved = interleaved ? 1 : 0; p.inverse = inverse ? 1 : 0;
+  p.factor = (float)factor;
+  if (q.numel() > 0) check(fa_rotary_qk_launch(&p, dt_of(q), cur_stream(q)), "rotary (q and k)");
+  return {qo, ko};
+}
+
 }  // namespace
 
 // ------------------------------------------------------------------ rotary (q / k, one pass)
@@ -814,6 +1027,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("softcap"), py::arg("alibi"), py::arg("cu_q"), py::arg("max_tokens"), py::arg("leftpad"),
         py::arg("rotary_cos"), py::arg("rotary_sin"), py::arg("rotary_interleaved"), py::arg("rotary_pos"),
         py::arg("return_lse"));
+  m.def("linear_fwd", &linear_fwd, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("log_decay"), py::arg("scale"),
+        py::arg("state_in"), py::arg("state_out"), py::arg("state_index"), py::arg("seen"), py::arg("cu_seqlens"),
+        py::arg("max_seqlen"), py::arg("keep_states"));
+  m.def("linear_bwd", &linear_bwd, py::arg("dout"), py::arg("q"), py::arg("k"), py::arg("v"), py::arg("log_decay"),
+        py::arg("scale"), py::arg("initial"), py::arg("dfinal"), py::arg("want_dinitial"), py::arg("cu_seqlens"),
+        py::arg("max_seqlen"), py::arg("states"), py::arg("seg_len"), py::arg("nseg"));
+  m.def("rotary_qk", &rotary_qk, py::arg("q"), py::arg("k"), py::arg("inv_freq"), py::arg("positions"), py::arg("offsets"),
+        py::arg("interleaved"), py::arg("inplace"), py::arg("factor"), py::arg("inverse"));
   m.def("combine", &combine, py::arg("out_partial"), py::arg("lse_partial"), py::arg("out_dtype"),
         py::arg("return_lse") = false);
   m.def("combine_packed", &combine_packed, py::arg("buf"), py::arg("nsplit"), py::arg("B"), py::arg("S"),

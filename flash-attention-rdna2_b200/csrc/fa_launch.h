@@ -24,6 +24,7 @@ int dec_tc_device_error(int clear);
 int rot_device_error(int clear);        // bit 0: a rotary position outside the cos/sin table
 int kv_device_error(int clear);        // bits of the paged-cache append / gather (kvcache.cu)
 int dec8_device_error(int clear);      // bits of the 8-bit decode
+int lin_device_error(int clear);       // linear attention: bit 0 a bad state slot, bit 1 a wait that gave up
 int fwd_simt_device_error(int clear);   // bit 0: an invalid block-table entry (paged forward)
 // FABLE_ATTN_NO_PDL set: launch every kernel plainly (no programmatic dependent launch)
 bool pdl_enabled();

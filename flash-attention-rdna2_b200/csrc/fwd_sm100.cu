@@ -1336,5 +1336,5 @@ extern "C" FA_API int fa_device_error(int clear) {
   }
   return v | (fa::dec_device_error(clear) ? 64 : 0) | (fa::bwd_device_error(clear) ? 128 : 0) |
          (fa::rot_device_error(clear) ? 256 : 0) | (fa::fwd_simt_device_error(clear) ? 1024 : 0) |
-         fa::kv_device_error(clear) | fa::dec8_device_error(clear);
+         fa::kv_device_error(clear) | fa::dec8_device_error(clear) | fa::lin_device_error(clear) * 131072;
 }

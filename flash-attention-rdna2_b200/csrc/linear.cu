@@ -1,0 +1,466 @@
+// linear.cu — linear attention with a decay per head: the recurrent kernel for few tokens, the CUDA-core kernels that take
+// every type and head dim, the kernel that joins segments, and the entry points.
+#include <algorithm>
+#include "linear_common.cuh"
+#include "fa_launch.h"
+
+namespace {
+
+using namespace fa;
+
+__device__ int g_lin_error = 0;
+
+// =====================================================================================
+// Recurrent kernel: S_t = lam S_{t-1} + k_t v_t^T, o_t = scale S_t^T q_t, token by token.
+// Bound by reading and writing the state once: 8 dk dv bytes a sequence and head.  A block holds 32 columns of one state
+// (a 128-byte line of each row) in registers, so that a state of 128 columns gives four blocks and small batches still spread;
+// all its loads are issued before the first token is looked at.
+// =====================================================================================
+constexpr int STEP_THREADS = 128, STEP_COLS = 32;
+
+template <typename T, int ROWS>   // ROWS = rows of the state a thread holds: dk <= 16 * ROWS
+__global__ void __launch_bounds__(STEP_THREADS)
+    lin_step_kernel(const LinSeqs q, const LinRole r, const LinPool pool, const int blocks_v) {
+  constexpr int GMAX = 4;                                    // query heads of a group that are summed together
+  __shared__ float sk[256], sq[GMAX][256], sred[4][GMAX][STEP_COLS];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int vb = blockIdx.x % blocks_v, h = (blockIdx.x / blocks_v) % q.nhk, z = blockIdx.x / blocks_v / q.nhk;
+  if (vb == 0) lin_zero_outside<T>(q, r, z, h * r.na, 0, 1, STEP_THREADS);
+  const LinSpan span = lin_span(q, z);
+  const int slot = lin_slot(pool, z, STEP_THREADS, &g_lin_error);
+  T* out = (T*)r.out + (q.cu ? 0 : z * r.so.b) + span.row0 * r.so.s + (long long)h * r.na * r.so.h;
+  const int col = vb * STEP_COLS + (tid & 7) * 4, row0 = tid >> 3;
+  const bool mine = col < r.dc;
+  if (slot < 0) {
+    for (int e = tid; e < span.len * r.na * STEP_COLS; e += STEP_THREADS) {
+      const int c = vb * STEP_COLS + e % STEP_COLS, g = e / STEP_COLS % r.na, t = e / STEP_COLS / r.na;
+      if (c < r.dc) out[t * r.so.s + g * r.so.h + c] = Elem<T>::from_f(0.f);
+    }
+    return;
+  }
+  const long long at = ((long long)slot * q.nhk + h) * r.da * r.dc + col;
+  const bool old = pool.in && !(pool.seen && pool.seen[z] <= 0);
+  float4 x[ROWS];
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int row = row0 + 16 * i;
+    x[i] = old && mine && row < r.da ? *reinterpret_cast<const float4*>(pool.in + at + (long long)row * r.dc) : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  const float lam = exp2f(lin_log2_decay(q.log_decay, h));
+  const T* a = (const T*)r.a + (q.cu ? 0 : z * r.sa.b) + span.row0 * r.sa.s + (long long)h * r.na * r.sa.h;
+  const T* b = (const T*)r.b + (q.cu ? 0 : z * r.sb.b) + span.row0 * r.sb.s + (long long)h * r.sb.h;
+  const T* c = (const T*)r.c + (q.cu ? 0 : z * r.sc.b) + span.row0 * r.sc.s + (long long)h * r.sc.h;
+  for (int t = 0; t < span.len; ++t) {
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (mine) {
+      const T* cr = c + t * r.sc.s + col;
+      v = make_float4(Elem<T>::to_f(cr[0]), Elem<T>::to_f(cr[1]), Elem<T>::to_f(cr[2]), Elem<T>::to_f(cr[3]));
+    }
+    for (int g0 = 0; g0 < r.na; g0 += GMAX) {
+      const int ng = min(GMAX, r.na - g0);
+      __syncthreads();
+      if (g0 == 0)
+        for (int e = tid; e < r.da; e += STEP_THREADS) sk[e] = Elem<T>::to_f(b[t * r.sb.s + e]);
+      for (int e = tid; e < ng * r.da; e += STEP_THREADS)
+        sq[e / r.da][e % r.da] = Elem<T>::to_f(a[t * r.sa.s + (g0 + e / r.da) * r.sa.h + e % r.da]);
+      __syncthreads();
+      float4 o[GMAX];
+#pragma unroll
+      for (int g = 0; g < GMAX; ++g) o[g] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) {
+        const int row = row0 + 16 * i;
+        if (row < r.da) {
+          if (g0 == 0) {
+            const float k = sk[row];
+            x[i].x = fmaf(lam, x[i].x, k * v.x);
+            x[i].y = fmaf(lam, x[i].y, k * v.y);
+            x[i].z = fmaf(lam, x[i].z, k * v.z);
+            x[i].w = fmaf(lam, x[i].w, k * v.w);
+          }
+#pragma unroll
+          for (int g = 0; g < GMAX; ++g)
+            if (g < ng) {
+              const float w = sq[g][row];
+              o[g].x = fmaf(w, x[i].x, o[g].x);
+              o[g].y = fmaf(w, x[i].y, o[g].y);
+              o[g].z = fmaf(w, x[i].z, o[g].z);
+              o[g].w = fmaf(w, x[i].w, o[g].w);
+            }
+        }
+      }
+      // lanes of one column group differ in bits 3 and 4; then the four warps
+#pragma unroll
+      for (int g = 0; g < GMAX; ++g)
+        if (g < ng) {
+#pragma unroll
+          for (int m = 8; m <= 16; m *= 2) {
+            o[g].x += __shfl_xor_sync(0xffffffffu, o[g].x, m);
+            o[g].y += __shfl_xor_sync(0xffffffffu, o[g].y, m);
+            o[g].z += __shfl_xor_sync(0xffffffffu, o[g].z, m);
+            o[g].w += __shfl_xor_sync(0xffffffffu, o[g].w, m);
+          }
+          if (lane < 8) *reinterpret_cast<float4*>(&sred[warp][g][lane * 4]) = o[g];
+        }
+      __syncthreads();
+      const int g = tid / STEP_COLS, cc = tid % STEP_COLS;
+      if (g < ng && vb * STEP_COLS + cc < r.dc)
+        out[t * r.so.s + (g0 + g) * r.so.h + vb * STEP_COLS + cc] =
+            Elem<T>::from_f(r.w_inter * (sred[0][g][cc] + sred[1][g][cc] + sred[2][g][cc] + sred[3][g][cc]));
+    }
+  }
+  if (!pool.out || !mine) return;
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int row = row0 + 16 * i;
+    if (row < r.da) *reinterpret_cast<float4*>(pool.out + at + (long long)row * r.dc) = x[i];
+  }
+}
+
+// =====================================================================================
+// CUDA-core chunked kernel: every type, dims up to 256, any strides.  A block walks one segment of one state in chunks of
+// 32 tokens, for 64 of the c dim's columns, all in fp32: the state, the chunk's rows and the pair products in shared memory.
+// =====================================================================================
+constexpr int SC = 32, SCOL = 64, SIMT_THREADS = 256;
+
+__host__ __device__ inline int simt_smem_floats(int da) { return 2 * SC * (da + 1) + SC * SCOL + da * SCOL + SC * (SC + 1) + 3 * SC; }
+
+template <typename T, bool REV, bool STATES>
+__global__ void __launch_bounds__(SIMT_THREADS)
+    lin_simt_kernel(const LinSeqs q, const LinRole r, const float* ws, float* ws_out, const LinPool pool, const int blocks_c) {
+  extern __shared__ float sm[];
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  const int ld = r.da + 1;
+  float* sa = sm;
+  float* sb = sa + SC * ld;
+  float* sc = sb + SC * ld;                 // [SC][SCOL], 16-byte aligned below
+  float* sx = sc + SC * SCOL;               // [da][SCOL]
+  float* sp = sx + r.da * SCOL;             // [SC][SC + 1]
+  float* lam = sp + SC * (SC + 1);          // lam^n, n <= SC
+  const int cb = blockIdx.x % blocks_c;
+  const int n = blockIdx.x / blocks_c % q.nseg;
+  const int h = blockIdx.x / blocks_c / q.nseg % q.nhk, z = blockIdx.x / blocks_c / q.nseg / q.nhk;
+  const int c0 = cb * SCOL;
+  if (!STATES && cb == 0) lin_zero_outside<T>(q, r, z, h * r.na, n, q.nseg, SIMT_THREADS);
+  const LinSpan span = lin_span(q, z);
+  int t0, t1;
+  lin_segment(q, span.len, n, t0, t1);
+  const int slot = STATES ? z : lin_slot(pool, z, SIMT_THREADS, &g_lin_error);
+  T* out = (T*)r.out + (q.cu ? 0 : z * r.so.b) + span.row0 * r.so.s + (long long)h * r.na * r.so.h;
+  const T* a = (const T*)r.a + (q.cu ? 0 : z * r.sa.b) + span.row0 * r.sa.s + (long long)h * r.na * r.sa.h;
+  const T* b = (const T*)r.b + (q.cu ? 0 : z * r.sb.b) + span.row0 * r.sb.s + (long long)h * r.nb * r.sb.h;
+  const T* c = (const T*)r.c + (q.cu ? 0 : z * r.sc.b) + span.row0 * r.sc.s + (long long)h * r.nb * r.sc.h;
+  if (!STATES && slot < 0) {
+    for (int g = 0; g < r.na; ++g)
+      for (long long e = tid; e < (long long)(t1 - t0) * SCOL; e += SIMT_THREADS)
+        if (c0 + e % SCOL < r.dc) out[(t0 + e / SCOL) * r.so.s + g * r.so.h + c0 + e % SCOL] = Elem<T>::from_f(0.f);
+    return;
+  }
+  const float g2 = lin_log2_decay(q.log_decay, h);
+  for (int e = tid; e <= SC; e += SIMT_THREADS) lam[e] = lin_power(g2, e);
+  // the state that enters the segment
+  const long long per = (long long)r.da * r.dc, segs = ((long long)z * q.nhk + h) * q.nseg + n;
+  const float* x0 = nullptr;
+  if (!STATES) {
+    if (q.nseg > 1) x0 = ws + segs * per;
+    else if (pool.in && !(pool.seen && pool.seen[z] <= 0)) x0 = pool.in + ((long long)slot * q.nhk + h) * per;
+  }
+  for (int e = tid; e < r.da * SCOL; e += SIMT_THREADS) {
+    const int i = e / SCOL, j = c0 + e % SCOL;
+    sx[e] = x0 && j < r.dc ? x0[r.transposed ? (long long)j * r.da + i : (long long)i * r.dc + j] : 0.f;
+  }
+  const int chunks = (t1 - t0 + SC - 1) / SC, groups = max(r.na, r.nb);
+  for (int m = 0; m < chunks; ++m) {
+    const int at = t0 + (REV ? chunks - 1 - m : m) * SC, cn = min(SC, t1 - at);
+    float4 o[2];
+    for (int g = 0; g < groups; ++g) {
+      const bool load_a = !STATES && (g == 0 || r.na > 1), load_b = g == 0 || r.nb > 1;
+      __syncthreads();
+      for (int e = tid; e < SC * r.da; e += SIMT_THREADS) {
+        const int j = e / r.da, i = e % r.da;
+        if (load_a) sa[j * ld + i] = j < cn ? Elem<T>::to_f(a[(at + j) * r.sa.s + (r.na > 1 ? g : 0) * r.sa.h + i]) : 0.f;
+        if (load_b) sb[j * ld + i] = j < cn ? Elem<T>::to_f(b[(at + j) * r.sb.s + (r.nb > 1 ? g : 0) * r.sb.h + i]) : 0.f;
+      }
+      if (load_b)
+        for (int e = tid; e < SC * SCOL; e += SIMT_THREADS) {
+          const int j = e / SCOL, i = c0 + e % SCOL;
+          sc[e] = j < cn && i < r.dc ? Elem<T>::to_f(c[(at + j) * r.sc.s + (r.nb > 1 ? g : 0) * r.sc.h + i]) : 0.f;
+        }
+      __syncthreads();
+      if constexpr (!STATES) {
+        float p[2][2] = {};
+        for (int i = 0; i < r.da; ++i) {
+          const float a0 = sa[(2 * ty) * ld + i], a1 = sa[(2 * ty + 1) * ld + i], b0 = sb[tx * ld + i], b1 = sb[(tx + 16) * ld + i];
+          p[0][0] = fmaf(a0, b0, p[0][0]);
+          p[0][1] = fmaf(a0, b1, p[0][1]);
+          p[1][0] = fmaf(a1, b0, p[1][0]);
+          p[1][1] = fmaf(a1, b1, p[1][1]);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const int i = 2 * ty + u, j = tx + 16 * w, gap = REV ? j - i : i - j;
+            sp[i * (SC + 1) + j] = gap >= 0 && i < cn && j < cn ? r.w_intra * p[u][w] * lam[gap] : 0.f;
+          }
+        if (g == 0 || r.na > 1) {
+          o[0] = o[1] = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int i = 0; i < r.da; ++i) {
+            const float a0 = sa[(2 * ty) * ld + i], a1 = sa[(2 * ty + 1) * ld + i];
+            const float4 x = *reinterpret_cast<const float4*>(sx + i * SCOL + tx * 4);
+            o[0].x = fmaf(a0, x.x, o[0].x); o[0].y = fmaf(a0, x.y, o[0].y); o[0].z = fmaf(a0, x.z, o[0].z); o[0].w = fmaf(a0, x.w, o[0].w);
+            o[1].x = fmaf(a1, x.x, o[1].x); o[1].y = fmaf(a1, x.y, o[1].y); o[1].z = fmaf(a1, x.z, o[1].z); o[1].w = fmaf(a1, x.w, o[1].w);
+          }
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int i = 2 * ty + u, steps = REV ? cn - 1 - i : i + 1;
+            const float w = steps >= 0 && i < cn ? r.w_inter * lam[steps] : 0.f;
+            o[u].x *= w; o[u].y *= w; o[u].z *= w; o[u].w *= w;
+          }
+        }
+        __syncthreads();
+        for (int j = 0; j < cn; ++j) {
+          const float4 v = *reinterpret_cast<const float4*>(sc + j * SCOL + tx * 4);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const float w = sp[(2 * ty + u) * (SC + 1) + j];
+            o[u].x = fmaf(w, v.x, o[u].x); o[u].y = fmaf(w, v.y, o[u].y); o[u].z = fmaf(w, v.z, o[u].z); o[u].w = fmaf(w, v.w, o[u].w);
+          }
+        }
+        if (r.na > 1 || g == groups - 1) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int i = 2 * ty + u, j = c0 + tx * 4;
+            if (i < cn && j < r.dc) {
+              T* w = out + (at + i) * r.so.s + (r.na > 1 ? g : 0) * r.so.h + j;
+              w[0] = Elem<T>::from_f(o[u].x); w[1] = Elem<T>::from_f(o[u].y); w[2] = Elem<T>::from_f(o[u].z); w[3] = Elem<T>::from_f(o[u].w);
+            }
+          }
+        }
+      }
+      if (r.nb > 1 || g == groups - 1) {      // the state: its old value has been used by every reader of this chunk
+        const float keep = r.nb > 1 && g > 0 ? 1.f : lam[cn];
+        for (int i = ty; i < r.da; i += 16) {
+          float4 s = *reinterpret_cast<const float4*>(sx + i * SCOL + tx * 4), acc = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int j = 0; j < cn; ++j) {
+            const float w = sb[j * ld + i] * lam[REV ? j + 1 : cn - 1 - j];
+            const float4 v = *reinterpret_cast<const float4*>(sc + j * SCOL + tx * 4);
+            acc.x = fmaf(w, v.x, acc.x); acc.y = fmaf(w, v.y, acc.y); acc.z = fmaf(w, v.z, acc.z); acc.w = fmaf(w, v.w, acc.w);
+          }
+          s.x = fmaf(r.w_up, acc.x, keep * s.x); s.y = fmaf(r.w_up, acc.y, keep * s.y);
+          s.z = fmaf(r.w_up, acc.z, keep * s.z); s.w = fmaf(r.w_up, acc.w, keep * s.w);
+          *reinterpret_cast<float4*>(sx + i * SCOL + tx * 4) = s;
+        }
+      }
+    }
+  }
+  float* x1 = nullptr;
+  if (STATES) x1 = t1 > t0 ? ws_out + segs * per : nullptr;
+  else if (q.nseg == 1 && pool.out) x1 = pool.out + ((long long)slot * q.nhk + h) * per;
+  if (!x1) return;
+  __syncthreads();
+  for (int e = tid; e < r.da * SCOL; e += SIMT_THREADS) {
+    const int i = e / SCOL, j = c0 + e % SCOL;
+    if (j < r.dc) x1[r.transposed ? (long long)j * r.da + i : (long long)i * r.dc + j] = sx[e];
+  }
+}
+
+// =====================================================================================
+// Joining segments: ws[n] holds what segment n adds from a state of 0; it becomes the state that enters the segment, and
+// the state past the last one goes to the pool.  One thread a float4 of the state; the next segment's load is in flight
+// while the running state is scaled.
+// =====================================================================================
+template <bool REV>
+__global__ void __launch_bounds__(256) lin_join_kernel(const LinSeqs q, float* ws, const LinPool pool, const int per4) {
+  const int z = blockIdx.x / q.nhk, h = blockIdx.x % q.nhk;
+  const int slot = lin_slot(pool, z, 256, &g_lin_error);
+  const int e = blockIdx.y * 256 + threadIdx.x;
+  if (slot < 0 || e >= per4) return;
+  const LinSpan span = lin_span(q, z);
+  const float g2 = lin_log2_decay(q.log_decay, h);
+  const int real = min(q.nseg, max(1, (span.len + q.seg_len - 1) / q.seg_len));
+  float4* w = reinterpret_cast<float4*>(ws) + (long long)blockIdx.x * q.nseg * per4 + e;
+  const long long at = ((long long)slot * q.nhk + h) * per4 + e;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (pool.in && !(pool.seen && pool.seen[z] <= 0)) x = reinterpret_cast<const float4*>(pool.in)[at];
+  const auto seg = [&](int m) { return REV ? real - 1 - m : m; };
+  float4 u = span.len > 0 ? w[(long long)seg(0) * per4] : make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int m = 0; m < real; ++m) {
+    const int n = seg(m);
+    int t0, t1;
+    lin_segment(q, span.len, n, t0, t1);
+    float4 next = u;
+    if (m + 1 < real) next = w[(long long)seg(m + 1) * per4];
+    w[(long long)n * per4] = x;
+    const float keep = lin_power(g2, t1 - t0);
+    x.x = fmaf(keep, x.x, u.x); x.y = fmaf(keep, x.y, u.y); x.z = fmaf(keep, x.z, u.z); x.w = fmaf(keep, x.w, u.w);
+    u = next;
+  }
+  if (pool.out) reinterpret_cast<float4*>(pool.out)[at] = x;
+}
+
+template <typename T>
+int simt_launch(const LinSeqs& q, const LinRole& r, bool rev, bool states, const float* ws, float* ws_out, const LinPool& pool,
+                cudaStream_t st) {
+  const int bytes = simt_smem_floats(r.da) * 4, blocks_c = (r.dc + SCOL - 1) / SCOL;
+  const long long grid = (long long)q.batch * q.nhk * q.nseg * blocks_c;
+  FA_CHECK_ARG(grid < (1ll << 31), "linear attention: %lld blocks", grid);
+  const auto go = [&](auto kernel, unsigned long long* done) -> int {
+    if (int rc = ensure_smem((const void*)kernel, simt_smem_floats(256) * 4, done)) return rc;
+    kernel<<<(int)grid, SIMT_THREADS, bytes, st>>>(q, r, ws, ws_out, pool, blocks_c);
+    count_launch();
+    return cuda_status(cudaGetLastError(), "linear attention launch");
+  };
+  static unsigned long long done[4] = {};
+  if (states) return rev ? go(lin_simt_kernel<T, true, true>, done) : go(lin_simt_kernel<T, false, true>, done + 1);
+  return rev ? go(lin_simt_kernel<T, true, false>, done + 2) : go(lin_simt_kernel<T, false, false>, done + 3);
+}
+
+template <typename T>
+int step_launch(const LinSeqs& q, const LinRole& r, const LinPool& pool, cudaStream_t st) {
+  const int blocks_v = (r.dc + STEP_COLS - 1) / STEP_COLS;
+  const long long grid = (long long)q.batch * q.nhk * blocks_v;
+  FA_CHECK_ARG(grid < (1ll << 31), "linear attention: %lld blocks", grid);
+  if (r.da <= 64) lin_step_kernel<T, 4><<<(int)grid, STEP_THREADS, 0, st>>>(q, r, pool, blocks_v);
+  else if (r.da <= 128) lin_step_kernel<T, 8><<<(int)grid, STEP_THREADS, 0, st>>>(q, r, pool, blocks_v);
+  else lin_step_kernel<T, 16><<<(int)grid, STEP_THREADS, 0, st>>>(q, r, pool, blocks_v);
+  count_launch();
+  return cuda_status(cudaGetLastError(), "linear attention (recurrent) launch");
+}
+
+int join(const LinSeqs& q, bool rev, float* ws, const LinPool& pool, int per, cudaStream_t st) {
+  const dim3 grid(q.batch * q.nhk, (per / 4 + 255) / 256);
+  if (rev) lin_join_kernel<true><<<grid, 256, 0, st>>>(q, ws, pool, per / 4);
+  else lin_join_kernel<false><<<grid, 256, 0, st>>>(q, ws, pool, per / 4);
+  count_launch();
+  return cuda_status(cudaGetLastError(), "linear attention (join) launch");
+}
+
+int states(const LinSeqs& q, const LinRole& r, bool rev, float* ws, int dtype, cudaStream_t st) {
+  return lin_simt_states(q, r, rev, ws, dtype, st);
+}
+int main_pass(const LinSeqs& q, const LinRole& r, bool rev, const float* ws, const LinPool& pool, int dtype, cudaStream_t st) {
+  return lin_simt_main(q, r, rev, ws, pool, dtype, st);
+}
+
+bool dims_ok(int dk, int dv) { return dk > 0 && dv > 0 && dk <= 256 && dv <= 256 && dk % 8 == 0 && dv % 8 == 0; }
+bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
+
+// Up to this many tokens a sequence the recurrent kernel is taken.
+constexpr int STEP_TOKENS = 16;
+
+}  // namespace
+
+namespace fa {
+int lin_simt_states(const LinSeqs& q, const LinRole& r, bool rev, float* ws, int dtype, cudaStream_t st) {
+  const LinPool none{};
+  if (dtype == FA_DTYPE_F16) return simt_launch<__half>(q, r, rev, true, nullptr, ws, none, st);
+  if (dtype == FA_DTYPE_BF16) return simt_launch<__nv_bfloat16>(q, r, rev, true, nullptr, ws, none, st);
+  return simt_launch<float>(q, r, rev, true, nullptr, ws, none, st);
+}
+int lin_simt_main(const LinSeqs& q, const LinRole& r, bool rev, const float* ws, const LinPool& pool, int dtype, cudaStream_t st) {
+  if (dtype == FA_DTYPE_F16) return simt_launch<__half>(q, r, rev, false, ws, nullptr, pool, st);
+  if (dtype == FA_DTYPE_BF16) return simt_launch<__nv_bfloat16>(q, r, rev, false, ws, nullptr, pool, st);
+  return simt_launch<float>(q, r, rev, false, ws, nullptr, pool, st);
+}
+int lin_device_error(int clear) {
+  int v = 0;
+  cudaMemcpyFromSymbol(&v, g_lin_error, sizeof(int));
+  if (clear && v) {
+    const int zero = 0;
+    cudaMemcpyToSymbol(g_lin_error, &zero, sizeof(int));
+  }
+  return v;
+}
+}  // namespace fa
+
+extern "C" FA_API long long fa_linear_plan(int batch, int S, long long total, int NH, int gqa, int dk, int dv, int dtype, int* seg_len,
+                                           int* nseg) {
+  if (seg_len) *seg_len = 128;
+  if (nseg) *nseg = 1;
+  if (!seg_len || !nseg || batch <= 0 || S <= 0 || gqa <= 0 || NH < gqa || !dims_ok(dk, dv)) return 0;
+  // Enough segments that every SM has two blocks, none shorter than 128 tokens (each costs a state written and read
+  // again, 8 dk dv bytes, and its keys and values read twice).
+  const long long states = (long long)batch * (NH / gqa);
+  const long long tokens = total > 0 && total < (long long)batch * S ? std::max(1ll, total / batch) : S;
+  const int cols = (dv + 63) / 64;
+  const long long want = std::max(1ll, 2ll * num_sms() / std::max(1ll, states * cols));
+  long long len = (tokens + want - 1) / want;
+  len = std::max(128ll, (len + 127) / 128 * 128);
+  if (len >= S) len = (S + 127ll) / 128 * 128;
+  *seg_len = (int)std::min(len, (1ll << 30));
+  *nseg = (int)((S + (long long)*seg_len - 1) / *seg_len);
+  return *nseg > 1 ? states * *nseg * dk * dv : 0;
+}
+
+extern "C" FA_API int fa_linear_launch(const FaLinearParams* pp, int dtype, void* stream) {
+  FA_ABI_GUARD(pp, FaLinearParams);
+  const FaLinearParams& p = *pp;
+  cudaStream_t st = (cudaStream_t)stream;
+  FA_CHECK_ARG(dtype >= FA_DTYPE_F16 && dtype <= FA_DTYPE_F32, "linear attention: dtype code %d", dtype);
+  const bool rows = p.cu ? p.total > 0 : (long long)p.batch * p.S > 0;
+  FA_CHECK_ARG(p.log_decay && (!rows || (p.q && p.k && p.v && p.o)), "linear attention: q, k, v, o, log_decay must be non-null");
+  FA_CHECK_ARG(p.batch >= 0 && p.S >= 0 && p.NH > 0 && p.gqa > 0 && p.NH % p.gqa == 0 && p.total >= 0,
+               "linear attention: batch=%d S=%d NH=%d gqa=%d total=%lld", p.batch, p.S, p.NH, p.gqa, p.total);
+  FA_CHECK_ARG(dims_ok(p.dk, p.dv), "linear attention: dk=%d and dv=%d must be multiples of 8 up to 256", p.dk, p.dv);
+  FA_CHECK_ARG(aligned16(p.state_in) && aligned16(p.state_out) && aligned16(p.states), "linear attention: states must lie on 16 bytes");
+  FA_CHECK_ARG(p.slots >= 0 && (p.state_index || !(p.state_in || p.state_out) || p.slots >= p.batch),
+               "linear attention: %lld slots for %d sequences", p.slots, p.batch);
+  FA_CHECK_ARG(!p.cu || p.batch > 0 || p.total == 0, "linear attention: %lld packed rows of no sequence", p.total);
+  if (p.batch == 0) return FA_OK;
+  const bool step = !p.keep_states && p.S <= STEP_TOKENS;
+  LinSeqs q{p.cu, p.log_decay, p.total, p.batch, p.S, p.NH / p.gqa, 0, 1};
+  if (!step) {
+    q.seg_len = p.seg_len;
+    q.nseg = p.nseg;
+    FA_CHECK_ARG(p.seg_len > 0 && p.nseg > 0 && (long long)p.seg_len * p.nseg >= p.S, "linear attention: %d segments of %d tokens for S=%d",
+                 p.nseg, p.seg_len, p.S);
+    FA_CHECK_ARG(p.nseg == 1 || p.states, "linear attention: %d segments need the workspace `states`", p.nseg);
+  }
+  const LinPool pool{p.state_in, p.state_out, p.state_index, p.seen, p.state_index ? p.slots : p.batch};
+  const LinRole r{p.q, p.k, p.v, p.o, p.sQ, p.sK, p.sV, p.sO, p.gqa, 1, p.dk, p.dv, 0, p.scale, p.scale, 1.f};
+  if (step) {
+    if (dtype == FA_DTYPE_F16) return step_launch<__half>(q, r, pool, st);
+    if (dtype == FA_DTYPE_BF16) return step_launch<__nv_bfloat16>(q, r, pool, st);
+    return step_launch<float>(q, r, pool, st);
+  }
+  if (q.nseg > 1) {
+    if (int rc = states(q, r, false, p.states, dtype, st)) return rc;
+    if (int rc = join(q, false, p.states, pool, p.dk * p.dv, st)) return rc;
+  }
+  return main_pass(q, r, false, p.states, pool, dtype, st);
+}
+
+extern "C" FA_API int fa_linear_backward_launch(const FaLinearBwdParams* pp, int dtype, void* stream) {
+  FA_ABI_GUARD(pp, FaLinearBwdParams);
+  const FaLinearBwdParams& p = *pp;
+  cudaStream_t st = (cudaStream_t)stream;
+  FA_CHECK_ARG(dtype >= FA_DTYPE_F16 && dtype <= FA_DTYPE_F32, "linear attention backward: dtype code %d", dtype);
+  const bool rows = p.cu ? p.total > 0 : (long long)p.batch * p.S > 0;
+  FA_CHECK_ARG(p.log_decay && (!rows || (p.q && p.k && p.v && p.dO && p.dQ && p.dK && p.dV)),
+               "linear attention backward: q, k, v, dO, dQ, dK, dV, log_decay must be non-null");
+  FA_CHECK_ARG(p.batch >= 0 && p.S >= 0 && p.NH > 0 && p.gqa > 0 && p.NH % p.gqa == 0 && p.total >= 0,
+               "linear attention backward: batch=%d S=%d NH=%d gqa=%d total=%lld", p.batch, p.S, p.NH, p.gqa, p.total);
+  FA_CHECK_ARG(dims_ok(p.dk, p.dv), "linear attention backward: dk=%d and dv=%d must be multiples of 8 up to 256", p.dk, p.dv);
+  FA_CHECK_ARG(aligned16(p.initial) && aligned16(p.dfinal) && aligned16(p.dinitial) && aligned16(p.states) && aligned16(p.work),
+               "linear attention backward: states must lie on 16 bytes");
+  FA_CHECK_ARG(!p.cu || p.batch > 0 || p.total == 0, "linear attention backward: %lld packed rows of no sequence", p.total);
+  if (p.batch == 0) return FA_OK;
+  FA_CHECK_ARG(p.seg_len > 0 && p.nseg > 0 && (long long)p.seg_len * p.nseg >= p.S,
+               "linear attention backward: %d segments of %d tokens for S=%d", p.nseg, p.seg_len, p.S);
+  FA_CHECK_ARG(p.nseg == 1 || (p.states && p.work), "linear attention backward: %d segments need `states` and `work`", p.nseg);
+  const LinSeqs q{p.cu, p.log_decay, p.total, p.batch, p.S, p.NH / p.gqa, p.seg_len, p.nseg};
+  const float s = p.scale;
+  const LinRole dq{p.dO, p.v, p.k, p.dQ, p.sdO, p.sV, p.sK, p.sdQ, p.gqa, 1, p.dv, p.dk, 1, s, s, 1.f};
+  const LinRole dk{p.v, p.dO, p.q, p.dK, p.sV, p.sdO, p.sQ, p.sdK, 1, p.gqa, p.dv, p.dk, 1, s, 1.f, s};
+  const LinRole dv{p.k, p.q, p.dO, p.dV, p.sK, p.sQ, p.sdO, p.sdV, 1, p.gqa, p.dk, p.dv, 0, s, 1.f, s};
+  const LinPool forward{p.initial, nullptr, nullptr, nullptr, p.batch};
+  const LinPool back{p.dfinal, p.dinitial, nullptr, nullptr, p.batch}, back_only{p.dfinal, nullptr, nullptr, nullptr, p.batch};
+  if (q.nseg > 1) {
+    if (int rc = states(q, dv, true, p.work, dtype, st)) return rc;
+    if (int rc = join(q, true, p.work, back, p.dk * p.dv, st)) return rc;
+  }
+  if (int rc = main_pass(q, dq, false, p.states, forward, dtype, st)) return rc;
+  if (int rc = main_pass(q, dk, true, p.work, back_only, dtype, st)) return rc;
+  return main_pass(q, dv, true, p.work, q.nseg > 1 ? back_only : back, dtype, st);
+}

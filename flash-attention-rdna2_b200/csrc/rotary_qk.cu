@@ -1,0 +1,149 @@
+// rotary_qk.cu — rotary of q and k at each token's own position, from frequencies instead of tables.
+//
+// theta = position * inv_freq.  The frequency is held as a fraction of a turn in units of 2^-64, so that the 64-bit product
+// with the position wraps by itself at whole turns: no range reduction is left, and a position of 2^31 is as exact as a
+// small one.  The quadrant comes off in the integers too, and sincospi sees at most an eighth of a turn.
+//
+// Bound by memory: every element of q and k is read and written once.  A block takes `TOK` tokens: its threads form the
+// tokens' cos / sin once, in shared memory, and then walk all heads of q and k by 16-byte units, so that the 64-bit product and the
+// sine cost one evaluation per token and pair instead of one per head.  Blocks of 4 tokens where that still gives
+// every SM several blocks, else of 1 (a decode step has few tokens, and its time is latency).
+#include <algorithm>
+#include "fa_common.cuh"
+#include "fa_launch.h"
+
+namespace {
+
+constexpr int THREADS = 256, MAX_PAIRS = 128;
+
+template <typename T>
+__device__ __forceinline__ void turn(const T& a, const T& b, float2 e, T& oa, T& ob) {
+  const float x = Elem<T>::to_f(a), y = Elem<T>::to_f(b);
+  oa = Elem<T>::from_f(x * e.x - y * e.y);
+  ob = Elem<T>::from_f(y * e.x + x * e.y);
+}
+
+template <typename T, int U> struct alignas(U * sizeof(T) == 16 ? 16 : sizeof(T)) Unit { T e[U]; };
+
+// U: elements of a 16-byte unit, or 1 (2 where the pairs are neighbours) for rows that do not lie on 16 bytes: those are read
+// and written element by element
+template <typename T, int U, bool INTER, int TOK>
+__global__ void __launch_bounds__(THREADS) rotary_qk_kernel(const FaRotaryQkParams p, const long long tokens) {
+  __shared__ float2 sce[TOK][MAX_PAIRS];
+  const int half = p.rot_dim / 2;
+  const long long first = (long long)blockIdx.x * TOK;
+  const int nt = (int)min((long long)TOK, tokens - first);
+  for (int e = threadIdx.x; e < nt * half; e += THREADS) {
+    const int t = e / half, i = e % half;
+    const long long row = first + t;
+    long long pos;
+    if (p.positions) {
+      pos = p.pos_bytes == 8 ? ((const long long*)p.positions)[row] : ((const int*)p.positions)[row];
+    } else {
+      const long long z = row / p.seqlen;
+      pos = row - z * p.seqlen + p.offset + (p.offsets ? p.offsets[z] : 0);
+    }
+    double f = p.inv_freq[i] * 0.15915494309189533577;      // turns for each position
+    f -= floor(f);
+    const unsigned long long angle = (unsigned long long)pos * __double2ull_rn(f * 18446744073709551616.0);
+    const unsigned int hi = (unsigned int)((angle + 0x80000000ull) >> 32);     // to nearest: opposite positions turn alike
+    const unsigned int quarter = (hi + 0x20000000u) >> 30;
+    float s, c;
+    sincospif((float)(int)(hi - (quarter << 30)) * (1.f / 2147483648.f), &s, &c);
+    if (quarter & 1) {
+      const float x = c;
+      c = -s;
+      s = x;
+    }
+    if (quarter & 2) {
+      c = -c;
+      s = -s;
+    }
+    sce[t][i] = make_float2(p.factor * c, (p.inverse ? -p.factor : p.factor) * s);
+  }
+  __syncthreads();
+  // a head's units: first those that turn, then (unless q and k stay in place) those that are copied
+  const int turning = INTER ? p.rot_dim / U : half / U;
+  const int heads = p.heads_q + p.heads_k;
+  const bool copy_q = p.q_out != p.q, copy_k = p.k_out != p.k;
+  constexpr int C = U * sizeof(T) == 16 ? U : 1;      // elements of a copied unit
+  const int copied = copy_q || copy_k ? (p.dim - p.rot_dim) / C : 0;
+  const int per = turning + copied, all = nt * heads * per;
+  using V = Unit<T, U>;
+#pragma unroll 4
+  for (int e = threadIdx.x; e < all; e += THREADS) {
+    const int w = e % per, h = e / per % heads, t = e / per / heads;
+    const long long row = first + t, z = row / p.seqlen, s = row - z * p.seqlen;
+    const bool is_q = h < p.heads_q;
+    const FaStrides& si = is_q ? p.sQ : p.sK;
+    const FaStrides& so = is_q ? p.sQo : p.sKo;
+    const int hh = is_q ? h : h - p.heads_q;
+    const T* x = (const T*)(is_q ? p.q : p.k) + z * si.b + s * si.s + hh * si.h;
+    T* o = (T*)(is_q ? p.q_out : p.k_out) + z * so.b + s * so.s + hh * so.h;
+    if (w >= turning) {
+      const int d = p.rot_dim + (w - turning) * C;
+      if (is_q ? copy_q : copy_k) *reinterpret_cast<Unit<T, C>*>(o + d) = *reinterpret_cast<const Unit<T, C>*>(x + d);
+      continue;
+    }
+    const float2* ce = sce[t];
+    if constexpr (INTER) {
+      const V v = *reinterpret_cast<const V*>(x + w * U);
+      V r;
+#pragma unroll
+      for (int i = 0; i < U; i += 2) turn<T>(v.e[i], v.e[i + 1], ce[(w * U + i) / 2], r.e[i], r.e[i + 1]);
+      *reinterpret_cast<V*>(o + w * U) = r;
+    } else {
+      const V a = *reinterpret_cast<const V*>(x + w * U), b = *reinterpret_cast<const V*>(x + half + w * U);
+      V ra, rb;
+#pragma unroll
+      for (int i = 0; i < U; ++i) turn<T>(a.e[i], b.e[i], ce[w * U + i], ra.e[i], rb.e[i]);
+      *reinterpret_cast<V*>(o + w * U) = ra;
+      *reinterpret_cast<V*>(o + half + w * U) = rb;
+    }
+  }
+}
+
+template <typename T, int U, bool INTER>
+int go(const FaRotaryQkParams& p, cudaStream_t st) {
+  const long long tokens = (long long)p.batch * p.seqlen;
+  if (tokens >= 8ll * fa::num_sms()) {
+    FA_CHECK_ARG((tokens + 3) / 4 < (1ll << 31), "rotary of q and k: %lld tokens", tokens);
+    rotary_qk_kernel<T, U, INTER, 4><<<(int)((tokens + 3) / 4), THREADS, 0, st>>>(p, tokens);
+  } else {
+    rotary_qk_kernel<T, U, INTER, 1><<<(int)tokens, THREADS, 0, st>>>(p, tokens);
+  }
+  fa::count_launch();
+  return fa::cuda_status(cudaGetLastError(), "rotary (q and k) launch");
+}
+
+template <typename T>
+int run(const FaRotaryQkParams& p, cudaStream_t st) {
+  constexpr int U = 16 / sizeof(T);
+  const auto on = [&](const void* x, const FaStrides& s) {
+    return (uintptr_t)x % 16 == 0 && (p.batch == 1 || s.b % U == 0) && (p.seqlen == 1 || s.s % U == 0) && s.h % U == 0;
+  };
+  const bool vec = p.dim % U == 0 && p.rot_dim % (p.interleaved ? U : 2 * U) == 0 && on(p.q, p.sQ) && on(p.q_out, p.sQo) &&
+                   (!p.k || (on(p.k, p.sK) && on(p.k_out, p.sKo)));
+  if (p.interleaved) return vec ? go<T, U, true>(p, st) : go<T, 2, true>(p, st);
+  return vec ? go<T, U, false>(p, st) : go<T, 1, false>(p, st);
+}
+
+}  // namespace
+
+extern "C" FA_API int fa_rotary_qk_launch(const FaRotaryQkParams* pp, int dtype, void* stream) {
+  FA_ABI_GUARD(pp, FaRotaryQkParams);
+  FaRotaryQkParams p = *pp;
+  FA_CHECK_ARG(dtype >= FA_DTYPE_F16 && dtype <= FA_DTYPE_F32, "rotary of q and k: dtype code %d", dtype);
+  FA_CHECK_ARG(p.q && p.q_out && p.inv_freq && !p.k == !p.k_out, "rotary of q and k: q, q_out, inv_freq must be non-null, k goes with k_out");
+  FA_CHECK_ARG(p.batch >= 0 && p.seqlen >= 0 && p.heads_q > 0 && p.dim > 0 && (!p.k || p.heads_k > 0),
+               "rotary of q and k: batch=%d seqlen=%d heads %d / %d dim=%d", p.batch, p.seqlen, p.heads_q, p.heads_k, p.dim);
+  FA_CHECK_ARG(p.rot_dim > 0 && p.rot_dim % 2 == 0 && p.rot_dim <= p.dim && p.rot_dim <= 2 * MAX_PAIRS,
+               "rotary of q and k: rot_dim=%d must be even, at most dim=%d and at most %d", p.rot_dim, p.dim, 2 * MAX_PAIRS);
+  FA_CHECK_ARG(!p.positions || p.pos_bytes == 4 || p.pos_bytes == 8, "rotary of q and k: positions of %d bytes", p.pos_bytes);
+  if (!p.k) p.heads_k = 0;
+  if (p.batch == 0 || p.seqlen == 0) return FA_OK;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == FA_DTYPE_F16) return run<__half>(p, st);
+  if (dtype == FA_DTYPE_BF16) return run<__nv_bfloat16>(p, st);
+  return run<float>(p, st);
+}

@@ -25,6 +25,11 @@ from .kvcache import (
     kvcache_gather,
     new_cache_8bit,
 )
+from .linear_attention import (
+    linear_attn_func,
+    linear_attn_varlen_func,
+    linear_attn_with_state,
+)
 from . import bert_padding
 from . import torch_op
 
@@ -34,8 +39,8 @@ torch_op.register()
 
 def device_error(clear=False):
     """Error bits the kernels recorded on the current device (0 = none): a pipeline wait that gave
-    up (the kernel unwound and its outputs are not valid), a paged-K/V entry outside the cache, or
-    a rotary position outside its table.  Synchronises with the device; clear=True resets them."""
+    up (the kernel unwound and its outputs are not valid), a paged-K/V entry outside the cache, a rotary
+    position outside its table, or a state slot outside its pool or named twice.  Synchronises with the device; clear=True resets them."""
     from . import _C
     return int(_C.device_error(bool(clear)))
 
@@ -44,6 +49,7 @@ __all__ = [
     "device_error", "flash_attn_func", "flash_attn_qkvpacked_func", "flash_attn_kvpacked_func", "flash_attn_varlen_func",
     "flash_attn_varlen_qkvpacked_func", "flash_attn_varlen_kvpacked_func", "flash_attn_combine",
     "flash_attn_with_kvcache", "flash_attn_with_kvcache_8bit", "kvcache_append", "kvcache_gather", "new_cache_8bit",
+    "linear_attn_func", "linear_attn_varlen_func", "linear_attn_with_state",
     "bert_padding", "install_as_flash_attn",
 ]
 

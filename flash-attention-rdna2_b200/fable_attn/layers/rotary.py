@@ -8,13 +8,14 @@ x' = x*cos - y*sin, y' = y*cos + x*sin.  Same surface as the reference's
 package/fable_attn/layers/rotary.py:43-178; the varlen form computes every token's position
 in one vectorised gather instead of a per-sequence loop.
 """
+import math
 from typing import Optional, Union
 
 import torch
 from torch import nn
 
 __all__ = ["apply_rotary_emb", "apply_rotary_emb_func", "apply_rotary_emb_qkv_", "apply_rotary_emb_kv_",
-           "RotaryEmbedding"]
+           "RotaryEmbedding", "apply_rotary_emb_qk", "scaled_inv_freq", "rotary_tables"]
 
 
 def _rotate(x, cos, sin, interleaved):
@@ -117,6 +118,93 @@ def apply_rotary_emb_kv_(kv, cos, sin, interleaved=False, seqlen_offsets=0, cu_s
     """kv (batch, seqlen, 2, nheads, headdim): rotates k in place."""
     kv[:, :, 0].copy_(apply_rotary_emb(kv[:, :, 0], cos, sin, interleaved, False, seqlen_offsets))
     return kv
+
+
+def scaled_inv_freq(rotary_dim, base=10000.0, scaling=None, factor=1.0, original_max_position=None, beta_fast=32.0, beta_slow=1.0,
+                    device=None):
+    """(inv_freq fp64 (rotary_dim / 2,), factor of cos and sin) of base**(-2i / rotary_dim), scaled for contexts `factor` times as
+    long as those trained on:
+      None      as they are;
+      "linear"  all divided by `factor` (positions interpolated);
+      "ntk"     base * factor**(rotary_dim / (rotary_dim - 2)): the slowest divided by `factor`, the fastest kept;
+      "yarn"    frequencies that turn at least beta_fast times over original_max_position are kept, those that turn at most
+                beta_slow times divided by `factor`, those between blended linearly in their index, and cos and sin multiplied by
+                1 + 0.1 ln(factor) (Peng et al. 2023, YaRN)."""
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError(f"scaled_inv_freq: rotary_dim={rotary_dim} must be even and positive")
+    if not (math.isfinite(base) and base > 1 and math.isfinite(factor) and factor >= 1):
+        raise ValueError(f"scaled_inv_freq: base={base} must be above 1 and factor={factor} at least 1")
+    i = torch.arange(0, rotary_dim, 2, dtype=torch.float64)
+    if scaling == "ntk":
+        if rotary_dim == 2:
+            raise ValueError("scaled_inv_freq: ntk needs a rotary_dim above 2")
+        base = base * factor ** (rotary_dim / (rotary_dim - 2))
+    freq, times = base ** (-i / rotary_dim), 1.0
+    if scaling == "linear":
+        freq = freq / factor
+    elif scaling == "yarn":
+        if original_max_position is None or not original_max_position > 0 or not beta_fast > beta_slow > 0:
+            raise ValueError("scaled_inv_freq: yarn needs original_max_position > 0 and beta_fast > beta_slow > 0")
+
+        def index(turns):     # of the frequency that turns so often over the original length
+            return rotary_dim * math.log(original_max_position / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+        first, last = max(math.floor(index(beta_fast)), 0), min(math.ceil(index(beta_slow)), rotary_dim - 1)
+        blend = ((i / 2 - first) / max(last - first, 1e-3)).clamp(0, 1)
+        freq, times = freq * (1 - blend) + freq / factor * blend, 1.0 + 0.1 * math.log(factor)
+    elif scaling not in (None, "ntk"):
+        raise ValueError(f"scaled_inv_freq: scaling={scaling!r} is none of None, 'linear', 'ntk', 'yarn'")
+    return freq.to(device), times
+
+
+def rotary_tables(inv_freq, seqlen, factor=1.0):
+    """cos and sin (seqlen, rotary_dim / 2) fp32 of positions 0 .. seqlen - 1: the tables that kvcache_append,
+    flash_attn_with_kvcache and the other calls with rotary_cos / rotary_sin take, so that they turn as apply_rotary_emb_qk does."""
+    angle = torch.arange(seqlen, dtype=torch.float64, device=inv_freq.device)[:, None] * inv_freq.double()
+    return (angle.cos() * factor).float(), (angle.sin() * factor).float()
+
+
+class _RotaryQkFn(torch.autograd.Function):
+    """The gradient of a rotation by theta is the rotation of the incoming gradient by -theta, times the same factor; the
+    dims past rotary_dim pass through."""
+
+    @staticmethod
+    def forward(ctx, q, k, inv_freq, positions, offsets, interleaved, factor):
+        from .. import _C
+        ctx.save_for_backward(inv_freq, positions, offsets if torch.is_tensor(offsets) else None)
+        ctx.rest = (None if torch.is_tensor(offsets) else offsets, interleaved, factor)
+        return _C.rotary_qk(q, k, inv_freq, positions, offsets, interleaved, False, factor, False)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq, dk):
+        from .. import _C
+        inv_freq, positions, offsets = ctx.saved_tensors
+        offset, interleaved, factor = ctx.rest
+        dq, dk = _C.rotary_qk(dq, dk, inv_freq, positions, offset if offsets is None else offsets, interleaved, False, factor, True)
+        return dq, dk, None, None, None, None, None
+
+
+def apply_rotary_emb_qk(q, k, inv_freq, positions=None, *, seqlen_offsets=0, interleaved=False, factor=1.0, inplace=False):
+    """Rotate q and k, (batch, seqlen, heads, headdim) or packed (total, heads, headdim), in one pass; (q, k).
+
+    inv_freq (rotary_dim / 2,): radians for each position, best in fp64 (scaled_inv_freq makes them); the first rotary_dim dims turn,
+    the rest pass through.  positions (batch, seqlen) or (total,), int32 or int64: each token's own position, any
+    whole number, without a table to end; without them token t sits at seqlen_offsets + t (an int, or (batch,)).  The angle is exact
+    however far the position; cos and sin are multiplied by factor and applied in fp32 with one rounding at the end (apply_rotary_emb
+    rounds tables and products to the inputs' type instead, as torch arithmetic does).  interleaved pairs dims (2i, 2i + 1) instead of
+    (i, i + rotary_dim / 2).  inplace writes q and k themselves.  Carries gradients to q and k.  CUDA tensors only."""
+    for x, name in ((q, "q"), (k, "k"), (inv_freq, "inv_freq")):
+        if not x.is_cuda:
+            raise ValueError(f"fable_attn: {name} must be on a CUDA device")
+    if torch.is_grad_enabled() and inv_freq.requires_grad:
+        raise NotImplementedError("apply_rotary_emb_qk: inv_freq carries no gradient; pass inv_freq.detach()")
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
+        if inplace:
+            raise RuntimeError("apply_rotary_emb_qk: inplace rotation of a tensor that requires grad")
+        return _RotaryQkFn.apply(q, k, inv_freq, positions, seqlen_offsets, bool(interleaved), float(factor))
+    from .. import _C
+    return _C.rotary_qk(q, k, inv_freq, positions, seqlen_offsets, bool(interleaved), bool(inplace), float(factor), False)
 
 
 class RotaryEmbedding(nn.Module):

@@ -420,6 +420,95 @@ typedef struct FaCombineParams {
 FA_API int fa_combine_launch(const FaCombineParams* p, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Linear attention with a decay per head (no counterpart in the reference).  Per sequence and kv head, with
+ * lam = exp(min(log_decay, 0)):
+ *     S_t = lam S_{t-1} + k_t v_t^T   (fp32, [dk][dv])        o_t = scale * S_t^T q_t
+ * and gqa query heads share one state.  Layouts as in the forward: dense [batch, heads, S, dim] through the strides,
+ * or, with cu [batch + 1], packed rows cu[z] + t (S a bound on the lengths that chooses kernels and grids, strides.b ignored);
+ * rows of o that belong to no sequence are written as 0.  dk and dv are multiples of 8 up to 256.
+ *   state_in   [slots][NH / gqa][dk][dv] or null (every sequence starts from 0), state_out likewise or null; they
+ *              may be the same.  16-byte aligned.  Sequence z has slot state_index[z] (z without state_index); where
+ *              seen[z] <= 0 it starts from 0 whatever the slot holds.  A negative slot is padding: its sequence gives 0 and touches
+ *              no state.  So does a slot outside the pool, and the later of two sequences of the same slot; these raise
+ *              fa_device_error bit 131072.
+ *   states     workspace of fa_linear_plan floats, 16-byte aligned (null where that is 0).  With keep_states the
+ *              chunked kernels run whatever S is, and leave each segment's start state there for fa_linear_backward_launch.
+ * fa_linear_plan: segments of seg_len tokens (nseg for the longest sequence) that run side by side, and the floats of `states`.
+ * -------------------------------------------------------------------------------------------*/
+typedef struct FaLinearParams {
+  unsigned int struct_size;
+  const void *q, *k, *v;
+  void* o;
+  FaStrides sQ, sK, sV, sO;
+  const float* log_decay;              /* [NH / gqa], natural log of the factor per token */
+  const float* state_in;
+  float* state_out;
+  long long slots;
+  const int* state_index;              /* [batch] or null */
+  const int* seen;                     /* [batch] or null */
+  const int* cu;                       /* [batch + 1] or null */
+  long long total;                     /* packed rows (cu given) */
+  int batch, S, NH, gqa, dk, dv;
+  float scale;
+  int seg_len, nseg, keep_states;
+  float* states;
+} FaLinearParams;
+
+FA_API long long fa_linear_plan(int batch, int S, long long total, int NH, int gqa, int dk, int dv, int dtype, int* seg_len,
+                                int* nseg);
+FA_API int fa_linear_launch(const FaLinearParams* p, int dtype, void* stream);
+
+/* Gradients of dense or packed sequences whose states are [batch][NH / gqa][dk][dv] (no index, no seen):
+ * R_T = dfinal (0 where null), N_t = R_{t+1} + scale q_t dO_t^T (summed over the group's query heads), R_t = lam N_t:
+ * dq_t = scale S_t dO_t, dk_t = N_t v_t, dv_t = N_t^T k_t, dinitial = R_0.  Sums over a
+ * group's query heads are taken in fp32 in a fixed order.  states, initial, seg_len, nseg: the forward's;
+ * work: fa_linear_plan floats.  dQ, dK, dV in the inputs' type, their strides given. */
+typedef struct FaLinearBwdParams {
+  unsigned int struct_size;
+  const void *q, *k, *v, *dO;
+  void *dQ, *dK, *dV;
+  FaStrides sQ, sK, sV, sdO, sdQ, sdK, sdV;
+  const float* log_decay;
+  const float* initial;                /* the forward's state_in, or null */
+  const float* dfinal;                 /* or null */
+  float* dinitial;                     /* or null */
+  const int* cu;
+  long long total;
+  int batch, S, NH, gqa, dk, dv;
+  float scale;
+  int seg_len, nseg;
+  const float* states;
+  float* work;
+} FaLinearBwdParams;
+
+FA_API int fa_linear_backward_launch(const FaLinearBwdParams* p, int dtype, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Rotary of q and k at positions given for each token, from frequencies instead of tables (no counterpart in the
+ * reference, whose tables are layers/rotary.py:119-146).  Pair i of the first rot_dim dims of token t turns by
+ * positions * inv_freq[i] radians, counted in 2^-64 turns by one 64-bit product (exact for the frequency as rounded there,
+ * however far the position); x' = factor (x cos - y sin), y' = factor (y cos + x sin), in fp32 and rounded once.
+ * `inverse` turns back (the gradient: by -theta, with the same factor).
+ *   rows z * seqlen + t by strides (dim contiguous); k may be null.  Outputs may be the inputs.
+ *   positions  [batch * seqlen] int32 or int64 (pos_bytes 4 / 8), or null: offsets[z] (0 where null) + offset + t
+ * -------------------------------------------------------------------------------------------*/
+typedef struct FaRotaryQkParams {
+  unsigned int struct_size;
+  const void *q, *k;
+  void *q_out, *k_out;
+  FaStrides sQ, sK, sQo, sKo;
+  const double* inv_freq;              /* [rot_dim / 2] */
+  const void* positions;
+  const int* offsets;                  /* [batch] or null */
+  long long offset;
+  int pos_bytes;
+  int batch, seqlen, heads_q, heads_k, dim, rot_dim, interleaved, inverse;
+  float factor;
+} FaRotaryQkParams;
+
+FA_API int fa_rotary_qk_launch(const FaRotaryQkParams* p, int dtype, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Multi-GPU decode exchange over peer memory (no counterpart in the reference, which has no
  * multi-GPU layer; its merge rule is flash_attn_combine, package/fable_attn/flash_attn_interface.py
  * :567-580).  A decode whose KV range is split across `world` GPUs leaves on every rank a packed
@@ -474,7 +563,8 @@ FA_API const char* fa_last_error(void);       /* message of the last failing cal
 /* Error bits recorded on the device (0 = none).  A bounded wait in a tensor-core kernel that
  * times out records a bit here and the kernel unwinds instead of hanging (its outputs are then
  * not valid); bits 1024 / 4096 / 256 flag a paged-K/V entry outside the cache and a rotary
- * position outside the cos/sin table (8192 / 16384 in the 8-bit cache operators, where 32768 is a copy whose wait gave up).  Synchronous (device -> host copy); clear != 0 resets the
+ * position outside the cos/sin table (8192 / 16384 in the 8-bit cache operators, where 32768 is a copy whose wait gave up); 131072
+ * is a state slot outside its pool or named twice, 262144 a wait of linear attention that gave up.  Synchronous (device -> host copy); clear != 0 resets the
  * bits.  No counterpart in the reference (its kernels have no waits that can give up). */
 FA_API int fa_device_error(int clear);
 /* Bit of fa_device_error set by fa_wait_selftest. */
