@@ -26,7 +26,7 @@ NVFLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler"
            "--expt-relaxed-constexpr", "-I", INC, "-I", CSRC]
 
 KERNEL_SOURCES = ["api.cu", "fwd_simt.cu", "fwd_sm100.cu", "bwd_simt.cu", "bwd_sm100.cu", "decode.cu", "decode_sm100.cu", "dropout.cu", "rotary.cu",
-                  "decode_peer.cu", "kvcache.cu", "decode8.cu", "linear.cu", "rotary_qk.cu"]
+                  "decode_peer.cu", "kvcache.cu", "decode8.cu", "linear.cu", "linear_sm100.cu", "rotary_qk.cu"]
 LIB = os.path.join(PKG, "libfable_attn.so")
 
 

@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(SIMT_THREADS)
   const long long per = (long long)r.da * r.dc, segs = ((long long)z * q.nhk + h) * q.nseg + n;
   const float* x0 = nullptr;
   if (!STATES) {
-    if (q.nseg > 1) x0 = ws + segs * per;
+    if (ws) x0 = ws + segs * per;
     else if (pool.in && !(pool.seen && pool.seen[z] <= 0)) x0 = pool.in + ((long long)slot * q.nhk + h) * per;
   }
   for (int e = tid; e < r.da * SCOL; e += SIMT_THREADS) {
@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(SIMT_THREADS)
   }
   float* x1 = nullptr;
   if (STATES) x1 = t1 > t0 ? ws_out + segs * per : nullptr;
-  else if (q.nseg == 1 && pool.out) x1 = pool.out + ((long long)slot * q.nhk + h) * per;
+  else if (!ws && pool.out) x1 = pool.out + ((long long)slot * q.nhk + h) * per;
   if (!x1) return;
   __syncthreads();
   for (int e = tid; e < r.da * SCOL; e += SIMT_THREADS) {
@@ -337,10 +337,19 @@ int join(const LinSeqs& q, bool rev, float* ws, const LinPool& pool, int per, cu
 }
 
 int states(const LinSeqs& q, const LinRole& r, bool rev, float* ws, int dtype, cudaStream_t st) {
-  return lin_simt_states(q, r, rev, ws, dtype, st);
+  bool taken = false;
+  if (int rc = lin_tc_states(q, r, rev, ws, dtype, st, &taken)) return rc;
+  return taken ? FA_OK : lin_simt_states(q, r, rev, ws, dtype, st);
 }
 int main_pass(const LinSeqs& q, const LinRole& r, bool rev, const float* ws, const LinPool& pool, int dtype, cudaStream_t st) {
-  return lin_simt_main(q, r, rev, ws, pool, dtype, st);
+  bool taken = false;
+  if (int rc = lin_tc_main(q, r, rev, ws, pool, dtype, st, &taken)) return rc;
+  return taken ? FA_OK : lin_simt_main(q, r, rev, ws, pool, dtype, st);
+}
+// The tensor-core kernels' last state comes from the states kernel (whose sums keep fp32's bits), so one segment goes
+// through it too where a last state is asked for.
+bool through_states(const LinSeqs& q, const LinRole& r, const float* out, int dtype) {
+  return q.nseg > 1 || (out && lin_tc_takes(q, r, dtype));
 }
 
 bool dims_ok(int dk, int dv) { return dk > 0 && dv > 0 && dk <= 256 && dv <= 256 && dk % 8 == 0 && dv % 8 == 0; }
@@ -370,7 +379,7 @@ int lin_device_error(int clear) {
     const int zero = 0;
     cudaMemcpyToSymbol(g_lin_error, &zero, sizeof(int));
   }
-  return v;
+  return v | lin_tc_device_error(clear);
 }
 }  // namespace fa
 
@@ -379,18 +388,30 @@ extern "C" FA_API long long fa_linear_plan(int batch, int S, long long total, in
   if (seg_len) *seg_len = 128;
   if (nseg) *nseg = 1;
   if (!seg_len || !nseg || batch <= 0 || S <= 0 || gqa <= 0 || NH < gqa || !dims_ok(dk, dv)) return 0;
-  // Enough segments that every SM has two blocks, none shorter than 128 tokens (each costs a state written and read
-  // again, 8 dk dv bytes, and its keys and values read twice).
   const long long states = (long long)batch * (NH / gqa);
   const long long tokens = total > 0 && total < (long long)batch * S ? std::max(1ll, total / batch) : S;
-  const int cols = (dv + 63) / 64;
-  const long long want = std::max(1ll, 2ll * num_sms() / std::max(1ll, states * cols));
-  long long len = (tokens + want - 1) / want;
-  len = std::max(128ll, (len + 127) / 128 * 128);
+  const bool tc = dtype != FA_DTYPE_F32 && dk <= 128 && dv <= 128;
+  const long long chunks = (tokens + 127) / 128, sms = num_sms();
+  long long best = 1;
+  if (tc) {
+    // Blocks run one to an SM.  In units of a chunk's time in the output kernel: as many chunks as the fullest SM walks, 3 for
+    // each block's start, and with more than one segment the states kernel, which takes less than half of that, and 4 for it and the join.
+    double least = 1e30;
+    for (long long n = 1; n <= std::min(chunks, 256ll); ++n) {
+      const double waves = (double)((states * n + sms - 1) / sms), walk = (double)((chunks + n - 1) / n);
+      const double cost = waves * (walk * (n > 1 ? 1.45 : 1.0) + (n > 1 ? 5.0 : 3.0)) + (n > 1 ? 4.0 : 0.0);
+      if (cost < least) least = cost, best = n;
+    }
+  } else {
+    // Two blocks to an SM, no segment shorter than 128 tokens (each costs a state written and read again, and its keys and
+    // values read twice).
+    best = std::max(1ll, std::min(chunks, 2 * sms / std::max(1ll, states * ((dv + 63) / 64))));
+  }
+  long long len = (chunks + best - 1) / best * 128;
   if (len >= S) len = (S + 127ll) / 128 * 128;
-  *seg_len = (int)std::min(len, (1ll << 30));
+  *seg_len = (int)std::min(len, 1ll << 30);
   *nseg = (int)((S + (long long)*seg_len - 1) / *seg_len);
-  return *nseg > 1 ? states * *nseg * dk * dv : 0;
+  return *nseg > 1 || tc ? states * *nseg * dk * dv : 0;
 }
 
 extern "C" FA_API int fa_linear_launch(const FaLinearParams* pp, int dtype, void* stream) {
@@ -424,11 +445,13 @@ extern "C" FA_API int fa_linear_launch(const FaLinearParams* pp, int dtype, void
     if (dtype == FA_DTYPE_BF16) return step_launch<__nv_bfloat16>(q, r, pool, st);
     return step_launch<float>(q, r, pool, st);
   }
-  if (q.nseg > 1) {
+  const bool joined = through_states(q, r, p.state_out, dtype);
+  FA_CHECK_ARG(!joined || p.states, "linear attention: the workspace `states` is missing");
+  if (joined) {
     if (int rc = states(q, r, false, p.states, dtype, st)) return rc;
     if (int rc = join(q, false, p.states, pool, p.dk * p.dv, st)) return rc;
   }
-  return main_pass(q, r, false, p.states, pool, dtype, st);
+  return main_pass(q, r, false, joined ? p.states : nullptr, pool, dtype, st);
 }
 
 extern "C" FA_API int fa_linear_backward_launch(const FaLinearBwdParams* pp, int dtype, void* stream) {
@@ -456,11 +479,14 @@ extern "C" FA_API int fa_linear_backward_launch(const FaLinearBwdParams* pp, int
   const LinRole dv{p.k, p.q, p.dO, p.dV, p.sK, p.sQ, p.sdO, p.sdV, 1, p.gqa, p.dk, p.dv, 0, s, 1.f, s};
   const LinPool forward{p.initial, nullptr, nullptr, nullptr, p.batch};
   const LinPool back{p.dfinal, p.dinitial, nullptr, nullptr, p.batch}, back_only{p.dfinal, nullptr, nullptr, nullptr, p.batch};
-  if (q.nseg > 1) {
+  const bool joined = through_states(q, dv, p.dinitial, dtype);
+  FA_CHECK_ARG(!joined || p.work, "linear attention backward: the workspace `work` is missing");
+  if (joined) {
     if (int rc = states(q, dv, true, p.work, dtype, st)) return rc;
     if (int rc = join(q, true, p.work, back, p.dk * p.dv, st)) return rc;
   }
-  if (int rc = main_pass(q, dq, false, p.states, forward, dtype, st)) return rc;
-  if (int rc = main_pass(q, dk, true, p.work, back_only, dtype, st)) return rc;
-  return main_pass(q, dv, true, p.work, q.nseg > 1 ? back_only : back, dtype, st);
+  const float* from = joined ? p.work : nullptr;
+  if (int rc = main_pass(q, dq, false, q.nseg > 1 ? p.states : nullptr, forward, dtype, st)) return rc;
+  if (int rc = main_pass(q, dk, true, from, back_only, dtype, st)) return rc;
+  return main_pass(q, dv, true, from, joined ? back_only : back, dtype, st);
 }

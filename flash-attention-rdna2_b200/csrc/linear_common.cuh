@@ -107,12 +107,14 @@ __device__ void lin_zero_outside(const LinSeqs& q, const LinRole& r, int z, int 
   }
 }
 
-// kernel families (host)
+// kernel families (host).  ws: the states that segments start from, joined already; null = one segment that starts from the
+// pool and leaves its last state there.
 int lin_simt_states(const LinSeqs& q, const LinRole& r, bool reversed, float* ws, int dtype, cudaStream_t st);
 int lin_simt_main(const LinSeqs& q, const LinRole& r, bool reversed, const float* ws, const LinPool& pool, int dtype, cudaStream_t st);
 int lin_tc_states(const LinSeqs& q, const LinRole& r, bool reversed, float* ws, int dtype, cudaStream_t st, bool* taken);
 int lin_tc_main(const LinSeqs& q, const LinRole& r, bool reversed, const float* ws, const LinPool& pool, int dtype, cudaStream_t st,
                 bool* taken);
+bool lin_tc_takes(const LinSeqs& q, const LinRole& r, int dtype);
 int lin_device_error(int clear);
 int lin_tc_device_error(int clear);
 }  // namespace fa

@@ -431,7 +431,7 @@ FA_API int fa_combine_launch(const FaCombineParams* p, void* stream);
  *              seen[z] <= 0 it starts from 0 whatever the slot holds.  A negative slot is padding: its sequence gives 0 and touches
  *              no state.  So does a slot outside the pool, and the later of two sequences of the same slot; these raise
  *              fa_device_error bit 131072.
- *   states     workspace of fa_linear_plan floats, 16-byte aligned (null where that is 0).  With keep_states the
+ *   states     workspace of fa_linear_plan floats, 16-byte aligned (null where that is 0, or with one segment and no state_out).  With keep_states the
  *              chunked kernels run whatever S is, and leave each segment's start state there for fa_linear_backward_launch.
  * fa_linear_plan: segments of seg_len tokens (nseg for the longest sequence) that run side by side, and the floats of `states`.
  * -------------------------------------------------------------------------------------------*/
