@@ -548,8 +548,10 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 
 // =====================================================================================
 // states: what a segment adds to the state, X = sum_j (lam^m_j b_j)^T c_j with powers up to the segment's own end, so that
-// nothing is scaled on the way: one product over all its tokens.  The result is a state that a caller may keep, in fp32, so the decayed rows
-// enter as three bf16 numbers (2^-24 of a term) or two fp16 ones (2^-22).  Bound by reading b and c once.
+// nothing is scaled on the way.  The result is a state that a caller may keep, in fp32, so the decayed rows enter as three bf16 numbers
+// (2^-24 of a term) or two fp16 ones (2^-22).  The tensor cores truncate each accumulation; so every item is summed from 0, its small
+// terms first (only the eight steps of the largest one then cut at the sum's full size), and items are added in registers, to nearest.
+// One accumulator over a whole segment had left 2e-6 of the state.  Bound by reading b and c once.
 // =====================================================================================
 template <int D, bool BF16>
 struct StCfg {
@@ -560,7 +562,7 @@ struct StCfg {
   static_assert(SMEM <= 232448, "shared memory per CTA");
 };
 struct StBz {
-  static constexpr int FULL = 0, EMPTY = 32, BT_READY = 64, BT_FREE = 80, DRAIN = 96, TMEM_ADDR = 104;
+  static constexpr int FULL = 0, EMPTY = 32, BT_READY = 64, DONE = 80, X_READ = 88, DRAIN = 96, TMEM_ADDR = 104;
 };
 
 template <int D, bool BF16, bool REV>
@@ -587,10 +589,9 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       mbar_init(bar + StBz::FULL + 8 * s, 1);
       mbar_init(bar + StBz::EMPTY + 8 * s, 1);
     }
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(bar + StBz::BT_READY + 8 * s, NELEM);
-      mbar_init(bar + StBz::BT_FREE + 8 * s, 1);
-    }
+    for (int s = 0; s < 2; ++s) mbar_init(bar + StBz::BT_READY + 8 * s, NELEM);
+    mbar_init(bar + StBz::DONE, 1);
+    mbar_init(bar + StBz::X_READ, NELEM);
     mbar_init(bar + StBz::DRAIN, 1);
     fence_barrier_init();
   }
@@ -634,17 +635,18 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         __syncwarp();
       }
       ok = ok && mbar_wait_warp(bar + StBz::BT_READY + 8 * (i & 1), (i >> 1) & 1);
+      if (i > 0) ok = ok && mbar_wait_warp(bar + StBz::X_READ, (i - 1) & 1);
       tc_fence_after();
       if (ok && lane == 0) {
         const uint64_t d = desc_mn(sbase + tile(i) + K::TILE, C);
         const uint32_t bt = tmem + K::BT_COL + (i & 1) * K::BT_COLS;
 #pragma unroll
-        for (int kk = 0; kk < C / 16; ++kk)
+        for (int w = K::TERMS - 1; w >= 0; --w)
 #pragma unroll
-          for (int w = 0; w < K::TERMS; ++w)
-            mma_ts(tmem + K::X_COL, bt + 64 * w + 8 * kk, desc_add(d, kk * 128), ID, i > 0 || kk > 0 || w > 0);
+          for (int kk = 0; kk < C / 16; ++kk)
+            mma_ts(tmem + K::X_COL, bt + 64 * w + 8 * kk, desc_add(d, kk * 128), ID, kk > 0 || w < K::TERMS - 1);
         mma_commit(bar + StBz::EMPTY + 8 * s);
-        mma_commit(bar + StBz::BT_FREE + 8 * (i & 1));
+        mma_commit(bar + StBz::DONE);
       }
       __syncwarp();
     }
@@ -656,12 +658,29 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     const int qd = warp & 3, hf = warp >> 2, row = qd * 32 + lane;
     const uint32_t la = tmem + ((uint32_t)(qd * 32) << 16);
     bool ok = true;
-    for (int i = 0; i < items; ++i) {
-      const int at = i / r.nb * C, cn = min(C, t1 - t0 - at);
-      ok = ok && mbar_wait_warp(bar + StBz::FULL + 8 * (i % K::NS), (i / K::NS) & 1);
-      if (i >= 2) ok = ok && mbar_wait_warp(bar + StBz::BT_FREE + 8 * (i & 1), ((i >> 1) - 1) & 1);
+    float acc[D / 2];
+#pragma unroll
+    for (int i = 0; i < D / 2; ++i) acc[i] = 0.f;
+    const auto add = [&](int i) {      // item i's sum
+      ok = ok && mbar_wait_warp(bar + StBz::DONE, i & 1);
       __syncwarp();
       tc_fence_after();
+#pragma unroll
+      for (int c0 = 0; c0 < D / 2; c0 += 32) {
+        float v[32];
+        tmem_ld32(la + K::X_COL + hf * (D / 2) + c0, v);
+        tc_wait_ld();
+#pragma unroll
+        for (int k = 0; k < 32; ++k) acc[c0 + k] += v[k];
+      }
+      tc_fence_before();
+      mbar_arrive(bar + StBz::X_READ);
+    };
+    for (int i = 0; i < items; ++i) {
+      // the buffer of decayed rows is free: item i - 2 was added up
+      const int at = i / r.nb * C, cn = min(C, t1 - t0 - at);
+      ok = ok && mbar_wait_warp(bar + StBz::FULL + 8 * (i % K::NS), (i / K::NS) & 1);
+      __syncwarp();
       const float far = lin_power(g2, REV ? at : t1 - t0 - at - cn);
       if (row < D) {
         const uint8_t* b = sgen + tile(i) + (row / 64) * C * 128 + (row % 8) * 2;
@@ -693,25 +712,15 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       tc_wait_st();
       tc_fence_before();
       mbar_arrive(bar + StBz::BT_READY + 8 * (i & 1));
+      if (i > 0) add(i - 1);
     }
-    const int e = items - 1;
-    ok = ok && mbar_wait_warp(bar + StBz::BT_FREE + 8 * (e & 1), (e >> 1) & 1);
-    __syncwarp();
-    tc_fence_after();
+    add(items - 1);
     float* x = ws + (((long long)z * q.nhk + h) * q.nseg + n) * r.da * r.dc + (long long)row * r.dc;
-    if (qd * 32 < D) {
 #pragma unroll
-      for (int c0 = 0; c0 < D / 2; c0 += 32) {
-        float v[32];
-        tmem_ld32(la + K::X_COL + hf * (D / 2) + c0, v);
-        tc_wait_ld();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int col = hf * (D / 2) + c0 + 4 * i;
-          if (row < r.da && col < r.dc)
-            *reinterpret_cast<float4*>(x + col) = make_float4(r.w_up * v[4 * i], r.w_up * v[4 * i + 1], r.w_up * v[4 * i + 2], r.w_up * v[4 * i + 3]);
-        }
-      }
+    for (int i = 0; i < D / 8; ++i) {
+      const int col = hf * (D / 2) + 4 * i;
+      if (row < r.da && col < r.dc)
+        *reinterpret_cast<float4*>(x + col) = make_float4(r.w_up * acc[4 * i], r.w_up * acc[4 * i + 1], r.w_up * acc[4 * i + 2], r.w_up * acc[4 * i + 3]);
     }
     if (!ok) record_error(LIN_ERR_WAIT);
   }
