@@ -16,9 +16,9 @@
 // left as they are: where they fall below 2^-14 their steps are 2^-24, which is fp16's own step for such inputs.
 //
 // Warp roles (320 threads): warps 0-7 elementwise, two to a TMEM lane quadrant (w and w + 4 share 32 lanes, w / 4 takes half
-// of the columns or tokens), warp 8 TMA, warp 9 MMA.  The elementwise warps run one item ahead of the epilogue: state and
-// decayed rows of item t, epilogue of item t - 1, pair products of item t, so that each waits for an MMA that has had another
-// step's time.  Every wait is bounded.
+// of the columns or tokens), warp 8 TMA, warp 9 MMA.  The elementwise warps take the decayed rows of item t, the epilogue of
+// item t - 1, then the state, the pair products and a X of item t, so that each waits for an MMA that has had another step's
+// time.  Every wait is bounded.
 #include <cudaTypedefs.h>
 #include "linear_common.cuh"
 #include "fa_launch.h"
@@ -49,17 +49,75 @@ __device__ __forceinline__ float2 unpack2(uint32_t w) {
   if constexpr (BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
   else return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
+// what is left of a pair once it is rounded to 16 bits (exact)
+template <bool BF16>
+__device__ __forceinline__ float2 rest2(float2 d, uint32_t hi) {
+  return __ffma2_rn(unpack2<BF16>(hi), make_float2(-1.f, -1.f), d);
+}
 // a pair as hi + lo 16-bit pairs
 template <bool BF16>
 __device__ __forceinline__ void split2(float2 d, uint32_t& hi, uint32_t& lo) {
   hi = pack2<BF16>(d.x, d.y);
-  const float2 h = unpack2<BF16>(hi);
-  lo = pack2<BF16>(d.x - h.x, d.y - h.y);
+  const float2 l = rest2<BF16>(d, hi);
+  lo = pack2<BF16>(l.x, l.y);
 }
-template <bool BF16>
-__device__ __forceinline__ float elem(uint16_t w) {
-  if constexpr (BF16) return __uint_as_float((uint32_t)w << 16);
-  else return __half2float(__ushort_as_half(w));
+
+// Four 8 x 8 blocks of 16-bit elements, transposed: a thread gets of each block the dim lane / 4 of tokens 2 (lane % 4) and + 1
+__device__ __forceinline__ void ldsm_t4(uint32_t addr, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// 16 TMEM lanes x 8 columns: thread T's r[2 n + e] goes to lane 8 e + T / 4, column 4 n + T % 4, which is where ldsm_t4 of
+// 16 dims x 16 tokens leaves token pairs
+__device__ __forceinline__ void tmem_st_16x8(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+}
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];"
+               ::"l"((uint64_t)map), "r"(src), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+
+// The decayed rows of a chunk, transposed for the A operand in TMEM: a warp takes 32 dims and 64 tokens (half hf).  Its thread
+// reads pairs of tokens 64 hf + 16 s + 8 m + 2 (lane % 4) (+ 1), whose factors w[2 s + m] stay in registers from chunk to
+// chunk.  Element by element from shared memory this took 6000 cycles a chunk, and half of the kernel's time.
+template <bool REV>
+__device__ __forceinline__ void row_factors(float2* w, const float* lam, float times, int hf, int lane, int cn) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int j = 64 * hf + 8 * i + 2 * (lane & 3);
+    w[i].x = j < cn ? times * lam[REV ? j + 1 : cn - 1 - j] : 0.f;
+    w[i].y = j + 1 < cn ? times * lam[REV ? j + 2 : cn - 2 - j] : 0.f;
+  }
+}
+template <bool BF16, int TERMS>
+__device__ __forceinline__ void decay_rows(uint32_t tile, uint32_t bt, const float2* w, int qd, int hf, int lane, int cn) {
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {          // 16 dims each
+    const int unit = 4 * (qd & 1) + 2 * half + ((lane >> 3) & 1), token = 64 * hf + 8 * (lane >> 4) + (lane & 7);
+    const uint32_t from = tile + (qd >> 1) * C * 128 + token * 128 + ((unit ^ (lane & 7)) << 4);
+    const uint32_t to = bt + ((uint32_t)(16 * half) << 16) + 32 * hf;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {                 // 16 tokens each
+      uint32_t r[4], o[3][4];
+      ldsm_t4(from + s * 16 * 128, r);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {               // blocks: dims 0-7 and 8-15 of the first 8 tokens, then of the next 8
+        if (cn < C) {                             // rows past the sequence may hold anything: a factor of 0 is not enough
+          const int j = 64 * hf + 16 * s + 8 * (i >> 1) + 2 * (lane & 3);
+          r[i] &= (j < cn ? 0xffffu : 0u) | (j + 1 < cn ? 0xffff0000u : 0u);
+        }
+        float2 x = __fmul2_rn(unpack2<BF16>(r[i]), w[2 * s + (i >> 1)]);
+#pragma unroll
+        for (int u = 0; u < TERMS; ++u) {
+          o[u][i] = pack2<BF16>(x.x, x.y);
+          if (u + 1 < TERMS) x = rest2<BF16>(x, o[u][i]);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < TERMS; ++u) tmem_st_16x8(to + 64 * u + 8 * s, o[u]);
+    }
+  }
 }
 
 // descriptors of a [rows][D] tile stored as D / 64 chunks of rows x 128 bytes (128-byte swizzle)
@@ -92,9 +150,10 @@ struct Cfg {
   static constexpr int NCH = D / 64;
   static constexpr int TILE = C * D * 2;            // a, b or c
   static constexpr int XT = D * D * 2;              // X hi or lo
-  static constexpr int NA = 2, NB = D == 128 ? 1 : 2, NC = 2;
+  static constexpr int NA = D == 128 ? 1 : 2, NB = D == 128 ? 1 : 2, NC = 2;
   static constexpr int OFF_X = 0, OFF_A = 2 * XT, OFF_B = OFF_A + NA * TILE, OFF_C = OFF_B + NB * TILE;
-  static constexpr int OFF_BAR = OFF_C + NC * TILE;
+  static constexpr int OFF_O = OFF_C + NC * TILE;   // outputs on their way: a box of 32 rows x D / 2 columns for each warp
+  static constexpr int OFF_BAR = OFF_O + TILE;
   static constexpr int OFF_LAM = OFF_BAR + 256;     // lam^n, n = 0 .. 128
   static constexpr int OFF_MAX = OFF_LAM + 132 * 4; // [2] largest |X|, then [2][128] largest |P| of half a row (fp16)
   static constexpr int SMEM = OFF_MAX + 16 + 2 * C * 4 + 1024;
@@ -110,7 +169,7 @@ struct Bz {
 template <int D, bool BF16, bool REV, bool SWAP>
 __global__ void __launch_bounds__(NTHREADS, 1)
     lin_tc_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb, const __grid_constant__ CUtensorMap tc,
-                  const LinSeqs q, const LinRole r, const float* ws, const LinPool pool) {
+                  const __grid_constant__ CUtensorMap to, const LinSeqs q, const LinRole r, const float* ws, const LinPool pool) {
   using K = Cfg<D>;
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
   extern __shared__ uint8_t smem_raw[];
@@ -342,10 +401,9 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       __syncwarp();
       tc_fence_after();
     };
+    const uint32_t obox = K::OFF_O + warp * 32 * HD * 2;
     const auto epilogue = [&](int t) {
-      const int cn = min(C, t1 - t0 - chunk_at(t)), g = r.na > 1 ? t % groups : 0;
-      const bool write = r.na > 1 || t % groups == groups - 1;
-      T* orow = out + (long long)(chunk_at(t) + row) * r.so.s + g * r.so.h;
+      const int at = chunk_at(t), cn = min(C, t1 - t0 - at), g = r.na > 1 ? t % groups : 0;
 #pragma unroll
       for (int c0 = 0; c0 < HD; c0 += 32) {
         float o[32];
@@ -356,110 +414,56 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       }
       tc_fence_before();
       mbar_arrive(bar + Bz::O_READ);
-      if (!write || row >= cn) return;
+      if ((r.na == 1 && t % groups != groups - 1) || hf * HD >= r.dc) return;
+      // 32 whole rows go out as one box; rows next to another sequence's one by one
+      const bool whole = qd * 32 + 32 <= cn;
+      T* orow = out + (long long)(at + row) * r.so.s + g * r.so.h + hf * HD;
+      if (whole) {
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        __syncwarp();
+      }
 #pragma unroll
       for (int i = 0; i < HD / 8; ++i) {
-        const int col = hf * HD + 8 * i;
-        if (col < r.dc)
-          *reinterpret_cast<uint4*>(orow + col) = make_uint4(pack2<BF16>(acc[8 * i], acc[8 * i + 1]), pack2<BF16>(acc[8 * i + 2], acc[8 * i + 3]),
-                                                             pack2<BF16>(acc[8 * i + 4], acc[8 * i + 5]), pack2<BF16>(acc[8 * i + 6], acc[8 * i + 7]));
+        const uint4 w = make_uint4(pack2<BF16>(acc[8 * i], acc[8 * i + 1]), pack2<BF16>(acc[8 * i + 2], acc[8 * i + 3]),
+                                   pack2<BF16>(acc[8 * i + 4], acc[8 * i + 5]), pack2<BF16>(acc[8 * i + 6], acc[8 * i + 7]));
+        if (whole)      // 128-byte or 64-byte swizzle
+          *reinterpret_cast<uint4*>(sgen + obox + lane * HD * 2 + ((i ^ (HD == 64 ? lane & 7 : (lane >> 1) & 3)) << 4)) = w;
+        else if (row < cn && hf * HD + 8 * i < r.dc)
+          *reinterpret_cast<uint4*>(orow + 8 * i) = w;
+      }
+      if (whole) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) tma_store_4d(&to, sbase + obox, hf * HD, (int)span.row0 + t0 + at + qd * 32, h * r.na + g, q.cu ? 0 : z);
       }
     };
+    float2 w_rows[8];
+    int w_cn = 0;
+    // Factors of the pair products: a block of 32 rows x 32 columns beside the diagonal takes lam^(rows from its near edge) times
+    // lam^(columns from it), both at most 1, so that nothing overflows however fast the decay
+    float u_blk[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int j0 = hf * 64 + 32 * b;
+      u_blk[b] = lam[REV ? max(j0 - row, 0) : max(row - j0 - 31, 0)];
+    }
     for (int t = 0; t < items; ++t) {
       const int g = t % groups;
       const bool first = g == 0, end = t / groups == chunks - 1;
       const bool do_b = (first || r.nb > 1) && !end, do_i = first || r.na > 1;
       const int cn = min(C, t1 - t0 - chunk_at(t));
-      // ---- the state: hi + lo to shared memory, lam^C X back to TMEM
-      if (first) {
-        if (t > 0) wait(Bz::X_DONE, nbt - 1);      // every update so far has landed
-        const float keep = lam[cn];
-        float xs = 1.f;
-        const auto load = [&](int c0, float* x) {
-          if (t > 0) {
-            tmem_ld32(la + K::X_COL + hf * HD + c0, x);
-            tc_wait_ld();
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const int col = hf * HD + c0 + i;
-              const int ii = SWAP ? col : row, jj = SWAP ? row : col;
-              x[i] = x0 && row < xl && col < xn ? x0[r.transposed ? (long long)jj * r.da + ii : (long long)ii * r.dc + jj] : 0.f;
-            }
-          }
-        };
-        if constexpr (!BF16) {
-          uint32_t top = 0;
-          if (row < D) {
-#pragma unroll
-            for (int c0 = 0; c0 < HD; c0 += 32) {
-              float x[32];
-              load(c0, x);
-#pragma unroll
-              for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-            }
-          }
-          top = __reduce_max_sync(0xffffffffu, top);
-          if (lane == 0) atomicMax(&xmax[nx & 1], top);
-          bar_elem();
-          xs = scale_to(xmax[nx & 1]);
-          if (tid == 0) xmax[(nx + 1) & 1] = 0;
-          x_inv = 1.f / xs;
-        }
-        if (row < D) {
-#pragma unroll
-          for (int c0 = 0; c0 < HD; c0 += 32) {
-            float x[32];
-            load(c0, x);
-            uint32_t hi[16], lo[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) split2<BF16>(make_float2(x[2 * i] * xs, x[2 * i + 1] * xs), hi[i], lo[i]);
-            const int col = hf * HD + c0;
-            uint8_t* xr = sgen + K::OFF_X + (col / 64) * D * 128 + row * 128;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int u = (((col % 64) / 8 + i) ^ (row & 7)) * 16;
-              *reinterpret_cast<uint4*>(xr + u) = make_uint4(hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
-              *reinterpret_cast<uint4*>(xr + K::XT + u) = make_uint4(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
-            }
-            uint32_t y[32];
-#pragma unroll
-            for (int i = 0; i < 32; ++i) y[i] = __float_as_uint(x[i] * keep);
-            tmem_st32(la + K::X_COL + hf * HD + c0, y);
-          }
-        }
-        tc_wait_st();
-        fence_proxy_async_smem();
-        tc_fence_before();
-        mbar_arrive(bar + Bz::XS_READY);
-        ++nx;
-      }
-      // ---- decayed rows, transposed: thread = dim, 64 tokens each
+      // ---- decayed rows, transposed
       if (first || r.nb > 1) ++cbw;
       if (do_b) {
+        if (cn != w_cn) {
+          row_factors<REV>(w_rows, lam, r.w_up, hf, lane, cn);
+          w_cn = cn;
+        }
         const int stages = SWAP ? K::NC : K::NB, s = cbw % stages;
         wait((SWAP ? Bz::C_FULL : Bz::B_FULL) + 8 * s, cbw / stages);
         if (nbt > 0) wait(Bz::X_DONE, nbt - 1);
-        if (row < D) {
-          const uint8_t* tile = sgen + (SWAP ? K::OFF_C : K::OFF_B) + s * K::TILE + (row / 64) * C * 128 + (row % 8) * 2;
-          const int unit = (row % 64) / 8;
-#pragma unroll
-          for (int b0 = 0; b0 < 64; b0 += 32) {
-            uint32_t hi[16], lo[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int j = hf * 64 + b0 + 2 * i;
-              float2 x;
-              x.x = elem<BF16>(*reinterpret_cast<const uint16_t*>(tile + j * 128 + ((unit ^ (j & 7)) * 16)));
-              x.y = elem<BF16>(*reinterpret_cast<const uint16_t*>(tile + (j + 1) * 128 + ((unit ^ ((j + 1) & 7)) * 16)));
-              x.x = j < cn ? x.x * (r.w_up * lam[REV ? j + 1 : max(cn - 1 - j, 0)]) : 0.f;
-              x.y = j + 1 < cn ? x.y * (r.w_up * lam[REV ? j + 2 : max(cn - 2 - j, 0)]) : 0.f;
-              split2<BF16>(x, hi[i], lo[i]);
-            }
-            tmem_st16(la + K::BT_COL + (hf * 64 + b0) / 2, hi);
-            tmem_st16(la + K::BT_COL + 64 + (hf * 64 + b0) / 2, lo);
-          }
-        }
+        if (qd * 32 < D)
+          decay_rows<BF16, 2>(sbase + (SWAP ? K::OFF_C : K::OFF_B) + s * K::TILE, la + K::BT_COL, w_rows, qd, hf, lane, cn);
         tc_wait_st();
         tc_fence_before();
         mbar_arrive(bar + Bz::BT_READY);
@@ -470,48 +474,117 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         wait(Bz::PV_DONE, t - 1);
         epilogue(t - 1);
       }
+      // ---- the state: hi + lo to shared memory, lam^C X back to TMEM
+      if (first) {
+        float x[HD];
+        if (t > 0) {
+          wait(Bz::X_DONE, nbt - 1 - (do_b ? 1 : 0));      // every update before this chunk's has landed
+          if (qd * 32 < D) {
+#pragma unroll
+            for (int c0 = 0; c0 < HD; c0 += 32) tmem_ld32(la + K::X_COL + hf * HD + c0, x + c0);
+            tc_wait_ld();
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < HD; ++i) {
+            const int col = hf * HD + i;
+            const int ii = SWAP ? col : row, jj = SWAP ? row : col;
+            x[i] = x0 && row < xl && col < xn ? x0[r.transposed ? (long long)jj * r.da + ii : (long long)ii * r.dc + jj] : 0.f;
+          }
+        }
+        float xs = 1.f;
+        if constexpr (!BF16) {
+          float top = 0.f;
+          if (qd * 32 < D) {
+#pragma unroll
+            for (int i = 0; i < HD; ++i) top = fmaxf(top, fabsf(x[i]));
+          }
+          const uint32_t all = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+          if (lane == 0) atomicMax(&xmax[nx & 1], all);
+          bar_elem();
+          xs = scale_to(xmax[nx & 1]);
+          if (tid == 0) xmax[(nx + 1) & 1] = 0;
+          x_inv = 1.f / xs;
+        }
+        const float keep = lam[cn];
+        if (qd * 32 < D) {
+          uint8_t* xr = sgen + K::OFF_X + row * 128;
+#pragma unroll
+          for (int i = 0; i < HD / 8; ++i) {
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) split2<BF16>(__fmul2_rn(make_float2(x[8 * i + 2 * k], x[8 * i + 2 * k + 1]), make_float2(xs, xs)), hi[k], lo[k]);
+            const int col = hf * HD + 8 * i;
+            uint8_t* to_x = xr + (col / 64) * D * 128 + ((((col % 64) / 8) ^ (row & 7)) << 4);
+            *reinterpret_cast<uint4*>(to_x) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            *reinterpret_cast<uint4*>(to_x + K::XT) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          }
+#pragma unroll
+          for (int i = 0; i < HD; ++i) x[i] *= keep;
+#pragma unroll
+          for (int c0 = 0; c0 < HD; c0 += 32) tmem_st32(la + K::X_COL + hf * HD + c0, reinterpret_cast<const uint32_t*>(x + c0));
+        }
+        tc_wait_st();
+        fence_proxy_async_smem();
+        tc_fence_before();
+        mbar_arrive(bar + Bz::XS_READY);
+        ++nx;
+      }
       // ---- pair products: decay, mask, back to TMEM as hi + lo
       wait(Bz::P_FULL, t);
       {
-        float ps = 1.f;
-        const auto load = [&](int c0, float* p) {
-          const int j0 = hf * 64 + c0;
-          // a block of 32 rows sees the blocks of 32 columns on its side of the diagonal
-          if (REV ? j0 / 32 < qd : j0 / 32 > qd) {
+        float2 p[2][16];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) p[i] = 0.f;
-            return;
+        for (int b = 0; b < 2; ++b) {
+          const int j0 = hf * 64 + 32 * b, side = REV ? j0 / 32 - qd : qd - j0 / 32;      // 0 on the diagonal, below 0 where nothing is seen
+          if (side < 0) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) p[b][i] = make_float2(0.f, 0.f);
+            continue;
           }
-          tmem_ld32(la + K::P_COL + j0, p);
+          tmem_ld32(la + K::P_COL + j0, reinterpret_cast<float*>(p[b]));
           tc_wait_ld();
+          if (side > 0) {
+            const float2 u = make_float2(u_blk[b], u_blk[b]);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const int gap = REV ? j0 + i - row : row - j0 - i;
-            p[i] = gap >= 0 && j0 + i < cn ? p[i] * lam[max(gap, 0)] : 0.f;
+            for (int i = 0; i < 16; ++i) {      // columns from the near edge: lam^(31 - j), or lam^j reversed
+              const float2 w = REV ? make_float2(lam[2 * i], lam[2 * i + 1]) : make_float2(lam[31 - 2 * i], lam[30 - 2 * i]);
+              p[b][i] = __fmul2_rn(p[b][i], __fmul2_rn(u, w));
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int gap = REV ? 2 * i - lane : lane - 2 * i, next = REV ? gap + 1 : gap - 1;
+              p[b][i].x = gap >= 0 ? p[b][i].x * lam[max(gap, 0)] : 0.f;
+              p[b][i].y = next >= 0 ? p[b][i].y * lam[max(next, 0)] : 0.f;
+            }
           }
-        };
+          if (REV && cn < C) {                  // forward, a row sees no token past its own
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              if (j0 + 2 * i >= cn) p[b][i].x = 0.f;
+              if (j0 + 2 * i + 1 >= cn) p[b][i].y = 0.f;
+            }
+          }
+        }
+        float ps = 1.f;
         if constexpr (!BF16) {
-          uint32_t top = 0;
+          float top = 0.f;
 #pragma unroll
-          for (int c0 = 0; c0 < 64; c0 += 32) {
-            float p[32];
-            load(c0, p);
+          for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(p[i]) & 0x7fffffffu);
-          }
-          pmax[hf * C + row] = top;
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, fmaxf(fabsf(p[b][i].x), fabsf(p[b][i].y)));
+          pmax[hf * C + row] = __float_as_uint(top);
           bar_pair(qd);
-          ps = scale_to(max(top, pmax[(hf ^ 1) * C + row]));
+          ps = scale_to(max(__float_as_uint(top), pmax[(hf ^ 1) * C + row]));
           bar_pair(qd);
         }
 #pragma unroll
-        for (int c0 = 0; c0 < 64; c0 += 32) {
-          float p[32];
-          load(c0, p);
+        for (int b = 0; b < 2; ++b) {
           uint32_t w[32];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) split2<BF16>(make_float2(p[2 * i] * ps, p[2 * i + 1] * ps), w[i], w[16 + i]);
-          tmem_st32(la + K::P_COL + hf * 64 + c0, w);
+          for (int i = 0; i < 16; ++i) split2<BF16>(BF16 ? p[b][i] : __fmul2_rn(p[b][i], make_float2(ps, ps)), w[i], w[16 + i]);
+          tmem_st32(la + K::P_COL + hf * 64 + 32 * b, w);
         }
         p_inv = r.w_intra / ps;
       }
@@ -524,10 +597,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         ++noi;
         const float mul = r.w_inter * lam[REV ? max(cn - 1 - row, 0) : min(row + 1, C)] * x_inv;
 #pragma unroll
-        for (int c0 = 0; c0 < HD; c0 += 32) {
-          tmem_ld32(la + K::O_COL + hf * HD + c0, acc + c0);
-          tc_wait_ld();
-        }
+        for (int c0 = 0; c0 < HD; c0 += 32) tmem_ld32(la + K::O_COL + hf * HD + c0, acc + c0);
+        tc_wait_ld();
         tc_fence_before();
         mbar_arrive(bar + Bz::OI_READ);
 #pragma unroll
@@ -536,6 +607,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     }
     wait(Bz::PV_DONE, items - 1);
     epilogue(items - 1);
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    __syncwarp();
     if (!ok) record_error(LIN_ERR_WAIT);
   }
   tc_fence_before();
@@ -676,39 +749,22 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       tc_fence_before();
       mbar_arrive(bar + StBz::X_READ);
     };
+    float2 w_rows[8];
+    int w_cn = 0;
     for (int i = 0; i < items; ++i) {
       // the buffer of decayed rows is free: item i - 2 was added up
       const int at = i / r.nb * C, cn = min(C, t1 - t0 - at);
       ok = ok && mbar_wait_warp(bar + StBz::FULL + 8 * (i % K::NS), (i / K::NS) & 1);
       __syncwarp();
-      const float far = lin_power(g2, REV ? at : t1 - t0 - at - cn);
-      if (row < D) {
-        const uint8_t* b = sgen + tile(i) + (row / 64) * C * 128 + (row % 8) * 2;
-        const int unit = (row % 64) / 8;
-        const uint32_t bt = la + K::BT_COL + (i & 1) * K::BT_COLS + hf * 32;
-#pragma unroll
-        for (int b0 = 0; b0 < 64; b0 += 32) {
-          uint32_t w[3][16];
-#pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            const int j = hf * 64 + b0 + 2 * k;
-            float2 x;
-            x.x = elem<BF16>(*reinterpret_cast<const uint16_t*>(b + j * 128 + ((unit ^ (j & 7)) * 16)));
-            x.y = elem<BF16>(*reinterpret_cast<const uint16_t*>(b + (j + 1) * 128 + ((unit ^ ((j + 1) & 7)) * 16)));
-            x.x = j < cn ? x.x * (far * lam[REV ? j + 1 : max(cn - 1 - j, 0)]) : 0.f;
-            x.y = j + 1 < cn ? x.y * (far * lam[REV ? j + 2 : max(cn - 2 - j, 0)]) : 0.f;
-#pragma unroll
-            for (int u = 0; u < K::TERMS; ++u) {
-              w[u][k] = pack2<BF16>(x.x, x.y);
-              const float2 y = unpack2<BF16>(w[u][k]);
-              x.x -= y.x;
-              x.y -= y.y;
-            }
-          }
-#pragma unroll
-          for (int u = 0; u < K::TERMS; ++u) tmem_st16(bt + 64 * u + b0 / 2, w[u]);
-        }
+      if (cn != w_cn) {
+        row_factors<REV>(w_rows, lam, 1.f, hf, lane, cn);
+        w_cn = cn;
       }
+      const float far = lin_power(g2, REV ? at : t1 - t0 - at - cn);
+      float2 w[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) w[k] = __fmul2_rn(w_rows[k], make_float2(far, far));
+      if (qd * 32 < D) decay_rows<BF16, K::TERMS>(sbase + tile(i), la + K::BT_COL + (i & 1) * K::BT_COLS, w, qd, hf, lane, cn);
       tc_wait_st();
       tc_fence_before();
       mbar_arrive(bar + StBz::BT_READY + 8 * (i & 1));
@@ -744,8 +800,9 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
-// boxes of 64 columns x 128 rows over [batch][heads][rows][dim]; false where the layout does not allow it
-bool map4(CUtensorMap* m, const void* base, bool bf16, int dim, long long rows, long long heads, long long batch, const FaStrides& st) {
+// boxes of `cols` columns (64, or 32) x `box_rows` rows over [batch][heads][rows][dim]; false where the layout does not allow it
+bool map4(CUtensorMap* m, const void* base, bool bf16, int dim, long long rows, long long heads, long long batch, const FaStrides& st,
+          int cols = 64, int box_rows = C) {
   const auto enc = encode_fn();
   if (!enc || (uintptr_t)base % 16) return false;
   // a stride that no second entry uses says nothing: any that is allowed will do
@@ -754,9 +811,9 @@ bool map4(CUtensorMap* m, const void* base, bool bf16, int dim, long long rows, 
   const cuuint64_t strides[3] = {(cuuint64_t)ss * 2, (cuuint64_t)sh * 2, (cuuint64_t)sb * 2};
   for (int i = 0; i < 3; ++i)
     if (strides[i] == 0 || strides[i] % 16 || strides[i] >= (1ull << 40)) return false;
-  const cuuint32_t box[4] = {64, C, 1, 1}, estr[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {(cuuint32_t)cols, (cuuint32_t)box_rows, 1, 1}, estr[4] = {1, 1, 1, 1};
   return enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, box,
-             estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             estr, CU_TENSOR_MAP_INTERLEAVE_NONE, cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -778,9 +835,9 @@ template <int D, bool BF16>
 int run_main(const LinSeqs& q, const LinRole& r, bool rev, const float* ws, const LinPool& pool, cudaStream_t st, const CUtensorMap* m) {
   static unsigned long long done[3] = {};
   // dk: the output is along the state's rows as it is stored
-  if (rev && r.transposed) return launch(lin_tc_kernel<D, BF16, true, true>, Cfg<D>::SMEM, done, q, st, m[0], m[1], m[2], q, r, ws, pool);
-  if (rev) return launch(lin_tc_kernel<D, BF16, true, false>, Cfg<D>::SMEM, done + 1, q, st, m[0], m[1], m[2], q, r, ws, pool);
-  return launch(lin_tc_kernel<D, BF16, false, false>, Cfg<D>::SMEM, done + 2, q, st, m[0], m[1], m[2], q, r, ws, pool);
+  if (rev && r.transposed) return launch(lin_tc_kernel<D, BF16, true, true>, Cfg<D>::SMEM, done, q, st, m[0], m[1], m[2], m[3], q, r, ws, pool);
+  if (rev) return launch(lin_tc_kernel<D, BF16, true, false>, Cfg<D>::SMEM, done + 1, q, st, m[0], m[1], m[2], m[3], q, r, ws, pool);
+  return launch(lin_tc_kernel<D, BF16, false, false>, Cfg<D>::SMEM, done + 2, q, st, m[0], m[1], m[2], m[3], q, r, ws, pool);
 }
 template <int D, bool BF16>
 int run_states(const LinSeqs& q, const LinRole& r, bool rev, float* ws, cudaStream_t st, const CUtensorMap* m) {
@@ -799,13 +856,13 @@ int lin_tc_main(const LinSeqs& q, const LinRole& r, bool rev, const float* ws, c
   if (!takes(q, r, dtype) || (pool.out && !ws)) return FA_OK;
   const bool bf16 = dtype == FA_DTYPE_BF16;
   const long long rows = q.cu ? q.total : q.S, zs = q.cu ? 1 : q.batch;
-  CUtensorMap m[3];
-  if (!map4(m, r.a, bf16, r.da, rows, (long long)q.nhk * r.na, zs, r.sa) || !map4(m + 1, r.b, bf16, r.da, rows, (long long)q.nhk * r.nb, zs, r.sb) ||
-      !map4(m + 2, r.c, bf16, r.dc, rows, (long long)q.nhk * r.nb, zs, r.sc))
-    return FA_OK;
-  if ((uintptr_t)r.out % 16 || r.so.s % 8 || r.so.h % 8 || (zs > 1 && r.so.b % 8)) return FA_OK;
-  *taken = true;
   const bool small = r.da <= 64 && r.dc <= 64;
+  CUtensorMap m[4];
+  if (!map4(m, r.a, bf16, r.da, rows, (long long)q.nhk * r.na, zs, r.sa) || !map4(m + 1, r.b, bf16, r.da, rows, (long long)q.nhk * r.nb, zs, r.sb) ||
+      !map4(m + 2, r.c, bf16, r.dc, rows, (long long)q.nhk * r.nb, zs, r.sc) ||
+      !map4(m + 3, r.out, bf16, r.dc, rows, (long long)q.nhk * r.na, zs, r.so, small ? 32 : 64, 32))
+    return FA_OK;
+  *taken = true;
   if (bf16) return small ? run_main<64, true>(q, r, rev, ws, pool, st, m) : run_main<128, true>(q, r, rev, ws, pool, st, m);
   return small ? run_main<64, false>(q, r, rev, ws, pool, st, m) : run_main<128, false>(q, r, rev, ws, pool, st, m);
 }
