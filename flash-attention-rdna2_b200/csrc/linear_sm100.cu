@@ -15,10 +15,14 @@
 // to a largest value of about 2^10 by a power of 2 each, and X by one for the tile, taken back in the epilogue; the decayed rows are
 // left as they are: where they fall below 2^-14 their steps are 2^-24, which is fp16's own step for such inputs.
 //
-// Warp roles (320 threads): warps 0-7 elementwise, two to a TMEM lane quadrant (w and w + 4 share 32 lanes, w / 4 takes half
-// of the columns or tokens), warp 8 TMA, warp 9 MMA.  The elementwise warps take the decayed rows of item t, the epilogue of
-// item t - 1, then the state, the pair products and a X of item t, so that each waits for an MMA that has had another step's
-// time.  Every wait is bounded.
+// Warp roles (640 threads, five warpgroups):
+//   0-7    outputs: pair products on their way back to TMEM, a X, epilogue; two warps to a TMEM lane quadrant (w % 4), half of the columns each
+//   8-15   state: decayed rows, X to shared memory and lam^C X back to TMEM; two warps to a quadrant likewise
+//   16, 17 TMA, MMA
+// What a chunk needs is a chain of short steps, each a TMEM or shared memory latency long, and not their instructions: one
+// set of warps that took all steps in turn needed 10000 cycles a chunk, issuing every third cycle.  Outputs of item t and the state
+// of the next chunk depend on each other through the MMAs alone, so two sets run them side by side, each waiting for an MMA
+// that has had another step's time.  Registers follow the need (setmaxnreg): the epilogue holds 64 columns.  Every wait is bounded.
 #include <cudaTypedefs.h>
 #include "linear_common.cuh"
 #include "fa_launch.h"
@@ -30,7 +34,13 @@ using namespace sm100;
 using namespace fa;
 
 constexpr int C = 128;               // tokens of a chunk
-constexpr int NTHREADS = 320, NELEM = 256, WARP_TMA = 8, WARP_MMA = 9;
+constexpr int NTHREADS = 640, NOUT = 256, NSTATE = 256, WARP_TMA = 16, WARP_MMA = 17;
+// registers a thread: launched with REGS; 2 x 136 + 2 x 80 + 48 = 5 x 96
+constexpr int REGS = 96;
+__device__ __forceinline__ void regs_out() { asm volatile("setmaxnreg.inc.sync.aligned.u32 136;"); }
+__device__ __forceinline__ void regs_state() { asm volatile("setmaxnreg.dec.sync.aligned.u32 80;"); }
+__device__ __forceinline__ void regs_few() { asm volatile("setmaxnreg.dec.sync.aligned.u32 48;"); }
+constexpr int NTHREADS_ST = 576, NELEM_ST = 512;      // the states kernel: 16 elementwise warps
 __device__ int g_lin_tc_error = 0;
 __device__ __forceinline__ void record_error(int code) { atomicOr(&g_lin_tc_error, code); }
 
@@ -78,36 +88,38 @@ __device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t sr
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 
-// The decayed rows of a chunk, transposed for the A operand in TMEM: a warp takes 32 dims and 64 tokens (half hf).  Its thread
-// reads pairs of tokens 64 hf + 16 s + 8 m + 2 (lane % 4) (+ 1), whose factors w[2 s + m] stay in registers from chunk to
-// chunk.  Element by element from shared memory this took 6000 cycles a chunk, and half of the kernel's time.
-template <bool REV>
-__device__ __forceinline__ void row_factors(float2* w, const float* lam, float times, int hf, int lane, int cn) {
+// The decayed rows of a chunk, transposed for the A operand in TMEM: a warp takes 32 dims and 16 N tokens from `first` on.  Its thread
+// reads pairs of tokens first + 16 s + 8 m + 2 (lane % 4) (+ 1), whose factors w[2 s + m] stay in registers from chunk to
+// chunk.  Element by element from shared memory this took 6000 cycles a chunk.
+template <bool REV, int N>
+__device__ __forceinline__ void row_factors(float2* w, const float* lam, float times, int first, int lane, int cn) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int j = 64 * hf + 8 * i + 2 * (lane & 3);
+  for (int i = 0; i < 2 * N; ++i) {
+    const int j = first + 8 * i + 2 * (lane & 3);
     w[i].x = j < cn ? times * lam[REV ? j + 1 : cn - 1 - j] : 0.f;
     w[i].y = j + 1 < cn ? times * lam[REV ? j + 2 : cn - 2 - j] : 0.f;
   }
 }
-template <bool BF16, int TERMS>
-__device__ __forceinline__ void decay_rows(uint32_t tile, uint32_t bt, const float2* w, int qd, int hf, int lane, int cn) {
-#pragma unroll
+template <bool BF16, int TERMS, int N>
+__device__ __forceinline__ void decay_rows(uint32_t tile, uint32_t bt, const float2* w, int qd, int first, int lane, int cn) {
+#pragma unroll 1
   for (int half = 0; half < 2; ++half) {          // 16 dims each
-    const int unit = 4 * (qd & 1) + 2 * half + ((lane >> 3) & 1), token = 64 * hf + 8 * (lane >> 4) + (lane & 7);
+    const int unit = 4 * (qd & 1) + 2 * half + ((lane >> 3) & 1), token = first + 8 * (lane >> 4) + (lane & 7);
     const uint32_t from = tile + (qd >> 1) * C * 128 + token * 128 + ((unit ^ (lane & 7)) << 4);
-    const uint32_t to = bt + ((uint32_t)(16 * half) << 16) + 32 * hf;
+    const uint32_t to = bt + ((uint32_t)(16 * half) << 16) + first / 2;
+    uint32_t r[N][4];
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {                 // 16 tokens each
-      uint32_t r[4], o[3][4];
-      ldsm_t4(from + s * 16 * 128, r);
+    for (int s = 0; s < N; ++s) ldsm_t4(from + s * 16 * 128, r[s]);
+#pragma unroll
+    for (int s = 0; s < N; ++s) {                 // 16 tokens each
+      uint32_t o[3][4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {               // blocks: dims 0-7 and 8-15 of the first 8 tokens, then of the next 8
         if (cn < C) {                             // rows past the sequence may hold anything: a factor of 0 is not enough
-          const int j = 64 * hf + 16 * s + 8 * (i >> 1) + 2 * (lane & 3);
-          r[i] &= (j < cn ? 0xffffu : 0u) | (j + 1 < cn ? 0xffff0000u : 0u);
+          const int j = first + 16 * s + 8 * (i >> 1) + 2 * (lane & 3);
+          r[s][i] &= (j < cn ? 0xffffu : 0u) | (j + 1 < cn ? 0xffff0000u : 0u);
         }
-        float2 x = __fmul2_rn(unpack2<BF16>(r[i]), w[2 * s + (i >> 1)]);
+        float2 x = __fmul2_rn(unpack2<BF16>(r[s][i]), w[2 * s + (i >> 1)]);
 #pragma unroll
         for (int u = 0; u < TERMS; ++u) {
           o[u][i] = pack2<BF16>(x.x, x.y);
@@ -120,14 +132,36 @@ __device__ __forceinline__ void decay_rows(uint32_t tile, uint32_t bt, const flo
   }
 }
 
+// N = 16 or 32 fp32 columns of this thread's lane
+template <int N>
+__device__ __forceinline__ void tmem_load(uint32_t taddr, float2* v) {
+  if constexpr (N == 32) tmem_ld32(taddr, reinterpret_cast<float*>(v));
+  else tmem_ld16(taddr, reinterpret_cast<float*>(v));
+  tc_wait_ld();
+}
+template <int N>
+__device__ __forceinline__ void tmem_store(uint32_t taddr, const float2* v) {
+  if constexpr (N == 32) tmem_st32(taddr, reinterpret_cast<const uint32_t*>(v));
+  else tmem_st16(taddr, reinterpret_cast<const uint32_t*>(v));
+}
+
 // descriptors of a [rows][D] tile stored as D / 64 chunks of rows x 128 bytes (128-byte swizzle)
 __device__ __forceinline__ uint64_t desc_k(uint32_t tile) { return sdesc_sw128(tile, 16, 1024); }
 __device__ __forceinline__ uint64_t desc_mn(uint32_t tile, int rows) { return sdesc_sw128(tile, rows * 128, 1024); }
 // 16 steps along the contracted dim, in 16-byte units
 __device__ __forceinline__ uint32_t step_k(int kk, int rows) { return (uint32_t)(((kk / 4) * rows * 128 + (kk % 4) * 32) >> 4); }
 
-__device__ __forceinline__ void bar_elem() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
-__device__ __forceinline__ void bar_pair(int quadrant) { asm volatile("bar.sync %0, 64;" ::"r"(2 + quadrant) : "memory"); }
+// Bounded warp-uniform wait, in few instructions: the kernel has some thirty of them, and what bounded it was the fetching of
+// instructions (a quarter of all stalls) while its steps were unrolled in full.  Gives up after 8e9 cycles, about 4 s.
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity) {
+  const long long from = clock64();
+  while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity)))
+    if (__any_sync(0xffffffffu, clock64() - from > 8000000000ll)) return false;
+  return true;
+}
+
+__device__ __forceinline__ void bar_state() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ void bar_quadrant(int quadrant) { asm volatile("bar.sync %0, 64;" ::"r"(2 + quadrant) : "memory"); }
 
 // power of 2 that brings a largest value of `top` to [2^10, 2^11); 1 for 0 and for what is not finite
 __device__ __forceinline__ float scale_to(uint32_t top_bits) {
@@ -152,10 +186,11 @@ struct Cfg {
   static constexpr int XT = D * D * 2;              // X hi or lo
   static constexpr int NA = D == 128 ? 1 : 2, NB = D == 128 ? 1 : 2, NC = 2;
   static constexpr int OFF_X = 0, OFF_A = 2 * XT, OFF_B = OFF_A + NA * TILE, OFF_C = OFF_B + NB * TILE;
-  static constexpr int OFF_O = OFF_C + NC * TILE;   // outputs on their way: a box of 32 rows x D / 2 columns for each warp
+  static constexpr int OFF_O = OFF_C + NC * TILE;   // outputs on their way: a box of 32 rows x D / 2 columns for each output warp
   static constexpr int OFF_BAR = OFF_O + TILE;
-  static constexpr int OFF_LAM = OFF_BAR + 256;     // lam^n, n = 0 .. 128
-  static constexpr int OFF_MAX = OFF_LAM + 132 * 4; // [2] largest |X|, then [2][128] largest |P| of half a row (fp16)
+  static constexpr int OFF_LAM = OFF_BAR + 192;     // lam^n, n = 0 .. 128
+  static constexpr int OFF_LAMC = OFF_LAM + 528;    // of a block's 32 columns: lam^(31 - j), or lam^j reversed
+  static constexpr int OFF_MAX = OFF_LAMC + 128;    // fp16: [3] largest |X|, then [2][128] largest |P| of half a row
   static constexpr int SMEM = OFF_MAX + 16 + 2 * C * 4 + 1024;
   static constexpr uint32_t P_COL = 0, BT_COL = 128, X_COL = 256, O_COL = 256 + D;
   static_assert(SMEM <= 232448, "shared memory per CTA");
@@ -192,6 +227,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   uint8_t* sgen = smem_raw + (sbase - smem_u32(smem_raw));
   const uint32_t bar = sbase + K::OFF_BAR;
   float* lam = reinterpret_cast<float*>(sgen + K::OFF_LAM);
+  float* lamc = reinterpret_cast<float*>(sgen + K::OFF_LAMC);
   uint32_t* xmax = reinterpret_cast<uint32_t*>(sgen + K::OFF_MAX);
   uint32_t* pmax = xmax + 4;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sgen + K::OFF_BAR + Bz::TMEM_ADDR);
@@ -208,16 +244,16 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       mbar_init(bar + Bz::C_EMPTY + 8 * s, 1);
     }
     mbar_init(bar + Bz::P_FULL, 1);
-    mbar_init(bar + Bz::P_READY, NELEM);
+    mbar_init(bar + Bz::P_READY, NOUT);
     mbar_init(bar + Bz::PV_DONE, 1);
-    mbar_init(bar + Bz::XS_READY, NELEM);
-    mbar_init(bar + Bz::BT_READY, NELEM);
+    mbar_init(bar + Bz::XS_READY, NSTATE);
+    mbar_init(bar + Bz::BT_READY, NSTATE);
     mbar_init(bar + Bz::X_DONE, 1);
     mbar_init(bar + Bz::OI_FULL, 1);
-    mbar_init(bar + Bz::OI_READ, NELEM);
-    mbar_init(bar + Bz::O_READ, NELEM);
+    mbar_init(bar + Bz::OI_READ, NOUT);
+    mbar_init(bar + Bz::O_READ, NOUT);
     mbar_init(bar + Bz::DRAIN, 1);
-    xmax[0] = xmax[1] = 0;
+    xmax[0] = xmax[1] = xmax[2] = 0;
     fence_barrier_init();
   }
   if (warp == WARP_MMA) {
@@ -225,21 +261,37 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     tmem_relinquish();
   }
   if (tid <= C) lam[tid] = lin_power(g2, tid);
+  if (tid < 32) lamc[tid] = lin_power(g2, REV ? tid : 31 - tid);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  // item t: chunk t / groups (from the end where reversed), head t % groups of the side that has several
-  const auto chunk_at = [&](int t) { return (REV ? chunks - 1 - t / groups : t / groups) * C; };
+  // item t = ck * groups + g: chunk ck (from the end where reversed), head g of the side that has several
+  const auto chunk_at = [&](int ck) { return (REV ? chunks - 1 - ck : ck) * C; };
 
-  if (warp == WARP_TMA) {
-    if (lane == 0) {
+  if (warp >= WARP_TMA) {
+    regs_few();
+    if (warp == WARP_TMA && lane == 0) {
       int na = 0, nb = 0, nc = 0;
       bool ok = true;
       const int z4 = q.cu ? 0 : z;
-      for (int t = 0; ok && t < items; ++t) {
-        const int g = t % groups, row = (int)span.row0 + t0 + chunk_at(t);
+      for (int ck = 0, g = 0; ok && ck < chunks; ++g == groups ? g = 0, ++ck : 0) {
+        const int row = (int)span.row0 + t0 + chunk_at(ck);
+        // c has two buffers and b is free first; a waits for a X, the last to read it
+        if (g == 0 || r.nb > 1) {
+          const int hh = h * r.nb + (r.nb > 1 ? g : 0), s = nc % K::NC, s2 = nb % K::NB;
+          if (nc >= K::NC && !mbar_wait(bar + Bz::C_EMPTY + 8 * s, ((nc / K::NC) - 1) & 1)) { ok = false; break; }
+          mbar_expect_tx(bar + Bz::C_FULL + 8 * s, K::TILE);
+          for (int c = 0; c < K::NCH; ++c)
+            tma_load_4d(sbase + K::OFF_C + s * K::TILE + c * C * 128, &tc, c * 64, row, hh, z4, bar + Bz::C_FULL + 8 * s);
+          ++nc;
+          if (nb >= K::NB && !mbar_wait(bar + Bz::B_EMPTY + 8 * s2, ((nb / K::NB) - 1) & 1)) { ok = false; break; }
+          mbar_expect_tx(bar + Bz::B_FULL + 8 * s2, K::TILE);
+          for (int c = 0; c < K::NCH; ++c)
+            tma_load_4d(sbase + K::OFF_B + s2 * K::TILE + c * C * 128, &tb, c * 64, row, hh, z4, bar + Bz::B_FULL + 8 * s2);
+          ++nb;
+        }
         if (g == 0 || r.na > 1) {
           const int s = na % K::NA;
           if (na >= K::NA && !mbar_wait(bar + Bz::A_EMPTY + 8 * s, ((na / K::NA) - 1) & 1)) { ok = false; break; }
@@ -248,20 +300,6 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             tma_load_4d(sbase + K::OFF_A + s * K::TILE + c * C * 128, &ta, c * 64, row, h * r.na + (r.na > 1 ? g : 0), z4, bar + Bz::A_FULL + 8 * s);
           ++na;
         }
-        if (g == 0 || r.nb > 1) {
-          const int s = nb % K::NB, hh = h * r.nb + (r.nb > 1 ? g : 0);
-          if (nb >= K::NB && !mbar_wait(bar + Bz::B_EMPTY + 8 * s, ((nb / K::NB) - 1) & 1)) { ok = false; break; }
-          mbar_expect_tx(bar + Bz::B_FULL + 8 * s, K::TILE);
-          for (int c = 0; c < K::NCH; ++c)
-            tma_load_4d(sbase + K::OFF_B + s * K::TILE + c * C * 128, &tb, c * 64, row, hh, z4, bar + Bz::B_FULL + 8 * s);
-          ++nb;
-          const int s2 = nc % K::NC;
-          if (nc >= K::NC && !mbar_wait(bar + Bz::C_EMPTY + 8 * s2, ((nc / K::NC) - 1) & 1)) { ok = false; break; }
-          mbar_expect_tx(bar + Bz::C_FULL + 8 * s2, K::TILE);
-          for (int c = 0; c < K::NCH; ++c)
-            tma_load_4d(sbase + K::OFF_C + s2 * K::TILE + c * C * 128, &tc, c * 64, row, hh, z4, bar + Bz::C_FULL + 8 * s2);
-          ++nc;
-        }
       }
       if (!ok) record_error(LIN_ERR_WAIT);
       // copies must have landed before the block leaves
@@ -269,84 +307,58 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       for (int i = max(0, nb - K::NB); i < nb; ++i) mbar_wait(bar + Bz::B_FULL + 8 * (i % K::NB), (i / K::NB) & 1);
       for (int i = max(0, nc - K::NC); i < nc; ++i) mbar_wait(bar + Bz::C_FULL + 8 * (i % K::NC), (i / K::NC) & 1);
     }
-    __syncwarp();
-  } else if (warp == WARP_MMA) {
+    if (warp == WARP_MMA) {
     constexpr uint32_t ID_P = idesc_f16(BF16 ? 1 : 0, C, C, 0, 0);
     constexpr uint32_t ID_T = idesc_f16(BF16 ? 1 : 0, C, D, 0, 1);                       // B along its rows
     constexpr uint32_t ID_I = idesc_f16(BF16 ? 1 : 0, C, D, 0, SWAP ? 0 : 1);            // O = a X: X [da][dc], or (SWAP) [dc][da]
     int ca = -1, cb = -1, cc = -1, nx = 0, nbt = 0, noi = 0;    // tiles taken, and steps signalled so far
     bool ok = true;
-    for (int t = 0; ok && t < items; ++t) {
-      const int g = t % groups;
-      const bool first = g == 0, last = g == groups - 1, end = t / groups == chunks - 1;
-      const bool do_b = (first || r.nb > 1) && !end, do_i = first || r.na > 1;
-      const int cn = min(C, t1 - t0 - chunk_at(t));
+    for (int t = 0, ck = 0, g = 0; ok && t < items; ++t, ++g == groups ? g = 0, ++ck : 0) {
+      const bool first = g == 0, last = g == groups - 1, end = ck == chunks - 1;
+      const bool new_b = first || r.nb > 1, do_b = new_b && !end, do_i = first || r.na > 1;
+      const int cn = min(C, t1 - t0 - chunk_at(ck));
       // P = a b^T
-      if (first || r.na > 1) {
-        ++ca;
-        ok = ok && mbar_wait_warp(bar + Bz::A_FULL + 8 * (ca % K::NA), (ca / K::NA) & 1);
-      }
-      if (first || r.nb > 1) {
+      if (new_b) {
         ++cb;
         ++cc;
-        ok = ok && mbar_wait_warp(bar + Bz::B_FULL + 8 * (cb % K::NB), (cb / K::NB) & 1);
-        if (SWAP && cn < C && q.cu) {
+        ok = ok && wait_warp(bar + Bz::B_FULL + 8 * (cb % K::NB), (cb / K::NB) & 1);
+        if (SWAP && ok && cn < C && q.cu) {
           zero_rows(sgen + K::OFF_B + (cb % K::NB) * K::TILE, K::NCH, cn, lane);
           fence_proxy_async_smem();
           __syncwarp();
         }
       }
-      if (t > 0) ok = ok && mbar_wait_warp(bar + Bz::PV_DONE, (t - 1) & 1);
+      if (do_i) {
+        ++ca;
+        ok = ok && wait_warp(bar + Bz::A_FULL + 8 * (ca % K::NA), (ca / K::NA) & 1);
+      }
+      if (t > 0) ok = ok && wait_warp(bar + Bz::PV_DONE, (t - 1) & 1);
       if (!ok) break;
-      const uint32_t at = sbase + K::OFF_A + (ca % K::NA) * K::TILE, bt = sbase + K::OFF_B + (cb % K::NB) * K::TILE,
-                     ct = sbase + K::OFF_C + (cc % K::NC) * K::TILE;
+      uint32_t at = sbase + K::OFF_A + (ca % K::NA) * K::TILE, bt = sbase + K::OFF_B + (cb % K::NB) * K::TILE,
+               ct = sbase + K::OFF_C + (cc % K::NC) * K::TILE, xt = sbase + K::OFF_X;
+      // opaque: the steps' descriptors are formed where they are used; kept from item to item they would fill the registers
+      asm volatile("" : "+r"(at), "+r"(bt), "+r"(ct), "+r"(xt));
       tc_fence_after();
       if (lane == 0) {
         const uint64_t da = desc_k(at), db = desc_k(bt);
-#pragma unroll
+#pragma unroll 1
         for (int kk = 0; kk < D / 16; ++kk)
           mma_ss(tmem + K::P_COL, desc_add(da, step_k(kk, C)), desc_add(db, step_k(kk, C)), ID_P, kk > 0);
         mma_commit(bar + Bz::P_FULL);
       }
       __syncwarp();
-      if (first || r.nb > 1) {
-        ok = mbar_wait_warp(bar + Bz::C_FULL + 8 * (cc % K::NC), (cc / K::NC) & 1);
-        if (ok && cn < C && q.cu) {
-          zero_rows(sgen + K::OFF_C + (cc % K::NC) * K::TILE, K::NCH, cn, lane);
-          fence_proxy_async_smem();
-          __syncwarp();
-        }
-      }
+      // O = a X, once the epilogue has taken the item before
       if (first) {
-        ok = ok && mbar_wait_warp(bar + Bz::XS_READY, nx & 1);
+        ok = ok && wait_warp(bar + Bz::XS_READY, nx & 1);
         ++nx;
       }
-      // X += (decayed rows)^T (rows)
-      if (do_b) {
-        ok = ok && mbar_wait_warp(bar + Bz::BT_READY, nbt & 1);
-        ++nbt;
-        tc_fence_after();
-        if (ok && lane == 0) {
-          const uint64_t d = desc_mn(SWAP ? bt : ct, C);
-#pragma unroll
-          for (int kk = 0; kk < C / 16; ++kk) {
-            mma_ts(tmem + K::X_COL, tmem + K::BT_COL + 8 * kk, desc_add(d, kk * 128), ID_T, 1u);
-            mma_ts(tmem + K::X_COL, tmem + K::BT_COL + 64 + 8 * kk, desc_add(d, kk * 128), ID_T, 1u);
-          }
-          mma_commit(bar + Bz::X_DONE);
-        }
-        __syncwarp();
-      }
-      if (!ok) break;
-      if (lane == 0 && (last || r.nb > 1)) mma_commit(bar + Bz::B_EMPTY + 8 * (cb % K::NB));
-      // O = a X
       if (do_i) {
-        if (t > 0) ok = mbar_wait_warp(bar + Bz::O_READ, (t - 1) & 1);
+        if (t > 0) ok = ok && wait_warp(bar + Bz::O_READ, (t - 1) & 1);
         tc_fence_after();
         if (ok && lane == 0) {
           const uint64_t da = desc_k(at);
-          const uint64_t xh = SWAP ? desc_k(sbase + K::OFF_X) : desc_mn(sbase + K::OFF_X, D);
-#pragma unroll
+          const uint64_t xh = SWAP ? desc_k(xt) : desc_mn(xt, D);
+#pragma unroll 1
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint32_t s = SWAP ? step_k(kk, D) : (uint32_t)(kk * 128);
             mma_ss(tmem + K::O_COL, desc_add(da, step_k(kk, C)), desc_add(xh, s), ID_I, kk > 0);
@@ -357,21 +369,50 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         __syncwarp();
       }
       if (lane == 0 && (last || r.na > 1)) mma_commit(bar + Bz::A_EMPTY + 8 * (ca % K::NA));
-      // O = P c, over what the elementwise warps have taken of a X or of the item before
-      ok = ok && mbar_wait_warp(bar + Bz::P_READY, t & 1);
+      // X += (decayed rows)^T (rows)
+      if (do_b) {
+        ok = ok && wait_warp(bar + Bz::BT_READY, nbt & 1);
+        ++nbt;
+      }
+      // b has been read for the decayed rows, and P = a b^T is the last to read it (SWAP: X is)
+      if (!SWAP && ok && lane == 0 && (last || r.nb > 1)) mma_commit(bar + Bz::B_EMPTY + 8 * (cb % K::NB));
+      if (new_b) {
+        ok = ok && wait_warp(bar + Bz::C_FULL + 8 * (cc % K::NC), (cc / K::NC) & 1);
+        if (ok && cn < C && q.cu) {
+          zero_rows(sgen + K::OFF_C + (cc % K::NC) * K::TILE, K::NCH, cn, lane);
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+      }
+      if (do_b) {
+        tc_fence_after();
+        if (ok && lane == 0) {
+          const uint64_t d = desc_mn(SWAP ? bt : ct, C);
+#pragma unroll 1
+          for (int kk = 0; kk < C / 16; ++kk) {
+            mma_ts(tmem + K::X_COL, tmem + K::BT_COL + 8 * kk, desc_add(d, kk * 128), ID_T, 1u);
+            mma_ts(tmem + K::X_COL, tmem + K::BT_COL + 64 + 8 * kk, desc_add(d, kk * 128), ID_T, 1u);
+          }
+          mma_commit(bar + Bz::X_DONE);
+        }
+        __syncwarp();
+      }
+      if (SWAP && ok && lane == 0 && (last || r.nb > 1)) mma_commit(bar + Bz::B_EMPTY + 8 * (cb % K::NB));
+      // O = P c, over what the output warps have taken of a X or of the item before
+      ok = ok && wait_warp(bar + Bz::P_READY, t & 1);
       if (do_i) {
-        ok = ok && mbar_wait_warp(bar + Bz::OI_READ, noi & 1);
+        ok = ok && wait_warp(bar + Bz::OI_READ, noi & 1);
         ++noi;
       }
       if (!ok) break;
       tc_fence_after();
       if (lane == 0) {
         const uint64_t d = desc_mn(ct, C);
-#pragma unroll
+#pragma unroll 1
         for (int kk = 0; kk < C / 16; ++kk) {
-          const uint32_t p = tmem + K::P_COL + 32 * (kk / 2) + 8 * (kk % 2);
+          const uint32_t p = tmem + K::P_COL + 16 * kk;      // 16 tokens: 8 columns hi, 8 lo
           mma_ts(tmem + K::O_COL, p, desc_add(d, kk * 128), ID_T, kk > 0);
-          mma_ts(tmem + K::O_COL, p + 16, desc_add(d, kk * 128), ID_T, 1u);
+          mma_ts(tmem + K::O_COL, p + 8, desc_add(d, kk * 128), ID_T, 1u);
         }
         mma_commit(bar + Bz::PV_DONE);
         if (last || r.nb > 1) mma_commit(bar + Bz::C_EMPTY + 8 * (cc % K::NC));
@@ -381,234 +422,262 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     if (!ok) record_error(LIN_ERR_WAIT);
     if (lane == 0) mma_commit(bar + Bz::DRAIN);
     __syncwarp();
-    if (!mbar_wait_warp(bar + Bz::DRAIN, 0)) record_error(LIN_ERR_WAIT);
+    if (!wait_warp(bar + Bz::DRAIN, 0)) record_error(LIN_ERR_WAIT);
+    }
+    __syncwarp();
   } else {
-    // ------------------------------------------------------------ elementwise
-    const int qd = warp & 3, hf = warp >> 2, row = qd * 32 + lane;
+    const int qd = warp & 3, hf = (warp >> 2) & 1, row = qd * 32 + lane;
     const uint32_t la = tmem + ((uint32_t)(qd * 32) << 16);
     constexpr int HD = D / 2;                       // state or output columns of a thread
-    const int xl = SWAP ? r.dc : r.da, xn = SWAP ? r.da : r.dc;   // real rows (lanes) and columns of X
-    const long long per = (long long)r.da * r.dc;
-    const float* x0 = nullptr;
-    if (ws) x0 = ws + (((long long)z * q.nhk + h) * q.nseg + n) * per;
-    else if (pool.in && !(pool.seen && pool.seen[z] <= 0)) x0 = pool.in + ((long long)slot * q.nhk + h) * per;
-    float acc[HD];                    // this thread's part of an output row: a X first, then P c of each item
-    float p_inv = 1.f, x_inv = 1.f;
     bool ok = true;                   // false once a wait has given up: the warp goes on without waiting (the named barriers stay matched)
-    int nx = 0, nbt = 0, noi = 0, cbw = -1;
     const auto wait = [&](int which, int phase) {
-      ok = ok && mbar_wait_warp(bar + which, phase & 1);
+      ok = ok && wait_warp(bar + which, phase & 1);
       __syncwarp();
       tc_fence_after();
     };
-    const uint32_t obox = K::OFF_O + warp * 32 * HD * 2;
-    const auto epilogue = [&](int t) {
-      const int at = chunk_at(t), cn = min(C, t1 - t0 - at), g = r.na > 1 ? t % groups : 0;
+    if (warp >= 8) {
+      // ---------------------------------------------------------- state
+      regs_state();
+      const int xl = SWAP ? r.dc : r.da, xn = SWAP ? r.da : r.dc;   // real rows (lanes) and columns of X
+      const float* x0 = nullptr;
+      if (ws) x0 = ws + (((long long)z * q.nhk + h) * q.nseg + n) * r.da * r.dc;
+      else if (pool.in && !(pool.seen && pool.seen[z] <= 0)) x0 = pool.in + ((long long)slot * q.nhk + h) * r.da * r.dc;
+      int nx = 0, nbt = 0, noi = 0, cbw = -1, w_cn = 0;
+      float2 w_rows[8];
+      if (qd * 32 < D) {                // X as it enters the segment
+#pragma unroll 1
+        for (int c0 = hf * HD; c0 < hf * HD + HD; c0 += 16) {
+          float2 x[8];
 #pragma unroll
-      for (int c0 = 0; c0 < HD; c0 += 32) {
-        float o[32];
-        tmem_ld32(la + K::O_COL + hf * HD + c0, o);
-        tc_wait_ld();
-#pragma unroll
-        for (int i = 0; i < 32; ++i) acc[c0 + i] = fmaf(o[i], p_inv, acc[c0 + i]);
-      }
-      tc_fence_before();
-      mbar_arrive(bar + Bz::O_READ);
-      if ((r.na == 1 && t % groups != groups - 1) || hf * HD >= r.dc) return;
-      // 32 whole rows go out as one box; rows next to another sequence's one by one
-      const bool whole = qd * 32 + 32 <= cn;
-      T* orow = out + (long long)(at + row) * r.so.s + g * r.so.h + hf * HD;
-      if (whole) {
-        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-        __syncwarp();
-      }
-#pragma unroll
-      for (int i = 0; i < HD / 8; ++i) {
-        const uint4 w = make_uint4(pack2<BF16>(acc[8 * i], acc[8 * i + 1]), pack2<BF16>(acc[8 * i + 2], acc[8 * i + 3]),
-                                   pack2<BF16>(acc[8 * i + 4], acc[8 * i + 5]), pack2<BF16>(acc[8 * i + 6], acc[8 * i + 7]));
-        if (whole)      // 128-byte or 64-byte swizzle
-          *reinterpret_cast<uint4*>(sgen + obox + lane * HD * 2 + ((i ^ (HD == 64 ? lane & 7 : (lane >> 1) & 3)) << 4)) = w;
-        else if (row < cn && hf * HD + 8 * i < r.dc)
-          *reinterpret_cast<uint4*>(orow + 8 * i) = w;
-      }
-      if (whole) {
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) tma_store_4d(&to, sbase + obox, hf * HD, (int)span.row0 + t0 + at + qd * 32, h * r.na + g, q.cu ? 0 : z);
-      }
-    };
-    float2 w_rows[8];
-    int w_cn = 0;
-    // Factors of the pair products: a block of 32 rows x 32 columns beside the diagonal takes lam^(rows from its near edge) times
-    // lam^(columns from it), both at most 1, so that nothing overflows however fast the decay
-    float u_blk[2];
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const int j0 = hf * 64 + 32 * b;
-      u_blk[b] = lam[REV ? max(j0 - row, 0) : max(row - j0 - 31, 0)];
-    }
-    for (int t = 0; t < items; ++t) {
-      const int g = t % groups;
-      const bool first = g == 0, end = t / groups == chunks - 1;
-      const bool do_b = (first || r.nb > 1) && !end, do_i = first || r.na > 1;
-      const int cn = min(C, t1 - t0 - chunk_at(t));
-      // ---- decayed rows, transposed
-      if (first || r.nb > 1) ++cbw;
-      if (do_b) {
-        if (cn != w_cn) {
-          row_factors<REV>(w_rows, lam, r.w_up, hf, lane, cn);
-          w_cn = cn;
+          for (int i = 0; i < 16; ++i) {
+            const int col = c0 + i, ii = SWAP ? col : row, jj = SWAP ? row : col;
+            reinterpret_cast<float*>(x)[i] =
+                x0 && row < xl && col < xn ? x0[r.transposed ? (long long)jj * r.da + ii : (long long)ii * r.dc + jj] : 0.f;
+          }
+          tmem_store<16>(la + K::X_COL + c0, x);
         }
-        const int stages = SWAP ? K::NC : K::NB, s = cbw % stages;
-        wait((SWAP ? Bz::C_FULL : Bz::B_FULL) + 8 * s, cbw / stages);
-        if (nbt > 0) wait(Bz::X_DONE, nbt - 1);
-        if (qd * 32 < D)
-          decay_rows<BF16, 2>(sbase + (SWAP ? K::OFF_C : K::OFF_B) + s * K::TILE, la + K::BT_COL, w_rows, qd, hf, lane, cn);
         tc_wait_st();
-        tc_fence_before();
-        mbar_arrive(bar + Bz::BT_READY);
-        ++nbt;
       }
-      // ---- epilogue of the item before
-      if (t > 0) {
-        wait(Bz::PV_DONE, t - 1);
-        epilogue(t - 1);
+      for (int t = 0, ck = 0, g = 0; t < items; ++t, ++g == groups ? g = 0, ++ck : 0) {
+        const bool first = g == 0, end = ck == chunks - 1;
+        const bool do_b = (first || r.nb > 1) && !end;
+        const int cn = min(C, t1 - t0 - chunk_at(ck));
+        // the last a X, which reads X in shared memory, and the last update of X, which reads the decayed rows
+        if (t > 0 && (r.na > 1 || groups == 1 || g == 1)) {
+          wait(Bz::OI_FULL, noi);
+          ++noi;
+        }
+        if (nbt > 0 && (first || do_b)) wait(Bz::X_DONE, nbt - 1);
+        // X: hi + lo to shared memory, lam^C X back to TMEM
+        if (first) {
+          float xs = 1.f;
+          if constexpr (!BF16) {
+            float top = 0.f;
+            if (qd * 32 < D) {
+#pragma unroll 1
+              for (int c0 = 0; c0 < HD; c0 += 32) {
+                float2 x[16];
+                tmem_load<32>(la + K::X_COL + hf * HD + c0, x);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, fmaxf(fabsf(x[i].x), fabsf(x[i].y)));
+              }
+            }
+            const uint32_t all = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+            if (lane == 0) atomicMax(&xmax[nx], all);
+            bar_state();
+            xs = scale_to(xmax[nx]);
+            nx = nx == 2 ? 0 : nx + 1;
+            if (tid == 256) xmax[nx] = 0;     // three slots: the output warps may still read the one before
+          }
+          const float keep = lam[cn];
+          if (qd * 32 < D) {
+#pragma unroll 1
+            for (int col = hf * HD; col < hf * HD + HD; col += 16) {
+              float2 x[8];
+              tmem_load<16>(la + K::X_COL + col, x);
+              uint32_t hi[8], lo[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                split2<BF16>(BF16 ? x[i] : __fmul2_rn(x[i], make_float2(xs, xs)), hi[i], lo[i]);
+                x[i] = __fmul2_rn(x[i], make_float2(keep, keep));
+              }
+              tmem_store<16>(la + K::X_COL + col, x);
+              uint8_t* xr = sgen + K::OFF_X + (col / 64) * D * 128 + row * 128;
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                uint8_t* to_x = xr + ((((col % 64) / 8 + i) ^ (row & 7)) << 4);
+                *reinterpret_cast<uint4*>(to_x) = make_uint4(hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
+                *reinterpret_cast<uint4*>(to_x + K::XT) = make_uint4(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
+              }
+            }
+          }
+          tc_wait_st();
+          fence_proxy_async_smem();
+          tc_fence_before();
+          mbar_arrive(bar + Bz::XS_READY);
+        }
+        // decayed rows, transposed
+        if (first || r.nb > 1) ++cbw;
+        if (do_b) {
+          if (cn != w_cn) {
+            row_factors<REV, 4>(w_rows, lam, r.w_up, 64 * hf, lane, cn);
+            w_cn = cn;
+          }
+          const int stages = SWAP ? K::NC : K::NB, s = cbw % stages;
+          wait((SWAP ? Bz::C_FULL : Bz::B_FULL) + 8 * s, cbw / stages);
+          if (qd * 32 < D)
+            decay_rows<BF16, 2, 4>(sbase + (SWAP ? K::OFF_C : K::OFF_B) + s * K::TILE, la + K::BT_COL, w_rows, qd, 64 * hf, lane, cn);
+          tc_wait_st();
+          tc_fence_before();
+          mbar_arrive(bar + Bz::BT_READY);
+          ++nbt;
+        }
       }
-      // ---- the state: hi + lo to shared memory, lam^C X back to TMEM
-      if (first) {
-        float x[HD];
+    } else {
+      // ---------------------------------------------------------- outputs
+      regs_out();
+      float2 acc[HD / 2];               // this thread's part of an output row: a X first, then P c of each item
+      float p_inv = 1.f, x_inv = 1.f;
+      int nx = 0, noi = 0, at = 0, cn = 0, head = 0;
+      bool write = false;
+      const uint32_t obox = K::OFF_O + warp * 32 * HD * 2;
+      for (int t = 0, ck = 0, g = 0;; ++t, ++g == groups ? g = 0, ++ck : 0) {
         if (t > 0) {
-          wait(Bz::X_DONE, nbt - 1 - (do_b ? 1 : 0));      // every update before this chunk's has landed
-          if (qd * 32 < D) {
+          // epilogue of the item before
+          wait(Bz::PV_DONE, t - 1);
 #pragma unroll
-            for (int c0 = 0; c0 < HD; c0 += 32) tmem_ld32(la + K::X_COL + hf * HD + c0, x + c0);
-            tc_wait_ld();
+          for (int c0 = 0; c0 < HD; c0 += 32) {
+            float2 o[16];
+            tmem_load<32>(la + K::O_COL + hf * HD + c0, o);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[c0 / 2 + i] = __ffma2_rn(o[i], make_float2(p_inv, p_inv), acc[c0 / 2 + i]);
           }
-        } else {
+          tc_fence_before();
+          mbar_arrive(bar + Bz::O_READ);
+          if (write && hf * HD < r.dc) {
+            // 32 whole rows go out as one box; rows next to another sequence's one by one
+            const bool whole = qd * 32 + 32 <= cn;
+            uint8_t* to_row = sgen + obox + lane * HD * 2;
+            int swizzle = HD == 64 ? lane & 7 : (lane >> 1) & 3, units = HD / 8;      // 128-byte or 64-byte swizzle
+            if (whole) {
+              if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+              __syncwarp();
+            } else {
+              to_row = reinterpret_cast<uint8_t*>(out + (long long)(at + row) * r.so.s + head * r.so.h + hf * HD);
+              swizzle = 0;
+              units = row < cn ? min(units, (r.dc - hf * HD) / 8) : 0;
+            }
 #pragma unroll
-          for (int i = 0; i < HD; ++i) {
-            const int col = hf * HD + i;
-            const int ii = SWAP ? col : row, jj = SWAP ? row : col;
-            x[i] = x0 && row < xl && col < xn ? x0[r.transposed ? (long long)jj * r.da + ii : (long long)ii * r.dc + jj] : 0.f;
+            for (int i = 0; i < HD / 8; ++i)
+              if (i < units)
+                *reinterpret_cast<uint4*>(to_row + ((i ^ swizzle) << 4)) =
+                    make_uint4(pack2<BF16>(acc[4 * i].x, acc[4 * i].y), pack2<BF16>(acc[4 * i + 1].x, acc[4 * i + 1].y),
+                               pack2<BF16>(acc[4 * i + 2].x, acc[4 * i + 2].y), pack2<BF16>(acc[4 * i + 3].x, acc[4 * i + 3].y));
+            if (whole) {
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) tma_store_4d(&to, sbase + obox, hf * HD, (int)span.row0 + t0 + at + qd * 32, h * r.na + head, q.cu ? 0 : z);
+            }
           }
         }
-        float xs = 1.f;
-        if constexpr (!BF16) {
-          float top = 0.f;
-          if (qd * 32 < D) {
+        if (t == items) break;
+        const bool first = g == 0, do_i = first || r.na > 1;
+        at = chunk_at(ck);
+        cn = min(C, t1 - t0 - at);
+        head = r.na > 1 ? g : 0;
+        write = r.na > 1 || g == groups - 1;
+        // Pair products: decay, mask, back to TMEM as hi + lo, in pieces of 16 columns.  A piece beside the diagonal block of 32 x 32 takes
+        // lam^(rows from its block's near edge) times lam^(columns from it), both at most 1, so that nothing overflows however
+        // fast the decay
+        wait(Bz::P_FULL, t);
+        {
+          const auto load = [&](int piece, float2* p) {      // false: all 0, not loaded
+            const int j0 = hf * 64 + 32 * (piece >> 1), c0 = 16 * (piece & 1), side = REV ? j0 / 32 - qd : qd - j0 / 32;
+            if (side < 0) return false;
+            tmem_load<16>(la + K::P_COL + j0 + c0, p);
+            if (side > 0) {
+              const float4* w = reinterpret_cast<const float4*>(lamc + c0);
+              const float blk = lam[REV ? j0 - row : row - j0 - 31];
+              const float2 u = make_float2(blk, blk);
 #pragma unroll
-            for (int i = 0; i < HD; ++i) top = fmaxf(top, fabsf(x[i]));
+              for (int i = 0; i < 4; ++i) {
+                const float4 f = w[i];
+                p[2 * i] = __fmul2_rn(p[2 * i], __fmul2_rn(u, make_float2(f.x, f.y)));
+                p[2 * i + 1] = __fmul2_rn(p[2 * i + 1], __fmul2_rn(u, make_float2(f.z, f.w)));
+              }
+            } else {
+              const float* w = lam + (REV ? c0 - lane : lane - c0);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int gap = REV ? c0 + 2 * i - lane : lane - c0 - 2 * i, next = REV ? gap + 1 : gap - 1;
+                p[i].x = gap >= 0 ? p[i].x * w[REV ? 2 * i : -2 * i] : 0.f;
+                p[i].y = next >= 0 ? p[i].y * w[REV ? 2 * i + 1 : -2 * i - 1] : 0.f;
+              }
+            }
+            if (REV && cn < C) {                  // forward, a row sees no token past its own
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                if (j0 + c0 + 2 * i >= cn) p[i].x = 0.f;
+                if (j0 + c0 + 2 * i + 1 >= cn) p[i].y = 0.f;
+              }
+            }
+            return true;
+          };
+          float ps = 1.f;
+          if constexpr (!BF16) {
+            float top = 0.f;
+#pragma unroll 1
+            for (int piece = 0; piece < 4; ++piece) {
+              float2 p[8];
+              if (!load(piece, p)) continue;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) top = fmaxf(top, fmaxf(fabsf(p[i].x), fabsf(p[i].y)));
+            }
+            uint32_t* most = pmax + row;
+            most[hf * C] = __float_as_uint(top);      // the item before was read before its P c, which this P waited for
+            bar_quadrant(qd);
+            ps = scale_to(max(most[0], most[C]));
           }
-          const uint32_t all = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
-          if (lane == 0) atomicMax(&xmax[nx & 1], all);
-          bar_elem();
-          xs = scale_to(xmax[nx & 1]);
-          if (tid == 0) xmax[(nx + 1) & 1] = 0;
-          x_inv = 1.f / xs;
-        }
-        const float keep = lam[cn];
-        if (qd * 32 < D) {
-          uint8_t* xr = sgen + K::OFF_X + row * 128;
+#pragma unroll 1
+          for (int piece = 0; piece < 4; ++piece) {
+            float2 p[8];
+            uint32_t w[16];
+            if (load(piece, p)) {
 #pragma unroll
-          for (int i = 0; i < HD / 8; ++i) {
-            uint32_t hi[4], lo[4];
+              for (int i = 0; i < 8; ++i) split2<BF16>(BF16 ? p[i] : __fmul2_rn(p[i], make_float2(ps, ps)), w[i], w[8 + i]);
+            } else {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) split2<BF16>(__fmul2_rn(make_float2(x[8 * i + 2 * k], x[8 * i + 2 * k + 1]), make_float2(xs, xs)), hi[k], lo[k]);
-            const int col = hf * HD + 8 * i;
-            uint8_t* to_x = xr + (col / 64) * D * 128 + ((((col % 64) / 8) ^ (row & 7)) << 4);
-            *reinterpret_cast<uint4*>(to_x) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            *reinterpret_cast<uint4*>(to_x + K::XT) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+              for (int i = 0; i < 16; ++i) w[i] = 0;
+            }
+            tmem_st16(la + K::P_COL + hf * 64 + 16 * piece, w);
           }
-#pragma unroll
-          for (int i = 0; i < HD; ++i) x[i] *= keep;
-#pragma unroll
-          for (int c0 = 0; c0 < HD; c0 += 32) tmem_st32(la + K::X_COL + hf * HD + c0, reinterpret_cast<const uint32_t*>(x + c0));
+          p_inv = r.w_intra / ps;
         }
         tc_wait_st();
-        fence_proxy_async_smem();
         tc_fence_before();
-        mbar_arrive(bar + Bz::XS_READY);
-        ++nx;
-      }
-      // ---- pair products: decay, mask, back to TMEM as hi + lo
-      wait(Bz::P_FULL, t);
-      {
-        float2 p[2][16];
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const int j0 = hf * 64 + 32 * b, side = REV ? j0 / 32 - qd : qd - j0 / 32;      // 0 on the diagonal, below 0 where nothing is seen
-          if (side < 0) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) p[b][i] = make_float2(0.f, 0.f);
-            continue;
-          }
-          tmem_ld32(la + K::P_COL + j0, reinterpret_cast<float*>(p[b]));
-          tc_wait_ld();
-          if (side > 0) {
-            const float2 u = make_float2(u_blk[b], u_blk[b]);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {      // columns from the near edge: lam^(31 - j), or lam^j reversed
-              const float2 w = REV ? make_float2(lam[2 * i], lam[2 * i + 1]) : make_float2(lam[31 - 2 * i], lam[30 - 2 * i]);
-              p[b][i] = __fmul2_rn(p[b][i], __fmul2_rn(u, w));
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int gap = REV ? 2 * i - lane : lane - 2 * i, next = REV ? gap + 1 : gap - 1;
-              p[b][i].x = gap >= 0 ? p[b][i].x * lam[max(gap, 0)] : 0.f;
-              p[b][i].y = next >= 0 ? p[b][i].y * lam[max(next, 0)] : 0.f;
+        mbar_arrive(bar + Bz::P_READY);
+        // a X
+        if (do_i) {
+          wait(Bz::OI_FULL, noi);
+          ++noi;
+          if constexpr (!BF16) {
+            if (first) {
+              x_inv = 1.f / scale_to(xmax[nx]);
+              nx = nx == 2 ? 0 : nx + 1;
             }
           }
-          if (REV && cn < C) {                  // forward, a row sees no token past its own
+          const float mul = r.w_inter * lam[REV ? max(cn - 1 - row, 0) : min(row + 1, C)] * x_inv;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              if (j0 + 2 * i >= cn) p[b][i].x = 0.f;
-              if (j0 + 2 * i + 1 >= cn) p[b][i].y = 0.f;
-            }
-          }
+          for (int c0 = 0; c0 < HD; c0 += 32) tmem_load<32>(la + K::O_COL + hf * HD + c0, acc + c0 / 2);
+          tc_fence_before();
+          mbar_arrive(bar + Bz::OI_READ);
+#pragma unroll
+          for (int i = 0; i < HD / 2; ++i) acc[i] = __fmul2_rn(acc[i], make_float2(mul, mul));
         }
-        float ps = 1.f;
-        if constexpr (!BF16) {
-          float top = 0.f;
-#pragma unroll
-          for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) top = fmaxf(top, fmaxf(fabsf(p[b][i].x), fabsf(p[b][i].y)));
-          pmax[hf * C + row] = __float_as_uint(top);
-          bar_pair(qd);
-          ps = scale_to(max(__float_as_uint(top), pmax[(hf ^ 1) * C + row]));
-          bar_pair(qd);
-        }
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          uint32_t w[32];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) split2<BF16>(BF16 ? p[b][i] : __fmul2_rn(p[b][i], make_float2(ps, ps)), w[i], w[16 + i]);
-          tmem_st32(la + K::P_COL + hf * 64 + 32 * b, w);
-        }
-        p_inv = r.w_intra / ps;
       }
-      tc_wait_st();
-      tc_fence_before();
-      mbar_arrive(bar + Bz::P_READY);
-      // ---- a X
-      if (do_i) {
-        wait(Bz::OI_FULL, noi);
-        ++noi;
-        const float mul = r.w_inter * lam[REV ? max(cn - 1 - row, 0) : min(row + 1, C)] * x_inv;
-#pragma unroll
-        for (int c0 = 0; c0 < HD; c0 += 32) tmem_ld32(la + K::O_COL + hf * HD + c0, acc + c0);
-        tc_wait_ld();
-        tc_fence_before();
-        mbar_arrive(bar + Bz::OI_READ);
-#pragma unroll
-        for (int i = 0; i < HD; ++i) acc[i] *= mul;
-      }
+      if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+      __syncwarp();
     }
-    wait(Bz::PV_DONE, items - 1);
-    epilogue(items - 1);
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-    __syncwarp();
     if (!ok) record_error(LIN_ERR_WAIT);
   }
   tc_fence_before();
@@ -639,7 +708,7 @@ struct StBz {
 };
 
 template <int D, bool BF16, bool REV>
-__global__ void __launch_bounds__(NTHREADS, 1)
+__global__ void __launch_bounds__(NTHREADS_ST, 1)
     lin_tc_states_kernel(const __grid_constant__ CUtensorMap tb, const __grid_constant__ CUtensorMap tc, const LinSeqs q, const LinRole r,
                          float* ws) {
   using K = StCfg<D, BF16>;
@@ -662,9 +731,9 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       mbar_init(bar + StBz::FULL + 8 * s, 1);
       mbar_init(bar + StBz::EMPTY + 8 * s, 1);
     }
-    for (int s = 0; s < 2; ++s) mbar_init(bar + StBz::BT_READY + 8 * s, NELEM);
+    for (int s = 0; s < 2; ++s) mbar_init(bar + StBz::BT_READY + 8 * s, NELEM_ST);
     mbar_init(bar + StBz::DONE, 1);
-    mbar_init(bar + StBz::X_READ, NELEM);
+    mbar_init(bar + StBz::X_READ, NELEM_ST);
     mbar_init(bar + StBz::DRAIN, 1);
     fence_barrier_init();
   }
@@ -728,28 +797,25 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     __syncwarp();
     if (!mbar_wait_warp(bar + StBz::DRAIN, 0)) record_error(LIN_ERR_WAIT);
   } else {
-    const int qd = warp & 3, hf = warp >> 2, row = qd * 32 + lane;
+    const int qd = warp & 3, qr = warp >> 2, row = qd * 32 + lane;
     const uint32_t la = tmem + ((uint32_t)(qd * 32) << 16);
+    constexpr int HD = D / 4;
     bool ok = true;
-    float acc[D / 2];
+    float2 acc[HD / 2];
 #pragma unroll
-    for (int i = 0; i < D / 2; ++i) acc[i] = 0.f;
+    for (int i = 0; i < HD / 2; ++i) acc[i] = make_float2(0.f, 0.f);
     const auto add = [&](int i) {      // item i's sum
       ok = ok && mbar_wait_warp(bar + StBz::DONE, i & 1);
       __syncwarp();
       tc_fence_after();
-#pragma unroll
-      for (int c0 = 0; c0 < D / 2; c0 += 32) {
-        float v[32];
-        tmem_ld32(la + K::X_COL + hf * (D / 2) + c0, v);
-        tc_wait_ld();
-#pragma unroll
-        for (int k = 0; k < 32; ++k) acc[c0 + k] += v[k];
-      }
+      float2 v[HD / 2];
+      tmem_load<HD>(la + K::X_COL + qr * HD, v);
       tc_fence_before();
       mbar_arrive(bar + StBz::X_READ);
+#pragma unroll
+      for (int k = 0; k < HD / 2; ++k) acc[k] = __fadd2_rn(acc[k], v[k]);
     };
-    float2 w_rows[8];
+    float2 w_rows[4];
     int w_cn = 0;
     for (int i = 0; i < items; ++i) {
       // the buffer of decayed rows is free: item i - 2 was added up
@@ -757,14 +823,14 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       ok = ok && mbar_wait_warp(bar + StBz::FULL + 8 * (i % K::NS), (i / K::NS) & 1);
       __syncwarp();
       if (cn != w_cn) {
-        row_factors<REV>(w_rows, lam, 1.f, hf, lane, cn);
+        row_factors<REV, 2>(w_rows, lam, 1.f, 32 * qr, lane, cn);
         w_cn = cn;
       }
       const float far = lin_power(g2, REV ? at : t1 - t0 - at - cn);
-      float2 w[8];
+      float2 w[4];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) w[k] = __fmul2_rn(w_rows[k], make_float2(far, far));
-      if (qd * 32 < D) decay_rows<BF16, K::TERMS>(sbase + tile(i), la + K::BT_COL + (i & 1) * K::BT_COLS, w, qd, hf, lane, cn);
+      for (int k = 0; k < 4; ++k) w[k] = __fmul2_rn(w_rows[k], make_float2(far, far));
+      if (qd * 32 < D) decay_rows<BF16, K::TERMS, 2>(sbase + tile(i), la + K::BT_COL + (i & 1) * K::BT_COLS, w, qd, 32 * qr, lane, cn);
       tc_wait_st();
       tc_fence_before();
       mbar_arrive(bar + StBz::BT_READY + 8 * (i & 1));
@@ -773,10 +839,10 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     add(items - 1);
     float* x = ws + (((long long)z * q.nhk + h) * q.nseg + n) * r.da * r.dc + (long long)row * r.dc;
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i) {
-      const int col = hf * (D / 2) + 4 * i;
+    for (int i = 0; i < HD / 4; ++i) {
+      const int col = qr * HD + 4 * i;
       if (row < r.da && col < r.dc)
-        *reinterpret_cast<float4*>(x + col) = make_float4(r.w_up * acc[4 * i], r.w_up * acc[4 * i + 1], r.w_up * acc[4 * i + 2], r.w_up * acc[4 * i + 3]);
+        *reinterpret_cast<float4*>(x + col) = make_float4(r.w_up * acc[2 * i].x, r.w_up * acc[2 * i].y, r.w_up * acc[2 * i + 1].x, r.w_up * acc[2 * i + 1].y);
     }
     if (!ok) record_error(LIN_ERR_WAIT);
   }
@@ -800,7 +866,7 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
-// boxes of `cols` columns (64, or 32) x `box_rows` rows over [batch][heads][rows][dim]; false where the layout does not allow it
+// boxes of `cols` columns (64 or 32) x `box_rows` rows over [batch][heads][rows][dim]; false where the layout does not allow it
 bool map4(CUtensorMap* m, const void* base, bool bf16, int dim, long long rows, long long heads, long long batch, const FaStrides& st,
           int cols = 64, int box_rows = C) {
   const auto enc = encode_fn();
@@ -821,30 +887,44 @@ bool takes(const LinSeqs& q, const LinRole& r, int dtype) {
   return dtype != FA_DTYPE_F32 && r.da <= 128 && r.dc <= 128 && (q.cu ? q.total > 0 : q.S > 0) && q.total < (1ll << 31) - 256;
 }
 
+// The register split of lin_tc_kernel waits for good unless the block starts with REGS a thread: looked up once for each kernel.
+template <typename Kernel>
+bool regs_fit(Kernel kernel) {
+  cudaFuncAttributes a;
+  return cudaFuncGetAttributes(&a, (const void*)kernel) == cudaSuccess && a.numRegs == REGS;
+}
+
 template <typename Kernel, typename... Args>
-int launch(Kernel kernel, int smem, unsigned long long* done, const LinSeqs& q, cudaStream_t st, const Args&... args) {
+int launch(Kernel kernel, int threads, int smem, unsigned long long* done, const LinSeqs& q, cudaStream_t st, const Args&... args) {
   const long long grid = (long long)q.batch * q.nhk * q.nseg;
   FA_CHECK_ARG(grid < (1ll << 31), "linear attention: %lld blocks", grid);
   if (int rc = ensure_smem((const void*)kernel, smem, done)) return rc;
-  kernel<<<(int)grid, NTHREADS, smem, st>>>(args...);
+  kernel<<<(int)grid, threads, smem, st>>>(args...);
   count_launch();
   return cuda_status(cudaGetLastError(), "linear attention (tensor cores) launch");
 }
 
+template <int D, bool BF16, bool REV, bool SWAP>
+int run_one(const LinSeqs& q, const LinRole& r, const float* ws, const LinPool& pool, cudaStream_t st, const CUtensorMap* m, bool* taken) {
+  static unsigned long long done = 0;
+  static const bool fits = regs_fit(lin_tc_kernel<D, BF16, REV, SWAP>);
+  if (!fits) return FA_OK;
+  *taken = true;
+  return launch(lin_tc_kernel<D, BF16, REV, SWAP>, NTHREADS, Cfg<D>::SMEM, &done, q, st, m[0], m[1], m[2], m[3], q, r, ws, pool);
+}
 template <int D, bool BF16>
-int run_main(const LinSeqs& q, const LinRole& r, bool rev, const float* ws, const LinPool& pool, cudaStream_t st, const CUtensorMap* m) {
-  static unsigned long long done[3] = {};
+int run_main(const LinSeqs& q, const LinRole& r, bool rev, const float* ws, const LinPool& pool, cudaStream_t st, const CUtensorMap* m, bool* taken) {
   // dk: the output is along the state's rows as it is stored
-  if (rev && r.transposed) return launch(lin_tc_kernel<D, BF16, true, true>, Cfg<D>::SMEM, done, q, st, m[0], m[1], m[2], m[3], q, r, ws, pool);
-  if (rev) return launch(lin_tc_kernel<D, BF16, true, false>, Cfg<D>::SMEM, done + 1, q, st, m[0], m[1], m[2], m[3], q, r, ws, pool);
-  return launch(lin_tc_kernel<D, BF16, false, false>, Cfg<D>::SMEM, done + 2, q, st, m[0], m[1], m[2], m[3], q, r, ws, pool);
+  if (rev && r.transposed) return run_one<D, BF16, true, true>(q, r, ws, pool, st, m, taken);
+  if (rev) return run_one<D, BF16, true, false>(q, r, ws, pool, st, m, taken);
+  return run_one<D, BF16, false, false>(q, r, ws, pool, st, m, taken);
 }
 template <int D, bool BF16>
 int run_states(const LinSeqs& q, const LinRole& r, bool rev, float* ws, cudaStream_t st, const CUtensorMap* m) {
   static unsigned long long done[2] = {};
   using K = StCfg<D, BF16>;
-  if (rev) return launch(lin_tc_states_kernel<D, BF16, true>, K::SMEM, done, q, st, m[0], m[1], q, r, ws);
-  return launch(lin_tc_states_kernel<D, BF16, false>, K::SMEM, done + 1, q, st, m[0], m[1], q, r, ws);
+  if (rev) return launch(lin_tc_states_kernel<D, BF16, true>, NTHREADS_ST, K::SMEM, done, q, st, m[0], m[1], q, r, ws);
+  return launch(lin_tc_states_kernel<D, BF16, false>, NTHREADS_ST, K::SMEM, done + 1, q, st, m[0], m[1], q, r, ws);
 }
 }  // namespace
 
@@ -862,9 +942,8 @@ int lin_tc_main(const LinSeqs& q, const LinRole& r, bool rev, const float* ws, c
       !map4(m + 2, r.c, bf16, r.dc, rows, (long long)q.nhk * r.nb, zs, r.sc) ||
       !map4(m + 3, r.out, bf16, r.dc, rows, (long long)q.nhk * r.na, zs, r.so, small ? 32 : 64, 32))
     return FA_OK;
-  *taken = true;
-  if (bf16) return small ? run_main<64, true>(q, r, rev, ws, pool, st, m) : run_main<128, true>(q, r, rev, ws, pool, st, m);
-  return small ? run_main<64, false>(q, r, rev, ws, pool, st, m) : run_main<128, false>(q, r, rev, ws, pool, st, m);
+  if (bf16) return small ? run_main<64, true>(q, r, rev, ws, pool, st, m, taken) : run_main<128, true>(q, r, rev, ws, pool, st, m, taken);
+  return small ? run_main<64, false>(q, r, rev, ws, pool, st, m, taken) : run_main<128, false>(q, r, rev, ws, pool, st, m, taken);
 }
 
 int lin_tc_states(const LinSeqs& q, const LinRole& r, bool rev, float* ws, int dtype, cudaStream_t st, bool* taken) {
