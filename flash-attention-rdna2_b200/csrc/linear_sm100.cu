@@ -18,7 +18,8 @@
 // Warp roles (640 threads, five warpgroups):
 //   0-7    outputs: pair products on their way back to TMEM, a X, epilogue; two warps to a TMEM lane quadrant (w % 4), half of the columns each
 //   8-15   state: decayed rows, X to shared memory and lam^C X back to TMEM; two warps to a quadrant likewise
-//   16, 17 TMA, MMA
+//   16     TMA
+//   17, 18 MMAs: P = a b^T and O = P c, O = a X and X += ..; one thread alone issues an MMA in 85 to 110 cycles and the pipe takes 64
 // What a chunk needs is a chain of short steps, each a TMEM or shared memory latency long, and not their instructions: one
 // set of warps that took all steps in turn needed 10000 cycles a chunk, issuing every third cycle.  Outputs of item t and the state
 // of the next chunk depend on each other through the MMAs alone, so two sets run them side by side, each waiting for an MMA
@@ -34,7 +35,7 @@ using namespace sm100;
 using namespace fa;
 
 constexpr int C = 128;               // tokens of a chunk
-constexpr int NTHREADS = 640, NOUT = 256, NSTATE = 256, WARP_TMA = 16, WARP_MMA = 17;
+constexpr int NTHREADS = 640, NOUT = 256, NSTATE = 256, WARP_TMA = 16, WARP_MMA = 17, WARP_MMA2 = 18;
 // registers a thread: launched with REGS; 2 x 136 + 2 x 80 + 48 = 5 x 96
 constexpr int REGS = 96;
 __device__ __forceinline__ void regs_out() { asm volatile("setmaxnreg.inc.sync.aligned.u32 136;"); }
@@ -198,7 +199,7 @@ struct Cfg {
 struct Bz {
   static constexpr int A_FULL = 0, A_EMPTY = 16, B_FULL = 32, B_EMPTY = 48, C_FULL = 64, C_EMPTY = 80, P_FULL = 96, P_READY = 104,
                        PV_DONE = 112, XS_READY = 120, BT_READY = 128, X_DONE = 136, OI_FULL = 144, OI_READ = 152, O_READ = 160,
-                       DRAIN = 168, TMEM_ADDR = 176;
+                       DRAIN = 168, TMEM_ADDR = 184;
 };
 
 template <int D, bool BF16, bool REV, bool SWAP>
@@ -237,11 +238,12 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   if (tid == 0) {
     for (int s = 0; s < 2; ++s) {
       mbar_init(bar + Bz::A_FULL + 8 * s, 1);
-      mbar_init(bar + Bz::A_EMPTY + 8 * s, 1);
+      mbar_init(bar + Bz::A_EMPTY + 8 * s, 2);      // both MMA warps
       mbar_init(bar + Bz::B_FULL + 8 * s, 1);
-      mbar_init(bar + Bz::B_EMPTY + 8 * s, 1);
+      mbar_init(bar + Bz::B_EMPTY + 8 * s, 2);
       mbar_init(bar + Bz::C_FULL + 8 * s, 1);
-      mbar_init(bar + Bz::C_EMPTY + 8 * s, 1);
+      mbar_init(bar + Bz::C_EMPTY + 8 * s, 2);
+      mbar_init(bar + Bz::DRAIN + 8 * s, 1);
     }
     mbar_init(bar + Bz::P_FULL, 1);
     mbar_init(bar + Bz::P_READY, NOUT);
@@ -252,7 +254,6 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     mbar_init(bar + Bz::OI_FULL, 1);
     mbar_init(bar + Bz::OI_READ, NOUT);
     mbar_init(bar + Bz::O_READ, NOUT);
-    mbar_init(bar + Bz::DRAIN, 1);
     xmax[0] = xmax[1] = xmax[2] = 0;
     fence_barrier_init();
   }
@@ -278,7 +279,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       const int z4 = q.cu ? 0 : z;
       for (int ck = 0, g = 0; ok && ck < chunks; ++g == groups ? g = 0, ++ck : 0) {
         const int row = (int)span.row0 + t0 + chunk_at(ck);
-        // c has two buffers and b is free first; a waits for a X, the last to read it
+        // c has two buffers; b is free once P and the decayed rows are formed, a waits for a X
         if (g == 0 || r.nb > 1) {
           const int hh = h * r.nb + (r.nb > 1 ? g : 0), s = nc % K::NC, s2 = nb % K::NB;
           if (nc >= K::NC && !mbar_wait(bar + Bz::C_EMPTY + 8 * s, ((nc / K::NC) - 1) & 1)) { ok = false; break; }
@@ -307,122 +308,144 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       for (int i = max(0, nb - K::NB); i < nb; ++i) mbar_wait(bar + Bz::B_FULL + 8 * (i % K::NB), (i / K::NB) & 1);
       for (int i = max(0, nc - K::NC); i < nc; ++i) mbar_wait(bar + Bz::C_FULL + 8 * (i % K::NC), (i / K::NC) & 1);
     }
-    if (warp == WARP_MMA) {
     constexpr uint32_t ID_P = idesc_f16(BF16 ? 1 : 0, C, C, 0, 0);
     constexpr uint32_t ID_T = idesc_f16(BF16 ? 1 : 0, C, D, 0, 1);                       // B along its rows
     constexpr uint32_t ID_I = idesc_f16(BF16 ? 1 : 0, C, D, 0, SWAP ? 0 : 1);            // O = a X: X [da][dc], or (SWAP) [dc][da]
-    int ca = -1, cb = -1, cc = -1, nx = 0, nbt = 0, noi = 0;    // tiles taken, and steps signalled so far
+    const uint32_t st = sbase;
     bool ok = true;
-    for (int t = 0, ck = 0, g = 0; ok && t < items; ++t, ++g == groups ? g = 0, ++ck : 0) {
-      const bool first = g == 0, last = g == groups - 1, end = ck == chunks - 1;
-      const bool new_b = first || r.nb > 1, do_b = new_b && !end, do_i = first || r.na > 1;
-      const int cn = min(C, t1 - t0 - chunk_at(ck));
-      // P = a b^T
-      if (new_b) {
-        ++cb;
-        ++cc;
-        ok = ok && wait_warp(bar + Bz::B_FULL + 8 * (cb % K::NB), (cb / K::NB) & 1);
-        if (SWAP && ok && cn < C && q.cu) {
-          zero_rows(sgen + K::OFF_B + (cb % K::NB) * K::TILE, K::NCH, cn, lane);
-          fence_proxy_async_smem();
-          __syncwarp();
-        }
-      }
-      if (do_i) {
-        ++ca;
-        ok = ok && wait_warp(bar + Bz::A_FULL + 8 * (ca % K::NA), (ca / K::NA) & 1);
-      }
-      if (t > 0) ok = ok && wait_warp(bar + Bz::PV_DONE, (t - 1) & 1);
-      if (!ok) break;
-      uint32_t at = sbase + K::OFF_A + (ca % K::NA) * K::TILE, bt = sbase + K::OFF_B + (cb % K::NB) * K::TILE,
-               ct = sbase + K::OFF_C + (cc % K::NC) * K::TILE, xt = sbase + K::OFF_X;
-      // opaque: the steps' descriptors are formed where they are used; kept from item to item they would fill the registers
-      asm volatile("" : "+r"(at), "+r"(bt), "+r"(ct), "+r"(xt));
-      tc_fence_after();
-      if (lane == 0) {
-        const uint64_t da = desc_k(at), db = desc_k(bt);
+    if (warp == WARP_MMA) {
+      // ------------------------------------------------------------ P = a b^T, O = P c
+      int ca = -1, cb = -1, noi = 0;
+      for (int t = 0, ck = 0, g = 0; ok && t < items; ++t, ++g == groups ? g = 0, ++ck : 0) {
+        const bool first = g == 0, last = g == groups - 1, new_b = first || r.nb > 1, do_i = first || r.na > 1;
+        const int cn = min(C, t1 - t0 - chunk_at(ck));
+        cb += new_b ? 1 : 0;
+        ca += do_i ? 1 : 0;
+        const uint32_t at = st + K::OFF_A + (ca % K::NA) * K::TILE, bt = st + K::OFF_B + (cb % K::NB) * K::TILE,
+                       ct = st + K::OFF_C + (cb % K::NC) * K::TILE;
+        if (new_b) ok = wait_warp(bar + Bz::B_FULL + 8 * (cb % K::NB), (cb / K::NB) & 1);
+        if (do_i) ok = ok && wait_warp(bar + Bz::A_FULL + 8 * (ca % K::NA), (ca / K::NA) & 1);
+        if (t > 0) ok = ok && wait_warp(bar + Bz::PV_DONE, (t - 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (lane == 0) {
+          const uint64_t da = desc_k(at), db = desc_k(bt);
 #pragma unroll 1
-        for (int kk = 0; kk < D / 16; ++kk)
-          mma_ss(tmem + K::P_COL, desc_add(da, step_k(kk, C)), desc_add(db, step_k(kk, C)), ID_P, kk > 0);
-        mma_commit(bar + Bz::P_FULL);
+          for (int k0 = 0; k0 < K::NCH; ++k0)
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) {
+              const uint32_t s = k0 * (C * 128 >> 4) + kk * 2;
+              mma_ss(tmem + K::P_COL, desc_add(da, s), desc_add(db, s), ID_P, k0 + kk > 0);
+            }
+          mma_commit(bar + Bz::P_FULL);
+          if (last || r.na > 1) mma_commit(bar + Bz::A_EMPTY + 8 * (ca % K::NA));
+          if (last || r.nb > 1) mma_commit(bar + Bz::B_EMPTY + 8 * (cb % K::NB));
+        }
+        __syncwarp();
+        if (new_b) {
+          ok = wait_warp(bar + Bz::C_FULL + 8 * (cb % K::NC), (cb / K::NC) & 1);
+          if (ok && cn < C && q.cu) {
+            zero_rows(sgen + K::OFF_C + (cb % K::NC) * K::TILE, K::NCH, cn, lane);
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+        }
+        // over what the output warps have taken of a X or of the item before
+        ok = ok && wait_warp(bar + Bz::P_READY, t & 1);
+        if (do_i) {
+          ok = ok && wait_warp(bar + Bz::OI_READ, noi & 1);
+          ++noi;
+        }
+        if (!ok) break;
+        tc_fence_after();
+        if (lane == 0) {
+          const uint64_t d = desc_mn(ct, C);
+#pragma unroll 1
+          for (int k0 = 0; k0 < C / 16; k0 += 4)
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) {
+              const uint32_t p = tmem + K::P_COL + 16 * (k0 + kk);      // 16 tokens: 8 columns hi, 8 lo
+              mma_ts(tmem + K::O_COL, p, desc_add(d, (k0 + kk) * 128), ID_T, k0 + kk > 0);
+              mma_ts(tmem + K::O_COL, p + 8, desc_add(d, (k0 + kk) * 128), ID_T, 1u);
+            }
+          mma_commit(bar + Bz::PV_DONE);
+          if (last || r.nb > 1) mma_commit(bar + Bz::C_EMPTY + 8 * (cb % K::NC));
+        }
+        __syncwarp();
       }
-      __syncwarp();
-      // O = a X, once the epilogue has taken the item before
-      if (first) {
-        ok = ok && wait_warp(bar + Bz::XS_READY, nx & 1);
-        ++nx;
-      }
-      if (do_i) {
+    } else if (warp == WARP_MMA2) {
+      // ------------------------------------------------------------ O = a X, X += (decayed rows)^T (rows)
+      int ca = -1, cb = -1, nx = 0, nbt = 0;
+      for (int t = 0, ck = 0, g = 0; ok && t < items; ++t, ++g == groups ? g = 0, ++ck : 0) {
+        const bool first = g == 0, last = g == groups - 1, end = ck == chunks - 1;
+        const bool new_b = first || r.nb > 1, do_b = new_b && !end, do_i = first || r.na > 1;
+        const int cn = min(C, t1 - t0 - chunk_at(ck));
+        cb += new_b ? 1 : 0;
+        ca += do_i ? 1 : 0;
+        const uint32_t at = st + K::OFF_A + (ca % K::NA) * K::TILE, bt = st + K::OFF_B + (cb % K::NB) * K::TILE,
+                       ct = st + K::OFF_C + (cb % K::NC) * K::TILE;
+        if (first) {
+          ok = wait_warp(bar + Bz::XS_READY, nx & 1);
+          ++nx;
+        }
+        // once the epilogue has taken the item before (waited for at every item, so that no phase is missed)
         if (t > 0) ok = ok && wait_warp(bar + Bz::O_READ, (t - 1) & 1);
-        tc_fence_after();
-        if (ok && lane == 0) {
-          const uint64_t da = desc_k(at);
-          const uint64_t xh = SWAP ? desc_k(xt) : desc_mn(xt, D);
+        if (do_i) {
+          ok = ok && wait_warp(bar + Bz::A_FULL + 8 * (ca % K::NA), (ca / K::NA) & 1);
+          tc_fence_after();
+          if (ok && lane == 0) {
+            const uint64_t da = desc_k(at), xh = SWAP ? desc_k(st + K::OFF_X) : desc_mn(st + K::OFF_X, D);
 #pragma unroll 1
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t s = SWAP ? step_k(kk, D) : (uint32_t)(kk * 128);
-            mma_ss(tmem + K::O_COL, desc_add(da, step_k(kk, C)), desc_add(xh, s), ID_I, kk > 0);
-            mma_ss(tmem + K::O_COL, desc_add(da, step_k(kk, C)), desc_add(xh, s + (K::XT >> 4)), ID_I, 1u);
+            for (int k0 = 0; k0 < K::NCH; ++k0)
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk) {
+                const uint32_t s = k0 * (C * 128 >> 4) + kk * 2, sx = SWAP ? k0 * (D * 128 >> 4) + kk * 2 : (4 * k0 + kk) * 128;
+                mma_ss(tmem + K::O_COL, desc_add(da, s), desc_add(xh, sx), ID_I, k0 + kk > 0);
+                mma_ss(tmem + K::O_COL, desc_add(da, s), desc_add(xh, sx + (K::XT >> 4)), ID_I, 1u);
+              }
+            mma_commit(bar + Bz::OI_FULL);
           }
-          mma_commit(bar + Bz::OI_FULL);
-        }
-        __syncwarp();
-      }
-      if (lane == 0 && (last || r.na > 1)) mma_commit(bar + Bz::A_EMPTY + 8 * (ca % K::NA));
-      // X += (decayed rows)^T (rows)
-      if (do_b) {
-        ok = ok && wait_warp(bar + Bz::BT_READY, nbt & 1);
-        ++nbt;
-      }
-      // b has been read for the decayed rows, and P = a b^T is the last to read it (SWAP: X is)
-      if (!SWAP && ok && lane == 0 && (last || r.nb > 1)) mma_commit(bar + Bz::B_EMPTY + 8 * (cb % K::NB));
-      if (new_b) {
-        ok = ok && wait_warp(bar + Bz::C_FULL + 8 * (cc % K::NC), (cc / K::NC) & 1);
-        if (ok && cn < C && q.cu) {
-          zero_rows(sgen + K::OFF_C + (cc % K::NC) * K::TILE, K::NCH, cn, lane);
-          fence_proxy_async_smem();
           __syncwarp();
         }
-      }
-      if (do_b) {
-        tc_fence_after();
-        if (ok && lane == 0) {
-          const uint64_t d = desc_mn(SWAP ? bt : ct, C);
-#pragma unroll 1
-          for (int kk = 0; kk < C / 16; ++kk) {
-            mma_ts(tmem + K::X_COL, tmem + K::BT_COL + 8 * kk, desc_add(d, kk * 128), ID_T, 1u);
-            mma_ts(tmem + K::X_COL, tmem + K::BT_COL + 64 + 8 * kk, desc_add(d, kk * 128), ID_T, 1u);
+        if (lane == 0 && (last || r.na > 1)) mma_commit(bar + Bz::A_EMPTY + 8 * (ca % K::NA));
+        if (do_b) {
+          ok = ok && wait_warp(bar + Bz::BT_READY, nbt & 1);
+          ++nbt;
+          ok = ok && wait_warp(bar + (SWAP ? Bz::B_FULL + 8 * (cb % K::NB) : Bz::C_FULL + 8 * (cb % K::NC)),
+                               (SWAP ? cb / K::NB : cb / K::NC) & 1);
+          if (ok && cn < C && q.cu) {
+            zero_rows(sgen + (SWAP ? K::OFF_B + (cb % K::NB) * K::TILE : K::OFF_C + (cb % K::NC) * K::TILE), K::NCH, cn, lane);
+            fence_proxy_async_smem();
+            __syncwarp();
           }
-          mma_commit(bar + Bz::X_DONE);
-        }
-        __syncwarp();
-      }
-      if (SWAP && ok && lane == 0 && (last || r.nb > 1)) mma_commit(bar + Bz::B_EMPTY + 8 * (cb % K::NB));
-      // O = P c, over what the output warps have taken of a X or of the item before
-      ok = ok && wait_warp(bar + Bz::P_READY, t & 1);
-      if (do_i) {
-        ok = ok && wait_warp(bar + Bz::OI_READ, noi & 1);
-        ++noi;
-      }
-      if (!ok) break;
-      tc_fence_after();
-      if (lane == 0) {
-        const uint64_t d = desc_mn(ct, C);
+          tc_fence_after();
+          if (ok && lane == 0) {
+            const uint64_t d = desc_mn(SWAP ? bt : ct, C);
 #pragma unroll 1
-        for (int kk = 0; kk < C / 16; ++kk) {
-          const uint32_t p = tmem + K::P_COL + 16 * kk;      // 16 tokens: 8 columns hi, 8 lo
-          mma_ts(tmem + K::O_COL, p, desc_add(d, kk * 128), ID_T, kk > 0);
-          mma_ts(tmem + K::O_COL, p + 8, desc_add(d, kk * 128), ID_T, 1u);
+            for (int k0 = 0; k0 < C / 16; k0 += 4)
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk) {
+                const uint32_t b = tmem + K::BT_COL + 8 * (k0 + kk);
+                mma_ts(tmem + K::X_COL, b, desc_add(d, (k0 + kk) * 128), ID_T, 1u);
+                mma_ts(tmem + K::X_COL, b + 64, desc_add(d, (k0 + kk) * 128), ID_T, 1u);
+              }
+            mma_commit(bar + Bz::X_DONE);
+          }
+          __syncwarp();
         }
-        mma_commit(bar + Bz::PV_DONE);
-        if (last || r.nb > 1) mma_commit(bar + Bz::C_EMPTY + 8 * (cc % K::NC));
+        if (!ok) break;
+        if (lane == 0 && (last || r.nb > 1)) {      // read here, or by the state warps, whose rows have been waited for
+          mma_commit(bar + Bz::B_EMPTY + 8 * (cb % K::NB));
+          mma_commit(bar + Bz::C_EMPTY + 8 * (cb % K::NC));
+        }
       }
-      __syncwarp();
     }
     if (!ok) record_error(LIN_ERR_WAIT);
-    if (lane == 0) mma_commit(bar + Bz::DRAIN);
-    __syncwarp();
-    if (!wait_warp(bar + Bz::DRAIN, 0)) record_error(LIN_ERR_WAIT);
+    if (warp == WARP_MMA || warp == WARP_MMA2) {
+      const uint32_t drain = bar + Bz::DRAIN + (warp == WARP_MMA2 ? 8 : 0);
+      if (lane == 0) mma_commit(drain);
+      __syncwarp();
+      if (!wait_warp(drain, 0)) record_error(LIN_ERR_WAIT);
     }
     __syncwarp();
   } else {
