@@ -149,12 +149,11 @@ __device__ __forceinline__ void tmem_store(uint32_t taddr, const float2* v) {
 // descriptors of a [rows][D] tile stored as D / 64 chunks of rows x 128 bytes (128-byte swizzle)
 __device__ __forceinline__ uint64_t desc_k(uint32_t tile) { return sdesc_sw128(tile, 16, 1024); }
 __device__ __forceinline__ uint64_t desc_mn(uint32_t tile, int rows) { return sdesc_sw128(tile, rows * 128, 1024); }
-// 16 steps along the contracted dim, in 16-byte units
-__device__ __forceinline__ uint32_t step_k(int kk, int rows) { return (uint32_t)(((kk / 4) * rows * 128 + (kk % 4) * 32) >> 4); }
 
 // Bounded warp-uniform wait, in few instructions: the kernel has some thirty of them, and what bounded it was the fetching of
 // instructions (a quarter of all stalls) while its steps were unrolled in full.  Gives up after 8e9 cycles, about 4 s.
 __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
   const long long from = clock64();
   while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity)))
     if (__any_sync(0xffffffffu, clock64() - from > 8000000000ll)) return false;
@@ -180,16 +179,17 @@ __device__ __forceinline__ void zero_rows(uint8_t* tile, int chunks, int r0, int
 // =====================================================================================
 // outputs
 // =====================================================================================
-template <int D>
+template <int D, bool SWAP>
 struct Cfg {
   static constexpr int NCH = D / 64;
   static constexpr int TILE = C * D * 2;            // a, b or c
   static constexpr int XT = D * D * 2;              // X hi or lo
-  static constexpr int NA = D == 128 ? 1 : 2, NB = D == 128 ? 1 : 2, NC = 2;
+  // two buffers for the rows that the state warps run ahead with; the others are free again before they are missed
+  static constexpr int NA = D == 128 ? 1 : 2, NB = D == 128 && SWAP ? 1 : 2, NC = D == 128 && !SWAP ? 1 : 2;
   static constexpr int OFF_X = 0, OFF_A = 2 * XT, OFF_B = OFF_A + NA * TILE, OFF_C = OFF_B + NB * TILE;
   static constexpr int OFF_O = OFF_C + NC * TILE;   // outputs on their way: a box of 32 rows x D / 2 columns for each output warp
   static constexpr int OFF_BAR = OFF_O + TILE;
-  static constexpr int OFF_LAM = OFF_BAR + 192;     // lam^n, n = 0 .. 128
+  static constexpr int OFF_LAM = OFF_BAR + 208;     // lam^n, n = 0 .. 128
   static constexpr int OFF_LAMC = OFF_LAM + 528;    // of a block's 32 columns: lam^(31 - j), or lam^j reversed
   static constexpr int OFF_MAX = OFF_LAMC + 128;    // fp16: [3] largest |X|, then [2][128] largest |P| of half a row
   static constexpr int SMEM = OFF_MAX + 16 + 2 * C * 4 + 1024;
@@ -199,14 +199,15 @@ struct Cfg {
 struct Bz {
   static constexpr int A_FULL = 0, A_EMPTY = 16, B_FULL = 32, B_EMPTY = 48, C_FULL = 64, C_EMPTY = 80, P_FULL = 96, P_READY = 104,
                        PV_DONE = 112, XS_READY = 120, BT_READY = 128, X_DONE = 136, OI_FULL = 144, OI_READ = 152, O_READ = 160,
-                       DRAIN = 168, TMEM_ADDR = 184;
+                       DRAIN = 168, X_READ = 184, TMEM_ADDR = 192;
 };
 
-template <int D, bool BF16, bool REV, bool SWAP>
+// MULTI: b and c have several heads (nb > 1)
+template <int D, bool BF16, bool REV, bool SWAP, bool MULTI>
 __global__ void __launch_bounds__(NTHREADS, 1)
     lin_tc_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb, const __grid_constant__ CUtensorMap tc,
                   const __grid_constant__ CUtensorMap to, const LinSeqs q, const LinRole r, const float* ws, const LinPool pool) {
-  using K = Cfg<D>;
+  using K = Cfg<D, SWAP>;
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
   extern __shared__ uint8_t smem_raw[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -251,6 +252,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     mbar_init(bar + Bz::XS_READY, NSTATE);
     mbar_init(bar + Bz::BT_READY, NSTATE);
     mbar_init(bar + Bz::X_DONE, 1);
+    mbar_init(bar + Bz::X_READ, 1);
     mbar_init(bar + Bz::OI_FULL, 1);
     mbar_init(bar + Bz::OI_READ, NOUT);
     mbar_init(bar + Bz::O_READ, NOUT);
@@ -279,28 +281,22 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       const int z4 = q.cu ? 0 : z;
       for (int ck = 0, g = 0; ok && ck < chunks; ++g == groups ? g = 0, ++ck : 0) {
         const int row = (int)span.row0 + t0 + chunk_at(ck);
-        // c has two buffers; b is free once P and the decayed rows are formed, a waits for a X
-        if (g == 0 || r.nb > 1) {
-          const int hh = h * r.nb + (r.nb > 1 ? g : 0), s = nc % K::NC, s2 = nb % K::NB;
-          if (nc >= K::NC && !mbar_wait(bar + Bz::C_EMPTY + 8 * s, ((nc / K::NC) - 1) & 1)) { ok = false; break; }
-          mbar_expect_tx(bar + Bz::C_FULL + 8 * s, K::TILE);
-          for (int c = 0; c < K::NCH; ++c)
-            tma_load_4d(sbase + K::OFF_C + s * K::TILE + c * C * 128, &tc, c * 64, row, hh, z4, bar + Bz::C_FULL + 8 * s);
-          ++nc;
-          if (nb >= K::NB && !mbar_wait(bar + Bz::B_EMPTY + 8 * s2, ((nb / K::NB) - 1) & 1)) { ok = false; break; }
-          mbar_expect_tx(bar + Bz::B_FULL + 8 * s2, K::TILE);
-          for (int c = 0; c < K::NCH; ++c)
-            tma_load_4d(sbase + K::OFF_B + s2 * K::TILE + c * C * 128, &tb, c * 64, row, hh, z4, bar + Bz::B_FULL + 8 * s2);
-          ++nb;
-        }
-        if (g == 0 || r.na > 1) {
-          const int s = na % K::NA;
-          if (na >= K::NA && !mbar_wait(bar + Bz::A_EMPTY + 8 * s, ((na / K::NA) - 1) & 1)) { ok = false; break; }
-          mbar_expect_tx(bar + Bz::A_FULL + 8 * s, K::TILE);
-          for (int c = 0; c < K::NCH; ++c)
-            tma_load_4d(sbase + K::OFF_A + s * K::TILE + c * C * 128, &ta, c * 64, row, h * r.na + (r.na > 1 ? g : 0), z4, bar + Bz::A_FULL + 8 * s);
-          ++na;
-        }
+        const auto load = [&](const CUtensorMap* map, int full, int empty, int off, int stages, int& i, int head) {
+          const int s = i % stages;
+          if (i >= stages) ok = ok && mbar_wait(bar + empty + 8 * s, ((i / stages) - 1) & 1);
+          if (!ok) return;
+          mbar_expect_tx(bar + full + 8 * s, K::TILE);
+          for (int c = 0; c < K::NCH; ++c) tma_load_4d(sbase + off + s * K::TILE + c * C * 128, map, c * 64, row, head, z4, bar + full + 8 * s);
+          ++i;
+        };
+        // the rows for the state first (two buffers), a next (free after a X), last what the end of an item reads
+        const bool new_b = g == 0 || r.nb > 1;
+        const int hb = h * r.nb + (r.nb > 1 ? g : 0);
+        if (new_b && SWAP) load(&tc, Bz::C_FULL, Bz::C_EMPTY, K::OFF_C, K::NC, nc, hb);
+        if (new_b && !SWAP) load(&tb, Bz::B_FULL, Bz::B_EMPTY, K::OFF_B, K::NB, nb, hb);
+        if (g == 0 || r.na > 1) load(&ta, Bz::A_FULL, Bz::A_EMPTY, K::OFF_A, K::NA, na, h * r.na + (r.na > 1 ? g : 0));
+        if (new_b && SWAP) load(&tb, Bz::B_FULL, Bz::B_EMPTY, K::OFF_B, K::NB, nb, hb);
+        if (new_b && !SWAP) load(&tc, Bz::C_FULL, Bz::C_EMPTY, K::OFF_C, K::NC, nc, hb);
       }
       if (!ok) record_error(LIN_ERR_WAIT);
       // copies must have landed before the block leaves
@@ -375,7 +371,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       }
     } else if (warp == WARP_MMA2) {
       // ------------------------------------------------------------ O = a X, X += (decayed rows)^T (rows)
-      int ca = -1, cb = -1, nx = 0, nbt = 0;
+      int ca = -1, cb = -1, nx = 0, nbt = 0, nor = 0;
       for (int t = 0, ck = 0, g = 0; ok && t < items; ++t, ++g == groups ? g = 0, ++ck : 0) {
         const bool first = g == 0, last = g == groups - 1, end = ck == chunks - 1;
         const bool new_b = first || r.nb > 1, do_b = new_b && !end, do_i = first || r.na > 1;
@@ -388,9 +384,11 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           ok = wait_warp(bar + Bz::XS_READY, nx & 1);
           ++nx;
         }
-        // once the epilogue has taken the item before (waited for at every item, so that no phase is missed)
-        if (t > 0) ok = ok && wait_warp(bar + Bz::O_READ, (t - 1) & 1);
         if (do_i) {
+          if (t > 0) {      // once the epilogue has taken the item before
+            ok = ok && wait_warp(bar + Bz::O_READ, nor & 1);
+            ++nor;
+          }
           ok = ok && wait_warp(bar + Bz::A_FULL + 8 * (ca % K::NA), (ca / K::NA) & 1);
           tc_fence_after();
           if (ok && lane == 0) {
@@ -404,6 +402,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                 mma_ss(tmem + K::O_COL, desc_add(da, s), desc_add(xh, sx + (K::XT >> 4)), ID_I, 1u);
               }
             mma_commit(bar + Bz::OI_FULL);
+            if (r.na == 1 || last) mma_commit(bar + Bz::X_READ);
           }
           __syncwarp();
         }
@@ -411,8 +410,13 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         if (do_b) {
           ok = ok && wait_warp(bar + Bz::BT_READY, nbt & 1);
           ++nbt;
-          ok = ok && wait_warp(bar + (SWAP ? Bz::B_FULL + 8 * (cb % K::NB) : Bz::C_FULL + 8 * (cb % K::NC)),
-                               (SWAP ? cb / K::NB : cb / K::NC) & 1);
+        }
+        // The state warps have read b (SWAP: it is still to be multiplied).  No buffer is given back before its tile has been
+        // seen to land, even where this warp has nothing to read: it would run ahead and give back the one before.
+        if (new_b && (SWAP || !do_b)) ok = ok && wait_warp(bar + Bz::B_FULL + 8 * (cb % K::NB), (cb / K::NB) & 1);
+        if (!SWAP && ok && lane == 0 && (last || r.nb > 1)) mbar_arrive(bar + Bz::B_EMPTY + 8 * (cb % K::NB));
+        if (new_b && (!SWAP || !do_b)) ok = ok && wait_warp(bar + Bz::C_FULL + 8 * (cb % K::NC), (cb / K::NC) & 1);
+        if (do_b) {
           if (ok && cn < C && q.cu) {
             zero_rows(sgen + (SWAP ? K::OFF_B + (cb % K::NB) * K::TILE : K::OFF_C + (cb % K::NC) * K::TILE), K::NCH, cn, lane);
             fence_proxy_async_smem();
@@ -435,7 +439,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         }
         if (!ok) break;
         if (lane == 0 && (last || r.nb > 1)) {      // read here, or by the state warps, whose rows have been waited for
-          mma_commit(bar + Bz::B_EMPTY + 8 * (cb % K::NB));
+          if (SWAP) mma_commit(bar + Bz::B_EMPTY + 8 * (cb % K::NB));
           mma_commit(bar + Bz::C_EMPTY + 8 * (cb % K::NC));
         }
       }
@@ -465,31 +469,47 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       const float* x0 = nullptr;
       if (ws) x0 = ws + (((long long)z * q.nhk + h) * q.nseg + n) * r.da * r.dc;
       else if (pool.in && !(pool.seen && pool.seen[z] <= 0)) x0 = pool.in + ((long long)slot * q.nhk + h) * r.da * r.dc;
-      int nx = 0, nbt = 0, noi = 0, cbw = -1, w_cn = 0;
+      int nx = 0, nbt = 0, cbw = -1, w_cn = 0;
       float2 w_rows[8];
-      if (qd * 32 < D) {                // X as it enters the segment
+      // X as it enters the segment.  Stored along its lanes it is read by whole lines; stored along its columns, a lane's row would be
+      // a line of its own in every load (20000 cycles of them), so it comes in by rows through the shared memory of X.
+      if (!r.transposed || SWAP) {
+        float4* stage = reinterpret_cast<float4*>(sgen + K::OFF_X);      // [D][D / 4], units swapped by row
+#pragma unroll 8
+        for (int e = tid - 256; e < D * D / 4; e += NSTATE) {
+          const int lane_x = e / (D / 4), col = e % (D / 4) * 4;
+          stage[lane_x * (D / 4) + ((col / 4) ^ (lane_x & 7))] =
+              x0 && lane_x < xl && col < xn ? *reinterpret_cast<const float4*>(x0 + (long long)lane_x * xn + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        bar_state();
+        if (qd * 32 < D) {
+#pragma unroll 1
+          for (int c0 = hf * HD; c0 < hf * HD + HD; c0 += 16) {
+            float2 x[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              reinterpret_cast<float4*>(x)[i] = stage[row * (D / 4) + ((c0 / 4 + i) ^ (row & 7))];
+            tmem_store<16>(la + K::X_COL + c0, x);
+          }
+        }
+        bar_state();
+      } else if (qd * 32 < D) {
 #pragma unroll 1
         for (int c0 = hf * HD; c0 < hf * HD + HD; c0 += 16) {
           float2 x[8];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int col = c0 + i, ii = SWAP ? col : row, jj = SWAP ? row : col;
-            reinterpret_cast<float*>(x)[i] =
-                x0 && row < xl && col < xn ? x0[r.transposed ? (long long)jj * r.da + ii : (long long)ii * r.dc + jj] : 0.f;
-          }
+          for (int i = 0; i < 16; ++i)
+            reinterpret_cast<float*>(x)[i] = x0 && row < xl && c0 + i < xn ? x0[(long long)(c0 + i) * xl + row] : 0.f;
           tmem_store<16>(la + K::X_COL + c0, x);
         }
-        tc_wait_st();
       }
+      tc_wait_st();
       for (int t = 0, ck = 0, g = 0; t < items; ++t, ++g == groups ? g = 0, ++ck : 0) {
         const bool first = g == 0, end = ck == chunks - 1;
         const bool do_b = (first || r.nb > 1) && !end;
         const int cn = min(C, t1 - t0 - chunk_at(ck));
         // the last a X, which reads X in shared memory, and the last update of X, which reads the decayed rows
-        if (t > 0 && (r.na > 1 || groups == 1 || g == 1)) {
-          wait(Bz::OI_FULL, noi);
-          ++noi;
-        }
+        if (t > 0 && first) wait(Bz::X_READ, ck - 1);
         if (nbt > 0 && (first || do_b)) wait(Bz::X_DONE, nbt - 1);
         // X: hi + lo to shared memory, lam^C X back to TMEM
         if (first) {
@@ -576,7 +596,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             for (int i = 0; i < 16; ++i) acc[c0 / 2 + i] = __ffma2_rn(o[i], make_float2(p_inv, p_inv), acc[c0 / 2 + i]);
           }
           tc_fence_before();
-          mbar_arrive(bar + Bz::O_READ);
+          if (write) mbar_arrive(bar + Bz::O_READ);      // a X comes next (else P c, which waits for the pair products)
           if (write && hf * HD < r.dc) {
             // 32 whole rows go out as one box; rows next to another sequence's one by one
             const bool whole = qd * 32 + 32 <= cn;
@@ -604,77 +624,77 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           }
         }
         if (t == items) break;
-        const bool first = g == 0, do_i = first || r.na > 1;
+        const bool first = g == 0, do_i = !MULTI || first;
         at = chunk_at(ck);
         cn = min(C, t1 - t0 - at);
         head = r.na > 1 ? g : 0;
         write = r.na > 1 || g == groups - 1;
-        // Pair products: decay, mask, back to TMEM as hi + lo, in pieces of 16 columns.  A piece beside the diagonal block of 32 x 32 takes
-        // lam^(rows from its block's near edge) times lam^(columns from it), both at most 1, so that nothing overflows however
-        // fast the decay
+        // Pair products: decay, mask, back to TMEM as hi + lo, in pieces of W columns (acc takes the registers where it lives on from
+        // head to head).  A block of 32 x 32 beside the diagonal's takes lam^(rows from its near edge) times lam^(columns from it), both at
+        // most 1, so that nothing overflows however fast the decay
+        constexpr int W = MULTI ? 16 : 32;
         wait(Bz::P_FULL, t);
-        {
-          const auto load = [&](int piece, float2* p) {      // false: all 0, not loaded
-            const int j0 = hf * 64 + 32 * (piece >> 1), c0 = 16 * (piece & 1), side = REV ? j0 / 32 - qd : qd - j0 / 32;
-            if (side < 0) return false;
-            tmem_load<16>(la + K::P_COL + j0 + c0, p);
-            if (side > 0) {
-              const float4* w = reinterpret_cast<const float4*>(lamc + c0);
-              const float blk = lam[REV ? j0 - row : row - j0 - 31];
-              const float2 u = make_float2(blk, blk);
+        float ps = 1.f;
+        if constexpr (!BF16) {
+          // the products before decay bound the row (factors are at most 1)
+          float top = 0.f;
+#pragma unroll 1
+          for (int j0 = hf * 64; j0 < hf * 64 + 64; j0 += W) {
+            if (REV ? j0 / 32 < qd : j0 / 32 > qd) continue;
+            float2 p[W / 2];
+            tmem_load<W>(la + K::P_COL + j0, p);
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < W / 2; ++i) top = fmaxf(top, fmaxf(fabsf(p[i].x), fabsf(p[i].y)));
+          }
+          uint32_t* most = pmax + row;
+          most[hf * C] = __float_as_uint(top);      // the item before was read before its P c, which this P waited for
+          bar_quadrant(qd);
+          ps = scale_to(max(most[0], most[C]));
+        }
+        p_inv = r.w_intra / ps;
+#pragma unroll 1
+        for (int j0 = hf * 64; j0 < hf * 64 + 64; j0 += W) {
+          const int edge = j0 & ~31, side = REV ? edge / 32 - qd : qd - edge / 32;
+          float2 p[W / 2];
+          if (side < 0) {
+#pragma unroll
+            for (int i = 0; i < W / 2; ++i) p[i] = make_float2(0.f, 0.f);
+          } else {
+            tmem_load<W>(la + K::P_COL + j0, p);
+            if (side > 0) {
+              const float4* w = reinterpret_cast<const float4*>(lamc + (j0 - edge));
+              const float blk = lam[REV ? edge - row : row - edge - 31] * ps;
+#pragma unroll
+              for (int i = 0; i < W / 4; ++i) {
                 const float4 f = w[i];
-                p[2 * i] = __fmul2_rn(p[2 * i], __fmul2_rn(u, make_float2(f.x, f.y)));
-                p[2 * i + 1] = __fmul2_rn(p[2 * i + 1], __fmul2_rn(u, make_float2(f.z, f.w)));
+                p[2 * i] = __fmul2_rn(p[2 * i], __fmul2_rn(make_float2(blk, blk), make_float2(f.x, f.y)));
+                p[2 * i + 1] = __fmul2_rn(p[2 * i + 1], __fmul2_rn(make_float2(blk, blk), make_float2(f.z, f.w)));
               }
             } else {
-              const float* w = lam + (REV ? c0 - lane : lane - c0);
+              // on the diagonal the exponent runs over both: exp2 of each, which costs less than a table read of each
+              const float from = (float)(REV ? j0 - row : row - j0);
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const int gap = REV ? c0 + 2 * i - lane : lane - c0 - 2 * i, next = REV ? gap + 1 : gap - 1;
-                p[i].x = gap >= 0 ? p[i].x * w[REV ? 2 * i : -2 * i] : 0.f;
-                p[i].y = next >= 0 ? p[i].y * w[REV ? 2 * i + 1 : -2 * i - 1] : 0.f;
+              for (int i = 0; i < W / 2; ++i) {
+                const float gap = REV ? from + 2 * i : from - 2 * i, next = REV ? gap + 1.f : gap - 1.f;
+                p[i].x = gap >= 0.f ? p[i].x * (ex2(g2 * gap) * ps) : 0.f;
+                p[i].y = next >= 0.f ? p[i].y * (ex2(g2 * next) * ps) : 0.f;
               }
             }
             if (REV && cn < C) {                  // forward, a row sees no token past its own
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                if (j0 + c0 + 2 * i >= cn) p[i].x = 0.f;
-                if (j0 + c0 + 2 * i + 1 >= cn) p[i].y = 0.f;
+              for (int i = 0; i < W / 2; ++i) {
+                if (j0 + 2 * i >= cn) p[i].x = 0.f;
+                if (j0 + 2 * i + 1 >= cn) p[i].y = 0.f;
               }
             }
-            return true;
-          };
-          float ps = 1.f;
-          if constexpr (!BF16) {
-            float top = 0.f;
-#pragma unroll 1
-            for (int piece = 0; piece < 4; ++piece) {
-              float2 p[8];
-              if (!load(piece, p)) continue;
-#pragma unroll
-              for (int i = 0; i < 8; ++i) top = fmaxf(top, fmaxf(fabsf(p[i].x), fabsf(p[i].y)));
-            }
-            uint32_t* most = pmax + row;
-            most[hf * C] = __float_as_uint(top);      // the item before was read before its P c, which this P waited for
-            bar_quadrant(qd);
-            ps = scale_to(max(most[0], most[C]));
           }
-#pragma unroll 1
-          for (int piece = 0; piece < 4; ++piece) {
-            float2 p[8];
+#pragma unroll
+          for (int c0 = 0; c0 < W / 2; c0 += 8) {
             uint32_t w[16];
-            if (load(piece, p)) {
 #pragma unroll
-              for (int i = 0; i < 8; ++i) split2<BF16>(BF16 ? p[i] : __fmul2_rn(p[i], make_float2(ps, ps)), w[i], w[8 + i]);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 16; ++i) w[i] = 0;
-            }
-            tmem_st16(la + K::P_COL + hf * 64 + 16 * piece, w);
+            for (int i = 0; i < 8; ++i) split2<BF16>(p[c0 + i], w[i], w[8 + i]);
+            tmem_st16(la + K::P_COL + j0 + 2 * c0, w);
           }
-          p_inv = r.w_intra / ps;
         }
         tc_wait_st();
         tc_fence_before();
@@ -927,20 +947,23 @@ int launch(Kernel kernel, int threads, int smem, unsigned long long* done, const
   return cuda_status(cudaGetLastError(), "linear attention (tensor cores) launch");
 }
 
-template <int D, bool BF16, bool REV, bool SWAP>
+template <int D, bool BF16, bool REV, bool SWAP, bool MULTI>
 int run_one(const LinSeqs& q, const LinRole& r, const float* ws, const LinPool& pool, cudaStream_t st, const CUtensorMap* m, bool* taken) {
   static unsigned long long done = 0;
-  static const bool fits = regs_fit(lin_tc_kernel<D, BF16, REV, SWAP>);
+  static const bool fits = regs_fit(lin_tc_kernel<D, BF16, REV, SWAP, MULTI>);
   if (!fits) return FA_OK;
   *taken = true;
-  return launch(lin_tc_kernel<D, BF16, REV, SWAP>, NTHREADS, Cfg<D>::SMEM, &done, q, st, m[0], m[1], m[2], m[3], q, r, ws, pool);
+  return launch(lin_tc_kernel<D, BF16, REV, SWAP, MULTI>, NTHREADS, Cfg<D, SWAP>::SMEM, &done, q, st, m[0], m[1], m[2], m[3], q, r, ws, pool);
 }
 template <int D, bool BF16>
 int run_main(const LinSeqs& q, const LinRole& r, bool rev, const float* ws, const LinPool& pool, cudaStream_t st, const CUtensorMap* m, bool* taken) {
   // dk: the output is along the state's rows as it is stored
-  if (rev && r.transposed) return run_one<D, BF16, true, true>(q, r, ws, pool, st, m, taken);
-  if (rev) return run_one<D, BF16, true, false>(q, r, ws, pool, st, m, taken);
-  return run_one<D, BF16, false, false>(q, r, ws, pool, st, m, taken);
+  if (!rev) return run_one<D, BF16, false, false, false>(q, r, ws, pool, st, m, taken);
+  if (r.nb > 1)
+    return r.transposed ? run_one<D, BF16, true, true, true>(q, r, ws, pool, st, m, taken)
+                        : run_one<D, BF16, true, false, true>(q, r, ws, pool, st, m, taken);
+  return r.transposed ? run_one<D, BF16, true, true, false>(q, r, ws, pool, st, m, taken)
+                      : run_one<D, BF16, true, false, false>(q, r, ws, pool, st, m, taken);
 }
 template <int D, bool BF16>
 int run_states(const LinSeqs& q, const LinRole& r, bool rev, float* ws, cudaStream_t st, const CUtensorMap* m) {
