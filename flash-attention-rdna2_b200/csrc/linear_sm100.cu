@@ -17,13 +17,14 @@
 //
 // Warp roles (640 threads, five warpgroups):
 //   0-7    outputs: pair products on their way back to TMEM, a X, epilogue; two warps to a TMEM lane quadrant (w % 4), half of the columns each
-//   8-15   state: decayed rows, X to shared memory and lam^C X back to TMEM; two warps to a quadrant likewise
+//   8-15   state: X to shared memory and lam^C X back to TMEM, decayed rows; two warps to a quadrant likewise (four warps for each of the
+//          two steps took longer)
 //   16     TMA
-//   17, 18 MMAs: P = a b^T and O = P c, O = a X and X += ..; one thread alone issues an MMA in 85 to 110 cycles and the pipe takes 64
+//   17-19  MMAs: P = a b^T and O = P c; O = a X; X += ..  One thread alone issues an MMA in 85 to 110 cycles and the pipe takes 64, and
+//          none of the three waits for what only another needs
 // What a chunk needs is a chain of short steps, each a TMEM or shared memory latency long, and not their instructions: one
 // set of warps that took all steps in turn needed 10000 cycles a chunk, issuing every third cycle.  Outputs of item t and the state
-// of the next chunk depend on each other through the MMAs alone, so two sets run them side by side, each waiting for an MMA
-// that has had another step's time.  Registers follow the need (setmaxnreg): the epilogue holds 64 columns.  Every wait is bounded.
+// of the next chunk depend on each other through the MMAs alone, so two sets run them side by side.  Registers follow the need (setmaxnreg): the epilogue holds 64 columns.  Every wait is bounded.
 #include <cudaTypedefs.h>
 #include "linear_common.cuh"
 #include "fa_launch.h"
@@ -35,7 +36,7 @@ using namespace sm100;
 using namespace fa;
 
 constexpr int C = 128;               // tokens of a chunk
-constexpr int NTHREADS = 640, NOUT = 256, NSTATE = 256, WARP_TMA = 16, WARP_MMA = 17, WARP_MMA2 = 18;
+constexpr int NTHREADS = 640, NOUT = 256, NSTATE = 256, WARP_TMA = 16, WARP_MMA = 17, WARP_MMA2 = 18, WARP_MMA3 = 19;
 // registers a thread: launched with REGS; 2 x 136 + 2 x 80 + 48 = 5 x 96
 constexpr int REGS = 96;
 __device__ __forceinline__ void regs_out() { asm volatile("setmaxnreg.inc.sync.aligned.u32 136;"); }
@@ -189,7 +190,7 @@ struct Cfg {
   static constexpr int OFF_X = 0, OFF_A = 2 * XT, OFF_B = OFF_A + NA * TILE, OFF_C = OFF_B + NB * TILE;
   static constexpr int OFF_O = OFF_C + NC * TILE;   // outputs on their way: a box of 32 rows x D / 2 columns for each output warp
   static constexpr int OFF_BAR = OFF_O + TILE;
-  static constexpr int OFF_LAM = OFF_BAR + 208;     // lam^n, n = 0 .. 128
+  static constexpr int OFF_LAM = OFF_BAR + 224;     // lam^n, n = 0 .. 128
   static constexpr int OFF_LAMC = OFF_LAM + 528;    // of a block's 32 columns: lam^(31 - j), or lam^j reversed
   static constexpr int OFF_MAX = OFF_LAMC + 128;    // fp16: [3] largest |X|, then [2][128] largest |P| of half a row
   static constexpr int SMEM = OFF_MAX + 16 + 2 * C * 4 + 1024;
@@ -199,7 +200,7 @@ struct Cfg {
 struct Bz {
   static constexpr int A_FULL = 0, A_EMPTY = 16, B_FULL = 32, B_EMPTY = 48, C_FULL = 64, C_EMPTY = 80, P_FULL = 96, P_READY = 104,
                        PV_DONE = 112, XS_READY = 120, BT_READY = 128, X_DONE = 136, OI_FULL = 144, OI_READ = 152, O_READ = 160,
-                       DRAIN = 168, X_READ = 184, TMEM_ADDR = 192;
+                       DRAIN = 168, X_READ = 192, TMEM_ADDR = 200;
 };
 
 // MULTI: b and c have several heads (nb > 1)
@@ -253,6 +254,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     mbar_init(bar + Bz::BT_READY, NSTATE);
     mbar_init(bar + Bz::X_DONE, 1);
     mbar_init(bar + Bz::X_READ, 1);
+    mbar_init(bar + Bz::DRAIN + 16, 1);
     mbar_init(bar + Bz::OI_FULL, 1);
     mbar_init(bar + Bz::OI_READ, NOUT);
     mbar_init(bar + Bz::O_READ, NOUT);
@@ -370,21 +372,17 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         __syncwarp();
       }
     } else if (warp == WARP_MMA2) {
-      // ------------------------------------------------------------ O = a X, X += (decayed rows)^T (rows)
-      int ca = -1, cb = -1, nx = 0, nbt = 0, nor = 0;
+      // ------------------------------------------------------------ O = a X
+      int ca = -1, nx = 0, nor = 0;
       for (int t = 0, ck = 0, g = 0; ok && t < items; ++t, ++g == groups ? g = 0, ++ck : 0) {
-        const bool first = g == 0, last = g == groups - 1, end = ck == chunks - 1;
-        const bool new_b = first || r.nb > 1, do_b = new_b && !end, do_i = first || r.na > 1;
-        const int cn = min(C, t1 - t0 - chunk_at(ck));
-        cb += new_b ? 1 : 0;
-        ca += do_i ? 1 : 0;
-        const uint32_t at = st + K::OFF_A + (ca % K::NA) * K::TILE, bt = st + K::OFF_B + (cb % K::NB) * K::TILE,
-                       ct = st + K::OFF_C + (cb % K::NC) * K::TILE;
+        const bool first = g == 0, last = g == groups - 1, do_i = first || r.na > 1;
         if (first) {
           ok = wait_warp(bar + Bz::XS_READY, nx & 1);
           ++nx;
         }
         if (do_i) {
+          ++ca;
+          const uint32_t at = st + K::OFF_A + (ca % K::NA) * K::TILE;
           if (t > 0) {      // once the epilogue has taken the item before
             ok = ok && wait_warp(bar + Bz::O_READ, nor & 1);
             ++nor;
@@ -406,7 +404,21 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           }
           __syncwarp();
         }
-        if (lane == 0 && (last || r.na > 1)) mma_commit(bar + Bz::A_EMPTY + 8 * (ca % K::NA));
+        if (ok && lane == 0 && (last || r.na > 1)) mma_commit(bar + Bz::A_EMPTY + 8 * (ca % K::NA));
+      }
+    } else if (warp == WARP_MMA3) {
+      // ------------------------------------------------------------ X += (decayed rows)^T (rows)
+      int cb = -1, nx = 0, nbt = 0;
+      for (int t = 0, ck = 0, g = 0; ok && t < items; ++t, ++g == groups ? g = 0, ++ck : 0) {
+        const bool first = g == 0, last = g == groups - 1, end = ck == chunks - 1;
+        const bool new_b = first || r.nb > 1, do_b = new_b && !end;
+        const int cn = min(C, t1 - t0 - chunk_at(ck));
+        cb += new_b ? 1 : 0;
+        const uint32_t bt = st + K::OFF_B + (cb % K::NB) * K::TILE, ct = st + K::OFF_C + (cb % K::NC) * K::TILE;
+        if (first && !end) {
+          ok = wait_warp(bar + Bz::XS_READY, nx & 1);
+          ++nx;
+        }
         if (do_b) {
           ok = ok && wait_warp(bar + Bz::BT_READY, nbt & 1);
           ++nbt;
@@ -445,8 +457,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       }
     }
     if (!ok) record_error(LIN_ERR_WAIT);
-    if (warp == WARP_MMA || warp == WARP_MMA2) {
-      const uint32_t drain = bar + Bz::DRAIN + (warp == WARP_MMA2 ? 8 : 0);
+    if (warp >= WARP_MMA) {
+      const uint32_t drain = bar + Bz::DRAIN + 8 * (warp - WARP_MMA);
       if (lane == 0) mma_commit(drain);
       __syncwarp();
       if (!wait_warp(drain, 0)) record_error(LIN_ERR_WAIT);
