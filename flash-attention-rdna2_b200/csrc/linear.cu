@@ -14,59 +14,62 @@ __device__ int g_lin_error = 0;
 // Recurrent kernel: S_t = lam S_{t-1} + k_t v_t^T, o_t = scale S_t^T q_t, token by token.
 // Bound by reading and writing the state once: 8 dk dv bytes a sequence and head.  A block holds 32 columns of one state
 // (a 128-byte line of each row) in registers, so that a state of 128 columns gives four blocks and small batches still spread;
-// all its loads are issued before the first token is looked at.
+// all its loads are issued before anything else is looked at, the other sequences' slots among them.
 // =====================================================================================
 constexpr int STEP_THREADS = 128, STEP_COLS = 32;
 
-template <typename T, int ROWS>   // ROWS = rows of the state a thread holds: dk <= 16 * ROWS
-__global__ void __launch_bounds__(STEP_THREADS)
+// ROWS = rows of the state a thread holds: dk <= 16 * ROWS; G = query heads of a group that are summed together
+template <typename T, int ROWS, int G>
+__global__ void __launch_bounds__(STEP_THREADS, ROWS > 8 ? 3 : G == 1 ? 6 : 5)
     lin_step_kernel(const LinSeqs q, const LinRole r, const LinPool pool, const int blocks_v) {
-  constexpr int GMAX = 4;                                    // query heads of a group that are summed together
-  __shared__ float sk[256], sq[GMAX][256], sred[4][GMAX][STEP_COLS];
+  __shared__ float sk[256], sq[G][256], sred[4][G][STEP_COLS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int vb = blockIdx.x % blocks_v, h = (blockIdx.x / blocks_v) % q.nhk, z = blockIdx.x / blocks_v / q.nhk;
-  if (vb == 0) lin_zero_outside<T>(q, r, z, h * r.na, 0, 1, STEP_THREADS);
-  const LinSpan span = lin_span(q, z);
-  const int slot = lin_slot(pool, z, STEP_THREADS, &g_lin_error);
-  T* out = (T*)r.out + (q.cu ? 0 : z * r.so.b) + span.row0 * r.so.s + (long long)h * r.na * r.so.h;
-  const int col = vb * STEP_COLS + (tid & 7) * 4, row0 = tid >> 3;
-  const bool mine = col < r.dc;
-  if (slot < 0) {
-    for (int e = tid; e < span.len * r.na * STEP_COLS; e += STEP_THREADS) {
-      const int c = vb * STEP_COLS + e % STEP_COLS, g = e / STEP_COLS % r.na, t = e / STEP_COLS / r.na;
-      if (c < r.dc) out[t * r.so.s + g * r.so.h + c] = Elem<T>::from_f(0.f);
-    }
-    return;
-  }
-  const long long at = ((long long)slot * q.nhk + h) * r.da * r.dc + col;
+  const int vb = blockIdx.x % blocks_v, hz = blockIdx.x / blocks_v, h = hz % q.nhk, z = hz / q.nhk;
+  const int named = pool.index ? pool.index[z] : z;
   const bool old = pool.in && !(pool.seen && pool.seen[z] <= 0);
+  const LinSpan span = lin_span(q, z);
+  const float lam = exp2f(lin_log2_decay(q.log_decay, h));
+  const int col = vb * STEP_COLS + (tid & 7) * 4, row0 = tid >> 3;
+  const bool mine = col < r.dc, inside = named >= 0 && (!pool.index || named < pool.slots);
+  const long long at = ((long long)named * q.nhk + h) * r.da * r.dc + col;
   float4 x[ROWS];
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
     const int row = row0 + 16 * i;
-    x[i] = old && mine && row < r.da ? *reinterpret_cast<const float4*>(pool.in + at + (long long)row * r.dc) : make_float4(0.f, 0.f, 0.f, 0.f);
+    x[i] = old && mine && inside && row < r.da ? __ldcs(reinterpret_cast<const float4*>(pool.in + at + (long long)row * r.dc))
+                                               : make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  const float lam = exp2f(lin_log2_decay(q.log_decay, h));
   const T* a = (const T*)r.a + (q.cu ? 0 : z * r.sa.b) + span.row0 * r.sa.s + (long long)h * r.na * r.sa.h;
   const T* b = (const T*)r.b + (q.cu ? 0 : z * r.sb.b) + span.row0 * r.sb.s + (long long)h * r.sb.h;
   const T* c = (const T*)r.c + (q.cu ? 0 : z * r.sc.b) + span.row0 * r.sc.s + (long long)h * r.sc.h;
+  T* out = (T*)r.out + (q.cu ? 0 : z * r.so.b) + span.row0 * r.so.s + (long long)h * r.na * r.so.h;
+  if (vb == 0) lin_zero_outside<T>(q, r, z, h * r.na, 0, 1, STEP_THREADS);
+  if (lin_slot(pool, z, STEP_THREADS, &g_lin_error) < 0) {
+    for (int e = tid; e < span.len * r.na * STEP_COLS; e += STEP_THREADS) {
+      const int cc = vb * STEP_COLS + e % STEP_COLS, g = e / STEP_COLS % r.na, t = e / STEP_COLS / r.na;
+      if (cc < r.dc) out[t * r.so.s + g * r.so.h + cc] = Elem<T>::from_f(0.f);
+    }
+    return;
+  }
   for (int t = 0; t < span.len; ++t) {
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (mine) {
       const T* cr = c + t * r.sc.s + col;
       v = make_float4(Elem<T>::to_f(cr[0]), Elem<T>::to_f(cr[1]), Elem<T>::to_f(cr[2]), Elem<T>::to_f(cr[3]));
     }
-    for (int g0 = 0; g0 < r.na; g0 += GMAX) {
-      const int ng = min(GMAX, r.na - g0);
-      __syncthreads();
+    for (int g0 = 0; g0 < r.na; g0 += G) {
+      const int ng = min(G, r.na - g0);
+      if (t > 0 || g0 > 0) __syncthreads();
       if (g0 == 0)
         for (int e = tid; e < r.da; e += STEP_THREADS) sk[e] = Elem<T>::to_f(b[t * r.sb.s + e]);
-      for (int e = tid; e < ng * r.da; e += STEP_THREADS)
-        sq[e / r.da][e % r.da] = Elem<T>::to_f(a[t * r.sa.s + (g0 + e / r.da) * r.sa.h + e % r.da]);
-      __syncthreads();
-      float4 o[GMAX];
 #pragma unroll
-      for (int g = 0; g < GMAX; ++g) o[g] = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int g = 0; g < G; ++g)
+        if (g < ng)
+          for (int e = tid; e < r.da; e += STEP_THREADS) sq[g][e] = Elem<T>::to_f(a[t * r.sa.s + (g0 + g) * r.sa.h + e]);
+      __syncthreads();
+      float4 o[G];
+#pragma unroll
+      for (int g = 0; g < G; ++g) o[g] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int i = 0; i < ROWS; ++i) {
         const int row = row0 + 16 * i;
@@ -79,7 +82,7 @@ __global__ void __launch_bounds__(STEP_THREADS)
             x[i].w = fmaf(lam, x[i].w, k * v.w);
           }
 #pragma unroll
-          for (int g = 0; g < GMAX; ++g)
+          for (int g = 0; g < G; ++g)
             if (g < ng) {
               const float w = sq[g][row];
               o[g].x = fmaf(w, x[i].x, o[g].x);
@@ -89,9 +92,17 @@ __global__ void __launch_bounds__(STEP_THREADS)
             }
         }
       }
+      // the state is on its way back before the sums are joined
+      if (t == span.len - 1 && g0 + G >= r.na && pool.out && mine) {
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+          const int row = row0 + 16 * i;
+          if (row < r.da) __stcs(reinterpret_cast<float4*>(pool.out + at + (long long)row * r.dc), x[i]);
+        }
+      }
       // lanes of one column group differ in bits 3 and 4; then the four warps
 #pragma unroll
-      for (int g = 0; g < GMAX; ++g)
+      for (int g = 0; g < G; ++g)
         if (g < ng) {
 #pragma unroll
           for (int m = 8; m <= 16; m *= 2) {
@@ -103,13 +114,15 @@ __global__ void __launch_bounds__(STEP_THREADS)
           if (lane < 8) *reinterpret_cast<float4*>(&sred[warp][g][lane * 4]) = o[g];
         }
       __syncthreads();
-      const int g = tid / STEP_COLS, cc = tid % STEP_COLS;
-      if (g < ng && vb * STEP_COLS + cc < r.dc)
-        out[t * r.so.s + (g0 + g) * r.so.h + vb * STEP_COLS + cc] =
-            Elem<T>::from_f(r.w_inter * (sred[0][g][cc] + sred[1][g][cc] + sred[2][g][cc] + sred[3][g][cc]));
+      for (int e = tid; e < ng * STEP_COLS; e += STEP_THREADS) {
+        const int g = e / STEP_COLS, cc = e % STEP_COLS;
+        if (vb * STEP_COLS + cc < r.dc)
+          out[t * r.so.s + (g0 + g) * r.so.h + vb * STEP_COLS + cc] =
+              Elem<T>::from_f(r.w_inter * (sred[0][g][cc] + sred[1][g][cc] + sred[2][g][cc] + sred[3][g][cc]));
+      }
     }
   }
-  if (!pool.out || !mine) return;
+  if (span.len > 0 || !pool.out || !mine) return;      // without tokens the state is passed on
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
     const int row = row0 + 16 * i;
@@ -120,23 +133,32 @@ __global__ void __launch_bounds__(STEP_THREADS)
 // =====================================================================================
 // CUDA-core chunked kernel: every type, dims up to 256, any strides.  A block walks one segment of one state in chunks of
 // 32 tokens, for 64 of the c dim's columns, all in fp32: the state, the chunk's rows and the pair products in shared memory.
+// Every product reads its operands four at a time (rows padded to an odd number of 16-byte units, so that the lanes of a
+// quarter warp meet different banks): 16 to 32 multiply-adds for each pair of 16-byte reads; scalar reads took three times as long.
 // =====================================================================================
-constexpr int SC = 32, SCOL = 64, SIMT_THREADS = 256;
+constexpr int SC = 32, SCOL = 64, SIMT_THREADS = 256, SPLD = SC + 4;
 
-__host__ __device__ inline int simt_smem_floats(int da) { return 2 * SC * (da + 1) + SC * SCOL + da * SCOL + SC * (SC + 1) + 3 * SC; }
+__host__ __device__ inline int simt_smem_floats(int da) { return 2 * SC * (da + 4) + SC * SCOL + da * SCOL + SC * SPLD + SC + 4; }
+
+__device__ __forceinline__ float dot4(const float4& a, const float4& b, float s) {
+  return fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, fmaf(a.x, b.x, s))));
+}
+__device__ __forceinline__ void axpy4(float w, const float4& v, float4& s) {
+  s.x = fmaf(w, v.x, s.x); s.y = fmaf(w, v.y, s.y); s.z = fmaf(w, v.z, s.z); s.w = fmaf(w, v.w, s.w);
+}
 
 template <typename T, bool REV, bool STATES>
 __global__ void __launch_bounds__(SIMT_THREADS)
     lin_simt_kernel(const LinSeqs q, const LinRole r, const float* ws, float* ws_out, const LinPool pool, const int blocks_c) {
-  extern __shared__ float sm[];
-  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  const int ld = r.da + 1;
-  float* sa = sm;
+  extern __shared__ __align__(16) float sm[];
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, lane = tid & 31, warp = tid >> 5;
+  const int ld = r.da + 4;
+  float* sa = sm;                           // [SC][ld]
   float* sb = sa + SC * ld;
-  float* sc = sb + SC * ld;                 // [SC][SCOL], 16-byte aligned below
+  float* sc = sb + SC * ld;                 // [SC][SCOL]
   float* sx = sc + SC * SCOL;               // [da][SCOL]
-  float* sp = sx + r.da * SCOL;             // [SC][SC + 1]
-  float* lam = sp + SC * (SC + 1);          // lam^n, n <= SC
+  float* sp = sx + r.da * SCOL;             // [SC][SPLD]
+  float* lam = sp + SC * SPLD;              // lam^n, n <= SC
   const int cb = blockIdx.x % blocks_c;
   const int n = blockIdx.x / blocks_c % q.nseg;
   const int h = blockIdx.x / blocks_c / q.nseg % q.nhk, z = blockIdx.x / blocks_c / q.nseg / q.nhk;
@@ -170,46 +192,49 @@ __global__ void __launch_bounds__(SIMT_THREADS)
     sx[e] = x0 && j < r.dc ? x0[r.transposed ? (long long)j * r.da + i : (long long)i * r.dc + j] : 0.f;
   }
   const int chunks = (t1 - t0 + SC - 1) / SC, groups = max(r.na, r.nb);
+  const auto rows = [&](float* to, int ld_to, const T* from, long long step, int first, int dims, int real, int cn) {
+    for (int j = warp; j < SC; j += SIMT_THREADS / 32)
+      for (int i = lane; i < dims; i += 32) to[j * ld_to + i] = j < cn && first + i < real ? Elem<T>::to_f(from[j * step + first + i]) : 0.f;
+  };
   for (int m = 0; m < chunks; ++m) {
     const int at = t0 + (REV ? chunks - 1 - m : m) * SC, cn = min(SC, t1 - at);
     float4 o[2];
     for (int g = 0; g < groups; ++g) {
       const bool load_a = !STATES && (g == 0 || r.na > 1), load_b = g == 0 || r.nb > 1;
       __syncthreads();
-      for (int e = tid; e < SC * r.da; e += SIMT_THREADS) {
-        const int j = e / r.da, i = e % r.da;
-        if (load_a) sa[j * ld + i] = j < cn ? Elem<T>::to_f(a[(at + j) * r.sa.s + (r.na > 1 ? g : 0) * r.sa.h + i]) : 0.f;
-        if (load_b) sb[j * ld + i] = j < cn ? Elem<T>::to_f(b[(at + j) * r.sb.s + (r.nb > 1 ? g : 0) * r.sb.h + i]) : 0.f;
+      if (load_a) rows(sa, ld, a + at * r.sa.s + (r.na > 1 ? g : 0) * r.sa.h, r.sa.s, 0, r.da, r.da, cn);
+      if (load_b) {
+        rows(sb, ld, b + at * r.sb.s + (r.nb > 1 ? g : 0) * r.sb.h, r.sb.s, 0, r.da, r.da, cn);
+        rows(sc, SCOL, c + at * r.sc.s + (r.nb > 1 ? g : 0) * r.sc.h, r.sc.s, c0, SCOL, r.dc, cn);
       }
-      if (load_b)
-        for (int e = tid; e < SC * SCOL; e += SIMT_THREADS) {
-          const int j = e / SCOL, i = c0 + e % SCOL;
-          sc[e] = j < cn && i < r.dc ? Elem<T>::to_f(c[(at + j) * r.sc.s + (r.nb > 1 ? g : 0) * r.sc.h + i]) : 0.f;
-        }
       __syncthreads();
       if constexpr (!STATES) {
+        const float *a0 = sa + (2 * ty) * ld, *a1 = a0 + ld, *b0 = sb + tx * ld, *b1 = b0 + 16 * ld;
         float p[2][2] = {};
-        for (int i = 0; i < r.da; ++i) {
-          const float a0 = sa[(2 * ty) * ld + i], a1 = sa[(2 * ty + 1) * ld + i], b0 = sb[tx * ld + i], b1 = sb[(tx + 16) * ld + i];
-          p[0][0] = fmaf(a0, b0, p[0][0]);
-          p[0][1] = fmaf(a0, b1, p[0][1]);
-          p[1][0] = fmaf(a1, b0, p[1][0]);
-          p[1][1] = fmaf(a1, b1, p[1][1]);
+        for (int i = 0; i < r.da; i += 4) {
+          const float4 x0_ = *reinterpret_cast<const float4*>(a0 + i), x1_ = *reinterpret_cast<const float4*>(a1 + i);
+          const float4 y0 = *reinterpret_cast<const float4*>(b0 + i), y1 = *reinterpret_cast<const float4*>(b1 + i);
+          p[0][0] = dot4(x0_, y0, p[0][0]);
+          p[0][1] = dot4(x0_, y1, p[0][1]);
+          p[1][0] = dot4(x1_, y0, p[1][0]);
+          p[1][1] = dot4(x1_, y1, p[1][1]);
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
             const int i = 2 * ty + u, j = tx + 16 * w, gap = REV ? j - i : i - j;
-            sp[i * (SC + 1) + j] = gap >= 0 && i < cn && j < cn ? r.w_intra * p[u][w] * lam[gap] : 0.f;
+            sp[i * SPLD + j] = gap >= 0 && i < cn && j < cn ? r.w_intra * p[u][w] * lam[gap] : 0.f;
           }
         if (g == 0 || r.na > 1) {
           o[0] = o[1] = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int i = 0; i < r.da; ++i) {
-            const float a0 = sa[(2 * ty) * ld + i], a1 = sa[(2 * ty + 1) * ld + i];
-            const float4 x = *reinterpret_cast<const float4*>(sx + i * SCOL + tx * 4);
-            o[0].x = fmaf(a0, x.x, o[0].x); o[0].y = fmaf(a0, x.y, o[0].y); o[0].z = fmaf(a0, x.z, o[0].z); o[0].w = fmaf(a0, x.w, o[0].w);
-            o[1].x = fmaf(a1, x.x, o[1].x); o[1].y = fmaf(a1, x.y, o[1].y); o[1].z = fmaf(a1, x.z, o[1].z); o[1].w = fmaf(a1, x.w, o[1].w);
+          const float* x = sx + tx * 4;
+          for (int i = 0; i < r.da; i += 4) {
+            const float4 u0 = *reinterpret_cast<const float4*>(a0 + i), u1 = *reinterpret_cast<const float4*>(a1 + i);
+            const float4 s0 = *reinterpret_cast<const float4*>(x + i * SCOL), s1 = *reinterpret_cast<const float4*>(x + (i + 1) * SCOL),
+                         s2 = *reinterpret_cast<const float4*>(x + (i + 2) * SCOL), s3 = *reinterpret_cast<const float4*>(x + (i + 3) * SCOL);
+            axpy4(u0.x, s0, o[0]); axpy4(u0.y, s1, o[0]); axpy4(u0.z, s2, o[0]); axpy4(u0.w, s3, o[0]);
+            axpy4(u1.x, s0, o[1]); axpy4(u1.y, s1, o[1]); axpy4(u1.z, s2, o[1]); axpy4(u1.w, s3, o[1]);
           }
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
@@ -219,13 +244,13 @@ __global__ void __launch_bounds__(SIMT_THREADS)
           }
         }
         __syncthreads();
-        for (int j = 0; j < cn; ++j) {
-          const float4 v = *reinterpret_cast<const float4*>(sc + j * SCOL + tx * 4);
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const float w = sp[(2 * ty + u) * (SC + 1) + j];
-            o[u].x = fmaf(w, v.x, o[u].x); o[u].y = fmaf(w, v.y, o[u].y); o[u].z = fmaf(w, v.z, o[u].z); o[u].w = fmaf(w, v.w, o[u].w);
-          }
+        const float *p0 = sp + (2 * ty) * SPLD, *p1 = p0 + SPLD, *v = sc + tx * 4;
+        for (int j = 0; j < cn; j += 4) {       // rows past the sequence are 0
+          const float4 u0 = *reinterpret_cast<const float4*>(p0 + j), u1 = *reinterpret_cast<const float4*>(p1 + j);
+          const float4 s0 = *reinterpret_cast<const float4*>(v + j * SCOL), s1 = *reinterpret_cast<const float4*>(v + (j + 1) * SCOL),
+                       s2 = *reinterpret_cast<const float4*>(v + (j + 2) * SCOL), s3 = *reinterpret_cast<const float4*>(v + (j + 3) * SCOL);
+          axpy4(u0.x, s0, o[0]); axpy4(u0.y, s1, o[0]); axpy4(u0.z, s2, o[0]); axpy4(u0.w, s3, o[0]);
+          axpy4(u1.x, s0, o[1]); axpy4(u1.y, s1, o[1]); axpy4(u1.z, s2, o[1]); axpy4(u1.w, s3, o[1]);
         }
         if (r.na > 1 || g == groups - 1) {
 #pragma unroll
@@ -240,16 +265,22 @@ __global__ void __launch_bounds__(SIMT_THREADS)
       }
       if (r.nb > 1 || g == groups - 1) {      // the state: its old value has been used by every reader of this chunk
         const float keep = r.nb > 1 && g > 0 ? 1.f : lam[cn];
-        for (int i = ty; i < r.da; i += 16) {
-          float4 s = *reinterpret_cast<const float4*>(sx + i * SCOL + tx * 4), acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = 4 * ty; i < r.da; i += 64) {
+          float4 acc[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
           for (int j = 0; j < cn; ++j) {
-            const float w = sb[j * ld + i] * lam[REV ? j + 1 : cn - 1 - j];
-            const float4 v = *reinterpret_cast<const float4*>(sc + j * SCOL + tx * 4);
-            acc.x = fmaf(w, v.x, acc.x); acc.y = fmaf(w, v.y, acc.y); acc.z = fmaf(w, v.z, acc.z); acc.w = fmaf(w, v.w, acc.w);
+            const float4 w4 = *reinterpret_cast<const float4*>(sb + j * ld + i), v = *reinterpret_cast<const float4*>(sc + j * SCOL + tx * 4);
+            const float w = lam[REV ? j + 1 : cn - 1 - j];
+            axpy4(w4.x * w, v, acc[0]); axpy4(w4.y * w, v, acc[1]); axpy4(w4.z * w, v, acc[2]); axpy4(w4.w * w, v, acc[3]);
           }
-          s.x = fmaf(r.w_up, acc.x, keep * s.x); s.y = fmaf(r.w_up, acc.y, keep * s.y);
-          s.z = fmaf(r.w_up, acc.z, keep * s.z); s.w = fmaf(r.w_up, acc.w, keep * s.w);
-          *reinterpret_cast<float4*>(sx + i * SCOL + tx * 4) = s;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            float4& s = *reinterpret_cast<float4*>(sx + (i + k) * SCOL + tx * 4);
+            s = make_float4(fmaf(r.w_up, acc[k].x, keep * s.x), fmaf(r.w_up, acc[k].y, keep * s.y), fmaf(r.w_up, acc[k].z, keep * s.z),
+                            fmaf(r.w_up, acc[k].w, keep * s.w));
+          }
         }
       }
     }
@@ -321,9 +352,13 @@ int step_launch(const LinSeqs& q, const LinRole& r, const LinPool& pool, cudaStr
   const int blocks_v = (r.dc + STEP_COLS - 1) / STEP_COLS;
   const long long grid = (long long)q.batch * q.nhk * blocks_v;
   FA_CHECK_ARG(grid < (1ll << 31), "linear attention: %lld blocks", grid);
-  if (r.da <= 64) lin_step_kernel<T, 4><<<(int)grid, STEP_THREADS, 0, st>>>(q, r, pool, blocks_v);
-  else if (r.da <= 128) lin_step_kernel<T, 8><<<(int)grid, STEP_THREADS, 0, st>>>(q, r, pool, blocks_v);
-  else lin_step_kernel<T, 16><<<(int)grid, STEP_THREADS, 0, st>>>(q, r, pool, blocks_v);
+  const auto go = [&](auto one, auto four) {
+    if (r.na == 1) one<<<(int)grid, STEP_THREADS, 0, st>>>(q, r, pool, blocks_v);
+    else four<<<(int)grid, STEP_THREADS, 0, st>>>(q, r, pool, blocks_v);
+  };
+  if (r.da <= 64) go(lin_step_kernel<T, 4, 1>, lin_step_kernel<T, 4, 4>);
+  else if (r.da <= 128) go(lin_step_kernel<T, 8, 1>, lin_step_kernel<T, 8, 4>);
+  else go(lin_step_kernel<T, 16, 1>, lin_step_kernel<T, 16, 4>);
   count_launch();
   return cuda_status(cudaGetLastError(), "linear attention (recurrent) launch");
 }
@@ -392,7 +427,7 @@ extern "C" FA_API long long fa_linear_plan(int batch, int S, long long total, in
   const long long tokens = total > 0 && total < (long long)batch * S ? std::max(1ll, total / batch) : S;
   const bool tc = dtype != FA_DTYPE_F32 && dk <= 128 && dv <= 128;
   const long long chunks = (tokens + 127) / 128, sms = num_sms();
-  long long best = 1;
+  long long best = 1, unit = 128;
   if (tc) {
     // Blocks run one to an SM.  In units of a chunk's time in the output kernel: as many chunks as the fullest SM walks, 3 for
     // each block's start, and with more than one segment the states kernel, which takes less than half of that, and 4 for it and the join.
@@ -403,12 +438,16 @@ extern "C" FA_API long long fa_linear_plan(int batch, int S, long long total, in
       if (cost < least) least = cost, best = n;
     }
   } else {
-    // Two blocks to an SM, no segment shorter than 128 tokens (each costs a state written and read again, and its keys and
-    // values read twice).
-    best = std::max(1ll, std::min(chunks, 2 * sms / std::max(1ll, states * ((dv + 63) / 64))));
+    // As many segments as give every SM four blocks, none shorter than a chunk of 32 tokens (each costs a state written and read
+    // again, and its keys and values read twice): 8 heads x 512 tokens took 5 us a kernel in 16 segments and 15 in 4.
+    const long long cols = (dv + 63) / 64, small = (tokens + 31) / 32;
+    const long long n = std::max(1ll, std::min(small, 4 * sms / std::max(1ll, states * cols)));
+    unit = 32;
+    best = n;
   }
-  long long len = (chunks + best - 1) / best * 128;
-  if (len >= S) len = (S + 127ll) / 128 * 128;
+  const long long units = (tokens + unit - 1) / unit;
+  long long len = (units + best - 1) / best * unit;
+  if (len >= S) len = (S + unit - 1ll) / unit * unit;
   *seg_len = (int)std::min(len, 1ll << 30);
   *nseg = (int)((S + (long long)*seg_len - 1) / *seg_len);
   return *nseg > 1 || tc ? states * *nseg * dk * dv : 0;

@@ -29,12 +29,20 @@ template <typename T, int U> struct alignas(U * sizeof(T) == 16 ? 16 : sizeof(T)
 // and written element by element
 template <typename T, int U, bool INTER, int TOK>
 __global__ void __launch_bounds__(THREADS) rotary_qk_kernel(const FaRotaryQkParams p, const long long tokens) {
-  __shared__ float2 sce[TOK][MAX_PAIRS];
+  __shared__ __align__(16) float2 sce[TOK][MAX_PAIRS];
+  __shared__ long long off[TOK][4];        // the tokens' rows in q, k and the outputs
   const int half = p.rot_dim / 2;
   const long long first = (long long)blockIdx.x * TOK;
   const int nt = (int)min((long long)TOK, tokens - first);
+  if (threadIdx.x < nt) {
+    const long long row = first + threadIdx.x, z = row / p.seqlen, s = row - z * p.seqlen;
+    off[threadIdx.x][0] = z * p.sQ.b + s * p.sQ.s;
+    off[threadIdx.x][1] = z * p.sK.b + s * p.sK.s;
+    off[threadIdx.x][2] = z * p.sQo.b + s * p.sQo.s;
+    off[threadIdx.x][3] = z * p.sKo.b + s * p.sKo.s;
+  }
   for (int e = threadIdx.x; e < nt * half; e += THREADS) {
-    const int t = e / half, i = e % half;
+    const int t = e / half, i = e - t * half;
     const long long row = first + t;
     long long pos;
     if (p.positions) {
@@ -68,37 +76,39 @@ __global__ void __launch_bounds__(THREADS) rotary_qk_kernel(const FaRotaryQkPara
   const bool copy_q = p.q_out != p.q, copy_k = p.k_out != p.k;
   constexpr int C = U * sizeof(T) == 16 ? U : 1;      // elements of a copied unit
   const int copied = copy_q || copy_k ? (p.dim - p.rot_dim) / C : 0;
-  const int per = turning + copied, all = nt * heads * per;
+  const int per = turning + copied;
   using V = Unit<T, U>;
-#pragma unroll 4
-  for (int e = threadIdx.x; e < all; e += THREADS) {
-    const int w = e % per, h = e / per % heads, t = e / per / heads;
-    const long long row = first + t, z = row / p.seqlen, s = row - z * p.seqlen;
-    const bool is_q = h < p.heads_q;
-    const FaStrides& si = is_q ? p.sQ : p.sK;
-    const FaStrides& so = is_q ? p.sQo : p.sKo;
-    const int hh = is_q ? h : h - p.heads_q;
-    const T* x = (const T*)(is_q ? p.q : p.k) + z * si.b + s * si.s + hh * si.h;
-    T* o = (T*)(is_q ? p.q_out : p.k_out) + z * so.b + s * so.s + hh * so.h;
-    if (w >= turning) {
-      const int d = p.rot_dim + (w - turning) * C;
-      if (is_q ? copy_q : copy_k) *reinterpret_cast<Unit<T, C>*>(o + d) = *reinterpret_cast<const Unit<T, C>*>(x + d);
-      continue;
-    }
-    const float2* ce = sce[t];
-    if constexpr (INTER) {
-      const V v = *reinterpret_cast<const V*>(x + w * U);
-      V r;
+  // a thread keeps its unit of the head and steps over heads and tokens
+  const int side = max(1, THREADS / per), lane_h = threadIdx.x / per;
+  for (int w = threadIdx.x - lane_h * per; w < per; w += THREADS) {
+    if (lane_h >= side) break;
+#pragma unroll 2
+    for (int e = lane_h; e < nt * heads; e += side) {
+      const int t = e / heads, h = e - t * heads;
+      const bool is_q = h < p.heads_q;
+      const int hh = is_q ? h : h - p.heads_q;
+      const T* x = (const T*)(is_q ? p.q : p.k) + off[t][is_q ? 0 : 1] + hh * (is_q ? p.sQ.h : p.sK.h);
+      T* o = (T*)(is_q ? p.q_out : p.k_out) + off[t][is_q ? 2 : 3] + hh * (is_q ? p.sQo.h : p.sKo.h);
+      if (w >= turning) {
+        const int d = p.rot_dim + (w - turning) * C;
+        if (is_q ? copy_q : copy_k) *reinterpret_cast<Unit<T, C>*>(o + d) = *reinterpret_cast<const Unit<T, C>*>(x + d);
+        continue;
+      }
+      const float2* ce = sce[t];
+      if constexpr (INTER) {
+        const V v = *reinterpret_cast<const V*>(x + w * U);
+        V r;
 #pragma unroll
-      for (int i = 0; i < U; i += 2) turn<T>(v.e[i], v.e[i + 1], ce[(w * U + i) / 2], r.e[i], r.e[i + 1]);
-      *reinterpret_cast<V*>(o + w * U) = r;
-    } else {
-      const V a = *reinterpret_cast<const V*>(x + w * U), b = *reinterpret_cast<const V*>(x + half + w * U);
-      V ra, rb;
+        for (int i = 0; i < U; i += 2) turn<T>(v.e[i], v.e[i + 1], ce[(w * U + i) / 2], r.e[i], r.e[i + 1]);
+        *reinterpret_cast<V*>(o + w * U) = r;
+      } else {
+        const V a = *reinterpret_cast<const V*>(x + w * U), b = *reinterpret_cast<const V*>(x + half + w * U);
+        V ra, rb;
 #pragma unroll
-      for (int i = 0; i < U; ++i) turn<T>(a.e[i], b.e[i], ce[w * U + i], ra.e[i], rb.e[i]);
-      *reinterpret_cast<V*>(o + w * U) = ra;
-      *reinterpret_cast<V*>(o + half + w * U) = rb;
+        for (int i = 0; i < U; ++i) turn<T>(a.e[i], b.e[i], ce[w * U + i], ra.e[i], rb.e[i]);
+        *reinterpret_cast<V*>(o + w * U) = ra;
+        *reinterpret_cast<V*>(o + half + w * U) = rb;
+      }
     }
   }
 }
