@@ -16,13 +16,13 @@ __device__ int g_lin_error = 0;
 // (a 128-byte line of each row) in registers, so that a state of 128 columns gives four blocks and small batches still spread;
 // all its loads are issued before anything else is looked at, the other sequences' slots among them.
 // =====================================================================================
-constexpr int STEP_THREADS = 128, STEP_COLS = 32;
+constexpr int STEP_THREADS = 128, STEP_COLS = 32, STEP_BATCH = 4;
 
 // ROWS = rows of the state a thread holds: dk <= 16 * ROWS; G = query heads of a group that are summed together
 template <typename T, int ROWS, int G>
-__global__ void __launch_bounds__(STEP_THREADS, ROWS > 8 ? 3 : G == 1 ? 6 : 5)
+__global__ void __launch_bounds__(STEP_THREADS, ROWS > 8 ? 3 : 6)
     lin_step_kernel(const LinSeqs q, const LinRole r, const LinPool pool, const int blocks_v) {
-  __shared__ float sk[256], sq[G][256], sred[4][G][STEP_COLS];
+  __shared__ __align__(16) float sk[STEP_BATCH][256], sq[STEP_BATCH][G][256], sv[STEP_BATCH][STEP_COLS], sred[STEP_BATCH][4][G][STEP_COLS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int vb = blockIdx.x % blocks_v, hz = blockIdx.x / blocks_v, h = hz % q.nhk, z = hz / q.nhk;
   const int named = pool.index ? pool.index[z] : z;
@@ -51,74 +51,93 @@ __global__ void __launch_bounds__(STEP_THREADS, ROWS > 8 ? 3 : G == 1 ? 6 : 5)
     }
     return;
   }
-  for (int t = 0; t < span.len; ++t) {
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (mine) {
-      const T* cr = c + t * r.sc.s + col;
-      v = make_float4(Elem<T>::to_f(cr[0]), Elem<T>::to_f(cr[1]), Elem<T>::to_f(cr[2]), Elem<T>::to_f(cr[3]));
-    }
+  // Tokens in batches: their rows come in together, and their sums are joined together (one by one a token cost 5 us, most of it
+  // waiting).  Groups of more than G query heads take one token at a time.
+  const int batch = r.na <= G ? STEP_BATCH : 1;
+  for (int t0 = 0; t0 < span.len; t0 += batch) {
+    const int nt = min(batch, span.len - t0);
     for (int g0 = 0; g0 < r.na; g0 += G) {
       const int ng = min(G, r.na - g0);
-      if (t > 0 || g0 > 0) __syncthreads();
-      if (g0 == 0)
-        for (int e = tid; e < r.da; e += STEP_THREADS) sk[e] = Elem<T>::to_f(b[t * r.sb.s + e]);
+      if (t0 > 0 || g0 > 0) __syncthreads();
+      if (g0 == 0 && tid < nt * STEP_COLS) {
+        const int cc = vb * STEP_COLS + tid % STEP_COLS;
+        sv[tid / STEP_COLS][tid % STEP_COLS] = cc < r.dc ? Elem<T>::to_f(c[(t0 + tid / STEP_COLS) * r.sc.s + cc]) : 0.f;
+      }
+      for (int e = tid; e < r.da; e += STEP_THREADS) {      // all rows of the batch in flight at once
+        T gk[STEP_BATCH], gq[STEP_BATCH][G];
 #pragma unroll
-      for (int g = 0; g < G; ++g)
-        if (g < ng)
-          for (int e = tid; e < r.da; e += STEP_THREADS) sq[g][e] = Elem<T>::to_f(a[t * r.sa.s + (g0 + g) * r.sa.h + e]);
-      __syncthreads();
-      float4 o[G];
-#pragma unroll
-      for (int g = 0; g < G; ++g) o[g] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int i = 0; i < ROWS; ++i) {
-        const int row = row0 + 16 * i;
-        if (row < r.da) {
-          if (g0 == 0) {
-            const float k = sk[row];
-            x[i].x = fmaf(lam, x[i].x, k * v.x);
-            x[i].y = fmaf(lam, x[i].y, k * v.y);
-            x[i].z = fmaf(lam, x[i].z, k * v.z);
-            x[i].w = fmaf(lam, x[i].w, k * v.w);
-          }
+        for (int tt = 0; tt < STEP_BATCH; ++tt) {
+          if (tt >= nt) break;
+          if (g0 == 0) gk[tt] = b[(t0 + tt) * r.sb.s + e];
 #pragma unroll
           for (int g = 0; g < G; ++g)
-            if (g < ng) {
-              const float w = sq[g][row];
-              o[g].x = fmaf(w, x[i].x, o[g].x);
-              o[g].y = fmaf(w, x[i].y, o[g].y);
-              o[g].z = fmaf(w, x[i].z, o[g].z);
-              o[g].w = fmaf(w, x[i].w, o[g].w);
-            }
+            if (g < ng) gq[tt][g] = a[(t0 + tt) * r.sa.s + (g0 + g) * r.sa.h + e];
+        }
+#pragma unroll
+        for (int tt = 0; tt < STEP_BATCH; ++tt) {
+          if (tt >= nt) break;
+          if (g0 == 0) sk[tt][e] = Elem<T>::to_f(gk[tt]);
+#pragma unroll
+          for (int g = 0; g < G; ++g)
+            if (g < ng) sq[tt][g][e] = Elem<T>::to_f(gq[tt][g]);
         }
       }
-      // the state is on its way back before the sums are joined
-      if (t == span.len - 1 && g0 + G >= r.na && pool.out && mine) {
+      __syncthreads();
+      for (int tt = 0; tt < nt; ++tt) {
+        const float4 v = *reinterpret_cast<const float4*>(&sv[tt][(tid & 7) * 4]);
+        float4 o[G];
+#pragma unroll
+        for (int g = 0; g < G; ++g) o[g] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int i = 0; i < ROWS; ++i) {
           const int row = row0 + 16 * i;
-          if (row < r.da) __stcs(reinterpret_cast<float4*>(pool.out + at + (long long)row * r.dc), x[i]);
-        }
-      }
-      // lanes of one column group differ in bits 3 and 4; then the four warps
+          if (row < r.da) {
+            if (g0 == 0) {
+              const float k = sk[tt][row];
+              x[i].x = fmaf(lam, x[i].x, k * v.x);
+              x[i].y = fmaf(lam, x[i].y, k * v.y);
+              x[i].z = fmaf(lam, x[i].z, k * v.z);
+              x[i].w = fmaf(lam, x[i].w, k * v.w);
+            }
 #pragma unroll
-      for (int g = 0; g < G; ++g)
-        if (g < ng) {
-#pragma unroll
-          for (int m = 8; m <= 16; m *= 2) {
-            o[g].x += __shfl_xor_sync(0xffffffffu, o[g].x, m);
-            o[g].y += __shfl_xor_sync(0xffffffffu, o[g].y, m);
-            o[g].z += __shfl_xor_sync(0xffffffffu, o[g].z, m);
-            o[g].w += __shfl_xor_sync(0xffffffffu, o[g].w, m);
+            for (int g = 0; g < G; ++g)
+              if (g < ng) {
+                const float w = sq[tt][g][row];
+                o[g].x = fmaf(w, x[i].x, o[g].x);
+                o[g].y = fmaf(w, x[i].y, o[g].y);
+                o[g].z = fmaf(w, x[i].z, o[g].z);
+                o[g].w = fmaf(w, x[i].w, o[g].w);
+              }
           }
-          if (lane < 8) *reinterpret_cast<float4*>(&sred[warp][g][lane * 4]) = o[g];
         }
+        // the state is on its way back before the sums are joined
+        if (t0 + tt == span.len - 1 && g0 + G >= r.na && pool.out && mine) {
+#pragma unroll
+          for (int i = 0; i < ROWS; ++i) {
+            const int row = row0 + 16 * i;
+            if (row < r.da) __stcs(reinterpret_cast<float4*>(pool.out + at + (long long)row * r.dc), x[i]);
+          }
+        }
+        // lanes of one column group differ in bits 3 and 4; then the four warps
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+          if (g < ng) {
+#pragma unroll
+            for (int m = 8; m <= 16; m *= 2) {
+              o[g].x += __shfl_xor_sync(0xffffffffu, o[g].x, m);
+              o[g].y += __shfl_xor_sync(0xffffffffu, o[g].y, m);
+              o[g].z += __shfl_xor_sync(0xffffffffu, o[g].z, m);
+              o[g].w += __shfl_xor_sync(0xffffffffu, o[g].w, m);
+            }
+            if (lane < 8) *reinterpret_cast<float4*>(&sred[tt][warp][g][lane * 4]) = o[g];
+          }
+      }
       __syncthreads();
-      for (int e = tid; e < ng * STEP_COLS; e += STEP_THREADS) {
-        const int g = e / STEP_COLS, cc = e % STEP_COLS;
+      for (int e = tid; e < nt * ng * STEP_COLS; e += STEP_THREADS) {
+        const int cc = e % STEP_COLS, g = e / STEP_COLS % ng, tt = e / STEP_COLS / ng;
         if (vb * STEP_COLS + cc < r.dc)
-          out[t * r.so.s + (g0 + g) * r.so.h + vb * STEP_COLS + cc] =
-              Elem<T>::from_f(r.w_inter * (sred[0][g][cc] + sred[1][g][cc] + sred[2][g][cc] + sred[3][g][cc]));
+          out[(t0 + tt) * r.so.s + (g0 + g) * r.so.h + vb * STEP_COLS + cc] =
+              Elem<T>::from_f(r.w_inter * (sred[tt][0][g][cc] + sred[tt][1][g][cc] + sred[tt][2][g][cc] + sred[tt][3][g][cc]));
       }
     }
   }

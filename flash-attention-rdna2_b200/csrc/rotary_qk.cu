@@ -28,7 +28,7 @@ template <typename T, int U> struct alignas(U * sizeof(T) == 16 ? 16 : sizeof(T)
 // U: elements of a 16-byte unit, or 1 (2 where the pairs are neighbours) for rows that do not lie on 16 bytes: those are read
 // and written element by element
 template <typename T, int U, bool INTER, int TOK>
-__global__ void __launch_bounds__(THREADS) rotary_qk_kernel(const FaRotaryQkParams p, const long long tokens) {
+__global__ void __launch_bounds__(THREADS, 5) rotary_qk_kernel(const FaRotaryQkParams p, const long long tokens) {
   __shared__ __align__(16) float2 sce[TOK][MAX_PAIRS];
   __shared__ long long off[TOK][4];        // the tokens' rows in q, k and the outputs
   const int half = p.rot_dim / 2;
@@ -70,46 +70,82 @@ __global__ void __launch_bounds__(THREADS) rotary_qk_kernel(const FaRotaryQkPara
     sce[t][i] = make_float2(p.factor * c, (p.inverse ? -p.factor : p.factor) * s);
   }
   __syncthreads();
-  // a head's units: first those that turn, then (unless q and k stay in place) those that are copied
-  const int turning = INTER ? p.rot_dim / U : half / U;
   const int heads = p.heads_q + p.heads_k;
-  const bool copy_q = p.q_out != p.q, copy_k = p.k_out != p.k;
-  constexpr int C = U * sizeof(T) == 16 ? U : 1;      // elements of a copied unit
-  const int copied = copy_q || copy_k ? (p.dim - p.rot_dim) / C : 0;
-  const int per = turning + copied;
   using V = Unit<T, U>;
-  // a thread keeps its unit of the head and steps over heads and tokens
-  const int side = max(1, THREADS / per), lane_h = threadIdx.x / per;
-  for (int w = threadIdx.x - lane_h * per; w < per; w += THREADS) {
-    if (lane_h >= side) break;
-#pragma unroll 2
-    for (int e = lane_h; e < nt * heads; e += side) {
-      const int t = e / heads, h = e - t * heads;
-      const bool is_q = h < p.heads_q;
-      const int hh = is_q ? h : h - p.heads_q;
-      const T* x = (const T*)(is_q ? p.q : p.k) + off[t][is_q ? 0 : 1] + hh * (is_q ? p.sQ.h : p.sK.h);
-      T* o = (T*)(is_q ? p.q_out : p.k_out) + off[t][is_q ? 2 : 3] + hh * (is_q ? p.sQo.h : p.sKo.h);
-      if (w >= turning) {
-        const int d = p.rot_dim + (w - turning) * C;
-        if (is_q ? copy_q : copy_k) *reinterpret_cast<Unit<T, C>*>(o + d) = *reinterpret_cast<const Unit<T, C>*>(x + d);
-        continue;
-      }
-      const float2* ce = sce[t];
-      if constexpr (INTER) {
-        const V v = *reinterpret_cast<const V*>(x + w * U);
-        V r;
+  const auto rows = [&](int t, int h, const T*& x, T*& o) {
+    const bool is_q = h < p.heads_q;
+    const int hh = is_q ? h : h - p.heads_q;
+    x = (const T*)(is_q ? p.q : p.k) + off[t][is_q ? 0 : 1] + hh * (is_q ? p.sQ.h : p.sK.h);
+    o = (T*)(is_q ? p.q_out : p.k_out) + off[t][is_q ? 2 : 3] + hh * (is_q ? p.sQo.h : p.sKo.h);
+    return is_q;
+  };
+  // A thread keeps its unit w of the head and steps over heads and tokens without a division; FLY units are in flight at a time
+  constexpr int FLY = 2;
+  {
+    const int turning = INTER ? p.rot_dim / U : half / U;      // units of a head that turn
+    const int side = max(1, THREADS / turning), mine = threadIdx.x / turning;      // heads at a time
+    for (int w = threadIdx.x - mine * turning; w < turning && mine < side; w += THREADS) {
+      int t = mine / heads, h = mine - t * heads;
+      while (t < nt) {
+        V a[FLY], b[FLY];
+        T* to[FLY];
+        const float2* ce[FLY];
 #pragma unroll
-        for (int i = 0; i < U; i += 2) turn<T>(v.e[i], v.e[i + 1], ce[(w * U + i) / 2], r.e[i], r.e[i + 1]);
-        *reinterpret_cast<V*>(o + w * U) = r;
-      } else {
-        const V a = *reinterpret_cast<const V*>(x + w * U), b = *reinterpret_cast<const V*>(x + half + w * U);
-        V ra, rb;
+        for (int k = 0; k < FLY; ++k) {
+          to[k] = nullptr;
+          if (t >= nt) break;
+          const T* x;
+          rows(t, h, x, to[k]);
+          x += w * U;
+          to[k] += w * U;
+          ce[k] = sce[t] + (INTER ? w * U / 2 : w * U);
+          a[k] = *reinterpret_cast<const V*>(x);
+          if constexpr (!INTER) b[k] = *reinterpret_cast<const V*>(x + half);
+          for (h += side; h >= heads; h -= heads) ++t;
+        }
 #pragma unroll
-        for (int i = 0; i < U; ++i) turn<T>(a.e[i], b.e[i], ce[w * U + i], ra.e[i], rb.e[i]);
-        *reinterpret_cast<V*>(o + w * U) = ra;
-        *reinterpret_cast<V*>(o + half + w * U) = rb;
+        for (int k = 0; k < FLY; ++k) {
+          if (!to[k]) break;
+          if constexpr (INTER) {
+            V r;
+#pragma unroll
+            for (int i = 0; i < U; i += 2) turn<T>(a[k].e[i], a[k].e[i + 1], ce[k][i / 2], r.e[i], r.e[i + 1]);
+            *reinterpret_cast<V*>(to[k]) = r;
+          } else {
+            V ra, rb;
+#pragma unroll
+            for (int i = 0; i < U; ++i) turn<T>(a[k].e[i], b[k].e[i], ce[k][i], ra.e[i], rb.e[i]);
+            *reinterpret_cast<V*>(to[k]) = ra;
+            *reinterpret_cast<V*>(to[k] + half) = rb;
+          }
+        }
       }
     }
+  }
+  // the dims past rot_dim, where q or k do not stay in place
+  const bool copy_q = p.q_out != p.q, copy_k = p.k_out != p.k;
+  if (!copy_q && !copy_k) return;
+  constexpr int C = U * sizeof(T) == 16 ? U : 1;      // elements of a copied unit
+  using W = Unit<T, C>;
+  const int copied = (p.dim - p.rot_dim) / C, all = nt * heads * copied;
+  for (int e0 = threadIdx.x; e0 < all; e0 += FLY * THREADS) {
+    W a[FLY];
+    T* to[FLY];
+#pragma unroll
+    for (int k = 0; k < FLY; ++k) {
+      const int e = e0 + k * THREADS;
+      to[k] = nullptr;
+      if (e >= all) break;
+      const int ht = e / copied, w = e - ht * copied, t = ht / heads;
+      const T* x;
+      T* o;
+      if (!(rows(t, ht - t * heads, x, o) ? copy_q : copy_k)) continue;
+      to[k] = o + p.rot_dim + w * C;
+      a[k] = *reinterpret_cast<const W*>(x + p.rot_dim + w * C);
+    }
+#pragma unroll
+    for (int k = 0; k < FLY; ++k)
+      if (e0 + k * THREADS < all && to[k]) *reinterpret_cast<W*>(to[k]) = a[k];
   }
 }
 
