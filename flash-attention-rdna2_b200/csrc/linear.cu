@@ -450,14 +450,30 @@ extern "C" FA_API long long fa_linear_plan(int batch, int S, long long total, in
   const long long chunks = (tokens + 127) / 128, sms = num_sms();
   long long best = 1, unit = 128;
   if (tc) {
-    // Blocks run one to an SM.  In units of a chunk's time in the output kernel: as many chunks as the fullest SM walks, 3 for
-    // each block's start, and with more than one segment the states kernel, which takes less than half of that, and 4 for it and the join.
+    // Blocks run one to an SM.  In units of one head's chunk in the output kernel (3 us): a chunk costs its query heads and 0.4 for the
+    // state, a block 2.5 to start, and the states kernel, which more than one segment needs, 0.5 a chunk and 1.5 to start, with
+    // 2 for it and the join.  Blocks of one length run in waves; where lengths differ they fill in, and the longest is what is left over.
+    const double heads = gqa, per_chunk = heads + 0.4;
     double least = 1e30;
-    for (long long n = 1; n <= std::min(chunks, 256ll); ++n) {
-      const double waves = (double)((states * n + sms - 1) / sms), walk = (double)((chunks + n - 1) / n);
-      const double cost = waves * (walk * (n > 1 ? 1.45 : 1.0) + (n > 1 ? 5.0 : 3.0)) + (n > 1 ? 4.0 : 0.0);
+    for (long long n = 1; n <= std::min((S + 127ll) / 128, 1024ll); ++n) {
+      const double walk = (double)(((S + 127ll) / 128 + n - 1) / n);
+      const bool ragged = tokens < S;
+      double cost;
+      if (ragged) {
+        const double blocks = (double)states * ((double)chunks / walk + 0.5) / (double)sms;
+        cost = blocks * 2.5 + (double)(states * chunks) / (double)sms * (per_chunk + (n > 1 ? 0.5 : 0.0)) + walk * per_chunk * 0.5;
+      } else {
+        const double waves = (double)((states * n + sms - 1) / sms);
+        cost = waves * (walk * (per_chunk + (n > 1 ? 0.5 : 0.0)) + (n > 1 ? 4.0 : 2.5)) + (n > 1 ? 2.0 : 0.0);
+      }
       if (cost < least) least = cost, best = n;
+      if (walk <= 1.0) break;
     }
+    unit = 128;
+    const long long whole = (S + 127ll) / 128;
+    *seg_len = (int)std::min((whole + best - 1) / best * 128, 1ll << 30);
+    *nseg = (int)((S + (long long)*seg_len - 1) / *seg_len);
+    return states * *nseg * dk * dv;
   } else {
     // As many segments as give every SM four blocks, none shorter than a chunk of 32 tokens (each costs a state written and read
     // again, and its keys and values read twice): 8 heads x 512 tokens took 5 us a kernel in 16 segments and 15 in 4.
@@ -471,7 +487,7 @@ extern "C" FA_API long long fa_linear_plan(int batch, int S, long long total, in
   if (len >= S) len = (S + unit - 1ll) / unit * unit;
   *seg_len = (int)std::min(len, 1ll << 30);
   *nseg = (int)((S + (long long)*seg_len - 1) / *seg_len);
-  return *nseg > 1 || tc ? states * *nseg * dk * dv : 0;
+  return *nseg > 1 ? states * *nseg * dk * dv : 0;
 }
 
 extern "C" FA_API int fa_linear_launch(const FaLinearParams* pp, int dtype, void* stream) {

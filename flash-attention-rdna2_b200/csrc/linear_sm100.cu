@@ -388,6 +388,9 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             ++nor;
           }
           ok = ok && wait_warp(bar + Bz::A_FULL + 8 * (ca % K::NA), (ca / K::NA) & 1);
+          // P goes first through the pipe: its readers have more to do.  (With several heads of b this may return a phase early,
+          // which changes the order and nothing else.)
+          ok = ok && wait_warp(bar + Bz::P_FULL, t & 1);
           tc_fence_after();
           if (ok && lane == 0) {
             const uint64_t da = desc_k(at), xh = SWAP ? desc_k(st + K::OFF_X) : desc_mn(st + K::OFF_X, D);
@@ -683,13 +686,32 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                 p[2 * i + 1] = __fmul2_rn(p[2 * i + 1], __fmul2_rn(make_float2(blk, blk), make_float2(f.z, f.w)));
               }
             } else {
-              // on the diagonal the exponent runs over both: exp2 of each, which costs less than a table read of each
-              const float from = (float)(REV ? j0 - row : row - j0);
+              // On the diagonal, in pieces of 8 columns: lam^(gap to the piece's far edge), which may be up to lam^-7, times the table's, and what
+              // lies on the other side is masked.  Where lam^-7 could overflow, exp2 of each gap (1200 cycles a block, not 600)
+              const float from = (float)(REV ? j0 - row : row - j0);      // gap of the piece's first column
+              if (g2 > -17.f) {
 #pragma unroll
-              for (int i = 0; i < W / 2; ++i) {
-                const float gap = REV ? from + 2 * i : from - 2 * i, next = REV ? gap + 1.f : gap - 1.f;
-                p[i].x = gap >= 0.f ? p[i].x * (ex2(g2 * gap) * ps) : 0.f;
-                p[i].y = next >= 0.f ? p[i].y * (ex2(g2 * next) * ps) : 0.f;
+                for (int s = 0; s < W / 8; ++s) {
+                  const float edge_gap = REV ? from + 8 * s : from - 8 * s - 7, u = ex2(g2 * edge_gap) * ps;
+                  const float4 w0 = *reinterpret_cast<const float4*>(lamc + (REV ? 0 : 24)), w1 = *reinterpret_cast<const float4*>(lamc + (REV ? 4 : 28));
+                  p[4 * s] = __fmul2_rn(p[4 * s], __fmul2_rn(make_float2(u, u), make_float2(w0.x, w0.y)));
+                  p[4 * s + 1] = __fmul2_rn(p[4 * s + 1], __fmul2_rn(make_float2(u, u), make_float2(w0.z, w0.w)));
+                  p[4 * s + 2] = __fmul2_rn(p[4 * s + 2], __fmul2_rn(make_float2(u, u), make_float2(w1.x, w1.y)));
+                  p[4 * s + 3] = __fmul2_rn(p[4 * s + 3], __fmul2_rn(make_float2(u, u), make_float2(w1.z, w1.w)));
+                }
+                const int gap = REV ? j0 - row : row - j0;
+#pragma unroll
+                for (int i = 0; i < W / 2; ++i) {
+                  if (REV ? gap + 2 * i < 0 : gap < 2 * i) p[i].x = 0.f;
+                  if (REV ? gap + 2 * i + 1 < 0 : gap < 2 * i + 1) p[i].y = 0.f;
+                }
+              } else {
+#pragma unroll
+                for (int i = 0; i < W / 2; ++i) {
+                  const float gap = REV ? from + 2 * i : from - 2 * i, next = REV ? gap + 1.f : gap - 1.f;
+                  p[i].x = gap >= 0.f ? p[i].x * (ex2(g2 * gap) * ps) : 0.f;
+                  p[i].y = next >= 0.f ? p[i].y * (ex2(g2 * next) * ps) : 0.f;
+                }
               }
             }
             if (REV && cn < C) {                  // forward, a row sees no token past its own
