@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         tc_fence_after();
         if (lane == 0) {
           const uint64_t da = desc_k(at), db = desc_k(bt);
-#pragma unroll 1
+#pragma unroll
           for (int k0 = 0; k0 < K::NCH; ++k0)
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk) {
@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         tc_fence_after();
         if (lane == 0) {
           const uint64_t d = desc_mn(ct, C);
-#pragma unroll 1
+#pragma unroll
           for (int k0 = 0; k0 < C / 16; k0 += 4)
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk) {
