@@ -824,9 +824,12 @@ std::tuple<torch::Tensor, torch::Tensor, int64_t, int64_t> linear_fwd(
   p.o = out.data_ptr();
   p.sO = rows_of_heads(out);
   p.keep_states = keep_states ? 1 : 0;
-  const long long floats = fa_linear_plan(p.batch, p.S, p.total, p.NH, p.gqa, p.dk, p.dv, dt_of(q), &p.seg_len, &p.nseg);
-  auto work = torch::empty({floats}, call.decay.options());
-  p.states = floats ? work.data_ptr<float>() : nullptr;
+  torch::Tensor work = call.decay;      // placeholder where no workspace is needed
+  if (keep_states || p.S > FA_LINEAR_STEP_TOKENS) {
+    const long long floats = fa_linear_plan(p.batch, p.S, p.total, p.NH, p.gqa, p.dk, p.dv, dt_of(q), &p.seg_len, &p.nseg);
+    work = torch::empty({floats}, call.decay.options());
+    p.states = floats ? work.data_ptr<float>() : nullptr;
+  }
   if (p.batch > 0) check(fa_linear_launch(&p, dt_of(q), cur_stream(q)), "linear attention");
   return {out, work, p.seg_len, p.nseg};
 }

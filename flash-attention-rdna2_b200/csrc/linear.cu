@@ -411,9 +411,6 @@ bool through_states(const LinSeqs& q, const LinRole& r, const float* out, int dt
 bool dims_ok(int dk, int dv) { return dk > 0 && dv > 0 && dk <= 256 && dv <= 256 && dk % 8 == 0 && dv % 8 == 0; }
 bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
 
-// Up to this many tokens a sequence the recurrent kernel is taken.
-constexpr int STEP_TOKENS = 16;
-
 }  // namespace
 
 namespace fa {
@@ -505,7 +502,7 @@ extern "C" FA_API int fa_linear_launch(const FaLinearParams* pp, int dtype, void
                "linear attention: %lld slots for %d sequences", p.slots, p.batch);
   FA_CHECK_ARG(!p.cu || p.batch > 0 || p.total == 0, "linear attention: %lld packed rows of no sequence", p.total);
   if (p.batch == 0) return FA_OK;
-  const bool step = !p.keep_states && p.S <= STEP_TOKENS;
+  const bool step = !p.keep_states && p.S <= FA_LINEAR_STEP_TOKENS;
   LinSeqs q{p.cu, p.log_decay, p.total, p.batch, p.S, p.NH / p.gqa, 0, 1};
   if (!step) {
     q.seg_len = p.seg_len;

@@ -194,12 +194,11 @@ def apply_rotary_emb_qk(q, k, inv_freq, positions=None, *, seqlen_offsets=0, int
     however far the position; cos and sin are multiplied by factor and applied in fp32 with one rounding at the end (apply_rotary_emb
     rounds tables and products to the inputs' type instead, as torch arithmetic does).  interleaved pairs dims (2i, 2i + 1) instead of
     (i, i + rotary_dim / 2).  inplace writes q and k themselves.  Carries gradients to q and k.  CUDA tensors only."""
-    for x, name in ((q, "q"), (k, "k"), (inv_freq, "inv_freq")):
-        if not x.is_cuda:
-            raise ValueError(f"fable_attn: {name} must be on a CUDA device")
-    if torch.is_grad_enabled() and inv_freq.requires_grad:
+    if not (q.is_cuda and k.is_cuda and inv_freq.is_cuda):
+        raise ValueError("fable_attn: q, k and inv_freq must be on a CUDA device")
+    if inv_freq.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError("apply_rotary_emb_qk: inv_freq carries no gradient; pass inv_freq.detach()")
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
+    if (q.requires_grad or k.requires_grad) and torch.is_grad_enabled():
         if inplace:
             raise RuntimeError("apply_rotary_emb_qk: inplace rotation of a tensor that requires grad")
         return _RotaryQkFn.apply(q, k, inv_freq, positions, seqlen_offsets, bool(interleaved), float(factor))

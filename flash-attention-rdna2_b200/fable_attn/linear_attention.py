@@ -25,9 +25,9 @@ from fable_attn import _C
 
 
 def _check(q, log_decay):
-    if not torch.is_tensor(log_decay):
+    if not isinstance(log_decay, torch.Tensor):
         raise TypeError(f"fable_attn: log_decay must be a tensor of (nheads_k,), got {type(log_decay).__name__}")
-    if torch.is_grad_enabled() and log_decay.requires_grad:
+    if log_decay.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError("fable_attn: log_decay carries no gradient; pass log_decay.detach()")
     if not q.is_cuda:
         raise ValueError("fable_attn: tensors must be on a CUDA device (q.is_cuda is False)")
@@ -103,7 +103,7 @@ def linear_attn_with_state(q, k, v, state, log_decay, scale=None, *, state_indic
     recorded in fable_attn.device_error().  Up to 16 tokens a sequence go through the state one by one; longer ones in
     chunks.  No gradients."""
     _check(q, log_decay)
-    if torch.is_grad_enabled() and any(x.requires_grad for x in (q, k, v, state)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
         raise NotImplementedError("fable_attn: linear_attn_with_state carries no gradients; use linear_attn_func")
     if scale is None:
         scale = q.shape[-1] ** -0.5

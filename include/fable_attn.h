@@ -431,10 +431,12 @@ FA_API int fa_combine_launch(const FaCombineParams* p, void* stream);
  *              seen[z] <= 0 it starts from 0 whatever the slot holds.  A negative slot is padding: its sequence gives 0 and touches
  *              no state.  So does a slot outside the pool, and the later of two sequences of the same slot; these raise
  *              fa_device_error bit 131072.
- *   states     workspace of fa_linear_plan floats, 16-byte aligned (null where that is 0, or with one segment and no state_out).  With keep_states the
- *              chunked kernels run whatever S is, and leave each segment's start state there for fa_linear_backward_launch.
+ *   states     workspace of fa_linear_plan floats, 16-byte aligned (null where that is 0, with one segment and no state_out, and for up to
+ *              FA_LINEAR_STEP_TOKENS tokens, which go through the state one by one).  With keep_states the chunked kernels run
+ *              whatever S is, and leave each segment's start state there for fa_linear_backward_launch.
  * fa_linear_plan: segments of seg_len tokens (nseg for the longest sequence) that run side by side, and the floats of `states`.
  * -------------------------------------------------------------------------------------------*/
+#define FA_LINEAR_STEP_TOKENS 16
 typedef struct FaLinearParams {
   unsigned int struct_size;
   const void *q, *k, *v;
