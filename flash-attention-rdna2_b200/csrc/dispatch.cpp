@@ -868,7 +868,9 @@ std::vector<torch::Tensor> linear_bwd(torch::Tensor dout, torch::Tensor q, torch
   p.dO = d.data_ptr(); p.dQ = dq.data_ptr(); p.dK = dk.data_ptr(); p.dV = dv.data_ptr();
   p.sdO = rows_of_heads(d); p.sdQ = rows_of_heads(dq); p.sdK = rows_of_heads(dk); p.sdV = rows_of_heads(dv);
   p.seg_len = (int)seg_len; p.nseg = (int)nseg;
-  TORCH_CHECK_VALUE(nseg <= 1 || states.numel() == nseg * p.batch * (p.NH / p.gqa) * p.dk * p.dv,
+  const int64_t len = std::max<int64_t>(seg_len, 1);
+  const int64_t slots = nseg == 1 ? p.batch : !call.packed ? nseg * p.batch : p.batch == 1 ? (p.total + len - 1) / len : p.total / len + p.batch;
+  TORCH_CHECK_VALUE(nseg <= 1 || states.numel() == slots * (p.NH / p.gqa) * p.dk * p.dv,
                     "fable_attn: `states` is not this forward's");
   p.states = states.numel() ? states.const_data_ptr<float>() : nullptr;
   p.work = states.numel() ? work.data_ptr<float>() : nullptr;

@@ -43,7 +43,7 @@ __global__ void __launch_bounds__(STEP_THREADS, ROWS > 8 ? 3 : 6)
   const T* b = (const T*)r.b + (q.cu ? 0 : z * r.sb.b) + span.row0 * r.sb.s + (long long)h * r.sb.h;
   const T* c = (const T*)r.c + (q.cu ? 0 : z * r.sc.b) + span.row0 * r.sc.s + (long long)h * r.sc.h;
   T* out = (T*)r.out + (q.cu ? 0 : z * r.so.b) + span.row0 * r.so.s + (long long)h * r.na * r.so.h;
-  if (vb == 0) lin_zero_outside<T>(q, r, z, h * r.na, 0, 1, STEP_THREADS);
+  if (vb == 0) lin_zero_outside<T>(q, r, h * r.na, z, q.batch, STEP_THREADS);
   if (lin_slot(pool, z, STEP_THREADS, &g_lin_error) < 0) {
     for (int e = tid; e < span.len * r.na * STEP_COLS; e += STEP_THREADS) {
       const int cc = vb * STEP_COLS + e % STEP_COLS, g = e / STEP_COLS % r.na, t = e / STEP_COLS / r.na;
@@ -181,13 +181,12 @@ __global__ void __launch_bounds__(SIMT_THREADS)
   float* sp = sx + r.da * SCOL;             // [SC][SPLD]
   float* lam = sp + SC * SPLD;              // lam^n, n <= SC
   const int cb = blockIdx.x % blocks_c;
-  const int n = blockIdx.x / blocks_c % q.nseg;
-  const int h = blockIdx.x / blocks_c / q.nseg % q.nhk, z = blockIdx.x / blocks_c / q.nseg / q.nhk;
+  const int h = blockIdx.x / blocks_c % q.nhk, seg = blockIdx.x / blocks_c / q.nhk;
   const int c0 = cb * SCOL;
-  if (!STATES && cb == 0) lin_zero_outside<T>(q, r, z, h * r.na, n, q.nseg, SIMT_THREADS);
-  const LinSpan span = lin_span(q, z);
-  int t0, t1;
-  lin_segment(q, span.len, n, t0, t1);
+  if (!STATES && cb == 0) lin_zero_outside<T>(q, r, h * r.na, seg, q.slots, SIMT_THREADS);
+  int z, t0, t1;
+  const LinSpan span = lin_segment(q, seg, z, t0, t1);
+  if (t1 <= t0 && (STATES || ws)) return;
   const int slot = STATES ? z : lin_slot(pool, z, SIMT_THREADS, &g_lin_error);
   T* out = (T*)r.out + (q.cu ? 0 : z * r.so.b) + span.row0 * r.so.s + (long long)h * r.na * r.so.h;
   const T* a = (const T*)r.a + (q.cu ? 0 : z * r.sa.b) + span.row0 * r.sa.s + (long long)h * r.na * r.sa.h;
@@ -202,7 +201,7 @@ __global__ void __launch_bounds__(SIMT_THREADS)
   const float g2 = lin_log2_decay(q.log_decay, h);
   for (int e = tid; e <= SC; e += SIMT_THREADS) lam[e] = lin_power(g2, e);
   // the state that enters the segment
-  const long long per = (long long)r.da * r.dc, segs = ((long long)z * q.nhk + h) * q.nseg + n;
+  const long long per = (long long)r.da * r.dc, segs = (long long)seg * q.nhk + h;
   const float* x0 = nullptr;
   if (!STATES) {
     if (ws) x0 = ws + segs * per;
@@ -330,21 +329,20 @@ __global__ void __launch_bounds__(256) lin_join_kernel(const LinSeqs q, float* w
   if (slot < 0 || e >= per4) return;
   const LinSpan span = lin_span(q, z);
   const float g2 = lin_log2_decay(q.log_decay, h);
-  const int real = min(q.nseg, max(1, (span.len + q.seg_len - 1) / q.seg_len));
-  float4* w = reinterpret_cast<float4*>(ws) + (long long)blockIdx.x * q.nseg * per4 + e;
+  const int real = max(1, lin_segments(q, span.len));
+  const long long step = (long long)q.nhk * per4;      // from one segment's state to the next
+  float4* w = reinterpret_cast<float4*>(ws) + lin_first_slot(q, z, span.row0) * step + (long long)h * per4 + e;
   const long long at = ((long long)slot * q.nhk + h) * per4 + e;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
   if (pool.in && !(pool.seen && pool.seen[z] <= 0)) x = reinterpret_cast<const float4*>(pool.in)[at];
   const auto seg = [&](int m) { return REV ? real - 1 - m : m; };
-  float4 u = span.len > 0 ? w[(long long)seg(0) * per4] : make_float4(0.f, 0.f, 0.f, 0.f);
+  float4 u = span.len > 0 ? w[seg(0) * step] : make_float4(0.f, 0.f, 0.f, 0.f);
   for (int m = 0; m < real; ++m) {
     const int n = seg(m);
-    int t0, t1;
-    lin_segment(q, span.len, n, t0, t1);
     float4 next = u;
-    if (m + 1 < real) next = w[(long long)seg(m + 1) * per4];
-    w[(long long)n * per4] = x;
-    const float keep = lin_power(g2, t1 - t0);
+    if (m + 1 < real) next = w[seg(m + 1) * step];
+    w[n * step] = x;
+    const float keep = lin_power(g2, n == real - 1 ? span.len - n * q.seg_len : q.seg_len);
     x.x = fmaf(keep, x.x, u.x); x.y = fmaf(keep, x.y, u.y); x.z = fmaf(keep, x.z, u.z); x.w = fmaf(keep, x.w, u.w);
     u = next;
   }
@@ -355,8 +353,8 @@ template <typename T>
 int simt_launch(const LinSeqs& q, const LinRole& r, bool rev, bool states, const float* ws, float* ws_out, const LinPool& pool,
                 cudaStream_t st) {
   const int bytes = simt_smem_floats(r.da) * 4, blocks_c = (r.dc + SCOL - 1) / SCOL;
-  const long long grid = (long long)q.batch * q.nhk * q.nseg * blocks_c;
-  FA_CHECK_ARG(grid < (1ll << 31), "linear attention: %lld blocks", grid);
+  const long long grid = (long long)q.slots * q.nhk * blocks_c;
+  FA_CHECK_ARG(grid < (1ll << 31) && (long long)q.batch * q.nhk < (1ll << 31), "linear attention: %lld blocks", grid);
   const auto go = [&](auto kernel, unsigned long long* done) -> int {
     if (int rc = ensure_smem((const void*)kernel, simt_smem_floats(256) * 4, done)) return rc;
     kernel<<<(int)grid, SIMT_THREADS, bytes, st>>>(q, r, ws, ws_out, pool, blocks_c);
@@ -436,6 +434,11 @@ int lin_device_error(int clear) {
 }
 }  // namespace fa
 
+// floats of the workspace, 0 where none is needed
+static long long workspace(long long total, int batch, int seg_len, int nseg, long long nhk, int dk, int dv, bool tc) {
+  return nseg > 1 || tc ? fa::lin_slots(total > 0, total, batch, seg_len, nseg) * nhk * dk * dv : 0;
+}
+
 extern "C" FA_API long long fa_linear_plan(int batch, int S, long long total, int NH, int gqa, int dk, int dv, int dtype, int* seg_len,
                                            int* nseg) {
   if (seg_len) *seg_len = 128;
@@ -470,7 +473,7 @@ extern "C" FA_API long long fa_linear_plan(int batch, int S, long long total, in
     const long long whole = (S + 127ll) / 128;
     *seg_len = (int)std::min((whole + best - 1) / best * 128, 1ll << 30);
     *nseg = (int)((S + (long long)*seg_len - 1) / *seg_len);
-    return states * *nseg * dk * dv;
+    return workspace(total, batch, *seg_len, *nseg, NH / gqa, dk, dv, true);
   } else {
     // As many segments as give every SM four blocks, none shorter than a chunk of 32 tokens (each costs a state written and read
     // again, and its keys and values read twice): 8 heads x 512 tokens took 5 us a kernel in 16 segments and 15 in 4.
@@ -484,7 +487,7 @@ extern "C" FA_API long long fa_linear_plan(int batch, int S, long long total, in
   if (len >= S) len = (S + unit - 1ll) / unit * unit;
   *seg_len = (int)std::min(len, 1ll << 30);
   *nseg = (int)((S + (long long)*seg_len - 1) / *seg_len);
-  return *nseg > 1 ? states * *nseg * dk * dv : 0;
+  return workspace(total, batch, *seg_len, *nseg, NH / gqa, dk, dv, false);
 }
 
 extern "C" FA_API int fa_linear_launch(const FaLinearParams* pp, int dtype, void* stream) {
@@ -503,12 +506,15 @@ extern "C" FA_API int fa_linear_launch(const FaLinearParams* pp, int dtype, void
   FA_CHECK_ARG(!p.cu || p.batch > 0 || p.total == 0, "linear attention: %lld packed rows of no sequence", p.total);
   if (p.batch == 0) return FA_OK;
   const bool step = !p.keep_states && p.S <= FA_LINEAR_STEP_TOKENS;
-  LinSeqs q{p.cu, p.log_decay, p.total, p.batch, p.S, p.NH / p.gqa, 0, 1};
+  LinSeqs q{p.cu, p.log_decay, p.total, p.batch, p.S, p.NH / p.gqa, 0, 1, p.batch};
   if (!step) {
     q.seg_len = p.seg_len;
     q.nseg = p.nseg;
     FA_CHECK_ARG(p.seg_len > 0 && p.nseg > 0 && (long long)p.seg_len * p.nseg >= p.S, "linear attention: %d segments of %d tokens for S=%d",
                  p.nseg, p.seg_len, p.S);
+    const long long slots = lin_slots(p.cu != nullptr, p.total, p.batch, p.seg_len, p.nseg);
+    FA_CHECK_ARG(slots < (1ll << 31), "linear attention: %lld segments", slots);
+    q.slots = (int)slots;
     FA_CHECK_ARG(p.nseg == 1 || p.states, "linear attention: %d segments need the workspace `states`", p.nseg);
   }
   const LinPool pool{p.state_in, p.state_out, p.state_index, p.seen, p.state_index ? p.slots : p.batch};
@@ -545,7 +551,9 @@ extern "C" FA_API int fa_linear_backward_launch(const FaLinearBwdParams* pp, int
   FA_CHECK_ARG(p.seg_len > 0 && p.nseg > 0 && (long long)p.seg_len * p.nseg >= p.S,
                "linear attention backward: %d segments of %d tokens for S=%d", p.nseg, p.seg_len, p.S);
   FA_CHECK_ARG(p.nseg == 1 || (p.states && p.work), "linear attention backward: %d segments need `states` and `work`", p.nseg);
-  const LinSeqs q{p.cu, p.log_decay, p.total, p.batch, p.S, p.NH / p.gqa, p.seg_len, p.nseg};
+  const long long slots = lin_slots(p.cu != nullptr, p.total, p.batch, p.seg_len, p.nseg);
+  FA_CHECK_ARG(slots < (1ll << 31), "linear attention backward: %lld segments", slots);
+  const LinSeqs q{p.cu, p.log_decay, p.total, p.batch, p.S, p.NH / p.gqa, p.seg_len, p.nseg, (int)slots};
   const float s = p.scale;
   const LinRole dq{p.dO, p.v, p.k, p.dQ, p.sdO, p.sV, p.sK, p.sdQ, p.gqa, 1, p.dv, p.dk, 1, s, s, 1.f};
   const LinRole dk{p.v, p.dO, p.q, p.dK, p.sV, p.sdO, p.sQ, p.sdK, 1, p.gqa, p.dv, p.dk, 1, s, 1.f, s};

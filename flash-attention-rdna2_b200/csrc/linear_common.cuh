@@ -29,7 +29,16 @@ struct LinSeqs {
   const float* log_decay;
   long long total;
   int batch, S, nhk, seg_len, nseg;
+  int slots;             // segments of all sequences (lin_slots): the states' workspace is [slots][nhk][da dc]
 };
+
+// Segments have slots: nseg for each dense sequence, and for packed ones, whatever their lengths, floor(total / seg_len) + batch, the first of
+// sequence z being floor(row0 / seg_len) + z (floor(x + y) + 1 >= floor(x) + ceil(y), so they do not meet); one sequence alone needs no
+// more than it has (32 empty blocks among 160 left the others on crowded SMs: 170 us, not 142).  nseg 1: one segment a sequence, of
+// any length.
+inline long long lin_slots(bool packed, long long total, int batch, int seg_len, int nseg) {
+  return nseg == 1 ? batch : packed ? (batch == 1 ? (total + seg_len - 1) / seg_len : total / seg_len + batch) : (long long)batch * nseg;
+}
 
 // the states that sequences start from and leave
 struct LinPool {
@@ -65,10 +74,29 @@ __device__ __forceinline__ LinSpan lin_span(const LinSeqs& q, int z) {
   }
   return s;
 }
-// tokens [t0, t1) of segment n; the last segment takes what a too small bound on the lengths leaves over
-__device__ __forceinline__ void lin_segment(const LinSeqs& q, int len, int n, int& t0, int& t1) {
-  t0 = (int)min((long long)n * q.seg_len, (long long)len);
-  t1 = n == q.nseg - 1 ? len : (int)min((long long)(n + 1) * q.seg_len, (long long)len);
+__device__ __forceinline__ long long lin_first_slot(const LinSeqs& q, int z, long long row0) {
+  return q.nseg == 1 ? z : q.cu ? row0 / q.seg_len + z : (long long)z * q.nseg;
+}
+__device__ __forceinline__ int lin_segments(const LinSeqs& q, int len) {
+  return q.nseg == 1 ? 1 : (len + q.seg_len - 1) / q.seg_len;
+}
+// the sequence of a slot and its tokens [t0, t1); t0 == t1 where the slot has none
+__device__ __forceinline__ LinSpan lin_segment(const LinSeqs& q, int slot, int& z, int& t0, int& t1) {
+  z = q.nseg == 1 ? slot : slot / q.nseg;
+  if (q.nseg > 1 && q.cu) {
+    int hi = q.batch;                      // the last sequence whose first slot is not past this one
+    z = 0;
+    while (hi - z > 1) {
+      const int mid = (z + hi) / 2;
+      if (lin_first_slot(q, mid, min(max((long long)q.cu[mid], 0ll), q.total)) <= slot) z = mid;
+      else hi = mid;
+    }
+  }
+  const LinSpan s = lin_span(q, z);
+  const long long n = slot - lin_first_slot(q, z, s.row0);
+  t0 = q.nseg == 1 ? 0 : (int)min(max(n, 0ll) * q.seg_len, (long long)s.len);
+  t1 = q.nseg == 1 ? s.len : n < 0 ? t0 : (int)min((long long)t0 + q.seg_len, (long long)s.len);
+  return s;
 }
 __device__ __forceinline__ float lin_log2_decay(const float* log_decay, int h) {
   const float g = log_decay[h];
@@ -90,16 +118,14 @@ __device__ __forceinline__ int lin_slot(const LinPool& p, int z, int nthreads, i
   return bad ? LIN_NONE : s;
 }
 
-// Packed rows that belong to no sequence are 0: the blocks of the first and the last sequence write them, `part` of
-// `parts` blocks each.  Heads [h0, h0 + nh).
+// Packed rows that belong to no sequence are 0: each of `parts` blocks of a head writes its share.
 template <typename T>
-__device__ void lin_zero_outside(const LinSeqs& q, const LinRole& r, int z, int h0, int part, int parts, int nthreads) {
+__device__ void lin_zero_outside(const LinSeqs& q, const LinRole& r, int h0, int part, int parts, int nthreads) {
   if (!q.cu) return;
   T* out = (T*)r.out;
   const LinSpan end = lin_span(q, q.batch - 1);
   const long long first = lin_span(q, 0).row0, last = end.row0 + end.len;
   for (int side = 0; side < 2; ++side) {
-    if (z != (side ? q.batch - 1 : 0)) continue;
     const long long r0 = side ? last : 0, r1 = side ? q.total : first;
     for (long long row = r0 + part; row < r1; row += parts)
       for (int e = threadIdx.x; e < r.na * r.dc; e += nthreads)

@@ -212,17 +212,17 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
   extern __shared__ uint8_t smem_raw[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int n = blockIdx.x % q.nseg, h = blockIdx.x / q.nseg % q.nhk, z = blockIdx.x / q.nseg / q.nhk;
-  lin_zero_outside<T>(q, r, z, h * r.na, n, q.nseg, NTHREADS);
-  const LinSpan span = lin_span(q, z);
-  int t0, t1;
-  lin_segment(q, span.len, n, t0, t1);
+  const int h = blockIdx.x % q.nhk, seg = blockIdx.x / q.nhk;
+  lin_zero_outside<T>(q, r, h * r.na, seg, q.slots, NTHREADS);
+  int z, t0, t1;
+  const LinSpan span = lin_segment(q, seg, z, t0, t1);
   if (t1 <= t0) return;
   const int slot = lin_slot(pool, z, NTHREADS, &g_lin_tc_error);
-  T* out = (T*)r.out + (q.cu ? 0 : z * r.so.b) + (span.row0 + t0) * r.so.s + (long long)h * r.na * r.so.h;
+  const int tokens = t1 - t0, row_first = (int)span.row0 + t0, z4 = q.cu ? 0 : z;      // rows of the maps
   if (slot < 0) {
+    T* out = (T*)r.out + z4 * r.so.b + row_first * r.so.s + (long long)h * r.na * r.so.h;
     for (int g = 0; g < r.na; ++g)
-      for (long long e = tid; e < (long long)(t1 - t0) * r.dc; e += NTHREADS)
+      for (long long e = tid; e < (long long)tokens * r.dc; e += NTHREADS)
         out[e / r.dc * r.so.s + g * r.so.h + e % r.dc] = Elem<T>::from_f(0.f);
     return;
   }
@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   uint32_t* xmax = reinterpret_cast<uint32_t*>(sgen + K::OFF_MAX);
   uint32_t* pmax = xmax + 4;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sgen + K::OFF_BAR + Bz::TMEM_ADDR);
-  const int chunks = (t1 - t0 + C - 1) / C, groups = max(r.na, r.nb), items = chunks * groups;
+  const int chunks = (tokens + C - 1) / C, groups = max(r.na, r.nb), items = chunks * groups;
   const float g2 = lin_log2_decay(q.log_decay, h);
 
   if (tid == 0) {
@@ -270,7 +270,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  constexpr uint32_t tmem = 0;        // all 512 columns are this block's
+  if (tid == 0 && *tmem_slot != tmem) record_error(LIN_ERR_WAIT);
 
   // item t = ck * groups + g: chunk ck (from the end where reversed), head g of the side that has several
   const auto chunk_at = [&](int ck) { return (REV ? chunks - 1 - ck : ck) * C; };
@@ -280,9 +281,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     if (warp == WARP_TMA && lane == 0) {
       int na = 0, nb = 0, nc = 0;
       bool ok = true;
-      const int z4 = q.cu ? 0 : z;
       for (int ck = 0, g = 0; ok && ck < chunks; ++g == groups ? g = 0, ++ck : 0) {
-        const int row = (int)span.row0 + t0 + chunk_at(ck);
+        const int row = row_first + chunk_at(ck);
         const auto load = [&](const CUtensorMap* map, int full, int empty, int off, int stages, int& i, int head) {
           const int s = i % stages;
           if (i >= stages) ok = ok && mbar_wait(bar + empty + 8 * s, ((i / stages) - 1) & 1);
@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       int ca = -1, cb = -1, noi = 0;
       for (int t = 0, ck = 0, g = 0; ok && t < items; ++t, ++g == groups ? g = 0, ++ck : 0) {
         const bool first = g == 0, last = g == groups - 1, new_b = first || r.nb > 1, do_i = first || r.na > 1;
-        const int cn = min(C, t1 - t0 - chunk_at(ck));
+        const int cn = min(C, tokens - chunk_at(ck));
         cb += new_b ? 1 : 0;
         ca += do_i ? 1 : 0;
         const uint32_t at = st + K::OFF_A + (ca % K::NA) * K::TILE, bt = st + K::OFF_B + (cb % K::NB) * K::TILE,
@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       for (int t = 0, ck = 0, g = 0; ok && t < items; ++t, ++g == groups ? g = 0, ++ck : 0) {
         const bool first = g == 0, last = g == groups - 1, end = ck == chunks - 1;
         const bool new_b = first || r.nb > 1, do_b = new_b && !end;
-        const int cn = min(C, t1 - t0 - chunk_at(ck));
+        const int cn = min(C, tokens - chunk_at(ck));
         cb += new_b ? 1 : 0;
         const uint32_t bt = st + K::OFF_B + (cb % K::NB) * K::TILE, ct = st + K::OFF_C + (cb % K::NC) * K::TILE;
         if (first && !end) {
@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       regs_state();
       const int xl = SWAP ? r.dc : r.da, xn = SWAP ? r.da : r.dc;   // real rows (lanes) and columns of X
       const float* x0 = nullptr;
-      if (ws) x0 = ws + (((long long)z * q.nhk + h) * q.nseg + n) * r.da * r.dc;
+      if (ws) x0 = ws + ((long long)seg * q.nhk + h) * r.da * r.dc;
       else if (pool.in && !(pool.seen && pool.seen[z] <= 0)) x0 = pool.in + ((long long)slot * q.nhk + h) * r.da * r.dc;
       int nx = 0, nbt = 0, cbw = -1, w_cn = 0;
       float2 w_rows[8];
@@ -522,7 +522,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       for (int t = 0, ck = 0, g = 0; t < items; ++t, ++g == groups ? g = 0, ++ck : 0) {
         const bool first = g == 0, end = ck == chunks - 1;
         const bool do_b = (first || r.nb > 1) && !end;
-        const int cn = min(C, t1 - t0 - chunk_at(ck));
+        const int cn = min(C, tokens - chunk_at(ck));
         // the last a X, which reads X in shared memory, and the last update of X, which reads the decayed rows
         if (t > 0 && first) wait(Bz::X_READ, ck - 1);
         if (nbt > 0 && (first || do_b)) wait(Bz::X_DONE, nbt - 1);
@@ -621,7 +621,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
               if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
               __syncwarp();
             } else {
-              to_row = reinterpret_cast<uint8_t*>(out + (long long)(at + row) * r.so.s + head * r.so.h + hf * HD);
+              to_row = reinterpret_cast<uint8_t*>((T*)r.out + z4 * r.so.b + (long long)(row_first + at + row) * r.so.s + (long long)(h * r.na + head) * r.so.h + hf * HD);
               swizzle = 0;
               units = row < cn ? min(units, (r.dc - hf * HD) / 8) : 0;
             }
@@ -634,14 +634,14 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             if (whole) {
               fence_proxy_async_smem();
               __syncwarp();
-              if (lane == 0) tma_store_4d(&to, sbase + obox, hf * HD, (int)span.row0 + t0 + at + qd * 32, h * r.na + head, q.cu ? 0 : z);
+              if (lane == 0) tma_store_4d(&to, sbase + obox, hf * HD, row_first + at + qd * 32, h * r.na + head, z4);
             }
           }
         }
         if (t == items) break;
         const bool first = g == 0, do_i = !MULTI || first;
         at = chunk_at(ck);
-        cn = min(C, t1 - t0 - at);
+        cn = min(C, tokens - at);
         head = r.na > 1 ? g : 0;
         write = r.na > 1 || g == groups - 1;
         // Pair products: decay, mask, back to TMEM as hi + lo, in pieces of W columns (acc takes the registers where it lives on from
@@ -791,10 +791,9 @@ __global__ void __launch_bounds__(NTHREADS_ST, 1)
   using K = StCfg<D, BF16>;
   extern __shared__ uint8_t smem_raw[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int n = blockIdx.x % q.nseg, h = blockIdx.x / q.nseg % q.nhk, z = blockIdx.x / q.nseg / q.nhk;
-  const LinSpan span = lin_span(q, z);
-  int t0, t1;
-  lin_segment(q, span.len, n, t0, t1);
+  const int h = blockIdx.x % q.nhk, seg = blockIdx.x / q.nhk;
+  int z, t0, t1;
+  const LinSpan span = lin_segment(q, seg, z, t0, t1);
   if (t1 <= t0) return;
   const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* sgen = smem_raw + (sbase - smem_u32(smem_raw));
@@ -914,7 +913,7 @@ __global__ void __launch_bounds__(NTHREADS_ST, 1)
       if (i > 0) add(i - 1);
     }
     add(items - 1);
-    float* x = ws + (((long long)z * q.nhk + h) * q.nseg + n) * r.da * r.dc + (long long)row * r.dc;
+    float* x = ws + ((long long)seg * q.nhk + h) * r.da * r.dc + (long long)row * r.dc;
 #pragma unroll
     for (int i = 0; i < HD / 4; ++i) {
       const int col = qr * HD + 4 * i;
@@ -973,7 +972,7 @@ bool regs_fit(Kernel kernel) {
 
 template <typename Kernel, typename... Args>
 int launch(Kernel kernel, int threads, int smem, unsigned long long* done, const LinSeqs& q, cudaStream_t st, const Args&... args) {
-  const long long grid = (long long)q.batch * q.nhk * q.nseg;
+  const long long grid = (long long)q.slots * q.nhk;
   FA_CHECK_ARG(grid < (1ll << 31), "linear attention: %lld blocks", grid);
   if (int rc = ensure_smem((const void*)kernel, smem, done)) return rc;
   kernel<<<(int)grid, threads, smem, st>>>(args...);

@@ -434,7 +434,9 @@ FA_API int fa_combine_launch(const FaCombineParams* p, void* stream);
  *   states     workspace of fa_linear_plan floats, 16-byte aligned (null where that is 0, with one segment and no state_out, and for up to
  *              FA_LINEAR_STEP_TOKENS tokens, which go through the state one by one).  With keep_states the chunked kernels run
  *              whatever S is, and leave each segment's start state there for fa_linear_backward_launch.
- * fa_linear_plan: segments of seg_len tokens (nseg for the longest sequence) that run side by side, and the floats of `states`.
+ * fa_linear_plan (total 0: dense): segments of seg_len tokens that run side by side, nseg for a sequence of S tokens (1: every sequence
+ * is one segment, however long), and the floats of `states`: [segments][NH / gqa][dk][dv], with batch * nseg segments or, packed,
+ * total / seg_len + batch (of one sequence, rounded up), whatever the lengths.
  * -------------------------------------------------------------------------------------------*/
 #define FA_LINEAR_STEP_TOKENS 16
 typedef struct FaLinearParams {

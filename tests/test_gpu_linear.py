@@ -479,3 +479,24 @@ def test_refusals(bad):
     if bad not in ("state", "state_grad", "slots", "index", "device_state"):
         with pytest.raises(err):
             fa.linear_attn_func(q, k, v, g)
+
+
+@pytest.mark.parametrize("dt", ALL)
+def test_workspace_follows_the_rows_and_not_the_bound(dt):
+    """Many short sequences beside a long one, without a bound on the lengths: segments are counted by the rows."""
+    lens = [3000] + [1, 0, 20] * 40 + [700]
+    q, k, v = inputs(DT[dt], lens, 2, 2, 64, 64)
+    state = torch.randn(len(lens), 2, 64, 64, device="cuda")
+    g, before = decays(2, "-0.01"), state.clone()
+    torch.cuda.reset_peak_memory_stats()
+    held = torch.cuda.memory_allocated()
+    out = fa.linear_attn_with_state(q, k, v, state, g, cu_seqlens=cum(lens))
+    assert torch.cuda.max_memory_allocated() - held < 64 << 20
+    at = 0
+    for z, n in enumerate(lens):
+        s = slice(at, at + n)
+        at += n
+        if z in (0, 1, 2, 3, 60, len(lens) - 1):
+            ref = R.both(q[s], k[s], v[s], g, 0.125, before[z])
+            R.close(out[s], *ref[0], n, (64, 64), g, DT[dt], f"sequence {z}")
+            R.close(state[z], *ref[1], n, (64, 64), g, DT[dt], f"state {z}")

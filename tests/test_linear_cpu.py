@@ -102,8 +102,32 @@ def test_plan_covers_every_token(batch, s, total, nh, gqa, dk, dv, dt):
     seg, n = C.c_int(), C.c_int()
     floats = L.fa_linear_plan(batch, s, C.c_longlong(total), nh, gqa, dk, dv, dt, C.byref(seg), C.byref(n))
     assert seg.value > 0 and n.value >= 1 and seg.value * n.value >= s and (n.value - 1) * seg.value < max(s, 1)
-    whole = batch * (nh // gqa) * n.value * dk * dv
+    slots = batch if n.value == 1 else batch * n.value if not total else -(-total // seg.value) if batch == 1 else total // seg.value + batch
+    whole = slots * (nh // gqa) * dk * dv
     assert floats == whole if n.value > 1 else floats in (0, whole)     # one segment: a last state may need it
+
+
+def test_segments_of_packed_sequences_have_slots_of_their_own():
+    """The first slot of sequence z is floor(row0 / seg_len) + z: ranges of ceil(len / seg_len) slots that do not meet and end in
+    total / seg_len + batch, and a bisection over them finds each slot's sequence."""
+    gen = torch.Generator().manual_seed(3)
+    for _ in range(300):
+        batch, seg = int(torch.randint(1, 9, (), generator=gen)), int(torch.randint(1, 40, (), generator=gen))
+        lens = (torch.randint(0, 90, (batch,), generator=gen) * (torch.rand(batch, generator=gen) > 0.3)).tolist()
+        row0 = [sum(lens[:z]) for z in range(batch)]
+        first = [r // seg + z for z, r in enumerate(row0)]
+        spans = [range(f, f + -(-n // seg)) for f, n in zip(first, lens)]
+        used = [s for r in spans for s in r]
+        assert len(set(used)) == len(used) and max(used, default=0) < sum(lens) // seg + batch
+        assert len(set(first)) == batch                                   # an empty sequence's slot is nobody else's
+        assert all(f not in r for z, f in enumerate(first) for y, r in enumerate(spans) if y != z)
+        for z, r in enumerate(spans):
+            for s in r:
+                lo, hi = 0, batch
+                while hi - lo > 1:
+                    mid = (lo + hi) // 2
+                    lo, hi = (mid, hi) if first[mid] <= s else (lo, mid)
+                assert lo == z
 
 
 def test_reference_gradients_against_differences():
