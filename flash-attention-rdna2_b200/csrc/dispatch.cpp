@@ -726,13 +726,23 @@ FaStrides rows_of_heads(const torch::Tensor& x) {
   return FaStrides{x.stride(0), x.stride(2), x.stride(1)};
 }
 
+// x with a contiguous last dimension and, for the chunked kernels of 16 bits (`tma`), as the tensor maps need it: rows on 16-byte boundaries
+// and no dimension that repeats itself.  A copy costs one pass over x; without it the CUDA-core kernels would run, several times as long.
+torch::Tensor rows_for_linear(const torch::Tensor& x, bool tma) {
+  if (x.stride(-1) != 1) return x.contiguous();
+  if (!tma || x.element_size() != 2) return x;
+  bool fits = (uintptr_t)x.const_data_ptr() % 16 == 0;
+  for (int64_t d = 0; d + 1 < x.dim(); ++d) fits = fits && (x.size(d) <= 1 || (x.stride(d) > 0 && x.stride(d) % 8 == 0));
+  return fits || x.numel() == 0 ? x : x.clone(at::MemoryFormat::Contiguous);
+}
+
 // what the forward and the backward check alike: shapes, types, the device, the packed rows' bounds
 template <typename P>
 struct LinearCall {
   torch::Tensor q, k, v, decay, cu;
   bool packed = false;
   LinearCall(P& p, const torch::Tensor& q_, const torch::Tensor& k_, const torch::Tensor& v_, const torch::Tensor& log_decay,
-             double scale, const c10::optional<torch::Tensor>& cu_, int64_t max_seqlen) {
+             double scale, const c10::optional<torch::Tensor>& cu_, int64_t max_seqlen, bool chunked) {
     const auto* c = opt_ptr(cu_);
     packed = c != nullptr;
     const int hd = packed ? 1 : 2;
@@ -757,23 +767,23 @@ struct LinearCall {
     TORCH_CHECK_VALUE(log_decay.is_cuda() && log_decay.device() == q_.device() && log_decay.dim() == 1 && log_decay.size(0) == hk &&
                           log_decay.is_floating_point(),
                       "fable_attn: log_decay must be (nheads_k,) = (", hk, ",) floating point values on q's device");
-    const auto last = [](const torch::Tensor& x) { return x.stride(-1) == 1 ? x : x.contiguous(); };
-    q = last(q_); k = last(k_); v = last(v_);
     decay = table_f32(log_decay);
     p.struct_size = sizeof(P);
     p.log_decay = decay.template data_ptr<float>();
     if (packed) {
-      cu = index_i32(*c, q.device(), "cu_seqlens");
+      cu = index_i32(*c, q_.device(), "cu_seqlens");
       TORCH_CHECK_VALUE(cu.dim() == 1 && cu.numel() >= 1, "fable_attn: cu_seqlens must be (batch + 1,)");
       p.cu = cu.template data_ptr<int>();
       p.batch = (int)cu.numel() - 1;
-      p.total = q.size(0);
+      p.total = q_.size(0);
       p.S = max_seqlen > 0 ? (int)std::min<int64_t>(max_seqlen, p.total) : (int)p.total;
       TORCH_CHECK_VALUE(p.batch > 0 || p.total == 0, "fable_attn: ", p.total, " rows and no sequence in cu_seqlens");
     } else {
-      p.batch = (int)q.size(0);
-      p.S = (int)q.size(1);
+      p.batch = (int)q_.size(0);
+      p.S = (int)q_.size(1);
     }
+    const bool tma = (chunked || p.S > FA_LINEAR_STEP_TOKENS) && q_.size(hd + 1) <= 128 && v_.size(hd + 1) <= 128;
+    q = rows_for_linear(q_, tma); k = rows_for_linear(k_, tma); v = rows_for_linear(v_, tma);
     p.q = q.data_ptr(); p.k = k.data_ptr(); p.v = v.data_ptr();
     p.sQ = rows_of_heads(q); p.sK = rows_of_heads(k); p.sV = rows_of_heads(v);
     p.NH = (int)hq; p.gqa = (int)(hq / hk);
@@ -798,7 +808,7 @@ std::tuple<torch::Tensor, torch::Tensor, int64_t, int64_t> linear_fwd(
   TORCH_CHECK_VALUE(q.is_cuda(), "fable_attn: linear attention needs CUDA tensors");
   const c10::cuda::CUDAGuard guard(q.device());
   FaLinearParams p{};
-  const LinearCall<FaLinearParams> call(p, q, k, v, log_decay, scale, cu, max_seqlen);
+  const LinearCall<FaLinearParams> call(p, q, k, v, log_decay, scale, cu, max_seqlen, keep_states);
   torch::Tensor idx, sn;
   const auto *si = opt_ptr(state_in), *so = opt_ptr(state_out);
   if (const auto* i = opt_ptr(index)) {
@@ -815,6 +825,7 @@ std::tuple<torch::Tensor, torch::Tensor, int64_t, int64_t> linear_fwd(
   const int64_t slots = p.state_index ? -1 : p.batch;
   if (si) call.check_states(p, *si, "the state", slots);
   if (so) call.check_states(p, *so, "the new state", si ? si->size(0) : slots);
+  if (si && so) at::assert_no_partial_overlap(*so, *si);
   p.slots = si ? si->size(0) : so ? so->size(0) : 0;
   p.state_in = si ? si->const_data_ptr<float>() : nullptr;
   p.state_out = so ? so->data_ptr<float>() : nullptr;
@@ -841,12 +852,12 @@ std::vector<torch::Tensor> linear_bwd(torch::Tensor dout, torch::Tensor q, torch
                                       int64_t seg_len, int64_t nseg) {
   const c10::cuda::CUDAGuard guard(q.device());
   FaLinearBwdParams p{};
-  const LinearCall<FaLinearBwdParams> call(p, q, k, v, log_decay, scale, cu, max_seqlen);
+  const LinearCall<FaLinearBwdParams> call(p, q, k, v, log_decay, scale, cu, max_seqlen, true);
   auto shape = call.q.sizes().vec();
   shape.back() = p.dv;
   TORCH_CHECK_VALUE(dout.is_cuda() && dout.sizes() == c10::IntArrayRef(shape) && dout.scalar_type() == q.scalar_type() && dout.device() == q.device(),
                     "fable_attn: the output's gradient must have the output's shape and type");
-  const torch::Tensor d = dout.stride(-1) == 1 ? dout : dout.contiguous();
+  const torch::Tensor d = rows_for_linear(dout, p.dk <= 128 && p.dv <= 128);
   torch::Tensor df;
   if (const auto* x = opt_ptr(dfinal)) {
     df = x->contiguous();
@@ -926,6 +937,7 @@ std::tuple<torch::Tensor, torch::Tensor> rotary_qk(torch::Tensor q, torch::Tenso
     TORCH_CHECK_VALUE(qs.is_same(q) && ks.is_same(k), "fable_attn: inplace rotary needs a contiguous last dimension");
     at::assert_no_internal_overlap(q);
     at::assert_no_internal_overlap(k);
+    at::assert_no_overlap(q, k);
   }
   const torch::Tensor qo = inplace ? q : torch::empty(q.sizes(), q.options()), ko = inplace ? k : torch::empty(k.sizes(), k.options());
   p.q = qs.const_data_ptr(); p.k = ks.const_data_ptr(); p.q_out = qo.data_ptr(); p.k_out = ko.data_ptr();

@@ -45,8 +45,8 @@ __global__ void __launch_bounds__(STEP_THREADS, ROWS > 8 ? 3 : 6)
   T* out = (T*)r.out + (q.cu ? 0 : z * r.so.b) + span.row0 * r.so.s + (long long)h * r.na * r.so.h;
   if (vb == 0) lin_zero_outside<T>(q, r, h * r.na, z, q.batch, STEP_THREADS);
   if (lin_slot(pool, z, STEP_THREADS, &g_lin_error) < 0) {
-    for (int e = tid; e < span.len * r.na * STEP_COLS; e += STEP_THREADS) {
-      const int cc = vb * STEP_COLS + e % STEP_COLS, g = e / STEP_COLS % r.na, t = e / STEP_COLS / r.na;
+    for (long long e = tid; e < (long long)span.len * r.na * STEP_COLS; e += STEP_THREADS) {
+      const int cc = vb * STEP_COLS + (int)(e % STEP_COLS), g = (int)(e / STEP_COLS % r.na), t = (int)(e / STEP_COLS / r.na);
       if (cc < r.dc) out[t * r.so.s + g * r.so.h + cc] = Elem<T>::from_f(0.f);
     }
     return;

@@ -114,6 +114,22 @@ def test_strided_inputs(dt):
     check_run(DT[dt], [3, 200, 77], 4, 2, 64, 64, decays(2), False, True, strided=True)
 
 
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+def test_rows_off_sixteen_bytes_and_repeated_heads(dt):
+    """Slices at odd places, a head that serves all, a gradient that is one row for all tokens: the same bits as of whole copies."""
+    dt, n, h, d = DT[dt], 150, 4, 64
+    wide = rand(0, n, 3 * h * d + 5, dtype=dt)
+    q, k, v = (wide[:, 3 + i * h * d:3 + (i + 1) * h * d].view(n, h, d)[None].requires_grad_() for i in range(3))
+    g, do = decays(h), rand(1, 1, 1, h, d, dtype=dt).expand(1, n, h, d)
+    near = [x.detach().clone(memory_format=torch.contiguous_format).requires_grad_() for x in (q, k, v)]
+    a, b = fa.linear_attn_func(q, k, v, g), fa.linear_attn_func(*near, g)
+    assert torch.equal(a, b)
+    for x, y in zip(torch.autograd.grad(a, (q, k, v), do), torch.autograd.grad(b, near, do.contiguous())):
+        assert torch.equal(x, y)
+    one = near[1].detach()[:, :, :1].expand(1, n, h, d)
+    assert torch.equal(fa.linear_attn_func(near[0], one, near[2], g), fa.linear_attn_func(near[0], one.contiguous(), near[2], g))
+
+
 def test_positive_decay_counts_as_none_and_nan_shows():
     q, k, v = inputs(torch.bfloat16, [130], 2, 2, 64, 64)
     g = torch.tensor([0.5, 0.0]).cuda()
@@ -454,7 +470,7 @@ def test_far_addresses():
         assert torch.equal(pool[[slots - 1, 0]], small)
 
 
-@pytest.mark.parametrize("bad", ["fp64", "heads", "dims", "batch", "decay", "decay_grad", "state", "state_grad", "slots", "index", "cpu", "dim7", "rank", "device_state"])
+@pytest.mark.parametrize("bad", ["fp64", "heads", "dims", "batch", "decay", "decay_grad", "state", "state_grad", "slots", "index", "cpu", "dim7", "rank", "device_state", "overlap"])
 def test_refusals(bad):
     b, n, h, d = 2, 20, 4, 64
     q, k, v = (rand(i, b, n, h, d, dtype=torch.bfloat16) for i in range(3))
@@ -474,9 +490,12 @@ def test_refusals(bad):
     if bad == "dim7": q, k, v, state = q[..., :7], k[..., :7], v[..., :7], state[..., :7, :7].contiguous()
     if bad == "rank": q, k, v = q[0], k[0], v[0]
     if bad == "device_state": state = state.cpu()
+    if bad == "overlap":
+        pool = rand(5, b + 1, h, d, d)
+        state, kw["state_out"], err = pool[:-1], pool[1:], RuntimeError
     with pytest.raises(err):
         fa.linear_attn_with_state(q, k, v, state, g, **kw)
-    if bad not in ("state", "state_grad", "slots", "index", "device_state"):
+    if bad not in ("state", "state_grad", "slots", "index", "device_state", "overlap"):
         with pytest.raises(err):
             fa.linear_attn_func(q, k, v, g)
 

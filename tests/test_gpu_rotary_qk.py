@@ -172,7 +172,7 @@ def test_non_finite_values_stay_in_their_pair():
     assert torch.equal(got[fine], want[fine]) and not got[~fine].isfinite().any()
 
 
-@pytest.mark.parametrize("bad", ["cpu", "types", "heads", "freq", "freq_grad", "pos", "pos_float", "both", "inplace_grad", "overlap", "rank", "dims"])
+@pytest.mark.parametrize("bad", ["cpu", "types", "heads", "freq", "freq_grad", "pos", "pos_float", "both", "inplace_grad", "overlap", "same", "rank", "dims"])
 def test_refusals(bad):
     freq, _ = scaled_inv_freq(64, device="cuda")
     q, k, pos, kw = rand(1, 2, 3, 4, 64), rand(2, 2, 3, 2, 64), torch.zeros(2, 3, dtype=torch.int32).cuda(), {}
@@ -187,6 +187,7 @@ def test_refusals(bad):
     if bad == "both": kw["seqlen_offsets"] = 3
     if bad == "inplace_grad": q, kw["inplace"] = q.requires_grad_(), True
     if bad == "overlap": k, kw["inplace"] = k[:, :, :1].expand(2, 3, 4, 64), True
+    if bad == "same": q, kw["inplace"] = k, True
     if bad == "rank": q, k = q[0, 0], k[0, 0]
     if bad == "dims": k = k[..., :32]
     with pytest.raises(err):
