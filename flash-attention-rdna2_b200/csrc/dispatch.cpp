@@ -727,7 +727,8 @@ FaStrides rows_of_heads(const torch::Tensor& x) {
 }
 
 // x with a contiguous last dimension and, for the chunked kernels of 16 bits (`tma`), as the tensor maps need it: rows on 16-byte boundaries
-// and no dimension that repeats itself.  A copy costs one pass over x; without it the CUDA-core kernels would run, several times as long.
+// and no dimension that repeats itself.  Otherwise the CUDA-core
+// kernels would have to run: 2 x 4096 tokens, 16 heads of 128 take 83 us as they are, 204 with all three copied, and 740 there.
 torch::Tensor rows_for_linear(const torch::Tensor& x, bool tma) {
   if (x.stride(-1) != 1) return x.contiguous();
   if (!tma || x.element_size() != 2) return x;

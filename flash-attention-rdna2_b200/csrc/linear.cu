@@ -153,30 +153,79 @@ __global__ void __launch_bounds__(STEP_THREADS, ROWS > 8 ? 3 : 6)
 
 // =====================================================================================
 // CUDA-core chunked kernel: every type, dims up to 256, any strides.  A block walks one segment of one state in chunks of
-// 32 tokens, for 64 of the c dim's columns, all in fp32: the state, the chunk's rows and the pair products in shared memory.
-// Every product reads its operands four at a time (rows padded to an odd number of 16-byte units, so that the lanes of a
-// quarter warp meet different banks): 16 to 32 multiply-adds for each pair of 16-byte reads; scalar reads took three times as long.
+// SC tokens, for 64 of the c dim's columns, all in fp32: the state, the chunk's rows and the pair products in shared memory.
+// The dims of a and b go by in slices of 64: a slice adds to the pair products and to a X, then its rows of X are brought up
+// to date; so the rows take the same room for every dim, and two blocks fit on an SM up to dims of 128.
+// Bound by shared memory's reads: a thread's tile is SC/16 rows by 4 columns, read four elements at a time (rows padded to an odd
+// number of 16-byte units, so that the lanes of a quarter warp meet different banks).  With 64 tokens eight 16-byte reads feed
+// 64 multiply-adds, with 32 tokens six feed 32; pairs that the order masks are neither multiplied nor read, and two adjacent
+// elements go through one packed multiply-add.  fp32, 4 x 4096 tokens, 16 heads of 64: 429 us, 15 TFLOP/s (with 2 x 4 outputs
+// a thread and whole rows of a and b in shared memory it was 809).
 // =====================================================================================
-constexpr int SC = 32, SCOL = 64, SIMT_THREADS = 256, SPLD = SC + 4;
+constexpr int SCOL = 64, SDIM = 64, SLD = SDIM + 4, SIMT_THREADS = 256;
+constexpr int SIMT_WIDE = 160;      // dims of a up to which an SM holds two blocks of 64-token chunks (110 KB)
 
-__host__ __device__ inline int simt_smem_floats(int da) { return 2 * SC * (da + 4) + SC * SCOL + da * SCOL + SC * SPLD + SC + 4; }
+template <int SC>
+__host__ __device__ constexpr int simt_smem_floats(int da) { return 2 * SC * SLD + SC * SCOL + da * SCOL + SC * (SC + 4) + SC + 4; }
 
-__device__ __forceinline__ float dot4(const float4& a, const float4& b, float s) {
-  return fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, fmaf(a.x, b.x, s))));
+__device__ __forceinline__ float2 twice(float w) { return make_float2(w, w); }
+struct Quad { float2 lo, hi; };      // four columns
+__device__ __forceinline__ Quad quad(const float* s) {
+  const float4 v = *reinterpret_cast<const float4*>(s);
+  return Quad{make_float2(v.x, v.y), make_float2(v.z, v.w)};
 }
-__device__ __forceinline__ void axpy4(float w, const float4& v, float4& s) {
-  s.x = fmaf(w, v.x, s.x); s.y = fmaf(w, v.y, s.y); s.z = fmaf(w, v.z, s.z); s.w = fmaf(w, v.w, s.w);
+__device__ __forceinline__ void axpy(float2 w, const Quad& v, Quad& s) {
+  s.lo = __ffma2_rn(w, v.lo, s.lo);
+  s.hi = __ffma2_rn(w, v.hi, s.hi);
+}
+// s[u] += p[u][0..3] rows 0..3 of v (row stride SCOL)
+template <int R>
+__device__ __forceinline__ void rows_by_four(const float* p, int ld, const float* v, Quad (&s)[R]) {
+  const Quad v0 = quad(v), v1 = quad(v + SCOL), v2 = quad(v + 2 * SCOL), v3 = quad(v + 3 * SCOL);
+#pragma unroll
+  for (int u = 0; u < R; ++u) {
+    const float4 w = *reinterpret_cast<const float4*>(p + u * ld);
+    axpy(twice(w.x), v0, s[u]);
+    axpy(twice(w.y), v1, s[u]);
+    axpy(twice(w.z), v2, s[u]);
+    axpy(twice(w.w), v3, s[u]);
+  }
 }
 
-template <typename T, bool REV, bool STATES>
-__global__ void __launch_bounds__(SIMT_THREADS)
+template <typename T> struct __align__(4 * sizeof(T)) Four { T x[4]; };
+
+// rows [0, n) of 64 columns, of which the first `real` exist (the rest, and the rows up to SC, are 0)
+template <typename T, int SC>
+__device__ __forceinline__ void simt_rows(float* to, int ld, const T* from, long long step, int real, int n, bool wide) {
+#pragma unroll 4
+  for (int e = threadIdx.x; e < SC * 16; e += SIMT_THREADS) {
+    const int j = e >> 4, i = (e & 15) * 4;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (j < n && i < real) {
+      const T* s = from + j * step + i;
+      Four<T> w;
+      if (wide) w = *reinterpret_cast<const Four<T>*>(s);
+      else w = Four<T>{{s[0], s[1], s[2], s[3]}};
+      x = make_float4(Elem<T>::to_f(w.x[0]), Elem<T>::to_f(w.x[1]), Elem<T>::to_f(w.x[2]), Elem<T>::to_f(w.x[3]));
+    }
+    *reinterpret_cast<float4*>(to + j * ld + i) = x;
+  }
+}
+// four elements at a time: base and strides on their boundary
+template <typename T>
+__device__ __forceinline__ bool simt_wide(const void* p, const FaStrides& s) {
+  return ((uintptr_t)p & (4 * sizeof(T) - 1)) == 0 && ((s.b | s.s | s.h) & 3) == 0;
+}
+
+template <typename T, int SC, bool REV, bool STATES>
+__global__ void __launch_bounds__(SIMT_THREADS, SC == 32 ? 3 : 2)
     lin_simt_kernel(const LinSeqs q, const LinRole r, const float* ws, float* ws_out, const LinPool pool, const int blocks_c) {
   extern __shared__ __align__(16) float sm[];
-  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, lane = tid & 31, warp = tid >> 5;
-  const int ld = r.da + 4;
-  float* sa = sm;                           // [SC][ld]
-  float* sb = sa + SC * ld;
-  float* sc = sb + SC * ld;                 // [SC][SCOL]
+  constexpr int R = SC / 16, SPLD = SC + 4;
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  float* sa = sm;                           // [SC][SLD]
+  float* sb = sa + SC * SLD;
+  float* sc = sb + SC * SLD;                // [SC][SCOL]
   float* sx = sc + SC * SCOL;               // [da][SCOL]
   float* sp = sx + r.da * SCOL;             // [SC][SPLD]
   float* lam = sp + SC * SPLD;              // lam^n, n <= SC
@@ -211,95 +260,99 @@ __global__ void __launch_bounds__(SIMT_THREADS)
     const int i = e / SCOL, j = c0 + e % SCOL;
     sx[e] = x0 && j < r.dc ? x0[r.transposed ? (long long)j * r.da + i : (long long)i * r.dc + j] : 0.f;
   }
-  const int chunks = (t1 - t0 + SC - 1) / SC, groups = max(r.na, r.nb);
-  const auto rows = [&](float* to, int ld_to, const T* from, long long step, int first, int dims, int real, int cn) {
-    for (int j = warp; j < SC; j += SIMT_THREADS / 32)
-      for (int i = lane; i < dims; i += 32) to[j * ld_to + i] = j < cn && first + i < real ? Elem<T>::to_f(from[j * step + first + i]) : 0.f;
-  };
+  const bool wide_a = simt_wide<T>(r.a, r.sa), wide_b = simt_wide<T>(r.b, r.sb), wide_c = simt_wide<T>(r.c, r.sc),
+             wide_o = simt_wide<T>(r.out, r.so);
+  const int chunks = (t1 - t0 + SC - 1) / SC, groups = STATES ? r.nb : max(r.na, r.nb), slices = (r.da + SDIM - 1) / SDIM;
+  const int diagonal = R * ty / 16;         // the 16 columns of P that hold this thread's rows (one for the whole warp)
   for (int m = 0; m < chunks; ++m) {
     const int at = t0 + (REV ? chunks - 1 - m : m) * SC, cn = min(SC, t1 - at);
-    float4 o[2];
+    Quad o[R];
     for (int g = 0; g < groups; ++g) {
-      const bool load_a = !STATES && (g == 0 || r.na > 1), load_b = g == 0 || r.nb > 1;
-      __syncthreads();
-      if (load_a) rows(sa, ld, a + at * r.sa.s + (r.na > 1 ? g : 0) * r.sa.h, r.sa.s, 0, r.da, r.da, cn);
-      if (load_b) {
-        rows(sb, ld, b + at * r.sb.s + (r.nb > 1 ? g : 0) * r.sb.h, r.sb.s, 0, r.da, r.da, cn);
-        rows(sc, SCOL, c + at * r.sc.s + (r.nb > 1 ? g : 0) * r.sc.h, r.sc.s, c0, SCOL, r.dc, cn);
+      const bool new_a = g == 0 || r.na > 1, new_b = g == 0 || r.nb > 1, last_a = r.na > 1 || g == groups - 1,
+                 last_b = r.nb > 1 || g == groups - 1;
+      float2 p[R][R] = {};
+      if (!STATES && new_a) {
+#pragma unroll
+        for (int u = 0; u < R; ++u) o[u] = Quad{};
       }
-      __syncthreads();
-      if constexpr (!STATES) {
-        const float *a0 = sa + (2 * ty) * ld, *a1 = a0 + ld, *b0 = sb + tx * ld, *b1 = b0 + 16 * ld;
-        float p[2][2] = {};
-        for (int i = 0; i < r.da; i += 4) {
-          const float4 x0_ = *reinterpret_cast<const float4*>(a0 + i), x1_ = *reinterpret_cast<const float4*>(a1 + i);
-          const float4 y0 = *reinterpret_cast<const float4*>(b0 + i), y1 = *reinterpret_cast<const float4*>(b1 + i);
-          p[0][0] = dot4(x0_, y0, p[0][0]);
-          p[0][1] = dot4(x0_, y1, p[0][1]);
-          p[1][0] = dot4(x1_, y0, p[1][0]);
-          p[1][1] = dot4(x1_, y1, p[1][1]);
-        }
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            const int i = 2 * ty + u, j = tx + 16 * w, gap = REV ? j - i : i - j;
-            sp[i * SPLD + j] = gap >= 0 && i < cn && j < cn ? r.w_intra * p[u][w] * lam[gap] : 0.f;
-          }
-        if (g == 0 || r.na > 1) {
-          o[0] = o[1] = make_float4(0.f, 0.f, 0.f, 0.f);
-          const float* x = sx + tx * 4;
-          for (int i = 0; i < r.da; i += 4) {
-            const float4 u0 = *reinterpret_cast<const float4*>(a0 + i), u1 = *reinterpret_cast<const float4*>(a1 + i);
-            const float4 s0 = *reinterpret_cast<const float4*>(x + i * SCOL), s1 = *reinterpret_cast<const float4*>(x + (i + 1) * SCOL),
-                         s2 = *reinterpret_cast<const float4*>(x + (i + 2) * SCOL), s3 = *reinterpret_cast<const float4*>(x + (i + 3) * SCOL);
-            axpy4(u0.x, s0, o[0]); axpy4(u0.y, s1, o[0]); axpy4(u0.z, s2, o[0]); axpy4(u0.w, s3, o[0]);
-            axpy4(u1.x, s0, o[1]); axpy4(u1.y, s1, o[1]); axpy4(u1.z, s2, o[1]); axpy4(u1.w, s3, o[1]);
-          }
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int i = 2 * ty + u, steps = REV ? cn - 1 - i : i + 1;
-            const float w = steps >= 0 && i < cn ? r.w_inter * lam[steps] : 0.f;
-            o[u].x *= w; o[u].y *= w; o[u].z *= w; o[u].w *= w;
-          }
-        }
+      for (int s = 0; s < slices; ++s) {
+        const int d0 = s * SDIM, width = min(SDIM, r.da - d0);
         __syncthreads();
-        const float *p0 = sp + (2 * ty) * SPLD, *p1 = p0 + SPLD, *v = sc + tx * 4;
-        for (int j = 0; j < cn; j += 4) {       // rows past the sequence are 0
-          const float4 u0 = *reinterpret_cast<const float4*>(p0 + j), u1 = *reinterpret_cast<const float4*>(p1 + j);
-          const float4 s0 = *reinterpret_cast<const float4*>(v + j * SCOL), s1 = *reinterpret_cast<const float4*>(v + (j + 1) * SCOL),
-                       s2 = *reinterpret_cast<const float4*>(v + (j + 2) * SCOL), s3 = *reinterpret_cast<const float4*>(v + (j + 3) * SCOL);
-          axpy4(u0.x, s0, o[0]); axpy4(u0.y, s1, o[0]); axpy4(u0.z, s2, o[0]); axpy4(u0.w, s3, o[0]);
-          axpy4(u1.x, s0, o[1]); axpy4(u1.y, s1, o[1]); axpy4(u1.z, s2, o[1]); axpy4(u1.w, s3, o[1]);
-        }
-        if (r.na > 1 || g == groups - 1) {
+        if (!STATES && (new_a || slices > 1))
+          simt_rows<T, SC>(sa, SLD, a + at * r.sa.s + (r.na > 1 ? g : 0) * r.sa.h + d0, r.sa.s, width, cn, wide_a);
+        if (new_b || slices > 1) simt_rows<T, SC>(sb, SLD, b + at * r.sb.s + (r.nb > 1 ? g : 0) * r.sb.h + d0, r.sb.s, width, cn, wide_b);
+        if (new_b && s == 0) simt_rows<T, SC>(sc, SCOL, c + at * r.sc.s + (r.nb > 1 ? g : 0) * r.sc.h + c0, r.sc.s, r.dc - c0, cn, wide_c);
+        __syncthreads();
+        if constexpr (!STATES) {
+          const float *ar = sa + R * ty * SLD, *br = sb + tx * SLD;
+          for (int i = 0; i < width; i += 4) {
+            Quad x[R];
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int i = 2 * ty + u, j = c0 + tx * 4;
-            if (i < cn && j < r.dc) {
-              T* w = out + (at + i) * r.so.s + (r.na > 1 ? g : 0) * r.so.h + j;
-              w[0] = Elem<T>::from_f(o[u].x); w[1] = Elem<T>::from_f(o[u].y); w[2] = Elem<T>::from_f(o[u].z); w[3] = Elem<T>::from_f(o[u].w);
+            for (int u = 0; u < R; ++u) x[u] = quad(ar + u * SLD + i);
+#pragma unroll
+            for (int w = 0; w < R; ++w) {
+              if (REV ? w < diagonal : w > diagonal) continue;
+              const Quad y = quad(br + 16 * w * SLD + i);
+#pragma unroll
+              for (int u = 0; u < R; ++u) p[u][w] = __ffma2_rn(x[u].hi, y.hi, __ffma2_rn(x[u].lo, y.lo, p[u][w]));
             }
           }
+          if (new_a)
+            for (int i = 0; i < width; i += 4) rows_by_four<R>(ar + i, SLD, sx + (d0 + i) * SCOL + tx * 4, o);
+          __syncthreads();
         }
-      }
-      if (r.nb > 1 || g == groups - 1) {      // the state: its old value has been used by every reader of this chunk
-        const float keep = r.nb > 1 && g > 0 ? 1.f : lam[cn];
-        for (int i = 4 * ty; i < r.da; i += 64) {
-          float4 acc[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        // this slice's rows of X: their old values have been used by every reader of the chunk
+        if (last_b && 4 * ty < width) {
+          const float keep = r.nb > 1 && g > 0 ? 1.f : lam[cn];
+          Quad x[4] = {};
 #pragma unroll 4
           for (int j = 0; j < cn; ++j) {
-            const float4 w4 = *reinterpret_cast<const float4*>(sb + j * ld + i), v = *reinterpret_cast<const float4*>(sc + j * SCOL + tx * 4);
-            const float w = lam[REV ? j + 1 : cn - 1 - j];
-            axpy4(w4.x * w, v, acc[0]); axpy4(w4.y * w, v, acc[1]); axpy4(w4.z * w, v, acc[2]); axpy4(w4.w * w, v, acc[3]);
+            const float4 w4 = *reinterpret_cast<const float4*>(sb + j * SLD + 4 * ty);
+            Quad v = quad(sc + j * SCOL + tx * 4);
+            const float2 w = twice(lam[REV ? j + 1 : cn - 1 - j]);
+            v.lo = __fmul2_rn(v.lo, w);
+            v.hi = __fmul2_rn(v.hi, w);
+            axpy(twice(w4.x), v, x[0]);
+            axpy(twice(w4.y), v, x[1]);
+            axpy(twice(w4.z), v, x[2]);
+            axpy(twice(w4.w), v, x[3]);
           }
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            float4& s = *reinterpret_cast<float4*>(sx + (i + k) * SCOL + tx * 4);
-            s = make_float4(fmaf(r.w_up, acc[k].x, keep * s.x), fmaf(r.w_up, acc[k].y, keep * s.y), fmaf(r.w_up, acc[k].z, keep * s.z),
-                            fmaf(r.w_up, acc[k].w, keep * s.w));
+            float4& to = *reinterpret_cast<float4*>(sx + (d0 + 4 * ty + k) * SCOL + tx * 4);
+            to = make_float4(fmaf(r.w_up, x[k].lo.x, keep * to.x), fmaf(r.w_up, x[k].lo.y, keep * to.y),
+                             fmaf(r.w_up, x[k].hi.x, keep * to.z), fmaf(r.w_up, x[k].hi.y, keep * to.w));
+          }
+        }
+      }
+      if constexpr (!STATES) {
+#pragma unroll
+        for (int u = 0; u < R; ++u) {
+          const int i = R * ty + u;
+          if (new_a) {
+            const int steps = REV ? cn - 1 - i : i + 1;
+            const float2 w = twice(i < cn ? r.w_inter * lam[max(steps, 0)] : 0.f);
+            o[u].lo = __fmul2_rn(o[u].lo, w);
+            o[u].hi = __fmul2_rn(o[u].hi, w);
+          }
+#pragma unroll
+          for (int w = 0; w < R; ++w) {
+            const int j = tx + 16 * w, gap = REV ? j - i : i - j;
+            sp[i * SPLD + j] = gap >= 0 && i < cn && j < cn ? r.w_intra * (p[u][w].x + p[u][w].y) * lam[gap] : 0.f;
+          }
+        }
+        __syncwarp();      // a warp reads its own rows of P only
+        const int j1 = REV ? cn : min(cn, R * (ty + 1));      // rows past the sequence are 0
+        for (int j = REV ? R * ty & ~3 : 0; j < j1; j += 4) rows_by_four<R>(sp + R * ty * SPLD + j, SPLD, sc + j * SCOL + tx * 4, o);
+        if (last_a && c0 + tx * 4 < r.dc) {
+#pragma unroll
+          for (int u = 0; u < R; ++u) {
+            const int i = R * ty + u;
+            if (i >= cn) continue;
+            T* to = out + (at + i) * r.so.s + (r.na > 1 ? g : 0) * r.so.h + c0 + tx * 4;
+            const Four<T> y{{Elem<T>::from_f(o[u].lo.x), Elem<T>::from_f(o[u].lo.y), Elem<T>::from_f(o[u].hi.x), Elem<T>::from_f(o[u].hi.y)}};
+            if (wide_o) *reinterpret_cast<Four<T>*>(to) = y;
+            else to[0] = y.x[0], to[1] = y.x[1], to[2] = y.x[2], to[3] = y.x[3];
           }
         }
       }
@@ -349,21 +402,27 @@ __global__ void __launch_bounds__(256) lin_join_kernel(const LinSeqs q, float* w
   if (pool.out) reinterpret_cast<float4*>(pool.out)[at] = x;
 }
 
-template <typename T>
-int simt_launch(const LinSeqs& q, const LinRole& r, bool rev, bool states, const float* ws, float* ws_out, const LinPool& pool,
-                cudaStream_t st) {
-  const int bytes = simt_smem_floats(r.da) * 4, blocks_c = (r.dc + SCOL - 1) / SCOL;
+// chunks of 64 tokens, or of 32 where segments are no longer than that or two blocks of 64 do not fit on an SM (fa_linear_plan has the times)
+template <typename T, int SC>
+int simt_go(const LinSeqs& q, const LinRole& r, bool rev, bool states, const float* ws, float* ws_out, const LinPool& pool,
+            cudaStream_t st) {
+  const int blocks_c = (r.dc + SCOL - 1) / SCOL;
   const long long grid = (long long)q.slots * q.nhk * blocks_c;
   FA_CHECK_ARG(grid < (1ll << 31) && (long long)q.batch * q.nhk < (1ll << 31), "linear attention: %lld blocks", grid);
   const auto go = [&](auto kernel, unsigned long long* done) -> int {
-    if (int rc = ensure_smem((const void*)kernel, simt_smem_floats(256) * 4, done)) return rc;
-    kernel<<<(int)grid, SIMT_THREADS, bytes, st>>>(q, r, ws, ws_out, pool, blocks_c);
+    if (int rc = ensure_smem((const void*)kernel, simt_smem_floats<SC>(256) * 4, done)) return rc;
+    kernel<<<(int)grid, SIMT_THREADS, simt_smem_floats<SC>(r.da) * 4, st>>>(q, r, ws, ws_out, pool, blocks_c);
     count_launch();
     return cuda_status(cudaGetLastError(), "linear attention launch");
   };
   static unsigned long long done[4] = {};
-  if (states) return rev ? go(lin_simt_kernel<T, true, true>, done) : go(lin_simt_kernel<T, false, true>, done + 1);
-  return rev ? go(lin_simt_kernel<T, true, false>, done + 2) : go(lin_simt_kernel<T, false, false>, done + 3);
+  if (states) return rev ? go(lin_simt_kernel<T, SC, true, true>, done) : go(lin_simt_kernel<T, SC, false, true>, done + 1);
+  return rev ? go(lin_simt_kernel<T, SC, true, false>, done + 2) : go(lin_simt_kernel<T, SC, false, false>, done + 3);
+}
+template <typename T>
+int simt_launch(const LinSeqs& q, const LinRole& r, bool rev, bool states, const float* ws, float* ws_out, const LinPool& pool,
+                cudaStream_t st) {
+  return q.seg_len <= 32 || r.da > SIMT_WIDE ? simt_go<T, 32>(q, r, rev, states, ws, ws_out, pool, st) : simt_go<T, 64>(q, r, rev, states, ws, ws_out, pool, st);
 }
 
 template <typename T>
@@ -475,12 +534,15 @@ extern "C" FA_API long long fa_linear_plan(int batch, int S, long long total, in
     *nseg = (int)((S + (long long)*seg_len - 1) / *seg_len);
     return workspace(total, batch, *seg_len, *nseg, NH / gqa, dk, dv, true);
   } else {
-    // As many segments as give every SM four blocks, none shorter than a chunk of 32 tokens (each costs a state written and read
-    // again, and its keys and values read twice): 8 heads x 512 tokens took 5 us a kernel in 16 segments and 15 in 4.
-    const long long cols = (dv + 63) / 64, small = (tokens + 31) / 32;
-    const long long n = std::max(1ll, std::min(small, 4 * sms / std::max(1ll, states * cols)));
-    unit = 32;
-    best = n;
+    // Segments of one chunk of 32 tokens while two blocks an SM can take them all (each costs a state written and read again, and its
+    // keys and values read twice): fp32, 8 heads of 64, 512 tokens in 21 us, against 26 with chunks of 64.  Past that chunks of 64, in as
+    // many segments as run at once: 2048 tokens 39 against 53 us, 4 x 4096 tokens of 16 heads 429 against 586.
+    // Dims of more than 160 keep to chunks of 32 (with 64 an SM holds one block: 2154 against 1580 us for 4096 tokens of
+    // 16 heads of 256), and to four blocks an SM, two waves of them.
+    const long long blocks = std::max(1ll, states * ((dv + 63) / 64)), small = (tokens + 31) / 32;
+    const bool large = std::max(dk, dv) > SIMT_WIDE;
+    unit = large || small <= 2 * sms / blocks ? 32 : 64;
+    best = std::max(1ll, std::min((tokens + unit - 1) / unit, (large ? 4 : 2) * sms / blocks));
   }
   const long long units = (tokens + unit - 1) / unit;
   long long len = (units + best - 1) / best * unit;

@@ -114,6 +114,33 @@ def test_strided_inputs(dt):
     check_run(DT[dt], [3, 200, 77], 4, 2, 64, 64, decays(2), False, True, strided=True)
 
 
+@pytest.mark.parametrize("dt,dk,dv", [("fp32", 64, 64), ("fp32", 128, 72), ("fp32", 200, 136), ("bf16", 160, 160), ("fp16", 256, 8)])
+@pytest.mark.parametrize("hq,hk", [(4, 4), (6, 2), (2, 2)])
+def test_cuda_core_chunks_of_64(dt, dk, dv, hq, hk):
+    """More heads than the SMs hold blocks of (chunks of 64 tokens), and one long sequence (segments of several chunks)."""
+    cols = (dv + 63) // 64
+    check_run(DT[dt], [70] * (300 // (hk * cols) + 1), hq, hk, dk, dv, decays(hk), True, False)
+    lens = [0, 1, 63, 64, 65, 130, 31]
+    check_run(DT[dt], lens * (600 // (hk * cols * len(lens)) + 1), hq, hk, dk, dv, decays(hk), True, True)
+    if hq == hk == 2:
+        check_run(DT[dt], [12000 // cols], hq, hk, dk, dv, decays(hk), True, False, grads=dt == "fp32")
+
+
+@pytest.mark.parametrize("dt,d", [("fp32", 64), ("fp32", 136), ("bf16", 136)])
+@pytest.mark.parametrize("n", [150, 5000])
+def test_cuda_core_rows_at_odd_places(dt, d, n):
+    """Elements one at a time where four are not on their boundary: the same bits."""
+    dt, h = DT[dt], 4
+    wide = rand(0, 2, n, 3 * h * d + 3, dtype=dt)
+    q, k, v = (wide[..., 1 + i * h * d:1 + (i + 1) * h * d].unflatten(-1, (h, d)).requires_grad_() for i in range(3))
+    near = [x.detach().clone(memory_format=torch.contiguous_format).requires_grad_() for x in (q, k, v)]
+    do = rand(1, 2, n, h, d + 1, dtype=dt)[..., 1:]
+    a, b = fa.linear_attn_func(q, k, v, decays(h)), fa.linear_attn_func(*near, decays(h))
+    assert torch.equal(a, b)
+    for x, y in zip(torch.autograd.grad(a, (q, k, v), do), torch.autograd.grad(b, near, do.contiguous())):
+        assert torch.equal(x, y)
+
+
 @pytest.mark.parametrize("dt", ["bf16", "fp16"])
 def test_rows_off_sixteen_bytes_and_repeated_heads(dt):
     """Slices at odd places, a head that serves all, a gradient that is one row for all tokens: the same bits as of whole copies."""
