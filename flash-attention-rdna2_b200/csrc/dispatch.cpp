@@ -726,6 +726,11 @@ FaStrides rows_of_heads(const torch::Tensor& x) {
   return FaStrides{x.stride(0), x.stride(2), x.stride(1)};
 }
 
+// x was written in place: a graph that saved it then fails in its backward pass instead of reading the new values
+void written(const torch::Tensor& x) {
+  if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
+}
+
 // x with a contiguous last dimension and, for the chunked kernels of 16 bits (`tma`), as the tensor maps need it: rows on 16-byte boundaries
 // and no dimension that repeats itself.  Otherwise the CUDA-core
 // kernels would have to run: 2 x 4096 tokens, 16 heads of 128 take 83 us as they are, 204 with all three copied, and 740 there.
@@ -843,6 +848,7 @@ std::tuple<torch::Tensor, torch::Tensor, int64_t, int64_t> linear_fwd(
     p.states = floats ? work.data_ptr<float>() : nullptr;
   }
   if (p.batch > 0) check(fa_linear_launch(&p, dt_of(q), cur_stream(q)), "linear attention");
+  if (so) written(*so);
   return {out, work, p.seg_len, p.nseg};
 }
 
@@ -946,6 +952,7 @@ std::tuple<torch::Tensor, torch::Tensor> rotary_qk(torch::Tensor q, torch::Tenso
   p.interleaved = interleaved ? 1 : 0; p.inverse = inverse ? 1 : 0;
   p.factor = (float)factor;
   if (q.numel() > 0) check(fa_rotary_qk_launch(&p, dt_of(q), cur_stream(q)), "rotary (q and k)");
+  if (inplace) written(q), written(k);
   return {qo, ko};
 }
 

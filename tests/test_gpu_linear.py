@@ -497,6 +497,21 @@ def test_far_addresses():
         assert torch.equal(pool[[slots - 1, 0]], small)
 
 
+@pytest.mark.parametrize("other", [False, True])
+def test_state_saved_for_a_gradient_and_then_written(other):
+    q, k, v = (rand(i, 2, 40, 2, 64, dtype=torch.bfloat16).requires_grad_() for i in range(3))
+    state, g = rand(4, 2, 2, 64, 64), decays(2)
+    near = [x.detach() for x in (q, k, v)]
+    out = fa.linear_attn_func(q, k, v, g, initial_state=state)
+    fa.linear_attn_with_state(*near, state.clone() if other else state, g, state_out=state if other else None)
+    with pytest.raises(RuntimeError, match="inplace"):
+        out.sum().backward()
+    with torch.inference_mode():
+        pool = torch.zeros(2, 2, 64, 64, device="cuda")
+        fa.linear_attn_with_state(*near, pool, g)
+    assert pool.any()
+
+
 @pytest.mark.parametrize("bad", ["fp64", "heads", "dims", "batch", "decay", "decay_grad", "state", "state_grad", "slots", "index", "cpu", "dim7", "rank", "device_state", "overlap"])
 def test_refusals(bad):
     b, n, h, d = 2, 20, 4, 64

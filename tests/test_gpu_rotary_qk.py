@@ -172,6 +172,21 @@ def test_non_finite_values_stay_in_their_pair():
     assert torch.equal(got[fine], want[fine]) and not got[~fine].isfinite().any()
 
 
+def test_saved_for_a_gradient_and_then_turned_in_place():
+    freq, _ = scaled_inv_freq(64, device="cuda")
+    q, k, w = rand(1, 2, 3, 4, 64), rand(2, 2, 3, 2, 64), torch.ones(64, device="cuda", requires_grad=True)
+    for x in (q, k):
+        y = (x * w).sum()
+        apply_rotary_emb_qk(q, k, freq, inplace=True)
+        with pytest.raises(RuntimeError, match="inplace"):
+            y.backward()
+    with torch.inference_mode():
+        q, k = q.clone(), k.clone()
+        before = q.clone()
+        apply_rotary_emb_qk(q, k, freq, seqlen_offsets=1, inplace=True)
+        assert not torch.equal(before, q)
+
+
 @pytest.mark.parametrize("bad", ["cpu", "types", "heads", "freq", "freq_grad", "pos", "pos_float", "both", "inplace_grad", "overlap", "same", "rank", "dims"])
 def test_refusals(bad):
     freq, _ = scaled_inv_freq(64, device="cuda")
