@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(STEP_THREADS, ROWS > 8 ? 3 : 6)
 // Bound by shared memory's reads: a thread's tile is SC/16 rows by 4 columns, read four elements at a time (rows padded to an odd
 // number of 16-byte units, so that the lanes of a quarter warp meet different banks).  With 64 tokens eight 16-byte reads feed
 // 64 multiply-adds, with 32 tokens six feed 32; pairs that the order masks are neither multiplied nor read, and two adjacent
-// elements go through one packed multiply-add.  fp32, 4 x 4096 tokens, 16 heads of 64: 429 us, 15 TFLOP/s (with 2 x 4 outputs
+// elements go through one packed multiply-add.  fp32, 4 x 4096 tokens, 16 heads of 64: 430 us, 15 TFLOP/s (with 2 x 4 outputs
 // a thread and whole rows of a and b in shared memory it was 809).
 // =====================================================================================
 constexpr int SCOL = 64, SDIM = 64, SLD = SDIM + 4, SIMT_THREADS = 256;
@@ -211,6 +211,26 @@ __device__ __forceinline__ void simt_rows(float* to, int ld, const T* from, long
     *reinterpret_cast<float4*>(to + j * ld + i) = x;
   }
 }
+__device__ __forceinline__ void copy16(float* to, const float* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy16_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// f(element of X in shared memory, place in the state, whether it exists) for every four elements that lie together in the state: of
+// a row of X, or (`across`, stored transposed) of a column, where a warp takes 8 columns by 4 units so that both sides go by 32 bytes or more
+template <typename F, typename G>
+__device__ __forceinline__ void simt_state(const LinRole& r, int c0, F along, G across, float* sx) {
+  const int n4 = r.da / 4;
+#pragma unroll 4
+  for (int e = threadIdx.x; e < r.da * (SCOL / 4); e += SIMT_THREADS) {
+    if (r.transposed) {
+      const int i = e / 8 % n4 * 4, j = e / 8 / n4 * 8 + (e & 7);
+      across(sx + i * SCOL + j, (long long)(c0 + j) * r.da + i, c0 + j < r.dc);
+    } else {
+      const int i = e / (SCOL / 4), j = e % (SCOL / 4) * 4;
+      along(sx + i * SCOL + j, (long long)i * r.dc + c0 + j, c0 + j < r.dc);
+    }
+  }
+}
 // four elements at a time: base and strides on their boundary
 template <typename T>
 __device__ __forceinline__ bool simt_wide(const void* p, const FaStrides& s) {
@@ -256,10 +276,16 @@ __global__ void __launch_bounds__(SIMT_THREADS, SC == 32 ? 3 : 2)
     if (ws) x0 = ws + segs * per;
     else if (pool.in && !(pool.seen && pool.seen[z] <= 0)) x0 = pool.in + ((long long)slot * q.nhk + h) * per;
   }
-  for (int e = tid; e < r.da * SCOL; e += SIMT_THREADS) {
-    const int i = e / SCOL, j = c0 + e % SCOL;
-    sx[e] = x0 && j < r.dc ? x0[r.transposed ? (long long)j * r.da + i : (long long)i * r.dc + j] : 0.f;
-  }
+  simt_state(r, c0, [&](float* to, long long from, bool real) {
+    if (real && x0) copy16(to, x0 + from);      // in flight while the first rows are loaded
+    else *reinterpret_cast<float4*>(to) = make_float4(0.f, 0.f, 0.f, 0.f);
+  }, [&](float* to, long long from, bool real) {
+    const float4 x = real && x0 ? *reinterpret_cast<const float4*>(x0 + from) : make_float4(0.f, 0.f, 0.f, 0.f);
+    to[0] = x.x, to[SCOL] = x.y, to[2 * SCOL] = x.z, to[3 * SCOL] = x.w;
+  }, sx);
+  float* x1 = nullptr;
+  if (STATES) x1 = ws_out + segs * per;
+  else if (!ws && pool.out) x1 = pool.out + ((long long)slot * q.nhk + h) * per;
   const bool wide_a = simt_wide<T>(r.a, r.sa), wide_b = simt_wide<T>(r.b, r.sb), wide_c = simt_wide<T>(r.c, r.sc),
              wide_o = simt_wide<T>(r.out, r.so);
   const int chunks = (t1 - t0 + SC - 1) / SC, groups = STATES ? r.nb : max(r.na, r.nb), slices = (r.da + SDIM - 1) / SDIM;
@@ -282,6 +308,7 @@ __global__ void __launch_bounds__(SIMT_THREADS, SC == 32 ? 3 : 2)
           simt_rows<T, SC>(sa, SLD, a + at * r.sa.s + (r.na > 1 ? g : 0) * r.sa.h + d0, r.sa.s, width, cn, wide_a);
         if (new_b || slices > 1) simt_rows<T, SC>(sb, SLD, b + at * r.sb.s + (r.nb > 1 ? g : 0) * r.sb.h + d0, r.sb.s, width, cn, wide_b);
         if (new_b && s == 0) simt_rows<T, SC>(sc, SCOL, c + at * r.sc.s + (r.nb > 1 ? g : 0) * r.sc.h + c0, r.sc.s, r.dc - c0, cn, wide_c);
+        copy16_wait();
         __syncthreads();
         if constexpr (!STATES) {
           const float *ar = sa + R * ty * SLD, *br = sb + tx * SLD;
@@ -301,8 +328,8 @@ __global__ void __launch_bounds__(SIMT_THREADS, SC == 32 ? 3 : 2)
             for (int i = 0; i < width; i += 4) rows_by_four<R>(ar + i, SLD, sx + (d0 + i) * SCOL + tx * 4, o);
           __syncthreads();
         }
-        // this slice's rows of X: their old values have been used by every reader of the chunk
-        if (last_b && 4 * ty < width) {
+        // this slice's rows of X: their old values have been used by every reader of the chunk (the last chunk's are kept only if asked for)
+        if (last_b && (x1 || m < chunks - 1) && 4 * ty < width) {
           const float keep = r.nb > 1 && g > 0 ? 1.f : lam[cn];
           Quad x[4] = {};
 #pragma unroll 4
@@ -358,15 +385,14 @@ __global__ void __launch_bounds__(SIMT_THREADS, SC == 32 ? 3 : 2)
       }
     }
   }
-  float* x1 = nullptr;
-  if (STATES) x1 = t1 > t0 ? ws_out + segs * per : nullptr;
-  else if (!ws && pool.out) x1 = pool.out + ((long long)slot * q.nhk + h) * per;
   if (!x1) return;
+  copy16_wait();
   __syncthreads();
-  for (int e = tid; e < r.da * SCOL; e += SIMT_THREADS) {
-    const int i = e / SCOL, j = c0 + e % SCOL;
-    if (j < r.dc) x1[r.transposed ? (long long)j * r.da + i : (long long)i * r.dc + j] = sx[e];
-  }
+  simt_state(r, c0, [&](const float* from, long long to, bool real) {
+    if (real) *reinterpret_cast<float4*>(x1 + to) = *reinterpret_cast<const float4*>(from);
+  }, [&](const float* from, long long to, bool real) {
+    if (real) *reinterpret_cast<float4*>(x1 + to) = make_float4(from[0], from[SCOL], from[2 * SCOL], from[3 * SCOL]);
+  }, sx);
 }
 
 // =====================================================================================
@@ -535,9 +561,9 @@ extern "C" FA_API long long fa_linear_plan(int batch, int S, long long total, in
     return workspace(total, batch, *seg_len, *nseg, NH / gqa, dk, dv, true);
   } else {
     // Segments of one chunk of 32 tokens while two blocks an SM can take them all (each costs a state written and read again, and its
-    // keys and values read twice): fp32, 8 heads of 64, 512 tokens in 21 us, against 26 with chunks of 64.  Past that chunks of 64, in as
-    // many segments as run at once: 2048 tokens 39 against 53 us, 4 x 4096 tokens of 16 heads 429 against 586.
-    // Dims of more than 160 keep to chunks of 32 (with 64 an SM holds one block: 2154 against 1580 us for 4096 tokens of
+    // keys and values read twice): fp32, 8 heads of 64, 512 tokens in 19 us, against 23 with chunks of 64.  Past that chunks of 64, in as
+    // many segments as run at once: 2048 tokens 35 against 40 us, 4 x 4096 tokens of 16 heads 430 against 543.
+    // Dims of more than 160 keep to chunks of 32 (with 64 an SM holds one block: 2085 against 1564 us for 4096 tokens of
     // 16 heads of 256), and to four blocks an SM, two waves of them.
     const long long blocks = std::max(1ll, states * ((dv + 63) / 64)), small = (tokens + 31) / 32;
     const bool large = std::max(dk, dv) > SIMT_WIDE;
