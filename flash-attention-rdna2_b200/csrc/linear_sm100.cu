@@ -102,7 +102,8 @@ __device__ __forceinline__ void row_factors(float2* w, const float* lam, float t
     w[i].y = j + 1 < cn ? times * lam[REV ? j + 2 : cn - 2 - j] : 0.f;
   }
 }
-template <bool BF16, int TERMS, int N>
+// With LO_SHIFT the second term is stored 2^LO_SHIFT times as large.
+template <bool BF16, int TERMS, int N, int LO_SHIFT = 0>
 __device__ __forceinline__ void decay_rows(uint32_t tile, uint32_t bt, const float2* w, int qd, int first, int lane, int cn) {
 #pragma unroll 1
   for (int half = 0; half < 2; ++half) {          // 16 dims each
@@ -126,6 +127,7 @@ __device__ __forceinline__ void decay_rows(uint32_t tile, uint32_t bt, const flo
         for (int u = 0; u < TERMS; ++u) {
           o[u][i] = pack2<BF16>(x.x, x.y);
           if (u + 1 < TERMS) x = rest2<BF16>(x, o[u][i]);
+          if (LO_SHIFT && u == 0) x = __fmul2_rn(x, make_float2(float(1 << LO_SHIFT), float(1 << LO_SHIFT)));
         }
       }
 #pragma unroll
@@ -768,13 +770,15 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 // =====================================================================================
 // states: what a segment adds to the state, X = sum_j (lam^m_j b_j)^T c_j with powers up to the segment's own end, so that
 // nothing is scaled on the way.  The result is a state that a caller may keep, in fp32, so the decayed rows enter as three bf16 numbers
-// (2^-24 of a term) or two fp16 ones (2^-22).  The tensor cores truncate each accumulation; so every item is summed from 0, its small
+// (2^-24 of a term) or two fp16 ones (2^-22).  fp16's smallest step is 2^-24, which fast decays meet; so the second fp16 number is what
+// the first left over times 2^11 (at most half a step of the first: it cannot overflow), and its sum is scaled back by the first
+// MMA on top of it.  The tensor cores truncate each accumulation; so every item is summed from 0, its small
 // terms first (only the eight steps of the largest one then cut at the sum's full size), and items are added in registers, to nearest.
 // One accumulator over a whole segment had left 2e-6 of the state.  Bound by reading b and c once.
 // =====================================================================================
 template <int D, bool BF16>
 struct StCfg {
-  static constexpr int NCH = D / 64, TILE = C * D * 2, NS = D == 128 ? 3 : 4, TERMS = BF16 ? 3 : 2;
+  static constexpr int NCH = D / 64, TILE = C * D * 2, NS = D == 128 ? 3 : 4, TERMS = BF16 ? 3 : 2, LO_SHIFT = BF16 ? 0 : 11;
   static constexpr int OFF_T = 0, OFF_BAR = NS * 2 * TILE, OFF_LAM = OFF_BAR + 128;
   static constexpr int SMEM = OFF_LAM + 132 * 4 + 1024;
   static constexpr uint32_t X_COL = 0, BT_COL = 128, BT_COLS = 192;      // two buffers of decayed rows
@@ -861,8 +865,10 @@ __global__ void __launch_bounds__(NTHREADS_ST, 1)
 #pragma unroll
         for (int w = K::TERMS - 1; w >= 0; --w)
 #pragma unroll
-          for (int kk = 0; kk < C / 16; ++kk)
-            mma_ts(tmem + K::X_COL, bt + 64 * w + 8 * kk, desc_add(d, kk * 128), ID, kk > 0 || w < K::TERMS - 1);
+          for (int kk = 0; kk < C / 16; ++kk) {
+            if (K::LO_SHIFT && w == 0 && kk == 0) mma_ts_onto<K::LO_SHIFT>(tmem + K::X_COL, bt, d, ID);
+            else mma_ts(tmem + K::X_COL, bt + 64 * w + 8 * kk, desc_add(d, kk * 128), ID, kk > 0 || w < K::TERMS - 1);
+          }
         mma_commit(bar + StBz::EMPTY + 8 * s);
         mma_commit(bar + StBz::DONE);
       }
@@ -906,7 +912,7 @@ __global__ void __launch_bounds__(NTHREADS_ST, 1)
       float2 w[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) w[k] = __fmul2_rn(w_rows[k], make_float2(far, far));
-      if (qd * 32 < D) decay_rows<BF16, K::TERMS, 2>(sbase + tile(i), la + K::BT_COL + (i & 1) * K::BT_COLS, w, qd, 32 * qr, lane, cn);
+      if (qd * 32 < D) decay_rows<BF16, K::TERMS, 2, K::LO_SHIFT>(sbase + tile(i), la + K::BT_COL + (i & 1) * K::BT_COLS, w, qd, 32 * qr, lane, cn);
       tc_wait_st();
       tc_fence_before();
       mbar_arrive(bar + StBz::BT_READY + 8 * (i & 1));

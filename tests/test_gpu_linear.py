@@ -99,6 +99,14 @@ def test_decays(dt, g):
 
 
 @pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("g", ["-7", "-9", "-12", "-16"])
+def test_states_of_fast_decays(dt, g):
+    """Rows whose decay takes them below fp16's smallest step, next to elements of the state that are as small."""
+    check_run(DT[dt], list(range(1, 41)), 8, 8, 72, 64, decays(8, g), True, True)
+    check_run(DT[dt], [130], 4, 4, 128, 128, decays(4, g), True, False)
+
+
+@pytest.mark.parametrize("dt", ALL)
 def test_many_segments(dt):
     check_run(DT[dt], [2500], 2, 1, 64, 64, decays(1, "-0.01"), True, False)
     check_run(DT[dt], [2500, 40, 1300], 2, 2, 128, 128, decays(2), True, True)
