@@ -188,8 +188,8 @@ class _RotaryQkFn(torch.autograd.Function):
 def apply_rotary_emb_qk(q, k, inv_freq, positions=None, *, seqlen_offsets=0, interleaved=False, factor=1.0, inplace=False):
     """Rotate q and k, (batch, seqlen, heads, headdim) or packed (total, heads, headdim), in one pass; (q, k).
 
-    inv_freq (rotary_dim / 2,): radians for each position, best in fp64 (scaled_inv_freq makes them); the first rotary_dim dims turn,
-    the rest pass through.  positions (batch, seqlen) or (total,), int32 or int64: each token's own position, any
+    inv_freq (rotary_dim / 2,): radians for each position, best in fp64 (scaled_inv_freq makes them); the first rotary_dim dims (up to 256)
+    turn, the rest pass through.  positions (batch, seqlen) or (total,), int32 or int64: each token's own position, any
     whole number, without a table to end; without them token t sits at seqlen_offsets + t (an int, or (batch,)).  The angle is exact
     however far the position; cos and sin are multiplied by factor and applied in fp32 with one rounding at the end (apply_rotary_emb
     rounds tables and products to the inputs' type instead, as torch arithmetic does).  interleaved pairs dims (2i, 2i + 1) instead of
