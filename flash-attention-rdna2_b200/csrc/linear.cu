@@ -397,8 +397,8 @@ __global__ void __launch_bounds__(SIMT_THREADS, SC == 32 ? 3 : 2)
 
 // =====================================================================================
 // Joining segments: ws[n] holds what segment n adds from a state of 0; it becomes the state that enters the segment, and
-// the state past the last one goes to the pool.  One thread a float4 of the state; the next segment's load is in flight
-// while the running state is scaled.
+// the state past the last one goes to the pool.  A sequence without tokens has no segment: its state goes through untouched.
+// One thread a float4 of the state; the next segment's load is in flight while the running state is scaled.
 // =====================================================================================
 template <bool REV>
 __global__ void __launch_bounds__(256) lin_join_kernel(const LinSeqs q, float* ws, const LinPool pool, const int per4) {
@@ -408,14 +408,14 @@ __global__ void __launch_bounds__(256) lin_join_kernel(const LinSeqs q, float* w
   if (slot < 0 || e >= per4) return;
   const LinSpan span = lin_span(q, z);
   const float g2 = lin_log2_decay(q.log_decay, h);
-  const int real = max(1, lin_segments(q, span.len));
+  const int real = lin_segments(q, span.len);
   const long long step = (long long)q.nhk * per4;      // from one segment's state to the next
   float4* w = reinterpret_cast<float4*>(ws) + lin_first_slot(q, z, span.row0) * step + (long long)h * per4 + e;
   const long long at = ((long long)slot * q.nhk + h) * per4 + e;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
   if (pool.in && !(pool.seen && pool.seen[z] <= 0)) x = reinterpret_cast<const float4*>(pool.in)[at];
   const auto seg = [&](int m) { return REV ? real - 1 - m : m; };
-  float4 u = span.len > 0 ? w[seg(0) * step] : make_float4(0.f, 0.f, 0.f, 0.f);
+  float4 u = real > 0 ? w[seg(0) * step] : make_float4(0.f, 0.f, 0.f, 0.f);
   for (int m = 0; m < real; ++m) {
     const int n = seg(m);
     float4 next = u;

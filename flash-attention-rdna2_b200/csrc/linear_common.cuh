@@ -64,7 +64,7 @@ struct LinSpan {
   int len;               // tokens of the sequence
 };
 
-__device__ __forceinline__ LinSpan lin_span(const LinSeqs& q, int z) {
+__host__ __device__ __forceinline__ LinSpan lin_span(const LinSeqs& q, int z) {
   LinSpan s{0, q.S};
   if (q.cu) {
     const long long lo = min(max((long long)q.cu[z], 0ll), q.total);
@@ -74,14 +74,15 @@ __device__ __forceinline__ LinSpan lin_span(const LinSeqs& q, int z) {
   }
   return s;
 }
-__device__ __forceinline__ long long lin_first_slot(const LinSeqs& q, int z, long long row0) {
+__host__ __device__ __forceinline__ long long lin_first_slot(const LinSeqs& q, int z, long long row0) {
   return q.nseg == 1 ? z : q.cu ? row0 / q.seg_len + z : (long long)z * q.nseg;
 }
-__device__ __forceinline__ int lin_segments(const LinSeqs& q, int len) {
-  return q.nseg == 1 ? 1 : (len + q.seg_len - 1) / q.seg_len;
+// an empty sequence has none, and its first slot may be the one past the last
+__host__ __device__ __forceinline__ int lin_segments(const LinSeqs& q, int len) {
+  return len <= 0 ? 0 : q.nseg == 1 ? 1 : (int)(((long long)len + q.seg_len - 1) / q.seg_len);
 }
 // the sequence of a slot and its tokens [t0, t1); t0 == t1 where the slot has none
-__device__ __forceinline__ LinSpan lin_segment(const LinSeqs& q, int slot, int& z, int& t0, int& t1) {
+__host__ __device__ __forceinline__ LinSpan lin_segment(const LinSeqs& q, int slot, int& z, int& t0, int& t1) {
   z = q.nseg == 1 ? slot : slot / q.nseg;
   if (q.nseg > 1 && q.cu) {
     int hi = q.batch;                      // the last sequence whose first slot is not past this one

@@ -1,0 +1,75 @@
+"""Linear attention on the GPU at the edges of what it is given, against the 64-bit formulas of lin_ref."""
+import ctypes as C
+
+import pytest
+import torch
+
+import fa_abi as A
+import fable_attn as fa
+import lin_ref as R
+from test_gpu_linear import ALL, DT, cum, decays, inputs, rand
+from test_linear_cpu import FaLinearBwdParams, FaLinearParams
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------ one sequence without tokens, behind the rows
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("cu", [[512, 512], [0, 0], [256, 256], [612, 712], [384, 512]])
+def test_one_empty_sequence_leaves_the_workspace_alone(dt, cu):
+    """The C entries with a workspace of exactly fa_linear_plan floats: what lies behind it stays as it was, the last state is
+    the first one, and so are their gradients."""
+    L, dev = A.lib(), "cuda"
+    L.fa_linear_plan.restype = C.c_longlong
+    n, h, d = 512, 8, 128
+    seg, nseg = C.c_int(), C.c_int()
+    floats = L.fa_linear_plan(1, n, C.c_longlong(n), h, 1, d, d, A.DT[dt], C.byref(seg), C.byref(nseg))
+    assert nseg.value > 1 and floats == -(-n // seg.value) * h * d * d
+    guard = 2 * h * d * d
+    # room for a slot on each side, so that even a write past the workspace stays in this test's memory
+    states, work = (torch.full((floats + 2 * guard,), 7.0, device=dev) for _ in range(2))
+    q, k, v, do = (rand(i, n, h, d, dtype=DT[dt]) for i in range(4))
+    o, dq, dk, dv = (torch.full_like(q, 3.0) for _ in range(4))
+    s0, ds = rand(5, 1, h, d, d), rand(6, 1, h, d, d)
+    s1, ds0 = torch.empty_like(s0), torch.empty_like(s0)
+    g, cut = decays(h), torch.tensor(cu, dtype=torch.int32, device=dev)
+    rows = A.FaStrides(0, d, h * d)
+    inside = lambda x: A.ptr(x[guard:])
+    p = FaLinearParams(struct_size=C.sizeof(FaLinearParams), q=A.ptr(q), k=A.ptr(k), v=A.ptr(v), o=A.ptr(o), sQ=rows, sK=rows, sV=rows, sO=rows,
+                       log_decay=A.ptr(g), state_in=A.ptr(s0), state_out=A.ptr(s1), slots=1, cu=A.ptr(cut), total=n, batch=1, S=n, NH=h, gqa=1,
+                       dk=d, dv=d, scale=0.125, seg_len=seg.value, nseg=nseg.value, keep_states=1, states=inside(states))
+    st = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    A.check(L.fa_linear_launch(C.byref(p), A.DT[dt], st))
+    b = FaLinearBwdParams(struct_size=C.sizeof(FaLinearBwdParams), q=A.ptr(q), k=A.ptr(k), v=A.ptr(v), dO=A.ptr(do), dQ=A.ptr(dq), dK=A.ptr(dk),
+                          dV=A.ptr(dv), sQ=rows, sK=rows, sV=rows, sdO=rows, sdQ=rows, sdK=rows, sdV=rows, log_decay=A.ptr(g), initial=A.ptr(s0),
+                          dfinal=A.ptr(ds), dinitial=A.ptr(ds0), cu=A.ptr(cut), total=n, batch=1, S=n, NH=h, gqa=1, dk=d, dv=d, scale=0.125,
+                          seg_len=seg.value, nseg=nseg.value, states=inside(states), work=inside(work))
+    A.check(L.fa_linear_backward_launch(C.byref(b), A.DT[dt], st))
+    torch.cuda.synchronize()
+    for x in (states, work):
+        assert bool((x[:guard] == 7).all()) and bool((x[guard + floats:] == 7).all())
+    lo, hi = min(cu[0], n), min(cu[1], n)
+    for x in (o, dq, dk, dv):
+        assert not x[:lo].any() and not x[hi:].any()
+    if hi == lo:
+        assert torch.equal(s1, s0) and torch.equal(ds0, ds)
+        return
+    ref = R.both(q[lo:hi], k[lo:hi], v[lo:hi], g, 0.125, s0[0], do[lo:hi], ds[0])
+    for x, (want, amp), name in zip((o[lo:hi], s1[0], dq[lo:hi], dk[lo:hi], dv[lo:hi], ds0[0]), ref, ("o", "final", "dq", "dk", "dv", "dinitial")):
+        R.close(x, want, amp, hi - lo, (d, d), g, DT[dt], name)
+
+
+@pytest.mark.parametrize("dt", ALL)
+def test_one_empty_sequence(dt):
+    n, h, d = 512, 8, 128
+    q, k, v = (x.requires_grad_() for x in inputs(DT[dt], [n], h, h, d, d))
+    s0, ds, g = rand(5, 1, h, d, d).requires_grad_(), rand(6, 1, h, d, d), decays(h)
+    cu = torch.tensor([n, n], dtype=torch.int32, device="cuda")
+    out, final = fa.linear_attn_varlen_func(q, k, v, g, cu, n, initial_state=s0, return_final_state=True)
+    assert torch.equal(final, s0) and not out.any()
+    grads = torch.autograd.grad((out, final), (q, k, v, s0), (torch.ones_like(out), ds))
+    assert not any(x.any() for x in grads[:3]) and torch.equal(grads[3], ds)
+    pool = s0.detach().clone()
+    with torch.no_grad():
+        assert not fa.linear_attn_with_state(q, k, v, pool, g, cu_seqlens=cu).any()
+    assert torch.equal(pool, s0)
