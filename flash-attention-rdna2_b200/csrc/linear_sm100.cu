@@ -689,12 +689,18 @@ __global__ void __launch_bounds__(NTHREADS, 1)
               }
             } else {
               // On the diagonal, in pieces of 8 columns: lam^(gap to the piece's far edge), which may be up to lam^-7, times the table's, and what
-              // lies on the other side is masked.  Where lam^-7 could overflow, exp2 of each gap (1200 cycles a block, not 600)
+              // lies on the other side is masked.  Where lam^-7 could overflow, exp2 of each gap (1200 cycles a block, not 600).
+              // fp16's row scale goes to the products: lam^-7 (up to 2^119) times a scale (2^10 and more) would overflow, while
+              // a scaled product is below 2^11 and lam^-7 times the table's factor at most 1 wherever it counts.
+              if constexpr (!BF16) {
+#pragma unroll
+                for (int i = 0; i < W / 2; ++i) p[i] = __fmul2_rn(p[i], make_float2(ps, ps));
+              }
               const float from = (float)(REV ? j0 - row : row - j0);      // gap of the piece's first column
               if (g2 > -17.f) {
 #pragma unroll
                 for (int s = 0; s < W / 8; ++s) {
-                  const float edge_gap = REV ? from + 8 * s : from - 8 * s - 7, u = ex2(g2 * edge_gap) * ps;
+                  const float edge_gap = REV ? from + 8 * s : from - 8 * s - 7, u = ex2(g2 * edge_gap);
                   const float4 w0 = *reinterpret_cast<const float4*>(lamc + (REV ? 0 : 24)), w1 = *reinterpret_cast<const float4*>(lamc + (REV ? 4 : 28));
                   p[4 * s] = __fmul2_rn(p[4 * s], __fmul2_rn(make_float2(u, u), make_float2(w0.x, w0.y)));
                   p[4 * s + 1] = __fmul2_rn(p[4 * s + 1], __fmul2_rn(make_float2(u, u), make_float2(w0.z, w0.w)));
@@ -711,8 +717,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 #pragma unroll
                 for (int i = 0; i < W / 2; ++i) {
                   const float gap = REV ? from + 2 * i : from - 2 * i, next = REV ? gap + 1.f : gap - 1.f;
-                  p[i].x = gap >= 0.f ? p[i].x * (ex2(g2 * gap) * ps) : 0.f;
-                  p[i].y = next >= 0.f ? p[i].y * (ex2(g2 * next) * ps) : 0.f;
+                  p[i].x = gap >= 0.f ? p[i].x * ex2(g2 * gap) : 0.f;
+                  p[i].y = next >= 0.f ? p[i].y * ex2(g2 * next) : 0.f;
                 }
               }
             }

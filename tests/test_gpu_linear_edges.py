@@ -6,6 +6,7 @@ import torch
 
 import fa_abi as A
 import fable_attn as fa
+import lin_floor as F
 import lin_ref as R
 from test_gpu_linear import ALL, DT, cum, decays, inputs, rand
 from test_linear_cpu import FaLinearBwdParams, FaLinearParams
@@ -73,3 +74,31 @@ def test_one_empty_sequence(dt):
     with torch.no_grad():
         assert not fa.linear_attn_with_state(q, k, v, pool, g, cu_seqlens=cu).any()
     assert torch.equal(pool, s0)
+
+
+# ------------------------------------------------------------------ operands of other sizes than 1
+def check_sizes(dt, n, hq, hk, d, g, sizes, carried=False, scale=None, seed=0):
+    """check_run of test_gpu_linear for one sequence, with q, k, v, dO (and the states) of given sizes and bounds that follow them."""
+    q, k, v = inputs(dt, [n], hq, hk, d, d, seed)
+    do = rand(seed + 5, n, hq, d, dtype=dt)
+    q, k, v, do = ((x.float() * s).to(dt) for x, s in zip((q, k, v, do), sizes))
+    s0, ds = (rand(seed + 3, 1, hk, d, d) * sizes[4], rand(seed + 4, 1, hk, d, d) * sizes[5]) if carried else (None, None)
+    leaves = [x[None].requires_grad_() for x in (q, k, v)] + ([s0.requires_grad_()] if carried else [])
+    scale = d ** -0.5 if scale is None else scale
+    out, final = fa.linear_attn_func(*leaves[:3], g, scale=scale, initial_state=s0, return_final_state=True)
+    grads = torch.autograd.grad((out, final) if carried else out, leaves, (do[None], ds) if carried else do[None])
+    one = (q, k, v, g, scale, s0[0] if carried else None, do, ds[0] if carried else None)
+    for x, (want, amp), floor, name in zip((out[0], final[0], *(x[0] for x in grads)), R.both(*one), F.floors(*one),
+                                           ("out", "final", "dq", "dk", "dv", "dinitial")):
+        F.close(x, want, amp, floor, n * max(1, hq // hk), (d, d), g, dt, name)
+
+
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+@pytest.mark.parametrize("g", ["-0.2", "-10", "-10.5", "-11", "-11.5", "-11.7", "-11.75", "-11.78", "-11.8"])
+@pytest.mark.parametrize("size", [1.0, 0.1, 0.01, 0.003])
+@pytest.mark.parametrize("hq,hk,d", [(2, 2, 64), (4, 2, 128)])
+def test_fast_decays_of_small_operands(dt, g, size, hq, hk, d):
+    """Around the decay where the factors of a diagonal piece are formed in another way, with rows whose largest product is small."""
+    check_sizes(DT[dt], 150, hq, hk, d, decays(hk, g), (size, size, 1.0, 1.0))
+    check_sizes(DT[dt], 40, hq, hk, d, decays(hk, g), (1.0, 1.0, 1.0, size * 2.0 ** -8))
+    check_sizes(DT[dt], 40, hq, hk, d, decays(hk, g), (1.0, 1.0, size, 1.0))
