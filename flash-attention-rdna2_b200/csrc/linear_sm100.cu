@@ -434,6 +434,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         if (!SWAP && ok && lane == 0 && (last || r.nb > 1)) mbar_arrive(bar + Bz::B_EMPTY + 8 * (cb % K::NB));
         if (new_b && (!SWAP || !do_b)) ok = ok && wait_warp(bar + Bz::C_FULL + 8 * (cb % K::NC), (cb / K::NC) & 1);
         if (do_b) {
+          // (SWAP: P = a b^T may read b's rows before or after this; nothing is taken from its columns past the sequence)
           if (ok && cn < C && q.cu) {
             zero_rows(sgen + (SWAP ? K::OFF_B + (cb % K::NB) * K::TILE : K::OFF_C + (cb % K::NC) * K::TILE), K::NCH, cn, lane);
             fence_proxy_async_smem();
@@ -653,13 +654,22 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         wait(Bz::P_FULL, t);
         float ps = 1.f;
         if constexpr (!BF16) {
-          // the products before decay bound the row (factors are at most 1)
+          // The products before decay bound the row (factors are at most 1), those that the row sees: past the sequence's end the
+          // columns are of other sequences, and may be as large as they like.
           float top = 0.f;
 #pragma unroll 1
           for (int j0 = hf * 64; j0 < hf * 64 + 64; j0 += W) {
             if (REV ? j0 / 32 < qd : j0 / 32 > qd) continue;
             float2 p[W / 2];
             tmem_load<W>(la + K::P_COL + j0, p);
+            if (j0 / 32 == qd || (REV && cn < C)) {
+#pragma unroll
+              for (int i = 0; i < W / 2; ++i) {
+                const int j = j0 + 2 * i;
+                if (REV ? j < row || j >= cn : j > row) p[i].x = 0.f;
+                if (REV ? j + 1 < row || j + 1 >= cn : j + 1 > row) p[i].y = 0.f;
+              }
+            }
 #pragma unroll
             for (int i = 0; i < W / 2; ++i) top = fmaxf(top, fmaxf(fabsf(p[i].x), fabsf(p[i].y)));
           }

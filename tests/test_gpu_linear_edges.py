@@ -102,3 +102,50 @@ def test_fast_decays_of_small_operands(dt, g, size, hq, hk, d):
     check_sizes(DT[dt], 150, hq, hk, d, decays(hk, g), (size, size, 1.0, 1.0))
     check_sizes(DT[dt], 40, hq, hk, d, decays(hk, g), (1.0, 1.0, 1.0, size * 2.0 ** -8))
     check_sizes(DT[dt], 40, hq, hk, d, decays(hk, g), (1.0, 1.0, size, 1.0))
+
+
+# ------------------------------------------------------------------ what stands next to a sequence
+def packed_grads(x, do, g, lens, first=0):
+    leaves = [y.detach().clone().requires_grad_() for y in x]
+    out = fa.linear_attn_varlen_func(*leaves, g, cum(lens, first), max(lens))
+    return (out,) + torch.autograd.grad(out, leaves, do)
+
+
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+@pytest.mark.parametrize("hq,hk,d", [(2, 2, 64), (2, 2, 128), (4, 2, 64), (4, 1, 128)])
+@pytest.mark.parametrize("sizes", [(1.0, 1.0, 1.0, 1.0), (1.0, 1.0, 1.0, 2.0 ** -18), (2.0 ** -9, 2.0 ** -9, 1.0, 1.0), (64.0, 64.0, 2.0 ** -8, 2.0 ** -12)])
+@pytest.mark.parametrize("bad", [float("inf"), 6e4, float("nan")])
+def test_neighbours_change_no_bit(dt, hq, hk, d, sizes, bad):
+    """A sequence's values and gradients are the same bits whatever the rows of other sequences, and of none, hold: small gradients,
+    small and large products next to infinities and to fp16's largest numbers."""
+    lens, pad = [70, 61, 130], 5
+    x = inputs(DT[dt], [pad] + lens + [pad], hq, hk, d, d)
+    do, g = rand(7, len(x[0]), hq, d, dtype=DT[dt]), decays(hk, "-0.1")
+    x, do = [(y.float() * s).to(DT[dt]) for y, s in zip(x, sizes)], (do.float() * sizes[3]).to(DT[dt])
+    want = packed_grads(x, do, g, lens, pad)
+    mine = slice(pad + 70, pad + 131)
+    for y in x + [do]:
+        keep = y[mine].clone()
+        y.fill_(bad)
+        y[mine] = keep
+    got = packed_grads(x, do, g, lens, pad)
+    for a, b, name in zip(want, got, ("out", "dq", "dk", "dv")):
+        assert torch.equal(a[mine], b[mine]) and a[mine].isfinite().all(), name
+        assert not b[:pad].any() and not b[-pad:].any()
+
+
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+@pytest.mark.parametrize("hq,hk,d", [(8, 2, 64), (4, 4, 128), (6, 2, 128)])
+def test_packed_runs_repeat(dt, hq, hk, d):
+    """Bit for bit, next to rows of very different sizes that meet in a chunk."""
+    lens = [60, 700, 1, 33, 129, 400] * 4
+    x = inputs(DT[dt], lens, hq, hk, d, d)
+    at = cum(lens).tolist()
+    for z in range(1, len(lens), 2):
+        for y in x[:2]:
+            y[at[z]:at[z + 1]] *= 64.0
+    do, g = rand(7, len(x[0]), hq, d, dtype=DT[dt]) * 2.0 ** -16, decays(hk)
+    first = packed_grads(x, do, g, lens)
+    for _ in range(6):
+        for a, b in zip(first, packed_grads(x, do, g, lens)):
+            assert torch.equal(a, b)
