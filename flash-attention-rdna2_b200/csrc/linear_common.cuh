@@ -57,6 +57,7 @@ struct LinRole {
   int da, dc;            // dims of a and b, of c and out
   int transposed;        // X[i][j] is stored at [j][i]
   float w_intra, w_inter, w_up;
+  float x_in = 1.f;      // the tensor-core kernel holds the state times this, and w_inter and w_up with it
 };
 
 struct LinSpan {

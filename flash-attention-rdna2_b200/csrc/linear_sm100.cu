@@ -13,7 +13,9 @@
 // Operands of 16 bits: what is computed (P, X, b~) enters as hi + lo, which leaves 2^-16 (bf16) or 2^-22 (fp16) of a term; the result's own rounding is
 // 2^-9 or 2^-12, and one 16-bit number each would add as much again.  fp16 has no range to spare: rows of P are brought
 // to a largest value of about 2^10 by a power of 2 each, and X by one for the tile, taken back in the epilogue; the decayed rows are
-// left as they are: where they fall below 2^-14 their steps are 2^-24, which is fp16's own step for such inputs.
+// left as they are: where they fall below 2^-14 their steps are 2^-24, which is fp16's own step for such inputs.  A scale that they carry
+// (w_up of the reversed passes) is brought to (1/2, 1] by a power of 2 that X is held in: a scale of 64 would take inputs of 1024 past
+// fp16's range, and one of 2^-14 leave them ten bits.
 //
 // Warp roles (640 threads, five warpgroups):
 //   0-7    outputs: pair products on their way back to TMEM, a X, epilogue; two warps to a TMEM lane quadrant (w % 4), half of the columns each
@@ -26,6 +28,8 @@
 // set of warps that took all steps in turn needed 10000 cycles a chunk, issuing every third cycle.  Outputs of item t and the state
 // of the next chunk depend on each other through the MMAs alone, so two sets run them side by side.  Registers follow the need (setmaxnreg): the epilogue holds 64 columns.  Every wait is bounded.
 #include <cudaTypedefs.h>
+#include <algorithm>
+#include <cmath>
 #include "linear_common.cuh"
 #include "fa_launch.h"
 #include "sm100_ptx.cuh"
@@ -496,8 +500,9 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 #pragma unroll 8
         for (int e = tid - 256; e < D * D / 4; e += NSTATE) {
           const int lane_x = e / (D / 4), col = e % (D / 4) * 4;
-          stage[lane_x * (D / 4) + ((col / 4) ^ (lane_x & 7))] =
-              x0 && lane_x < xl && col < xn ? *reinterpret_cast<const float4*>(x0 + (long long)lane_x * xn + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+          float4 x = x0 && lane_x < xl && col < xn ? *reinterpret_cast<const float4*>(x0 + (long long)lane_x * xn + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+          if constexpr (!BF16 && REV) x.x *= r.x_in, x.y *= r.x_in, x.z *= r.x_in, x.w *= r.x_in;
+          stage[lane_x * (D / 4) + ((col / 4) ^ (lane_x & 7))] = x;
         }
         bar_state();
         if (qd * 32 < D) {
@@ -981,6 +986,18 @@ bool map4(CUtensorMap* m, const void* base, bool bf16, int dim, long long rows, 
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// fp16: the role with X in units of the power of 2 next above |w_up| (up to 2^64 either way: gradients of scales past that leave
+// fp16 themselves)
+LinRole in_units(LinRole r) {
+  int e = 0;
+  if (r.w_up != 0.f && std::isfinite(r.w_up) && fabsf(frexpf(r.w_up, &e)) == 0.5f) --e;
+  const int u = std::min(std::max(e, -64), 64);
+  r.x_in = ldexpf(1.f, -u);
+  r.w_up *= r.x_in;
+  r.w_inter *= ldexpf(1.f, u);
+  return r;
+}
+
 bool takes(const LinSeqs& q, const LinRole& r, int dtype) {
   return dtype != FA_DTYPE_F32 && r.da <= 128 && r.dc <= 128 && (q.cu ? q.total > 0 : q.S > 0) && q.total < (1ll << 31) - 256;
 }
@@ -1032,10 +1049,11 @@ int run_states(const LinSeqs& q, const LinRole& r, bool rev, float* ws, cudaStre
 namespace fa {
 bool lin_tc_takes(const LinSeqs& q, const LinRole& r, int dtype) { return takes(q, r, dtype); }
 
-int lin_tc_main(const LinSeqs& q, const LinRole& r, bool rev, const float* ws, const LinPool& pool, int dtype, cudaStream_t st, bool* taken) {
+int lin_tc_main(const LinSeqs& q, const LinRole& role, bool rev, const float* ws, const LinPool& pool, int dtype, cudaStream_t st, bool* taken) {
   *taken = false;
-  if (!takes(q, r, dtype) || (pool.out && !ws)) return FA_OK;
+  if (!takes(q, role, dtype) || (pool.out && !ws)) return FA_OK;
   const bool bf16 = dtype == FA_DTYPE_BF16;
+  const LinRole r = bf16 ? role : in_units(role);
   const long long rows = q.cu ? q.total : q.S, zs = q.cu ? 1 : q.batch;
   const bool small = r.da <= 64 && r.dc <= 64;
   CUtensorMap m[4];

@@ -149,3 +149,31 @@ def test_packed_runs_repeat(dt, hq, hk, d):
     for _ in range(6):
         for a, b in zip(first, packed_grads(x, do, g, lens)):
             assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------ scales far from 1
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+@pytest.mark.parametrize("hq,hk,d", [(1, 1, 64), (2, 1, 128)])
+@pytest.mark.parametrize("scale,sizes", [(64.0, (1500.0, 2.0 ** -6, 2.0 ** -6, 2.0 ** -12)), (2.0 ** -20, (1.0, 1.0, 1.0, 256.0)), (-0.3, (1.0, 1.0, 1.0, 1.0)),
+                                         (1e-5, (8.0, 1.0, 1.0, 64.0)), (3e4, (2.0, 2.0 ** -10, 2.0 ** -10, 2.0 ** -13)), (0.0, (1.0, 1.0, 1.0, 1.0)), (2.0 ** -100, (1.0, 1.0, 1.0, 1.0))])
+def test_gradients_under_any_scale(dt, hq, hk, d, scale, sizes):
+    """Chunks that meet through the state, with a scale that fp16 inputs times it do not bear.  So many sequences that each is one segment."""
+    L, n, b = A.lib(), 300, 320
+    L.fa_linear_plan.restype = C.c_longlong
+    seg, nseg = C.c_int(), C.c_int()
+    L.fa_linear_plan(b, n, C.c_longlong(0), hq, hq // hk, d, d, A.DT[dt], C.byref(seg), C.byref(nseg))
+    assert nseg.value == 1
+    dt = DT[dt]
+    one = [(x.float() * s).to(dt) for x, s in zip((*inputs(dt, [n], hq, hk, d, d), rand(5, n, hq, d, dtype=dt)), sizes)]
+    size = min(1.0, abs(scale) * sizes[3] * sizes[0] * 16 + 2.0 ** -14)       # a last state's gradient next to the outputs' own
+    start = 1.0 / max(1.0, 16 * abs(scale) * sizes[0])                        # a first state whose outputs stay in fp16
+    s0, ds, g = rand(3, hk, d, d) * start, rand(4, hk, d, d) * size, decays(hk, "-0.02")
+    q, k, v, s = (x.expand(b, *x.shape).clone().requires_grad_() for x in (*one[:3], s0))
+    out, final = fa.linear_attn_func(q, k, v, g, scale=scale, initial_state=s, return_final_state=True)
+    grads = torch.autograd.grad((out, final), (q, k, v, s), (one[3].expand_as(out), ds.expand_as(final)))
+    args = (*one[:3], g, scale, s0, one[3], ds)
+    sizes_of = R.both(*one[:3], g, abs(scale), s0, one[3], ds)     # a term's size takes the scale's size; lin_ref's sums take the scale as it is
+    for x, (want, _), (_, amp), floor, name in zip((out, final, *grads), R.both(*args), sizes_of, F.floors(*args),
+                                                   ("out", "final", "dq", "dk", "dv", "dinitial")):
+        for z in (0, b - 1):
+            F.close(x[z], want, amp, floor, n * (hq // hk), (d, d), g, dt, name)
