@@ -230,3 +230,16 @@ extern "C" int fa_combine_launch(const FaCombineParams* pp, void* stream) {
                p.lse_split_stride);
   return fa::combine_run(p, (cudaStream_t)stream);
 }
+
+// latency alone: a few entries for each sequence of a batch
+__global__ void __launch_bounds__(256) narrow_index_kernel(const long long* from, int* to, long long n) {
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) to[i] = (int)min(max(from[i], -2147483648ll), 2147483647ll);
+}
+
+extern "C" int fa_narrow_index_launch(const long long* from, int* to, long long n, void* stream) {
+  FA_CHECK_ARG(n >= 0 && (n == 0 || (from && to)), "narrow index: %lld entries, from and to must be non-null", n);
+  if (n == 0) return FA_OK;
+  narrow_index_kernel<<<(int)std::min<long long>((n + 255) / 256, 8ll * fa::num_sms()), 256, 0, (cudaStream_t)stream>>>(from, to, n);
+  fa::count_launch();
+  return fa::cuda_status(cudaGetLastError(), "narrow index launch");
+}

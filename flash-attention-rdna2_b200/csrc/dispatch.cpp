@@ -398,11 +398,17 @@ std::vector<torch::Tensor> dec(torch::Tensor q, torch::Tensor k_cache, torch::Te
 // ------------------------------------------------------------------ paged caches held in 8 bits
 const torch::Tensor* opt_ptr(const c10::optional<torch::Tensor>& t) { return t.has_value() && t->defined() ? &*t : nullptr; }
 
-// an integer index tensor as contiguous int32 on `dev` (itself where it is that already)
+// An integer index tensor as contiguous int32 on `dev` (itself where it is that already).  What 32 bits do not hold becomes the nearest
+// number that they do: an index past every pool and table stays past it.
 torch::Tensor index_i32(const torch::Tensor& t, const torch::Device& dev, const char* name) {
   TORCH_CHECK_VALUE(!t.is_floating_point() && t.scalar_type() != torch::kBool, "fable_attn: ", name, " must be integers");
-  if (t.scalar_type() == torch::kInt32 && t.device() == dev && t.is_contiguous()) return t;
-  return t.to(dev, torch::kInt32).contiguous();
+  if (t.scalar_type() == torch::kInt32) return t.to(dev).contiguous();
+  if (t.element_size() < 4 || !dev.is_cuda()) return t.to(dev, torch::kInt32).contiguous();
+  const c10::cuda::CUDAGuard guard(dev);
+  const torch::Tensor wide = t.to(dev, torch::kInt64).contiguous();
+  torch::Tensor out = torch::empty(wide.sizes(), wide.options().dtype(torch::kInt32));
+  check(fa_narrow_index_launch((const long long*)wide.const_data_ptr<int64_t>(), out.data_ptr<int>(), wide.numel(), cur_stream(out)), name);
+  return out;
 }
 torch::Tensor table_f32(const torch::Tensor& t) {
   return t.scalar_type() == torch::kFloat32 && t.is_contiguous() ? t : t.to(torch::kFloat32).contiguous();
@@ -934,9 +940,16 @@ std::tuple<torch::Tensor, torch::Tensor> rotary_qk(torch::Tensor q, torch::Tenso
   } else if (py::isinstance<py::int_>(offsets)) {
     p.offset = offsets.cast<int64_t>();
   } else {
-    offs = index_i32(offsets.cast<torch::Tensor>(), q.device(), "seqlen_offsets");
-    TORCH_CHECK_VALUE(offs.numel() == p.batch, "fable_attn: seqlen_offsets needs one entry per sequence");
-    p.offsets = offs.data_ptr<int>();
+    const auto given = offsets.cast<torch::Tensor>();
+    TORCH_CHECK_VALUE(given.numel() == p.batch, "fable_attn: seqlen_offsets needs one entry per sequence");
+    if (given.scalar_type() == torch::kInt64) {      // every token's own position, which has 64 bits
+      pos = given.to(q.device()).reshape({p.batch, 1}) + torch::arange(p.seqlen, given.options().device(q.device()));
+      p.positions = pos.const_data_ptr();
+      p.pos_bytes = 8;
+    } else {
+      offs = index_i32(given, q.device(), "seqlen_offsets");
+      p.offsets = offs.data_ptr<int>();
+    }
   }
   const auto last = [](const torch::Tensor& x) { return x.stride(-1) == 1 || x.size(-1) == 1 ? x : x.contiguous(); };
   const torch::Tensor qs = last(q), ks = last(k);

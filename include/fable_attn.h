@@ -579,6 +579,9 @@ FA_API int fa_device_error(int clear);
  * the give-up path of the pipelines' waits without faulting or hanging a GPU.  No counterpart in
  * the reference. */
 FA_API int fa_wait_selftest(unsigned long long limit_ns, void* stream);
+/* n indices or lengths of 64 bits as 32: each becomes the nearest int, so that one that does not fit lies outside every pool, table and
+ * cache as it did before, and is not some other entry's low word.  No counterpart in the reference. */
+FA_API int fa_narrow_index_launch(const long long* from, int* to, long long n, void* stream);
 /* Number of this library's kernels launched since load (all threads, all devices). */
 FA_API unsigned long long fa_kernel_launch_count(void);
 /* 1 when the forward's two-query-tile kernel (dense fp16/bf16, head_dim 128, no softcap / alibi /

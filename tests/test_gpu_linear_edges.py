@@ -8,7 +8,7 @@ import fa_abi as A
 import fable_attn as fa
 import lin_floor as F
 import lin_ref as R
-from test_gpu_linear import ALL, DT, cum, decays, inputs, rand
+from test_gpu_linear import ALL, DT, SLOT, cum, decays, inputs, rand
 from test_linear_cpu import FaLinearBwdParams, FaLinearParams
 
 pytestmark = pytest.mark.gpu
@@ -177,3 +177,76 @@ def test_gradients_under_any_scale(dt, hq, hk, d, scale, sizes):
                                                    ("out", "final", "dq", "dk", "dv", "dinitial")):
         for z in (0, b - 1):
             F.close(x[z], want, amp, floor, n * (hq // hk), (d, d), g, dt, name)
+
+
+# ------------------------------------------------------------------ indices and lengths of 64 bits
+@pytest.mark.parametrize("n", [1, 40])
+def test_wide_indices_and_lengths(n):
+    """Slots past 32 bits are outside the pool and not their low word's; that many tokens seen are not none."""
+    b, h, d = 6, 2, 64
+    x = [rand(i, b, n, h, d, dtype=torch.bfloat16) for i in range(3)]
+    pool, g = rand(5, 4, h, d, d), decays(h)
+    before, want = pool.clone(), pool.clone()
+    at = torch.tensor([1, 2 ** 32 + 3, -2 ** 40, 2 ** 62, -1, 0]).cuda()
+    seen = torch.tensor([2 ** 31, 1, 1, 1, 1, 2 ** 40 + 7]).cuda()
+    fa.device_error(clear=True)
+    out = fa.linear_attn_with_state(*x, pool, g, state_indices=at, cache_seqlens=seen)
+    assert fa.device_error(clear=True) == SLOT
+    narrow = torch.tensor([1, -1, -1, -1, -1, 0], dtype=torch.int32).cuda()
+    assert torch.equal(out, fa.linear_attn_with_state(*x, want, g, state_indices=narrow)) and torch.equal(pool, want)
+    assert torch.equal(pool[2:], before[2:]) and not out[1:5].any() and fa.device_error() == 0
+    every = torch.stack((at, at), 1)[:, 0]                      # strided, and in each integer type that torch indexes with
+    fa.linear_attn_with_state(*x, pool, g, state_indices=every, cache_seqlens=seen)
+    fa.linear_attn_with_state(*x, want, g, state_indices=narrow.short())
+    assert torch.equal(pool, want)
+    fa.device_error(clear=True)
+
+
+def test_wide_indices_on_another_stream_and_captured():
+    x = [rand(i, 3, 1, 2, 64, dtype=torch.bfloat16) for i in range(3)]
+    pool, g, at = rand(5, 4, 2, 64, 64), decays(2), torch.tensor([2, 0, 3]).cuda()
+    new = torch.zeros_like(pool)
+    run = lambda: fa.linear_attn_with_state(*x, pool, g, state_indices=at, state_out=new)
+    run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    at.copy_(torch.tensor([1, 3, 2]))
+    graph.replay()
+    got = out.clone()
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        big = torch.zeros(64 << 20, device="cuda")
+        at.copy_(torch.tensor([1, 3, 2], device="cuda"))
+        want = run()
+    side.synchronize()
+    assert torch.equal(got, want) and not big.any()
+
+
+def test_wide_offsets_of_rotary():
+    from fable_attn.layers.rotary import apply_rotary_emb_qk, scaled_inv_freq
+    freq, _ = scaled_inv_freq(64, device="cuda")
+    q, k = (rand(i, 3, 5, 2, 64, dtype=torch.bfloat16).requires_grad_() for i in range(2))
+    far = torch.tensor([2 ** 32 + 5, -2 ** 35, 2 ** 31]).cuda()
+    pos = far[:, None] + torch.arange(5, device="cuda")
+    a, b = (apply_rotary_emb_qk(q, k, freq, **kw) for kw in (dict(seqlen_offsets=far), dict(positions=pos)))
+    ga, gb = (torch.autograd.grad(y, (q, k), (torch.ones_like(q), torch.ones_like(k))) for y in (a, b))
+    assert all(torch.equal(x, y) for x, y in zip((*a, *ga), (*b, *gb)))
+    near = torch.tensor([5, 0, 70000]).cuda()
+    a, b = (apply_rotary_emb_qk(q, k, freq, seqlen_offsets=o) for o in (near, near.int()))
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    one = [apply_rotary_emb_qk(q[i].detach(), k[i].detach(), freq, seqlen_offsets=far[i:i + 1]) for i in range(3)]      # packed: one offset
+    want = apply_rotary_emb_qk(q, k, freq, pos)
+    assert all(torch.equal(o[j], want[j][i]) for i, o in enumerate(one) for j in range(2))
+
+
+def test_wide_lengths_of_the_cache():
+    """The paged cache reads the same kind of lengths: 2^32 cached tokens are not none, and their pages are outside the table."""
+    k = rand(1, 2, 1, 2, 64, dtype=torch.bfloat16)
+    kc, vc = (torch.zeros(4, 16, 2, 64, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    table = torch.tensor([[0], [2]], dtype=torch.int32).cuda()
+    fa.device_error(clear=True)
+    fa.kvcache_append(k, k, kc, vc, torch.tensor([2 ** 32, 3]).cuda(), table)
+    assert fa.device_error(clear=True) == 8192
+    assert torch.equal(kc[2, 3], k[1, 0]) and int(kc.count_nonzero()) == int(k[1].count_nonzero())

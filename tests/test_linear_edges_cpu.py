@@ -1,4 +1,5 @@
 """Linear attention and the rotary of q and k at the edges of what they are given: the parts that run on the host."""
+import ctypes as C
 import os
 import random
 import subprocess
@@ -79,3 +80,11 @@ def test_the_join_stays_in_its_workspace(slots_program):
     lines.append("512 512 1 128 4 512 512")
     r = subprocess.run([slots_program], input="\n".join(lines), capture_output=True, text=True)
     assert r.returncode == 0 and r.stdout == str(len(lines)), r.stdout
+
+
+def test_narrowing_refusals():
+    L = A.lib()
+    L.fa_narrow_index_launch.argtypes = [C.c_void_p, C.c_void_p, C.c_longlong, C.c_void_p]
+    assert L.fa_narrow_index_launch(None, None, 0, None) == A.FA_OK
+    for args in ((None, 16, 3, None), (16, None, 3, None), (16, 16, -1, None)):
+        assert L.fa_narrow_index_launch(*args) == A.FA_ERR_INVALID
