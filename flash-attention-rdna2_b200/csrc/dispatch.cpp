@@ -737,6 +737,14 @@ void written(const torch::Tensor& x) {
   if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
 }
 
+// Forward-mode tangents are refused and not dropped.  (Here, where a look costs nothing: unpack_dual takes 0.5 us a tensor in Python, and a
+// decode step 6.6 in all.)
+void no_tangents(std::initializer_list<const torch::Tensor*> tensors, const char* what) {
+  for (const auto* t : tensors)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t || !t->defined() || !t->unsafeGetTensorImpl()->_fw_grad(0, *t).defined(), "fable_attn: ", what,
+                                " carries no forward-mode tangents");
+}
+
 // x with a contiguous last dimension and, for the chunked kernels of 16 bits (`tma`), as the tensor maps need it: rows on 16-byte boundaries
 // and no dimension that repeats itself.  Otherwise the CUDA-core
 // kernels would have to run: 2 x 4096 tokens, 16 heads of 128 take 83 us as they are, 204 with all three copied, and 740 there.
@@ -818,6 +826,7 @@ std::tuple<torch::Tensor, torch::Tensor, int64_t, int64_t> linear_fwd(
     c10::optional<torch::Tensor> state_out, c10::optional<torch::Tensor> index, c10::optional<torch::Tensor> seen,
     c10::optional<torch::Tensor> cu, int64_t max_seqlen, bool keep_states) {
   TORCH_CHECK_VALUE(q.is_cuda(), "fable_attn: linear attention needs CUDA tensors");
+  no_tangents({&q, &k, &v, &log_decay, opt_ptr(state_in), opt_ptr(state_out)}, "linear attention");
   const c10::cuda::CUDAGuard guard(q.device());
   FaLinearParams p{};
   const LinearCall<FaLinearParams> call(p, q, k, v, log_decay, scale, cu, max_seqlen, keep_states);
@@ -863,6 +872,7 @@ std::vector<torch::Tensor> linear_bwd(torch::Tensor dout, torch::Tensor q, torch
                                       double scale, c10::optional<torch::Tensor> initial, c10::optional<torch::Tensor> dfinal,
                                       bool want_dinitial, c10::optional<torch::Tensor> cu, int64_t max_seqlen, torch::Tensor states,
                                       int64_t seg_len, int64_t nseg) {
+  no_tangents({&dout, opt_ptr(dfinal)}, "the gradient of linear attention");
   const c10::cuda::CUDAGuard guard(q.device());
   FaLinearBwdParams p{};
   const LinearCall<FaLinearBwdParams> call(p, q, k, v, log_decay, scale, cu, max_seqlen, true);
@@ -908,6 +918,7 @@ std::tuple<torch::Tensor, torch::Tensor> rotary_qk(torch::Tensor q, torch::Tenso
                                                    bool inplace, double factor, bool inverse) {
   TORCH_CHECK_VALUE(q.is_cuda() && k.is_cuda() && k.device() == q.device() && k.scalar_type() == q.scalar_type(),
                     "fable_attn: rotary needs q and k of one type on one CUDA device");
+  no_tangents({&q, &k, &inv_freq}, "rotary of q and k");
   const int hd = (int)q.dim() - 2;
   TORCH_CHECK_VALUE((hd == 1 || hd == 2) && k.dim() == q.dim(), "fable_attn: rotary expects (batch, seqlen, nheads, headdim) or (total, "
                     "nheads, headdim), got ", q.sizes(), " and ", k.sizes());

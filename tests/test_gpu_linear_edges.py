@@ -250,3 +250,46 @@ def test_wide_lengths_of_the_cache():
     fa.kvcache_append(k, k, kc, vc, torch.tensor([2 ** 32, 3]).cuda(), table)
     assert fa.device_error(clear=True) == 8192
     assert torch.equal(kc[2, 3], k[1, 0]) and int(kc.count_nonzero()) == int(k[1].count_nonzero())
+
+
+# ------------------------------------------------------------------ forward-mode tangents
+@pytest.mark.parametrize("which", [0, 1, 2, 3, 4])
+def test_forward_mode_is_refused(which):
+    """A tangent is not dropped in silence: not the queries', nor any other input's, with or without gradients."""
+    from torch.autograd import forward_ad
+    from fable_attn.layers.rotary import apply_rotary_emb_qk, scaled_inv_freq
+    x = [rand(i, 2, 20, 2, 64) for i in range(3)] + [rand(3, 2, 2, 64, 64), decays(2)]
+    freq, _ = scaled_inv_freq(64, device="cuda")
+    with forward_ad.dual_level():
+        x[which] = forward_ad.make_dual(x[which], torch.ones_like(x[which]))
+        q, k, v, s, g = x
+        cu = cum([20, 20])
+        calls = [lambda: fa.linear_attn_func(q, k, v, g, initial_state=s), lambda: fa.linear_attn_with_state(q, k, v, s, g),
+                 lambda: fa.linear_attn_varlen_func(*(y.flatten(0, 1) for y in (q, k, v)), g, cu, 20, initial_state=s)]
+        for call in calls:
+            with pytest.raises(NotImplementedError):
+                call()
+            with torch.no_grad(), pytest.raises(NotImplementedError):
+                call()
+        if which < 2:
+            with pytest.raises(NotImplementedError):
+                apply_rotary_emb_qk(q, k, freq)
+            with torch.no_grad(), pytest.raises(NotImplementedError):
+                apply_rotary_emb_qk(q, k, freq, inplace=True)
+        if which == 0:
+            turn = forward_ad.make_dual(freq, freq)
+            with pytest.raises(NotImplementedError):
+                apply_rotary_emb_qk(k, k, turn)
+    if which < 2:
+        with pytest.raises(NotImplementedError):
+            torch.func.jvp(lambda y: apply_rotary_emb_qk(y, k, freq)[0], (q,), (q,))
+    q, k, v = (rand(i, 2, 20, 2, 64).requires_grad_() for i in range(3))
+    out, turned = fa.linear_attn_func(q, k, v, decays(2)), apply_rotary_emb_qk(q, k, freq)[0]
+    with forward_ad.dual_level():                    # of a gradient that comes in
+        do = forward_ad.make_dual(torch.ones_like(q), torch.ones_like(q))
+        for y in (out, turned):
+            with pytest.raises(NotImplementedError):
+                torch.autograd.grad(y, q, do)
+    q, k = q.detach(), k.detach()
+    a, b = apply_rotary_emb_qk(k, k, freq)
+    assert torch.equal(a, b) and fa.linear_attn_func(*(rand(i, 2, 20, 2, 64) for i in range(3)), decays(2)).isfinite().all()
