@@ -1,8 +1,10 @@
 // rotary_qk.cu — rotary of q and k at each token's own position, from frequencies instead of tables.
 //
 // theta = position * inv_freq.  The frequency is held as a fraction of a turn in units of 2^-64, so that the 64-bit product
-// with the position wraps by itself at whole turns: no range reduction is left, and a position of 2^31 is as exact as a
-// small one.  The quadrant comes off in the integers too, and sincospi sees at most an eighth of a turn.
+// with the position wraps by itself at whole turns: no range reduction is left.  inv_freq / (2 pi) is formed in twice fp64's
+// bits (a product and its rest, 1 / (2 pi) as two numbers), so that the unit is all that is rounded: the angle is off by
+// 2^-64 of a turn for each position, 2^-33 of one at 2^31.  The quadrant comes off in the integers too, and sincospi sees at
+// most an eighth of a turn.
 //
 // Bound by memory: every element of q and k is read and written once.  A block takes `TOK` tokens: its threads form the
 // tokens' cos / sin once, in shared memory, and then walk all heads of q and k by 16-byte units, so that the 64-bit product and the
@@ -21,6 +23,16 @@ __device__ __forceinline__ void turn(const T& a, const T& b, float2 e, T& oa, T&
   const float x = Elem<T>::to_f(a), y = Elem<T>::to_f(b);
   oa = Elem<T>::from_f(x * e.x - y * e.y);
   ob = Elem<T>::from_f(y * e.x + x * e.y);
+}
+
+// radians as a fraction of a turn in units of 2^-64
+__device__ __forceinline__ unsigned long long turns_of(double radians) {
+  constexpr double INV_2PI = 0.15915494309189535, INV_2PI_REST = -9.839338337591243e-18;      // their sum is 1 / (2 pi) to 2^-110
+  constexpr double UNITS = 18446744073709551616.0;
+  const double turns = radians * INV_2PI, rest = fma(radians, INV_2PI, -turns) + radians * INV_2PI_REST;
+  const double part = turns - trunc(turns);      // exact
+  const unsigned long long most = __double2ull_rn(fabs(part) * UNITS);
+  return (part < 0 ? 0 - most : most) + (unsigned long long)__double2ll_rn(rest * UNITS);
 }
 
 template <typename T, int U> struct alignas(U * sizeof(T) == 16 ? 16 : sizeof(T)) Unit { T e[U]; };
@@ -51,9 +63,7 @@ __global__ void __launch_bounds__(THREADS, 5) rotary_qk_kernel(const FaRotaryQkP
       const long long z = row / p.seqlen;
       pos = row - z * p.seqlen + p.offset + (p.offsets ? p.offsets[z] : 0);
     }
-    double f = p.inv_freq[i] * 0.15915494309189533577;      // turns for each position
-    f -= floor(f);
-    const unsigned long long angle = (unsigned long long)pos * __double2ull_rn(f * 18446744073709551616.0);
+    const unsigned long long angle = (unsigned long long)pos * turns_of(p.inv_freq[i]);
     const unsigned int hi = (unsigned int)((angle + 0x80000000ull) >> 32);     // to nearest: opposite positions turn alike
     const unsigned int quarter = (hi + 0x20000000u) >> 30;
     float s, c;

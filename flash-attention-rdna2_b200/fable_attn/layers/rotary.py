@@ -190,8 +190,8 @@ def apply_rotary_emb_qk(q, k, inv_freq, positions=None, *, seqlen_offsets=0, int
 
     inv_freq (rotary_dim / 2,): radians for each position, best in fp64 (scaled_inv_freq makes them); the first rotary_dim dims (up to 256)
     turn, the rest pass through.  positions (batch, seqlen) or (total,), int32 or int64: each token's own position, any
-    whole number, without a table to end; without them token t sits at seqlen_offsets + t (an int, or (batch,)).  The angle is exact
-    however far the position; cos and sin are multiplied by factor and applied in fp32 with one rounding at the end (apply_rotary_emb
+    whole number, without a table to end; without them token t sits at seqlen_offsets + t (an int, or (batch,)).  The angle is
+    position * inv_freq to 2^-64 of a turn for each position (2^-33 of one at 2^31); cos and sin are multiplied by factor and applied in fp32 with one rounding at the end (apply_rotary_emb
     rounds tables and products to the inputs' type instead, as torch arithmetic does).  interleaved pairs dims (2i, 2i + 1) instead of
     (i, i + rotary_dim / 2).  inplace writes q and k themselves.  Carries gradients to q and k.  CUDA tensors only."""
     if not (q.is_cuda and k.is_cuda and inv_freq.is_cuda):

@@ -490,8 +490,8 @@ FA_API int fa_linear_backward_launch(const FaLinearBwdParams* p, int dtype, void
 /* ------------------------------------------------------------------------------------------
  * Rotary of q and k at positions given for each token, from frequencies instead of tables (no counterpart in the
  * reference, whose tables are layers/rotary.py:119-146).  Pair i of the first rot_dim dims of token t turns by
- * positions * inv_freq[i] radians, counted in 2^-64 turns by one 64-bit product (exact for the frequency as rounded there,
- * however far the position); x' = factor (x cos - y sin), y' = factor (y cos + x sin), in fp32 and rounded once.
+ * positions * inv_freq[i] radians, counted in 2^-64 turns by one 64-bit product (exact for the frequency as rounded there: off
+ * by 2^-64 of a turn for each position); x' = factor (x cos - y sin), y' = factor (y cos + x sin), in fp32 and rounded once.
  * `inverse` turns back (the gradient: by -theta, with the same factor).
  *   rows z * seqlen + t by strides (dim contiguous); k may be null.  Outputs may be the inputs.
  *   positions  [batch * seqlen] int32 or int64 (pos_bytes 4 / 8), or null: offsets[z] (0 where null) + offset + t
