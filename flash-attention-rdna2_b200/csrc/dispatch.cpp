@@ -402,7 +402,7 @@ const torch::Tensor* opt_ptr(const c10::optional<torch::Tensor>& t) { return t.h
 // number that they do: an index past every pool and table stays past it.
 torch::Tensor index_i32(const torch::Tensor& t, const torch::Device& dev, const char* name) {
   TORCH_CHECK_VALUE(!t.is_floating_point() && t.scalar_type() != torch::kBool, "fable_attn: ", name, " must be integers");
-  if (t.scalar_type() == torch::kInt32) return t.to(dev).contiguous();
+  if (t.scalar_type() == torch::kInt32) return t.device() == dev && t.is_contiguous() ? t : t.to(dev).contiguous();
   if (t.element_size() < 4 || !dev.is_cuda()) return t.to(dev, torch::kInt32).contiguous();
   const c10::cuda::CUDAGuard guard(dev);
   const torch::Tensor wide = t.to(dev, torch::kInt64).contiguous();
