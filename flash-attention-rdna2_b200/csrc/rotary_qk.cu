@@ -77,6 +77,7 @@ __global__ void __launch_bounds__(THREADS, 5) rotary_qk_kernel(const FaRotaryQkP
       c = -c;
       s = -s;
     }
+    if (!isfinite(p.inv_freq[i])) c = s = __int_as_float(0x7fffffff);      // shows, and in its own pair alone
     sce[t][i] = make_float2(p.factor * c, (p.inverse ? -p.factor : p.factor) * s);
   }
   __syncthreads();

@@ -48,3 +48,18 @@ def test_frequencies_of_many_turns_and_of_almost_none():
             want, amp = turned(x[i], p, freq)
             bound = amp * (8 * 2.0 ** -24 + abs(p) * 2 * math.pi * 2.0 ** -64) + 2.0 ** -24 * want.abs()
             assert ((got[i].double().cpu() - want).abs() <= bound).all(), p
+
+
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("n", [1, 3000])
+def test_frequencies_that_are_no_numbers_show(inter, n):
+    freq, _ = scaled_inv_freq(64, device="cuda")
+    q, k = rand(1, 1, n, 2, 80), rand(2, 1, n, 1, 80)
+    want = apply_rotary_emb_qk(q, k, freq, interleaved=inter)
+    for i, bad in ((3, math.nan), (17, math.inf), (31, -math.inf)):
+        f = freq.clone()
+        f[i] = bad
+        pair = [2 * i, 2 * i + 1] if inter else [i, i + 32]
+        rest = [d for d in range(80) if d not in pair]
+        for a, b in zip(apply_rotary_emb_qk(q, k, f, interleaved=inter), want):
+            assert a[..., pair].isnan().all() and torch.equal(a[..., rest], b[..., rest])
