@@ -1102,10 +1102,11 @@ int map_of(CUtensorMap* m, const void* base, const FaDec8Params& p, int row, int
   const cuuint64_t strides[2] = {(cuuint64_t)p.dim, heads * p.dim};
   const cuuint32_t box[3] = {(cuuint32_t)row, 1, (cuuint32_t)std::min(p.page, strip)};
   const cuuint32_t one[3] = {1, 1, 1};
-  const CUresult e = !enc ? CUDA_ERROR_NOT_FOUND
-                          : enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, one,
-                                CU_TENSOR_MAP_INTERLEAVE_NONE, row == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUresult e = !enc ? CUDA_ERROR_NOT_FOUND : fa::encode_map([&] {
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               row == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  });
   if (e == CUDA_SUCCESS) return FA_OK;
   fa::set_error("8-bit decode: cuTensorMapEncodeTiled failed (%d)", (int)e);
   return FA_ERR_CUDA;

@@ -34,4 +34,13 @@ bool require_tc();   // FABLE_ATTN_REQUIRE_TC set: no CUDA-core fallback for fp1
 int current_device();
 // Raise the dynamic shared-memory limit of `func` to `bytes` once per device.
 int ensure_smem(const void* func, int bytes, unsigned long long* done_mask);
+// encode() is a call of cuTensorMapEncodeTiled.  It asks for a current context, which a thread has after its first call to the runtime: where
+// the operator is that first call (a thread of the host's own, autograd's) the context is made current and the call repeated.
+template <typename Encode>
+auto encode_map(const Encode& encode) -> decltype(encode()) {
+  const auto e = encode();
+  if ((int)e == 0) return e;
+  cudaSetDevice(current_device());
+  return encode();
+}
 }  // namespace fa

@@ -981,9 +981,11 @@ bool map4(CUtensorMap* m, const void* base, bool bf16, int dim, long long rows, 
   for (int i = 0; i < 3; ++i)
     if (strides[i] == 0 || strides[i] % 16 || strides[i] >= (1ull << 40)) return false;
   const cuuint32_t box[4] = {(cuuint32_t)cols, (cuuint32_t)box_rows, 1, 1}, estr[4] = {1, 1, 1, 1};
-  return enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, box,
-             estr, CU_TENSOR_MAP_INTERLEAVE_NONE, cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return encode_map([&] {
+    return enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, box,
+               estr, CU_TENSOR_MAP_INTERLEAVE_NONE, cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  }) == CUDA_SUCCESS;
 }
 
 // fp16: the role with X in units of the power of 2 next above |w_up| (up to 2^64 either way: gradients of scales past that leave
