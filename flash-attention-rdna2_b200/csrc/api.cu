@@ -45,7 +45,7 @@ int num_sms() {
   return cached[d];
 }
 
-// FABLE_ATTN_REQUIRE_TC=1: fp16/bf16 forward / backward requests that the tensor-core kernels do
+// FABLE_ATTN_REQUIRE_TC=1: fp16/bf16 forward / backward requests, and those of linear attention, that the tensor-core kernels do
 // not take fail with FA_ERR_UNSUPPORTED instead of running on the CUDA-core kernels (lets a caller,
 // or a test, be sure which kernels ran)
 bool require_tc() {

@@ -29,7 +29,7 @@ int fwd_simt_device_error(int clear);   // bit 0: an invalid block-table entry (
 // FABLE_ATTN_NO_PDL set: launch every kernel plainly (no programmatic dependent launch)
 bool pdl_enabled();
 int num_sms();
-bool require_tc();   // FABLE_ATTN_REQUIRE_TC set: no CUDA-core fallback for fp16/bf16 fwd / bwd
+bool require_tc();   // FABLE_ATTN_REQUIRE_TC set: no CUDA-core fallback for fp16/bf16 fwd / bwd / linear attention
 
 int current_device();
 // Raise the dynamic shared-memory limit of `func` to `bytes` once per device.

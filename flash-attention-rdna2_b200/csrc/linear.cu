@@ -475,15 +475,26 @@ int join(const LinSeqs& q, bool rev, float* ws, const LinPool& pool, int per, cu
   return cuda_status(cudaGetLastError(), "linear attention (join) launch");
 }
 
+// 16 bits on the CUDA cores take nine times as long: FABLE_ATTN_REQUIRE_TC refuses them
+int allow_cuda_cores(const LinSeqs& q, const LinRole& r, int dtype) {
+  if (dtype == FA_DTYPE_F32 || !(q.cu ? q.total > 0 : q.S > 0) || !require_tc()) return FA_OK;
+  set_error("linear attention: FABLE_ATTN_REQUIRE_TC is set and the tensor-core kernels do not take this request (dims %d and %d, "
+            "alignment or strides, or the build's register count)", r.da, r.dc);
+  return FA_ERR_UNSUPPORTED;
+}
 int states(const LinSeqs& q, const LinRole& r, bool rev, float* ws, int dtype, cudaStream_t st) {
   bool taken = false;
   if (int rc = lin_tc_states(q, r, rev, ws, dtype, st, &taken)) return rc;
-  return taken ? FA_OK : lin_simt_states(q, r, rev, ws, dtype, st);
+  if (taken) return FA_OK;
+  if (int rc = allow_cuda_cores(q, r, dtype)) return rc;
+  return lin_simt_states(q, r, rev, ws, dtype, st);
 }
 int main_pass(const LinSeqs& q, const LinRole& r, bool rev, const float* ws, const LinPool& pool, int dtype, cudaStream_t st) {
   bool taken = false;
   if (int rc = lin_tc_main(q, r, rev, ws, pool, dtype, st, &taken)) return rc;
-  return taken ? FA_OK : lin_simt_main(q, r, rev, ws, pool, dtype, st);
+  if (taken) return FA_OK;
+  if (int rc = allow_cuda_cores(q, r, dtype)) return rc;
+  return lin_simt_main(q, r, rev, ws, pool, dtype, st);
 }
 // The tensor-core kernels' last state comes from the states kernel (whose sums keep fp32's bits), so one segment goes
 // through it too where a last state is asked for.

@@ -1004,7 +1004,8 @@ bool takes(const LinSeqs& q, const LinRole& r, int dtype) {
   return dtype != FA_DTYPE_F32 && r.da <= 128 && r.dc <= 128 && (q.cu ? q.total > 0 : q.S > 0) && q.total < (1ll << 31) - 256;
 }
 
-// The register split of lin_tc_kernel waits for good unless the block starts with REGS a thread: looked up once for each kernel.
+// The register split of lin_tc_kernel waits for good unless the block starts with REGS a thread: looked up once for each kernel.  Another
+// count, of another compiler, leaves the request to the CUDA cores (FABLE_ATTN_REQUIRE_TC refuses it).
 template <typename Kernel>
 bool regs_fit(Kernel kernel) {
   cudaFuncAttributes a;

@@ -8,7 +8,7 @@ import fa_abi as A
 import fable_attn as fa
 import lin_floor as F
 import lin_ref as R
-from test_gpu_linear import ALL, DT, SLOT, cum, decays, inputs, rand
+from test_gpu_linear import ALL, DT, SLOT, check_run, cum, decays, inputs, rand
 from test_linear_cpu import FaLinearBwdParams, FaLinearParams
 
 pytestmark = pytest.mark.gpu
@@ -293,3 +293,34 @@ def test_forward_mode_is_refused(which):
     q, k = q.detach(), k.detach()
     a, b = apply_rotary_emb_qk(k, k, freq)
     assert torch.equal(a, b) and fa.linear_attn_func(*(rand(i, 2, 20, 2, 64) for i in range(3)), decays(2)).isfinite().all()
+
+
+# ------------------------------------------------------------------ which kernels run
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 128), (8, 40), (72, 128), (128, 16)])
+@pytest.mark.parametrize("hq,hk", [(2, 2), (4, 2)])
+def test_tensor_cores_take_16_bits(dt, dk, dv, hq, hk, monkeypatch):
+    """With FABLE_ATTN_REQUIRE_TC nothing runs on the CUDA cores instead: every direction, grouped heads, packed, states, rows off 16 bytes."""
+    monkeypatch.setenv("FABLE_ATTN_REQUIRE_TC", "1")
+    check_run(DT[dt], [130, 130], hq, hk, dk, dv, decays(hk), True, False)
+    check_run(DT[dt], [5, 300, 0, 40], hq, hk, dk, dv, decays(hk), True, True, strided=True)
+    x = [rand(i, 2, 40, h, d, dtype=DT[dt]) for i, (h, d) in enumerate(((hq, dk), (hk, dk), (hk, dv)))]
+    pool = torch.zeros(2, hk, dk, dv, device="cuda")
+    assert fa.linear_attn_with_state(*x, pool, decays(hk)).isfinite().all()
+    odd = [torch.cat((y[..., :1], y), -1)[..., 1:] for y in x]
+    assert torch.equal(fa.linear_attn_func(*odd, decays(hk)), fa.linear_attn_func(*x, decays(hk)))
+
+
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+def test_cuda_cores_are_refused_where_tensor_cores_are_required(dt, monkeypatch):
+    x = [rand(i, 2, 40, 2, 136, dtype=DT[dt]).requires_grad_() for i in range(3)]
+    g = decays(2)
+    out = fa.linear_attn_func(*x, g)
+    monkeypatch.setenv("FABLE_ATTN_REQUIRE_TC", "1")
+    for call in (lambda: fa.linear_attn_func(*x, g), lambda: torch.autograd.grad(out.sum(), x)):
+        with pytest.raises(Exception, match="FABLE_ATTN_REQUIRE_TC"):
+            call()
+    with torch.no_grad():
+        assert fa.linear_attn_func(*(y[:, :16] for y in x), g).isfinite().all()       # token by token
+        assert fa.linear_attn_func(*(y[:, :0] for y in x), g).numel() == 0
+        assert fa.linear_attn_func(*(y.float() for y in x), g).isfinite().all()
