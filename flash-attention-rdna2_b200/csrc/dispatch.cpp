@@ -884,6 +884,7 @@ std::vector<torch::Tensor> linear_bwd(torch::Tensor dout, torch::Tensor q, torch
   torch::Tensor df;
   if (const auto* x = opt_ptr(dfinal)) {
     df = x->contiguous();
+    if ((uintptr_t)df.const_data_ptr() % 16) df = df.clone();      // autograd may hand a slice of a flat gradient
     call.check_states(p, df, "the final state's gradient", p.batch);
     p.dfinal = df.const_data_ptr<float>();
   }

@@ -40,6 +40,8 @@ class _LinearAttn(torch.autograd.Function):
         final = None
         if initial is not None:
             initial = initial.contiguous()
+            if initial.data_ptr() % 16:              # a slice of a flat buffer
+                initial = initial.clone()
         if want_final:
             final = torch.empty(batch, k.shape[-2], k.shape[-1], v.shape[-1], dtype=torch.float32, device=q.device)
         out, states, seg_len, nseg = _C.linear_fwd(q, k, v, log_decay, scale, initial, final, None, None, cu_seqlens, max_seqlen, keep)
@@ -94,7 +96,7 @@ def linear_attn_with_state(q, k, v, state, log_decay, scale=None, *, state_indic
 
     q, k, v: (batch, seqlen, heads, dim) or, with cu_seqlens (batch + 1) int32, ragged counts packed as (total, heads, dim), where
     max_seqlen is a bound on the counts that helps to choose the kernel.  state (slots, nheads_k, headdim, headdim_v)
-    fp32, contiguous, is updated in place, or, with state_out of the same shape, left as it is while the new states go there (drafted tokens
+    fp32, contiguous and on a 16-byte boundary, is updated in place, or, with state_out of the same shape, left as it is while the new states go there (drafted tokens
     that are not accepted then cost nothing but the step back).  Sequence b has slot state_indices[b] (slot b, and
     slots == batch, without it); a negative index is padding, whose rows of out are 0.  cache_seqlens (batch): tokens seen before; where it
     is 0 the sequence starts from an empty state whatever its slot holds.

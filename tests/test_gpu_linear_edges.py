@@ -324,3 +324,28 @@ def test_cuda_cores_are_refused_where_tensor_cores_are_required(dt, monkeypatch)
         assert fa.linear_attn_func(*(y[:, :16] for y in x), g).isfinite().all()       # token by token
         assert fa.linear_attn_func(*(y[:, :0] for y in x), g).numel() == 0
         assert fa.linear_attn_func(*(y.float() for y in x), g).isfinite().all()
+
+
+# ------------------------------------------------------------------ states off 16 bytes
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("n", [40, 400])
+def test_states_that_are_slices_of_flat_buffers(dt, n):
+    """A first state and a last state's gradient at any place: the same bits.  A pool is refused there, since it is written in place."""
+    b, h, d = 2, 2, 64
+    x = [rand(i, b, n, h, d, dtype=DT[dt]).requires_grad_() for i in range(3)]
+    g, flat = decays(h), rand(3, b * h * d * d + 1)
+    for at in (0, 1):
+        part = flat[at:at + b * h * d * d]
+        s0 = part.view(b, h, d, d).requires_grad_()
+        out, final = fa.linear_attn_func(*x, g, initial_state=s0, return_final_state=True)
+        both = torch.cat((rand(4, 3 if at else 4), final.flatten()))      # the gradient of the second part starts 12 bytes, or 16, into one buffer
+        weight = rand(5, 4 + len(both))[:len(both)]
+        got = (out, final) + torch.autograd.grad((out, both), x + [s0], (torch.ones_like(out), weight))
+        near = part.detach().clone().view(b, h, d, d).requires_grad_()
+        out, final = fa.linear_attn_func(*x, g, initial_state=near, return_final_state=True)
+        ds = weight[-final.numel():].clone().view_as(final)
+        want = (out, final) + torch.autograd.grad((out, final), x + [near], (torch.ones_like(out), ds))
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+    pool = flat[1:].view(b, h, d, d).detach()
+    with torch.no_grad(), pytest.raises(ValueError):
+        fa.linear_attn_with_state(*x, pool, g)
