@@ -105,7 +105,8 @@ def linear_attn_with_state(q, k, v, state, log_decay, scale=None, *, state_indic
     recorded in fable_attn.device_error().  Up to 16 tokens a sequence go through the state one by one; longer ones in
     chunks.  No gradients."""
     _check(q, log_decay)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad or
+                                    (state_out is not None and state_out.requires_grad)):
         raise NotImplementedError("fable_attn: linear_attn_with_state carries no gradients; use linear_attn_func")
     if scale is None:
         scale = q.shape[-1] ** -0.5

@@ -349,3 +349,24 @@ def test_states_that_are_slices_of_flat_buffers(dt, n):
     pool = flat[1:].view(b, h, d, d).detach()
     with torch.no_grad(), pytest.raises(ValueError):
         fa.linear_attn_with_state(*x, pool, g)
+
+
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+@pytest.mark.parametrize("hq,hk,d", [(2, 2, 64), (4, 2, 128)])
+@pytest.mark.parametrize("g", ["0", "-0.02", "-1.5"])
+@pytest.mark.parametrize("sizes", [(1.0, 1.0, 1.0, 2.0 ** -18, 1.0, 2.0 ** -10), (2.0 ** -9, 2.0 ** -9, 1.0, 1.0, 2.0 ** -8, 1.0), (2.0 ** 5, 2.0 ** 5, 2.0 ** -6, 2.0 ** -14, 1.0, 2.0 ** -9),
+                                   (1.0, 2.0 ** -12, 2.0 ** 6, 2.0 ** -6, 1.0, 2.0 ** -4), (2.0 ** -6, 2.0 ** 6, 2.0 ** -10, 2.0 ** 6, 2.0 ** -6, 1.0)])
+@pytest.mark.parametrize("carried", [False, True])
+def test_operands_of_other_sizes(dt, hq, hk, d, g, sizes, carried):
+    """Small gradients, small and large queries, keys and values, over several chunks, with and without states."""
+    check_sizes(DT[dt], 300, hq, hk, d, decays(hk, g), sizes, carried)
+
+
+def test_written_states_may_not_want_gradients():
+    x = [rand(i, 2, 3, 2, 64) for i in range(3)]
+    pool, out = torch.zeros(2, 2, 64, 64, device="cuda"), torch.zeros(2, 2, 64, 64, device="cuda", requires_grad=True)
+    with pytest.raises(NotImplementedError):
+        fa.linear_attn_with_state(*x, pool, decays(2), state_out=out)
+    with torch.no_grad():
+        fa.linear_attn_with_state(*x, pool, decays(2), state_out=out)
+    assert out.any()
