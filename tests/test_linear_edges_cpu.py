@@ -1,5 +1,6 @@
 """Linear attention and the rotary of q and k at the edges of what they are given: the parts that run on the host."""
 import ctypes as C
+import math
 import os
 import random
 import subprocess
@@ -88,3 +89,21 @@ def test_narrowing_refusals():
     assert L.fa_narrow_index_launch(None, None, 0, None) == A.FA_OK
     for args in ((None, 16, 3, None), (16, None, 3, None), (16, 16, -1, None)):
         assert L.fa_narrow_index_launch(*args) == A.FA_ERR_INVALID
+
+
+@pytest.mark.parametrize("dim,base,factor,length", [(64, 10000.0, 4.0, 4096), (128, 500000.0, 32.0, 8192), (16, 10000.0, 8.0, 256), (128, 10000.0, 1.0, 2048)])
+def test_yarn_between_the_kept_and_the_divided(dim, base, factor, length):
+    """Pair i turns length * base^(-2 i / dim) / (2 pi) times over the original length.  From the pair below the one that turns beta_fast = 32 times to the
+    pair above the one that turns once, the share that is divided by `factor` grows by equal steps; every element against that, pair by pair."""
+    from fable_attn.layers.rotary import scaled_inv_freq
+    got, times = scaled_inv_freq(dim, base, "yarn", factor, length)
+    of = lambda turns: dim / 2 * math.log(length / (2 * math.pi * turns)) / math.log(base)      # the (real) pair that turns so often
+    first, last = max(math.floor(of(32.0)), 0), min(math.ceil(of(1.0)), dim - 1)
+    assert first < last and 0 < sum(first < i < last for i in range(dim // 2))
+    for i in range(dim // 2):
+        f = base ** (-2 * i / dim)
+        share = 0.0 if i <= first else 1.0 if i >= last else (i - first) / (last - first)
+        assert math.isclose(float(got[i]), f * ((1 - share) + share / factor), rel_tol=1e-12), i
+    assert math.isclose(times, 1 + 0.1 * math.log(factor))
+    slow, _ = scaled_inv_freq(dim, base, "yarn", factor, length, beta_fast=8.0, beta_slow=2.0)
+    assert bool((slow <= got * (1 + 1e-12)).any()) and float(slow[0]) == 1.0
