@@ -667,16 +667,24 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             if (REV ? j0 / 32 < qd : j0 / 32 > qd) continue;
             float2 p[W / 2];
             tmem_load<W>(la + K::P_COL + j0, p);
-            if (j0 / 32 == qd || (REV && cn < C)) {
+            if (REV && cn < C) {
 #pragma unroll
               for (int i = 0; i < W / 2; ++i) {
-                const int j = j0 + 2 * i;
-                if (REV ? j < row || j >= cn : j > row) p[i].x = 0.f;
-                if (REV ? j + 1 < row || j + 1 >= cn : j + 1 > row) p[i].y = 0.f;
+                if (j0 + 2 * i >= cn) p[i].x = 0.f;
+                if (j0 + 2 * i + 1 >= cn) p[i].y = 0.f;
               }
             }
+            if (j0 / 32 == qd) {
+              const int own = row - j0;
 #pragma unroll
-            for (int i = 0; i < W / 2; ++i) top = fmaxf(top, fmaxf(fabsf(p[i].x), fabsf(p[i].y)));
+              for (int i = 0; i < W / 2; ++i) {
+                if (REV ? 2 * i >= own : 2 * i <= own) top = fmaxf(top, fabsf(p[i].x));
+                if (REV ? 2 * i + 1 >= own : 2 * i + 1 <= own) top = fmaxf(top, fabsf(p[i].y));
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < W / 2; ++i) top = fmaxf(top, fmaxf(fabsf(p[i].x), fabsf(p[i].y)));
+            }
           }
           uint32_t* most = pmax + row;
           most[hf * C] = __float_as_uint(top);      // the item before was read before its P c, which this P waited for
@@ -705,17 +713,13 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             } else {
               // On the diagonal, in pieces of 8 columns: lam^(gap to the piece's far edge), which may be up to lam^-7, times the table's, and what
               // lies on the other side is masked.  Where lam^-7 could overflow, exp2 of each gap (1200 cycles a block, not 600).
-              // fp16's row scale goes to the products: lam^-7 (up to 2^119) times a scale (2^10 and more) would overflow, while
-              // a scaled product is below 2^11 and lam^-7 times the table's factor at most 1 wherever it counts.
-              if constexpr (!BF16) {
-#pragma unroll
-                for (int i = 0; i < W / 2; ++i) p[i] = __fmul2_rn(p[i], make_float2(ps, ps));
-              }
+              // fp16's row scale (2^10 and more where products are near 1 or smaller) goes to the factors as long as lam^-7 times it is in range
+              // for every row of the warp; exp2 of a gap that counts is at most 1
               const float from = (float)(REV ? j0 - row : row - j0);      // gap of the piece's first column
-              if (g2 > -17.f) {
+              if (BF16 ? g2 > -17.f : __all_sync(0xffffffffu, ex2(-7.f * g2) * ps < 0x1p126f)) {
 #pragma unroll
                 for (int s = 0; s < W / 8; ++s) {
-                  const float edge_gap = REV ? from + 8 * s : from - 8 * s - 7, u = ex2(g2 * edge_gap);
+                  const float edge_gap = REV ? from + 8 * s : from - 8 * s - 7, u = ex2(g2 * edge_gap) * ps;
                   const float4 w0 = *reinterpret_cast<const float4*>(lamc + (REV ? 0 : 24)), w1 = *reinterpret_cast<const float4*>(lamc + (REV ? 4 : 28));
                   p[4 * s] = __fmul2_rn(p[4 * s], __fmul2_rn(make_float2(u, u), make_float2(w0.x, w0.y)));
                   p[4 * s + 1] = __fmul2_rn(p[4 * s + 1], __fmul2_rn(make_float2(u, u), make_float2(w0.z, w0.w)));
@@ -732,8 +736,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 #pragma unroll
                 for (int i = 0; i < W / 2; ++i) {
                   const float gap = REV ? from + 2 * i : from - 2 * i, next = REV ? gap + 1.f : gap - 1.f;
-                  p[i].x = gap >= 0.f ? p[i].x * ex2(g2 * gap) : 0.f;
-                  p[i].y = next >= 0.f ? p[i].y * ex2(g2 * next) : 0.f;
+                  p[i].x = gap >= 0.f ? p[i].x * (ex2(g2 * gap) * ps) : 0.f;
+                  p[i].y = next >= 0.f ? p[i].y * (ex2(g2 * next) * ps) : 0.f;
                 }
               }
             }
