@@ -102,3 +102,57 @@ def test_first_backward_of_a_process(kind):
     root = os.path.dirname(os.path.dirname(os.path.abspath(fa.__file__)))
     r = subprocess.run([sys.executable, "-c", BACKWARD, root, kind], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "True" in r.stdout and "False" not in r.stdout, r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("name", ["prompt", "forward128", "packed"])
+def test_two_threads_at_once(name):
+    """Each on a stream of its own, many times over: nothing is shared that the calls write."""
+    calls = [CALLS[name]() for _ in range(2)]
+    want = [[x.clone() for x in c()] for c in calls]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                if not all(torch.equal(a, b) for a, b in zip(calls[i](), want[i])):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+CAPTURED = """
+import sys, torch
+sys.path.insert(0, sys.argv[1])
+import fable_attn as fa
+from fable_attn.layers.rotary import apply_rotary_emb_qk, scaled_inv_freq
+torch.manual_seed(0)
+x = [torch.randn(2, 300, 4, 64, device="cuda").bfloat16().requires_grad_() for _ in range(3)]
+do, g = torch.randn_like(x[0]), torch.full((4,), -0.02, device="cuda")
+freq = scaled_inv_freq(64, device="cuda")[0]
+
+def step():
+    q, k = apply_rotary_emb_qk(x[0], x[1], freq)
+    out = fa.linear_attn_func(q, k, x[2], g)
+    return (out,) + torch.autograd.grad(out, x, do)
+
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = step()
+graph.replay()
+torch.cuda.synchronize()
+print([bool(torch.equal(a, b)) for a, b in zip(got, step())], fa.device_error())
+"""
+
+
+def test_first_calls_of_a_process_captured():
+    """No call before the capture: kernels are loaded, and their limits raised, inside it."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(fa.__file__)))
+    r = subprocess.run([sys.executable, "-c", CAPTURED, root], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.split("]")[0] == "[True, True, True, True" and r.stdout.split()[-1] == "0", r.stdout + r.stderr
