@@ -15,7 +15,7 @@ nheads_k, headdim_v), fp16, bf16 or fp32; the nheads / nheads_k query heads of a
     linear_attn_with_state   serving: new tokens (a chunk of a prompt, or one or a few) continue states that live in a pool
 
 log_decay (nheads_k,) is the natural logarithm of the factor per token: 0 keeps everything, -infinity nothing but the token
-itself, and a value above 0 counts as 0.  It carries no gradient.  scale defaults to headdim ** -0.5.  A NaN or an infinity may
+itself, and a value above 0 counts as 0.  It carries no gradient, and forward-mode tangents are refused.  scale defaults to headdim ** -0.5.  A NaN or an infinity may
 reach every output of its own sequence and heads, the tokens before it among them, and no other sequence.  All calls run on the
 current stream and read lengths and indices on the device, with no host synchronisation.  The reference has no counterpart.
 """
