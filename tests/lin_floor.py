@@ -5,7 +5,9 @@ smallest step, 2^-25:
   pair products   a power of 2 brings a row's largest one to 2^10 or more, so that 2^-35 of that one is lost;
   the state       likewise, with the largest element of a state;
   decayed rows    b lam^m (dk: c lam^m) as they are: 2^-25 each, carried from their chunk's end on with the other operand.
-Last states are summed from rows whose second number is held 2^11 times as large: 2^-36 each.  A chunk is 128 tokens from the sequence's start."""
+Last states are summed from rows whose second number is held 2^11 times as large: 2^-36 each.  A chunk is 128 tokens from the sequence's start.
+(What the tensor cores cut from a sum of operands that small, about 2^-37 of the other operand's largest value for each sixteen tokens, is of
+the same size and not counted.)"""
 import torch
 
 CHUNK = 128
