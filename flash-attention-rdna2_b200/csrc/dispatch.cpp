@@ -954,10 +954,10 @@ std::tuple<torch::Tensor, torch::Tensor> rotary_qk(torch::Tensor q, torch::Tenso
   } else {
     const auto given = offsets.cast<torch::Tensor>();
     TORCH_CHECK_VALUE(given.numel() == p.batch, "fable_attn: seqlen_offsets needs one entry per sequence");
-    if (given.scalar_type() == torch::kInt64) {      // every token's own position, which has 64 bits
-      pos = given.to(q.device()).reshape({p.batch, 1}) + torch::arange(p.seqlen, given.options().device(q.device()));
-      p.positions = pos.const_data_ptr();
-      p.pos_bytes = 8;
+    if (given.scalar_type() == torch::kInt64) {
+      offs = given.to(q.device()).contiguous();
+      p.offsets = (const int*)offs.const_data_ptr();
+      p.pos_bytes = FA_ROTARY_OFFSETS_64;
     } else {
       offs = index_i32(given, q.device(), "seqlen_offsets");
       p.offsets = offs.data_ptr<int>();

@@ -61,7 +61,8 @@ __global__ void __launch_bounds__(THREADS, 5) rotary_qk_kernel(const FaRotaryQkP
       pos = p.pos_bytes == 8 ? ((const long long*)p.positions)[row] : ((const int*)p.positions)[row];
     } else {
       const long long z = row / p.seqlen;
-      pos = row - z * p.seqlen + p.offset + (p.offsets ? p.offsets[z] : 0);
+      pos = row - z * p.seqlen + p.offset;
+      if (p.offsets) pos += p.pos_bytes == FA_ROTARY_OFFSETS_64 ? ((const long long*)p.offsets)[z] : p.offsets[z];
     }
     const unsigned long long angle = (unsigned long long)pos * turns_of(p.inv_freq[i]);
     const unsigned int hi = (unsigned int)((angle + 0x80000000ull) >> 32);     // to nearest: opposite positions turn alike

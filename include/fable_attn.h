@@ -495,7 +495,9 @@ FA_API int fa_linear_backward_launch(const FaLinearBwdParams* p, int dtype, void
  * `inverse` turns back (the gradient: by -theta, with the same factor).
  *   rows z * seqlen + t by strides (dim contiguous); k may be null.  Outputs may be the inputs.
  *   positions  [batch * seqlen] int32 or int64 (pos_bytes 4 / 8), or null: offsets[z] (0 where null) + offset + t
+ *   offsets    int32, or int64 where positions is null and pos_bytes is FA_ROTARY_OFFSETS_64
  * -------------------------------------------------------------------------------------------*/
+#define FA_ROTARY_OFFSETS_64 (-8)
 typedef struct FaRotaryQkParams {
   unsigned int struct_size;
   const void *q, *k;
